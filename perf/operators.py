@@ -2,9 +2,9 @@
 
 Three operators, each as an inference program calls it on activations that are already on the device:
 
-  quantize   rows of bf16, fp16 or fp32 to MXFP4 (E2M1) or MXFP8 (E4M3), a power of two for every 32 columns, and back to
+  quantize   rows of bf16, fp16 or fp32 to MXFP4 (E2M1) or MXFP6 (E2M3), a power of two for every 32 columns, and back to
              the values they stand for
-  linear     one projection: activations quantised to MXFP4 ("a4") or MXFP8 ("a8"), times an MXFP4 tensor; with `glu` the
+  linear     one projection: activations quantised to MXFP4 ("a4") or MXFP6 ("a6"), times an MXFP4 tensor; with `glu` the
              tensor holds gate and up and the product leaves as silu(gate) * up
   experts    the same product grouped by expert: every (token, route) pair against the tensor of its expert, groups of any
              size; with `routed` every pair has an activation row of its own (the down projection)
@@ -24,8 +24,8 @@ import torch
 own = False
 
 DTYPE = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
-ACT = {"a4": "MXFP4", "a8": "MXFP8"}
-MAX_FLOPS = 1.47e12  # of a product with 4-bit activations; 8-bit ones cost twice as much
+ACT = {"a4": "MXFP4", "a6": "MXFP6"}
+MAX_FLOPS = 1.47e12
 
 
 def listed():
@@ -33,21 +33,21 @@ def listed():
         # the hidden state of one sequence before a projection: launch latency
         dict(name="quantize_a4_row1", kind="quantize", act="a4", rows=1, k=4096, dtype="bf16"),
         # the hidden rows of a prefill chunk in front of a down projection
-        dict(name="quantize_a8_rows2048", kind="quantize", act="a8", rows=2048, k=12288, dtype="bf16"),
+        dict(name="quantize_a6_rows2048", kind="quantize", act="a6", rows=2048, k=12288, dtype="bf16"),
         # the fp32 rows that the packed matmuls return, for every (token, route) pair of a chunk
         dict(name="quantize_a4_fp32_rows16383", kind="quantize", act="a4", rows=16383, k=4096, dtype="fp32"),
         # one projection of a decode step: the weights are read once
         dict(name="linear_a4_row1", kind="linear", act="a4", out=12288, k=4096, rows=1, dtype="bf16", glu=False, result="fp32"),
         # a batched decode step through a down projection
-        dict(name="linear_a8_rows13", kind="linear", act="a8", out=4096, k=12288, rows=13, dtype="bf16", glu=False, result="fp32"),
+        dict(name="linear_a6_rows13", kind="linear", act="a6", out=4096, k=12288, rows=13, dtype="bf16", glu=False, result="fp32"),
         # a prefill chunk of an odd length
         dict(name="linear_a4_rows601", kind="linear", act="a4", out=12288, k=4096, rows=601, dtype="bf16", glu=False, result="fp32"),
         # gate and up of a dense feed-forward block over a full prefill chunk
-        dict(name="linear_a8_glu_rows2048", kind="linear", act="a8", out=24576, k=4096, rows=2048, dtype="fp16", glu=True, result="fp16"),
+        dict(name="linear_a6_glu_rows2048", kind="linear", act="a6", out=24576, k=4096, rows=2048, dtype="fp16", glu=True, result="fp16"),
         # several prompts prefilled together: the most arithmetic
         dict(name="linear_a4_rows8192", kind="linear", act="a4", out=17408, k=5120, rows=8192, dtype="bf16", glu=False, result="bf16"),
         # gate and up of the routed experts of one token
-        dict(name="experts_a8_glu_row1", kind="experts", act="a8", experts=64, top_k=8, out=4096, k=4096, rows=1, dtype="bf16",
+        dict(name="experts_a6_glu_row1", kind="experts", act="a6", experts=64, top_k=8, out=4096, k=4096, rows=1, dtype="bf16",
              glu=True, routed=False, dropped=0.0, result="fp16"),
         # the down projection of a batched decode step that hits every expert, some routes dropped
         dict(name="experts_a4_rows61", kind="experts", act="a4", experts=64, top_k=8, out=4096, k=2048, rows=61, dtype="fp16",
@@ -56,7 +56,7 @@ def listed():
         dict(name="experts_a4_glu_rows2048", kind="experts", act="a4", experts=128, top_k=8, out=2048, k=2048, rows=2048, dtype="bf16",
              glu=True, routed=False, dropped=0.0, result="bf16"),
         # the down projection of a prefill chunk where rows end inside every tile
-        dict(name="experts_a8_rows1501", kind="experts", act="a8", experts=32, top_k=4, out=2880, k=1440, rows=1501, dtype="bf16",
+        dict(name="experts_a6_rows1501", kind="experts", act="a6", experts=32, top_k=4, out=2880, k=1440, rows=1501, dtype="bf16",
              glu=False, routed=True, dropped=0.0, result="fp32"),
     ]
 
@@ -67,7 +67,7 @@ def _log_int(rng, lo, hi):
 
 def draw(rng):
     while True:
-        c = dict(kind=rng.choice(("quantize",) + ("linear",) * 3 + ("experts",) * 3), act=rng.choice(("a4", "a8")))
+        c = dict(kind=rng.choice(("quantize",) + ("linear",) * 3 + ("experts",) * 3), act=rng.choice(("a4", "a6")))
         if c["kind"] == "quantize":
             c.update(rows=_log_int(rng, 1, 16384), k=32 * _log_int(rng, 32, 544), dtype=rng.choice(tuple(DTYPE)))
             if c["rows"] * c["k"] > 6.72e7:
@@ -81,7 +81,7 @@ def draw(rng):
             hidden, inter, experts = rng.choice(((4096, 2048, 64), (2048, 1024, 128), (2048, 768, 128), (2880, 1440, 32)))
             c.update(experts=experts, top_k=rng.choice((1, 2, 4, 8)), rows=_log_int(rng, 1, 4096), routed=not c["glu"],
                      out=2 * inter if c["glu"] else hidden, k=hidden if c["glu"] else inter, dropped=rng.choice((0.0, 0.0, 0.05)))
-        if work(c)["flops"] * (2 if c["act"] == "a8" else 1) <= MAX_FLOPS:
+        if work(c)["flops"] <= MAX_FLOPS:
             return c
 
 
@@ -134,14 +134,14 @@ def prepare(case, seed):
 # ---- the plain forms -------------------------------------------------------------------------------------------------
 def _quantized(x, act):
     """fp32 values of the rows after quantisation: in each block of 32 the scale 2^(e - emax), e = the exponent of the largest
-    magnitude; elements rounded to the nearest of E2M1 (emax 2, up to 6) or E4M3 (emax 8, up to 448), ties to even, the
-    largest where they are beyond it.  The scale's exponent is at least -127."""
-    emax, emin, mant, most = (2, 0, 1, 6.0) if act == "a4" else (8, -6, 3, 448.0)
+    magnitude and emax = 2; elements rounded to the nearest of E2M1 (up to 6) or E2M3 (up to 7.5), ties to even, the largest
+    where they are beyond it.  The scale's exponent is at least -127."""
+    mant, most = (1, 6.0) if act == "a4" else (3, 7.5)
     v = x.float().reshape(x.shape[0], -1, 32)
     e = torch.frexp(v.abs().amax(-1, keepdim=True))[1] - 1
-    scale = torch.ldexp(torch.ones_like(v[..., :1]), (e - emax).clamp(min=-127))
+    scale = torch.ldexp(torch.ones_like(v[..., :1]), (e - 2).clamp(min=-127))
     v = v / scale
-    step = torch.ldexp(torch.ones_like(v), (torch.frexp(v)[1] - 1).clamp(min=emin) - mant)
+    step = torch.ldexp(torch.ones_like(v), (torch.frexp(v)[1] - 1).clamp(min=0) - mant)
     return ((torch.round(v / step) * step).clamp(-most, most) * scale).reshape(x.shape[0], -1)
 
 
@@ -215,7 +215,7 @@ def work(case):
     of a quantisation also the codes and scales that it leaves."""
     c = case
     size = {"bf16": 2, "fp16": 2, "fp32": 4}
-    coded = {"a4": 17 / 32, "a8": 33 / 32}[c["act"]]
+    coded = {"a4": 17 / 32, "a6": 25 / 32}[c["act"]]
     if c["kind"] == "quantize":
         n = c["rows"] * c["k"]
         return {"bytes": n * (2 * size[c["dtype"]] + coded), "flops": 0}
@@ -234,7 +234,7 @@ def _grid(act):
     """every magnitude of the element type, in the order of its codes"""
     if act == "a4":
         return [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
-    return [(m / 8 if e == 0 else 1 + m / 8) * 2.0 ** (max(e, 1) - 7) for e in range(16) for m in range(8)][:127]
+    return [(m / 8 if e == 0 else 1 + m / 8) * 2.0 ** (max(e, 1) - 1) for e in range(4) for m in range(8)]
 
 
 def _rounded64(x, act):
@@ -246,7 +246,7 @@ def _rounded64(x, act):
     for v in x.split(max(1, (1 << 25) // x.shape[1])):
         v = v.double().reshape(v.shape[0], -1, 32)
         most = v.abs().amax(-1, keepdim=True)
-        unit = torch.exp2((torch.floor(torch.log2(most)) - (2 if act == "a4" else 8)).clamp(min=-127.0))
+        unit = torch.exp2((torch.floor(torch.log2(most)) - 2).clamp(min=-127.0))
         a = v.abs() / unit
         below = torch.searchsorted(mid, a.contiguous(), right=False)  # midpoints under the value
         at = below.clamp(max=len(mid) - 1)
