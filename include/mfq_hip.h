@@ -492,6 +492,49 @@ int mfq_hip_mx_gemv_pairs(int kind, const void *values, const void *scales, int 
                           const int32_t *expert_slot, int E, const void *x, int x_dtype, int64_t ldx, int routed_input,
                           const int32_t *ids, int T, int R, float *y, int64_t ldy, mfq_stream_t stream);
 
+/* Products of two microscaled operands: MXFP4 weights against activations quantised on the device to kind 4 = MXFP4 (E2M1) or
+ * kind 6 = MXFP6 (E2M3), in either case with one E8M0 scale for every 32 columns of a row.  The matrix cores take the codes
+ * and scales of both operands as they are, at one rate for both kinds, and sum in fp32.  No counterpart in the reference, which
+ * multiplies MX weights in fp16.
+ * Quantised rows: values [M, mfq_hip_mx_quantized_row_bytes(kind, cols)], 16-byte aligned, rows of whole groups of 256 columns with
+ * zeros behind the last: 128 bytes of E2M1 codes (low nibble = even column); or of the eight blocks' 192 bits of E2M3 codes (the first
+ * column lowest) the first 16 bytes of each and then the last 8 of each.  scales [M, mfq_hip_mx_scale_stride(cols)], 8-byte aligned:
+ * cols / 32 bytes and zeros up to a multiple of eight.
+ * The scale of a block is 2^(e - 2), e = the exponent of its largest magnitude, at least 2^-127; elements are rounded to nearest, ties
+ * to even, those beyond the largest element (6 or 7.5) to it.  A block that holds an infinity or a NaN takes scale 255 (NaN) and
+ * codes 0.  x: bf16, fp16 or fp32 [M, ldx]; cols must be divisible by 32. */
+int mfq_hip_mx_quantized_row_bytes(int kind, int cols);
+int mfq_hip_mx_scale_stride(int cols);
+int mfq_hip_mx_quantize_rows(int kind, const void *x, int x_dtype, int64_t ldx, int M, int cols, void *values, void *scales,
+                             mfq_stream_t stream);
+/* out[m][c] = element * scale in fp32, rounded once to out_dtype. */
+int mfq_hip_mx_dequant_quantized(int kind, const void *values, const void *scales, int M, int cols, int out_dtype, void *out,
+                                 int64_t ldo, mfq_stream_t stream);
+/* Scales of an MXFP4 payload [rows, cols / 32] at the row stride of the calls below; needed only where cols is no multiple of 256
+ * (elsewhere the payload has that stride). */
+int mfq_hip_mx_pad_scales(const void *scales, int64_t rows, int cols, void *out, mfq_stream_t stream);
+/* y[M, nrows] = q(x) . W^T over rows [row0, row0 + nrows) of an MXFP4 tensor [rows, cols], fp32 accumulation, rounded once to
+ * y_dtype (MFQ_X_*).  `scales` has rows of mfq_hip_mx_scale_stride(cols) bytes.  act: kind of q(x).  x is bf16, fp16 or fp32
+ * [M, ldx] and quantised by the call (x_scales null), or the values of quantised rows with their x_scales (x_dtype and ldx are
+ * not looked at then).  glu != 0: gate rows first, y[M, nrows / 2] = act(gate) * up with `activation` MFQ_GLU_*, 16-bit y_dtype.
+ * Rows of x that hold a NaN or an infinity give NaN.  Workspace (size from the query): the quantised rows, and partial sums of a
+ * split over K; without room for the latter K is split into fewer pieces.  Sums have a fixed order. */
+size_t mfq_hip_mx_scaled_gemm_workspace_bytes(int act, int nrows, int cols, int M, int x_quantized);
+int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scales, int rows, int cols, int row0, int nrows, int act,
+                                const void *x, int x_dtype, int64_t ldx, const void *x_scales, int M, int glu, int activation,
+                                void *y, int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, mfq_stream_t stream);
+/* The same grouped by expert: y[p] = q(x[p (routed_input) or p / R]) . W[ids[p]]^T for every pair p = t * R + r, W = a pool
+ * [experts * out_per_expert, cols].  ids device int32 [T, R]; ids outside [0, E) give rows of zeros.  expert_slot (device, [E]) =
+ * place of an expert in the pool, -1 for those of other pools, whose rows are left as they are; null: the experts as they lie.
+ * ids_dst and expert_bounds from mfq_hip_moe_route_map (any tile_m), or both null: every pair by itself, for a handful of tokens.
+ * x has T rows, with routed_input T * R.  Workspace: the quantised rows of calls with a route map. */
+size_t mfq_hip_mx_moe_workspace_bytes(int act, int cols, int x_rows, int mapped, int x_quantized);
+int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int rows, int cols, int out_per_expert, const int32_t *expert_slot,
+                          int E, int act, const void *x, int x_dtype, int64_t ldx, const void *x_scales, int routed_input,
+                          const int32_t *ids, int T, int R, const int32_t *ids_dst, const int32_t *expert_bounds, int glu,
+                          int activation, void *y, int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes,
+                          mfq_stream_t stream);
+
 /* ------------------------------------------------------------------------------------
  * NEPQ1-S / NEPQ1-L (cross-expert table pool, bank id per 96 weights).  Rows are the
  * flattened [experts * out_per_expert] neurons.  Replaces NepqWeight

@@ -138,6 +138,17 @@ _SIGS = {
     "mfq_hip_mx_gemm_rows_workspace_bytes": (sz, [C.c_int, C.c_int, C.c_int]),
     "mfq_hip_mx_gemv_pairs": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, i64, C.c_int, vp, C.c_int,
                               C.c_int, vp, i64, vp]),
+    "mfq_hip_mx_quantized_row_bytes": (C.c_int, [C.c_int, C.c_int]),
+    "mfq_hip_mx_scale_stride": (C.c_int, [C.c_int]),
+    "mfq_hip_mx_quantize_rows": (C.c_int, [C.c_int, vp, C.c_int, i64, C.c_int, C.c_int, vp, vp, vp]),
+    "mfq_hip_mx_dequant_quantized": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, vp, i64, vp]),
+    "mfq_hip_mx_pad_scales": (C.c_int, [vp, i64, C.c_int, vp, vp]),
+    "mfq_hip_mx_scaled_gemm_workspace_bytes": (sz, [C.c_int] * 5),
+    "mfq_hip_mx_scaled_gemm_rows": (C.c_int, [vp, vp] + [C.c_int] * 5 + [vp, C.c_int, i64, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, i64, vp,
+                                    sz, vp]),
+    "mfq_hip_mx_moe_workspace_bytes": (sz, [C.c_int] * 5),
+    "mfq_hip_mx_moe_matmul": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, C.c_int, vp, C.c_int, i64, vp, C.c_int, vp, C.c_int,
+                              C.c_int, vp, vp, C.c_int, C.c_int, vp, C.c_int, i64, vp, sz, vp]),
     "mfq_hip_mx_gemm_rows": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, C.c_int, i64, C.c_int, vp, i64,
                                        vp, sz, vp]),
     "mfq_hip_nepq_plan": (C.c_int, [C.c_int] * 4 + [C.POINTER(NepqDesc)]),

@@ -1,0 +1,194 @@
+// Products of two microscaled operands: MXFP4 weights (E2M1 nibbles) against activations quantised to MXFP4 or to MXFP6
+// (E2M3), a power of two (E8M0) for every 32 columns of a row of either operand.
+//   y[m, n] = sum over blocks b of 32 columns  2^(sw[n, b] - 127) * 2^(sx[m, b] - 127) * sum_k w[n, k] * x[m, k]
+// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 rows by 16 rows over 128 columns of codes as they lie in memory and
+// applies the eight scale bytes of each row pair itself, so nothing is converted on the way, and its sums are held in fp32.
+// (With an FP8 operand it is half as fast, and adds products in groups of eight aligned to the largest, of which it keeps 14 bits:
+// measured 5e-6 to 2e-5, 2-norm, from the same sums in 64 bits.  FP4 and FP6 gave exact sums where they fit 24 bits.)
+//
+// Lanes of that instruction, lane l = (r, g), r = l & 15, g = l >> 4: an operand holds columns 32 g .. 32 g + 31 of row r, four
+// registers of FP4 or six of FP6; its scale register holds in the byte that the instruction names the scale of block g of row r; the
+// result of lane l is row 4 g + i of the first operand by row r of the second.  A sum does not care which column sits in which slot as
+// long as both operands agree: the kernels take 256 columns ("a macro": 8 blocks) for two instructions, the first over blocks
+// 0, 2, 4, 6 and the second over blocks 1, 3, 5, 7, so that lane g's two scale bytes are neighbours, one 16-bit read.
+//
+// Quantised activations are rows of whole macros, zeros behind the last column: 128 bytes of FP4 codes in their order (low nibble =
+// even column), or of FP6 the first 16 bytes of each of the eight blocks' 24 and then their last 8 (a block's codes are 192 bits,
+// the first code lowest): both parts of a macro are then read from LDS 16 bytes at a time.
+//
+// Both operands pass through LDS, copied there directly and row by row: a request moves 8 lines of 128 bytes, eight lanes a line
+// (lanes of a load in different rows occupy a compute unit's address path four times as long).  The 16-byte pieces of a line
+// are turned by a key of the row, mx_key, with which each of the four passes in which the hardware serves a 16-byte read meets
+// every bank once; those of FP6's second part lie as in row_order_quarter.
+#pragma once
+#include "common.hpp"
+#include "gemv_common.hpp"
+#include "tile_gemm.hpp"
+#include "tune.hpp"
+
+namespace mfq {
+
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kMxMacro = 256;  // columns of a macro
+
+// bytes of a row of scales: those of whole macros
+__host__ __device__ __forceinline__ constexpr int mx_scale_stride(int K) { return (K / 32 + 7) & ~7; }
+// bytes of a macro of quantised activations, and of a row
+__host__ __device__ __forceinline__ constexpr int mx_macro_bytes(int kind) { return kind == 4 ? 128 : 192; }
+__host__ __device__ __forceinline__ constexpr int64_t mx_row_bytes(int kind, int K) { return static_cast<int64_t>((K + kMxMacro - 1) / kMxMacro) * mx_macro_bytes(kind); }
+
+// by which the pieces of a line are turned, from its row (0 .. 15): with rows p = 2, 3, 4, 5 (in pairs) in the upper half and 0, 1, 6, 7
+// in the lower, for each of which the hardware reads another lane group's piece in the same pass
+__device__ __forceinline__ int mx_key(int row) {
+    const int p = (row >> 1) & 7;
+    return (p & 1) | ((p >> 2) << 1) | ((((p >> 1) ^ (p >> 2)) & 1) << 2);
+}
+
+// a fragment of activations: FP4 fills x, FP6 also y
+struct MxFrag {
+    u32x4_t x;
+    u32x2_t y;
+};
+template <int AK, int SEL>
+__device__ __forceinline__ float4_t mx_scale_mfma(u32x4_t w, const MxFrag &f, float4_t c, uint32_t sw, uint32_t sx) {
+    const i32x8_t a = {static_cast<int>(w.x), static_cast<int>(w.y), static_cast<int>(w.z), static_cast<int>(w.w), 0, 0, 0, 0};
+    if constexpr (AK == 4) {
+        const i32x8_t b = {static_cast<int>(f.x.x), static_cast<int>(f.x.y), static_cast<int>(f.x.z), static_cast<int>(f.x.w), 0, 0, 0, 0};
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, SEL, static_cast<int>(sw), SEL, static_cast<int>(sx));
+    } else {
+        const i32x8_t b = {static_cast<int>(f.x.x), static_cast<int>(f.x.y), static_cast<int>(f.x.z), static_cast<int>(f.x.w),
+                           static_cast<int>(f.y.x), static_cast<int>(f.y.y), 0, 0};
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 2, SEL, static_cast<int>(sw), SEL, static_cast<int>(sx));
+    }
+}
+
+// Copies of a wave straight into LDS, 16 or 4 bytes a lane, lane after lane from `lds` on.  POLICY: as in load_unit_win.
+template <int POLICY>
+__device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t win, uint8_t *lds, uint32_t at, int base) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(win, (lds_void_t)lds, 16, at, base, 0, POLICY);
+}
+__device__ __forceinline__ void copy4(__amdgpu_buffer_rsrc_t win, uint8_t *lds, uint32_t at, int base) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(win, (lds_void_t)lds, 4, at, base, 0, 0);
+}
+
+// ---- quantisation of eight values of a block of 32, which lies in the four lanes of a quad --------------------------------------
+// Scale 2^(e - 2), e the exponent of the block's largest magnitude (both element types reach into the binade of 4), not below
+// 2^-127; elements to nearest, ties to even, those beyond the largest element (6, or 7.5) to it.  A block that holds an infinity
+// or a NaN takes the NaN scale 255 and codes of zero.
+template <int PERM>
+__device__ __forceinline__ uint32_t quad_perm(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), PERM, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t mx_scale_byte(const float (&v)[8]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+    most = max(most, quad_perm<0xB1>(most));
+    most = max(most, quad_perm<0x4E>(most));
+    const int e = static_cast<int>(most >> 23);  // of an fp32 subnormal 0: its scale is 2^-127 in any case
+    return e == 255 ? 255u : static_cast<uint32_t>(max(e - 2, 0));
+}
+// codes of eight values: 32 bits of E2M1, or 48 of E2M3
+template <int AK>
+__device__ __forceinline__ u32x2_t mx_codes(const float (&v)[8], uint32_t byte) {
+    u32x2_t q = {0u, 0u};
+    if constexpr (AK == 4) {
+        // the conversions divide by the power of two in the exponent field, of which 0 is 2^-127, and saturate
+        const float scale = __uint_as_float(byte << 23);
+        q.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q.x, v[0], v[1], scale, 0);
+        q.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q.x, v[2], v[3], scale, 1);
+        q.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q.x, v[4], v[5], scale, 2);
+        q.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q.x, v[6], v[7], scale, 3);
+    } else {
+        // From 1 on the three bits behind an fp32's leading one, rounded, are the code's fraction and what they carry its exponent;
+        // below 1 codes are eighths.  (The hardware converts whole blocks of one lane only.)
+        const float up = byte > 253u ? 0.f : __uint_as_float((254u - byte) << 23);  // 2^(127 - byte); 255 needs none
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = fabsf(v[i]) * up;
+            const uint32_t bits = __float_as_uint(a);
+            const uint32_t high = ((bits + 0x7ffffu + ((bits >> 20) & 1u)) >> 20) - (127u * 8u - 8u);
+            const uint32_t low = static_cast<uint32_t>(__builtin_rintf(a * 8.f));
+            const uint32_t c = min(a < 1.f ? low : high, 31u) | ((__float_as_uint(v[i]) >> 26) & 32u);
+            if (i < 5) q.x |= c << (6 * i);
+            else if (i == 5) { q.x |= c << 30; q.y |= c >> 2; }
+            else q.y |= c << (6 * i - 32);
+        }
+    }
+    return byte == 255u ? u32x2_t{0u, 0u} : q;
+}
+// Where the codes of piece p (eight columns, lane p & 3 of its quad) go in a row of quantised activations, and what: FP4 a dword a
+// lane; FP6 8 bytes of the block's 24 for lanes 0 to 2, each with what its neighbour holds of them.
+struct MxStore {
+    u32x2_t q;
+    uint32_t at;
+    bool any;
+};
+template <int AK>
+__device__ __forceinline__ MxStore mx_place(u32x2_t q, int p) {
+    const uint32_t mac = static_cast<uint32_t>(p) >> 5, in = p & 31, j = p & 3;
+    if constexpr (AK == 4) return {q, mac * 128u + in * 4u, true};
+    const uint32_t nx = quad_perm<0xF9>(q.x), ny = quad_perm<0xF9>(q.y);  // of the next lane
+    u32x2_t o;
+    if (j == 0) o = u32x2_t{q.x, q.y | (nx << 16)};
+    else if (j == 1) o = u32x2_t{(q.x >> 16) | (q.y << 16), nx};
+    else o = u32x2_t{q.y | (nx << 16), (nx >> 16) | (ny << 16)};
+    const uint32_t block = in >> 2;
+    return {o, mac * 192u + (j < 2 ? block * 16u + j * 8u : 128u + block * 8u), j < 3};
+}
+
+// Eight consecutive values of a row as fp32; VEC: the row's pieces of eight lie on 16-byte boundaries.
+template <int XD, bool VEC>
+__device__ __forceinline__ void mx_load8(const void *x, int64_t at, float (&v)[8]) {
+    if constexpr (XD == MFQ_X_F32) {
+        const float *p = static_cast<const float *>(x) + at;
+        if constexpr (VEC) {
+            const float4_t a = *reinterpret_cast<const float4_t *>(p), b = *reinterpret_cast<const float4_t *>(p + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = p[i];
+        }
+    } else {
+        const uint16_t *p = static_cast<const uint16_t *>(x) + at;
+        if constexpr (VEC) {
+            const u32x4_t q = *reinterpret_cast<const u32x4_t *>(p);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = x_to_f32<XD == MFQ_X_F16>(static_cast<uint16_t>(q[i >> 1] >> (16 * (i & 1))));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = x_to_f32<XD == MFQ_X_F16>(p[i]);
+        }
+    }
+}
+
+// two values rounded to a 16-bit type
+__device__ __forceinline__ uint32_t mx_pack16(float lo, float hi, int dtype) {
+    if (dtype == MFQ_X_F16) return static_cast<uint32_t>(f32_to_f16_rne(lo)) | (static_cast<uint32_t>(f32_to_f16_rne(hi)) << 16);
+    const bf16x2_t v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------------
+// Quantised rows in memory: values [M, mx_row_bytes], scales [M, mx_scale_stride] with zeros behind the row's blocks.
+int mx_quantize_launch(int kind, const void *x, int x_dtype, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st);
+
+struct MxsArgs {
+    const uint8_t *wv, *ws;  // weights of the pool: values, scales with rows of `sstride` bytes
+    const uint8_t *xv, *xs;  // quantised activations
+    void *y;
+    const int32_t *ids, *ids_dst, *bounds, *slot;  // grouped calls: expert of a pair, pairs by expert, their bounds, place of an expert in the pool
+    const void *xraw;        // activations before quantisation, for the kernel that does it itself
+    int64_t ldy, ldx;
+    int K, sstride, nrows;   // nrows: neurons of the tensor or of an expert
+    int M, E, R, pairs, routed;
+    int y_dtype, glu, gelu, x_dtype, x_wide;  // glu: gate rows first, nrows / 2 results; x_wide: xraw lies in pieces of 16 bytes
+    int splits;
+    float *part;             // partial results of a split over K [splits][M][nrows]
+};
+
+}  // namespace mfq

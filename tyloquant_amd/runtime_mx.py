@@ -2,14 +2,18 @@
 
 Mirrors the reference's Mxfp8Weight / mxfp8_matmul_f32 (cpp_runtime/mfq_decode.cpp:2060-2100, 8784-8802) and, for MXFP4
 expert pools, dequant_mxfp4_cpu / select_mxfp4_cpu_rows (:1920-1975): the payload's value and scale bytes are used on the
-device as they lie in the file."""
+device as they lie in the file.
+
+Products of two microscaled operands (mx_quantize, mx_scaled_matmul, mx_scaled_glu, mx_moe_matmul, mx_moe_glu) have no
+counterpart there: activations are quantised to MXFP4 or MXFP6 with a scale for every 32 columns, and the matrix cores
+multiply the codes."""
 from __future__ import annotations
 
 import torch
 
 from . import _lib as L
 from . import formats as F
-from .runtime import _Workspace, _as_2d, _like_rows, _ptr, _stream, _upload, _x_dtype
+from .runtime import _Workspace, _as_2d, _like_rows, _ptr, _stream, _upload, _x_dtype, borrow
 
 
 class MxWeight:
@@ -26,10 +30,40 @@ class MxWeight:
         self.n_experts = self.rows // self.out
         self.data = values                      # the device tensor other weights call `data`
         self._ws = _Workspace()
+        self._wide_scales = None
 
     @property
     def payload_bytes(self) -> int:
         return self.header.values_bytes + self.header.scales_bytes
+
+    @staticmethod
+    def from_tensors(dtype: str, values: torch.Tensor, scales: torch.Tensor, out: int | None = None) -> "MxWeight":
+        """The two byte matrices of a payload that are on the device already (uint8, contiguous, used as they are)."""
+        if values.dim() != 2 or scales.dim() != 2 or values.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise ValueError(f"{dtype}: values and scales must be uint8 matrices")
+        cols = values.shape[1] * (2 if dtype == "MXFP4" else 1)
+        storage, scale = F.mx_shapes(dtype, values.shape[0], cols)
+        if tuple(values.shape) != tuple(storage) or tuple(scales.shape) != tuple(scale):
+            raise ValueError(f"{dtype}: values {tuple(values.shape)} and scales {tuple(scales.shape)} must be {tuple(storage)} and {tuple(scale)}")
+        if not (values.is_cuda and scales.is_cuda and values.device == scales.device and values.is_contiguous() and scales.is_contiguous()):
+            raise ValueError(f"{dtype}: values and scales must be contiguous and on one GPU")
+        h = F.MxHeader(dtype, 4 if dtype == "MXFP4" else 8, values.shape[0], cols, 0, values.numel(), values.numel(), scales.numel())
+        return MxWeight(h, values, scales, out)
+
+    def wide_scales(self) -> torch.Tensor:
+        """Scales with rows of whole groups of eight, which the products of microscaled operands read: the payload's own where
+        the columns are a multiple of 256, else a copy made at the first call."""
+        if self.kind != 4:
+            raise ValueError(f"products of microscaled operands take MXFP4 weights, not {self.dtype}: use mx_matmul")
+        if self._wide_scales is None:
+            if self.neuron_len % 256 == 0 and self.scales.data_ptr() % 8 == 0:
+                self._wide_scales = self.scales
+            else:
+                stride = (self.neuron_len // 32 + 7) // 8 * 8
+                wide = torch.empty((self.rows, stride), dtype=torch.uint8, device=self.scales.device)
+                L.check(L.lib().mfq_hip_mx_pad_scales(_ptr(self.scales), self.rows, self.neuron_len, _ptr(wide), _stream()))
+                self._wide_scales = wide
+        return self._wide_scales
 
     @staticmethod
     def from_blob(dtype: str, blob, device="cuda", out: int | None = None) -> "MxWeight":
@@ -73,3 +107,155 @@ def mx_matmul(w: MxWeight, x: torch.Tensor, expert: int = 0) -> torch.Tensor:
     L.check(lib.mfq_hip_mx_gemm_rows(w.kind, _ptr(w.values), _ptr(w.scales), w.rows, w.neuron_len, row0, nrows, _ptr(x2),
                                      _x_dtype(x2), x2.stride(0), M, _ptr(y), nrows, _ptr(ws), need, _stream()))
     return _like_rows(y, x)
+
+
+# ---------------------------------------------------------------------------------------
+# Products of two microscaled operands
+# ---------------------------------------------------------------------------------------
+_ACT = {"MXFP4": 4, "MXFP6": 6}
+_OUT = {torch.float32: L.X_F32, torch.bfloat16: L.X_BF16, torch.float16: L.X_F16}
+
+
+def _row_bytes(kind: int, K: int) -> int:
+    return -(-K // 256) * (128 if kind == 4 else 192)
+
+
+class MxRows:
+    """Quantised activations [.., neuron_len]: value bytes of rows of whole groups of 256 columns (uint8 [M, 128 or 192 a group], the
+    layout of mfq_hip_mx_quantize_rows) and E8M0 scales (uint8 [M, 8 a group]), zeros behind the row's last column; `shape` is
+    that of the rows before quantisation."""
+
+    def __init__(self, dtype: str, values: torch.Tensor, scales: torch.Tensor, shape):
+        kind, self.shape = _act_kind(dtype), tuple(shape)
+        if not self.shape or self.shape[-1] <= 0 or self.shape[-1] % 32:
+            raise ValueError(f"{dtype} columns must be divisible by 32: {self.shape}")
+        self.dtype, self.kind, self.values, self.scales = dtype, kind, values, scales
+        self.neuron_len = self.shape[-1]
+        self.rows = torch.Size(self.shape[:-1]).numel()
+        want = (self.rows, _row_bytes(kind, self.neuron_len)), (self.rows, -(-self.neuron_len // 256) * 8)
+        if values.dtype != torch.uint8 or scales.dtype != torch.uint8 or (tuple(values.shape), tuple(scales.shape)) != want or \
+                not (values.is_contiguous() and scales.is_contiguous()) or values.device != scales.device:
+            raise ValueError(f"{dtype} rows of {self.shape}: values {tuple(values.shape)} and scales {tuple(scales.shape)} must be contiguous uint8 "
+                             f"{want[0]} and {want[1]} on one device")
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """element x scale in fp32, rounded once to `dtype`."""
+        out = torch.empty(self.shape, dtype=dtype, device=self.values.device)
+        if self.rows:
+            L.check(L.lib().mfq_hip_mx_dequant_quantized(self.kind, _ptr(self.values), _ptr(self.scales), self.rows, self.neuron_len,
+                                                         _out_dtype(dtype), _ptr(out), self.neuron_len, _stream()))
+        return out
+
+
+def _out_dtype(dtype) -> int:
+    try:
+        return _OUT[dtype]
+    except KeyError:
+        raise TypeError(f"results are float32, bfloat16 or float16, not {dtype}") from None
+
+
+def _act_kind(act: str) -> int:
+    try:
+        return _ACT[act]
+    except KeyError:
+        raise ValueError(f"activations are quantised to MXFP4 or MXFP6, not {act}") from None
+
+
+def _raw_rows(x: torch.Tensor, K: int) -> torch.Tensor:
+    """[rows, K] with neighbouring columns side by side"""
+    if x.dtype not in _OUT:
+        raise TypeError(f"activations must be float32, bfloat16 or float16, got {x.dtype}")
+    return _as_2d(x, K)
+
+
+def mx_quantize(x: torch.Tensor, dtype: str = "MXFP4") -> MxRows:
+    """Rows of bf16, fp16 or fp32 [..., K] to MXFP4 or MXFP6 with a power of two for every 32 columns: 2^(e - 2), e = the
+    exponent of the block's largest magnitude; elements to nearest, ties to even, the largest where they are beyond it.  A block
+    that holds an infinity or a NaN becomes NaN."""
+    kind, K = _act_kind(dtype), x.shape[-1]
+    if K % 32 or K == 0:
+        raise ValueError(f"{dtype} columns must be divisible by 32, got {K}")
+    x2 = _raw_rows(x, K)
+    M = x2.shape[0]
+    values = torch.empty((M, _row_bytes(kind, K)), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((M, -(-K // 256) * 8), dtype=torch.uint8, device=x.device)
+    if M:
+        L.check(L.lib().mfq_hip_mx_quantize_rows(kind, _ptr(x2), _OUT[x2.dtype], x2.stride(0), M, K, _ptr(values), _ptr(scales), _stream()))
+    return MxRows(dtype, values, scales, x.shape)
+
+
+def _operand(x, K: int, act: str):
+    """(kind, tensor, x_dtype, row stride, scales or None, rows, shape, device) of activations that come quantised or not"""
+    if isinstance(x, MxRows):
+        if x.neuron_len != K:
+            raise ValueError(f"activation width {x.neuron_len} != neuron length {K}")
+        return x.kind, x.values, 0, 0, x.scales, x.rows, x.shape, x.values.device
+    x2 = _raw_rows(x, K)
+    return _act_kind(act), x2, _OUT[x2.dtype], x2.stride(0), None, x2.shape[0], x.shape, x.device
+
+
+def _scaled(w: MxWeight, x, act: str, expert: int, glu: int, activation: int, out_dtype) -> torch.Tensor:
+    row0, nrows = w._rows(expert)
+    K = w.neuron_len
+    kind, x2, xd, ldx, xs, M, shape, dev = _operand(x, K, act)
+    yd = _out_dtype(out_dtype)
+    if glu and (nrows % 2 or yd == L.X_F32):
+        raise ValueError(f"a gated product takes a 16-bit type and gate and up rows, not {out_dtype} and {nrows} rows")
+    ws_scales = w.wide_scales()
+    width = nrows // 2 if glu else nrows
+    y = torch.empty((M, width), dtype=out_dtype, device=dev)
+    if M:
+        lib = L.lib()
+        need = lib.mfq_hip_mx_scaled_gemm_workspace_bytes(kind, nrows, K, M, xs is not None)
+        ws = borrow(need, dev)
+        L.check(lib.mfq_hip_mx_scaled_gemm_rows(w.values.data_ptr(), ws_scales.data_ptr(), w.rows, K, row0, nrows, kind, x2.data_ptr(), xd, ldx,
+                                                _ptr(xs), M, glu, activation, y.data_ptr(), yd, width, _ptr(ws), need if ws is not None else 0,
+                                                _stream()))
+    return y if len(shape) == 2 else y.reshape(*shape[:-1], width)
+
+
+def mx_scaled_matmul(w: MxWeight, x, act: str = "MXFP6", expert: int = 0, out_dtype=torch.float32) -> torch.Tensor:
+    """q(x) @ W^T of an MXFP4 tensor, fp32 sums rounded once to `out_dtype`.  x: bf16, fp16 or fp32 [..., K], quantised to `act` by the
+    call, or MxRows (their own type).  mx_matmul is the product with unquantised activations."""
+    return _scaled(w, x, act, expert, 0, 0, out_dtype)
+
+
+def mx_scaled_glu(w: MxWeight, x, act: str = "MXFP6", activation: int = L.GLU_SILU, expert: int = 0, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """act(gate) * up of an MXFP4 gate/up tensor (gate rows first), in 16 bits."""
+    return _scaled(w, x, act, expert, 1, int(activation), out_dtype)
+
+
+def _moe(w: MxWeight, x, route, act: str, routed: bool, glu: int, activation: int, out_dtype, slot=None, out=None) -> torch.Tensor:
+    K, T, R = w.neuron_len, route.tokens, route.routes
+    kind, x2, xd, ldx, xs, M, shape, dev = _operand(x, K, act)
+    if M != (T * R if routed else T):
+        raise ValueError(f"MoE activations must be [{'tokens * routes' if routed else 'tokens'}, K]: {M} rows for {T} tokens of {R} routes")
+    if slot is None and w.n_experts != route.n_experts:
+        raise ValueError(f"{w.n_experts} experts, a route plan for {route.n_experts}")
+    yd = _out_dtype(out_dtype)
+    if glu and (w.out % 2 or yd == L.X_F32):
+        raise ValueError(f"a gated product takes a 16-bit type and gate and up rows, not {out_dtype} and {w.out} rows")
+    ws_scales = w.wide_scales()
+    width = w.out // 2 if glu else w.out
+    y = torch.empty((T, R, width), dtype=out_dtype, device=dev) if out is None else out
+    if T * R:
+        lib = L.lib()
+        mapped = route.ids_dst is not None
+        need = lib.mfq_hip_mx_moe_workspace_bytes(kind, K, M, mapped, xs is not None)
+        ws = borrow(need, dev)
+        L.check(lib.mfq_hip_mx_moe_matmul(w.values.data_ptr(), ws_scales.data_ptr(), w.rows, K, w.out, _ptr(slot), route.n_experts, kind, x2.data_ptr(), xd,
+                                          ldx, _ptr(xs), int(routed), route.ids.data_ptr(), T, R, _ptr(route.ids_dst) if mapped else None,
+                                          _ptr(route.expert_bounds) if mapped else None, glu, activation, y.data_ptr(), yd, width, _ptr(ws),
+                                          need if ws is not None else 0, _stream()))
+    return y
+
+
+def mx_moe_matmul(w: MxWeight, x, route, act: str = "MXFP6", routed: bool = False, out_dtype=torch.float32) -> torch.Tensor:
+    """[tokens, routes, out] of a pool of MXFP4 experts: every (token, route) pair of `route` (build_moe_route_plan) against its expert;
+    zeros where the id is none.  x has a row per token, with `routed` one per pair."""
+    return _moe(w, x, route, act, routed, 0, 0, out_dtype)
+
+
+def mx_moe_glu(w: MxWeight, x, route, act: str = "MXFP6", activation: int = L.GLU_SILU, routed: bool = False, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """act(gate) * up of a pool of gate/up tensors, 16-bit [tokens, routes, out / 2]."""
+    return _moe(w, x, route, act, routed, 1, int(activation), out_dtype)
