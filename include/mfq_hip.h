@@ -498,23 +498,22 @@ int mfq_hip_mx_gemv_pairs(int kind, const void *values, const void *scales, int 
  * multiplies MX weights in fp16.
  * Quantised rows: values [M, mfq_hip_mx_quantized_row_bytes(kind, cols)], 16-byte aligned, rows of whole groups of 256 columns with
  * zeros behind the last: 128 bytes of E2M1 codes (low nibble = even column); or of the eight blocks' 192 bits of E2M3 codes (the first
- * column lowest) the first 16 bytes of each and then the last 8 of each.  scales [M, mfq_hip_mx_scale_stride(cols)], 8-byte aligned:
- * cols / 32 bytes and zeros up to a multiple of eight.
+ * column lowest) the first 16 bytes of each and then the last 8 of each.  scales: mfq_hip_mx_scale_bytes(M, cols) bytes, 8-byte aligned,
+ * [blocks of 32 rows][groups of 256 columns][32 rows][8 bytes], zeros behind the last column.
  * The scale of a block is 2^(e - 2), e = the exponent of its largest magnitude, at least 2^-127; elements are rounded to nearest, ties
  * to even, those beyond the largest element (6 or 7.5) to it.  A block that holds an infinity or a NaN takes scale 255 (NaN) and
  * codes 0.  x: bf16, fp16 or fp32 [M, ldx]; cols must be divisible by 32. */
 int mfq_hip_mx_quantized_row_bytes(int kind, int cols);
-int mfq_hip_mx_scale_stride(int cols);
+int64_t mfq_hip_mx_scale_bytes(int64_t rows, int cols);
 int mfq_hip_mx_quantize_rows(int kind, const void *x, int x_dtype, int64_t ldx, int M, int cols, void *values, void *scales,
                              mfq_stream_t stream);
 /* out[m][c] = element * scale in fp32, rounded once to out_dtype. */
 int mfq_hip_mx_dequant_quantized(int kind, const void *values, const void *scales, int M, int cols, int out_dtype, void *out,
                                  int64_t ldo, mfq_stream_t stream);
-/* Scales of an MXFP4 payload [rows, cols / 32] at the row stride of the calls below; needed only where cols is no multiple of 256
- * (elsewhere the payload has that stride). */
-int mfq_hip_mx_pad_scales(const void *scales, int64_t rows, int cols, void *out, mfq_stream_t stream);
+/* Scales of an MXFP4 payload [rows, cols / 32] in that layout, in which the calls below take them (once, at load time). */
+int mfq_hip_mx_lay_scales(const void *scales, int64_t rows, int cols, void *out, mfq_stream_t stream);
 /* y[M, nrows] = q(x) . W^T over rows [row0, row0 + nrows) of an MXFP4 tensor [rows, cols], fp32 accumulation, rounded once to
- * y_dtype (MFQ_X_*).  `scales` has rows of mfq_hip_mx_scale_stride(cols) bytes.  act: kind of q(x).  x is bf16, fp16 or fp32
+ * y_dtype (MFQ_X_*).  `scales`: those of all rows from mfq_hip_mx_lay_scales.  act: kind of q(x).  x is bf16, fp16 or fp32
  * [M, ldx] and quantised by the call (x_scales null), or the values of quantised rows with their x_scales (x_dtype and ldx are
  * not looked at then).  glu != 0: gate rows first, y[M, nrows / 2] = act(gate) * up with `activation` MFQ_GLU_*, 16-bit y_dtype.
  * Rows of x that hold a NaN or an infinity give NaN.  Workspace (size from the query): the quantised rows, and partial sums of a

@@ -6,8 +6,9 @@ E2M3 = np.array([(m / 8 if e == 0 else 1 + m / 8) * 2.0 ** (max(e, 1) - 1) for e
 GRID = {"MXFP4": E2M1, "MXFP6": E2M3}
 
 
-def stride(K):
-    return -(-(K // 32) // 8) * 8
+def plain_scales(laid, M, K):
+    """[M, whole groups of eight] of scales laid out [blocks of 32 rows][groups of 256 columns][32][8]"""
+    return laid.reshape(-(-M // 32), -(-K // 256), 32, 8).transpose(0, 2, 1, 3).reshape(-(-M // 32) * 32, -1)[:M]
 
 
 def quantize(x, dtype):

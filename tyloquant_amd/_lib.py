@@ -139,10 +139,10 @@ _SIGS = {
     "mfq_hip_mx_gemv_pairs": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, i64, C.c_int, vp, C.c_int,
                               C.c_int, vp, i64, vp]),
     "mfq_hip_mx_quantized_row_bytes": (C.c_int, [C.c_int, C.c_int]),
-    "mfq_hip_mx_scale_stride": (C.c_int, [C.c_int]),
+    "mfq_hip_mx_scale_bytes": (i64, [i64, C.c_int]),
     "mfq_hip_mx_quantize_rows": (C.c_int, [C.c_int, vp, C.c_int, i64, C.c_int, C.c_int, vp, vp, vp]),
     "mfq_hip_mx_dequant_quantized": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, vp, i64, vp]),
-    "mfq_hip_mx_pad_scales": (C.c_int, [vp, i64, C.c_int, vp, vp]),
+    "mfq_hip_mx_lay_scales": (C.c_int, [vp, i64, C.c_int, vp, vp]),
     "mfq_hip_mx_scaled_gemm_workspace_bytes": (sz, [C.c_int] * 5),
     "mfq_hip_mx_scaled_gemm_rows": (C.c_int, [vp, vp] + [C.c_int] * 5 + [vp, C.c_int, i64, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, i64, vp,
                                     sz, vp]),

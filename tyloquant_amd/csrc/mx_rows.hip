@@ -5,44 +5,109 @@
 namespace mfq {
 namespace {
 
-constexpr int kUnits = 4;  // pieces of eight values a thread takes, 256 pieces apart: their loads are in flight together
+constexpr int kUnits = 4;  // pieces of eight values a thread of the dequantizer takes, 256 pieces apart: their loads are in flight together
 
-// Pieces of a row run over whole macros: those behind the last column are zeros (scales too).
+typedef __bf16 bf16x32_t __attribute__((ext_vector_type(32)));
+typedef _Float16 half32_t __attribute__((ext_vector_type(32)));
+typedef uint32_t u32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x6_t __attribute__((ext_vector_type(6)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+
+// A thread takes a block of 32 values, whose conversion to E2M3 the hardware does in one instruction and to E2M1 in sixteen, from the
+// activations' own type; its codes are 16 bytes (and 8 more of E2M3) next to its neighbour's.  Its loads are 64 or 128 bytes from its
+// neighbour's, which takes the address path four or eight times as long as side by side and still is the lesser evil: with a quad of
+// threads a block and E2M3 rounded in integers, 2048 x 12288 bf16 to MXFP6 took 23.0 us.
 template <int AK, int XD, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const void *__restrict__ x, int64_t ldx, int M, int K, uint8_t *__restrict__ values,
                                                           uint8_t *__restrict__ scales) {
-    const int nmac = (K + kMxMacro - 1) / kMxMacro, per_row = nmac * 32;
-    const int64_t units = static_cast<int64_t>(M) * per_row, xrow = mx_row_bytes(AK, K);
-    const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (256 * kUnits) + threadIdx.x;
-    float v[kUnits][8];
-    int64_t row[kUnits];
-    int piece[kUnits];
+    const int nmac = mx_macros(K), per_row = nmac * 8;  // blocks behind the last column are zeros
+    const int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t row = static_cast<int64_t>(M) * per_row < (1ll << 31) ? static_cast<int64_t>(static_cast<uint32_t>(u) / static_cast<uint32_t>(per_row)) : u / per_row;
+    if (row >= M) return;
+    const int block = static_cast<int>(u - row * per_row);
+    const int64_t from = row * ldx + block * 32;
+    uint32_t byte = 0;
+    u32x6_t q = {};
+    if (block < K / 32) {
+        if constexpr (XD == MFQ_X_F32) {
+            const float *p = static_cast<const float *>(x) + from;
+            float16_t v[2];
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-        const int64_t u = min(u0 + 256 * i, units - 1);  // whole quads: units is a multiple of four
-        row[i] = units < (1ll << 31) ? static_cast<int64_t>(static_cast<uint32_t>(u) / static_cast<uint32_t>(per_row)) : u / per_row;
-        piece[i] = static_cast<int>(u - row[i] * per_row);
+            for (int i = 0; i < 8; ++i) {
+                float4_t f;
+                if constexpr (VEC) f = reinterpret_cast<const float4_t *>(p)[i];
+                else f = float4_t{p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]};
 #pragma unroll
-        for (int t = 0; t < 8; ++t) v[i][t] = 0.f;
-        if (piece[i] < K / 8) mx_load8<XD, VEC>(x, row[i] * ldx + piece[i] * 8, v[i]);
+                for (int t = 0; t < 4; ++t) v[t & 1][2 * i + (t >> 1)] = f[t];  // even and odd columns: the order of the conversion to E2M3
+            }
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) most = max(most, __float_as_uint(v[i & 1][i >> 1]) & 0x7fffffffu);
+            byte = mx_scale_of(most);
+            const float scale = __uint_as_float(byte << 23);
+            if constexpr (AK == 6) {
+                q = __builtin_bit_cast(u32x6_t, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(v[0], v[1], scale));
+            } else {
+                static_for<4>([&](auto D) {
+                    constexpr int d = D.value;
+                    static_for<4>([&](auto T) {
+                        constexpr int t = T.value;
+                        q[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q[d], v[0][4 * d + t], v[1][4 * d + t], scale, t);
+                    });
+                });
+            }
+        } else {
+            const uint16_t *p = static_cast<const uint16_t *>(x) + from;
+            u32x16_t v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (VEC) {
+                    const u32x4_t f = reinterpret_cast<const u32x4_t *>(p)[i];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) v[4 * i + t] = f[t];
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) v[4 * i + t] = p[8 * i + 2 * t] | (static_cast<uint32_t>(p[8 * i + 2 * t + 1]) << 16);
+                }
+            }
+            u16x2_t most = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t pair = v[i] & 0x7fff7fffu;
+                most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, pair));
+            }
+            const uint32_t m = max(most.x, most.y);
+            // of fp16 the exponent as an fp32 has it, infinities and NaN with theirs
+            byte = mx_scale_of(XD == MFQ_X_BF16 ? m << 16 : m >= 0x7c00u ? 0x7f800000u : __float_as_uint(f16_to_f32(static_cast<uint16_t>(m))));
+            const float scale = __uint_as_float(byte << 23);
+            if constexpr (AK == 6) {
+                if constexpr (XD == MFQ_X_F16) q = __builtin_bit_cast(u32x6_t, __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(__builtin_bit_cast(half32_t, v), scale));
+                else q = __builtin_bit_cast(u32x6_t, __builtin_amdgcn_cvt_scalef32_pk32_fp6_bf16(__builtin_bit_cast(bf16x32_t, v), scale));
+            } else {
+                static_for<4>([&](auto D) {
+                    constexpr int d = D.value;
+                    static_for<4>([&](auto T) {
+                        constexpr int t = T.value;
+                        const uint32_t pair = v[4 * d + t];  // by itself: a bit cast of the element reads the vector's first
+                        if constexpr (XD == MFQ_X_F16) q[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q[d], __builtin_bit_cast(half2_t, pair), scale, t);
+                        else q[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q[d], __builtin_bit_cast(bf16x2_t, pair), scale, t);
+                    });
+                });
+            }
+        }
+        if (byte == 255u) q = u32x6_t{};
     }
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-        const uint32_t byte = mx_scale_byte(v[i]);
-        const MxStore o = mx_place<AK>(mx_codes<AK>(v[i], byte), piece[i]);
-        if (u0 + 256 * i >= units) continue;
-        uint8_t *to = values + row[i] * xrow + o.at;
-        if constexpr (AK == 4) *reinterpret_cast<uint32_t *>(to) = o.q.x;
-        else if (o.any) *reinterpret_cast<u32x2_t *>(to) = o.q;
-        if ((piece[i] & 3) == 0) scales[row[i] * (nmac * 8) + (piece[i] >> 2)] = static_cast<uint8_t>(byte);
-    }
+    uint8_t *to = values + row * mx_row_bytes(AK, K) + (block >> 3) * mx_macro_bytes(AK);
+    *reinterpret_cast<u32x4_t *>(to + (block & 7) * 16) = u32x4_t{q[0], q[1], q[2], q[3]};
+    if constexpr (AK == 6) *reinterpret_cast<u32x2_t *>(to + 128 + (block & 7) * 8) = u32x2_t{q[4], q[5]};
+    scales[mx_scale_at(row, nmac) + (block >> 3) * 256 + (block & 7)] = static_cast<uint8_t>(byte);
 }
 
 // a thread per eight values
 template <int AK>
 __global__ __launch_bounds__(256) void mx_rows_dequant_kernel(const uint8_t *__restrict__ values, const uint8_t *__restrict__ scales, int M, int K,
                                                               void *__restrict__ out, int out_dtype, int64_t ldo, bool wide) {
-    const int per_row = K / 8, sstride = mx_scale_stride(K);
+    const int per_row = K / 8, nmac = mx_macros(K);
     const int64_t units = static_cast<int64_t>(M) * per_row, xrow = mx_row_bytes(AK, K);
     const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (256 * kUnits) + threadIdx.x;
     u32x2_t q[kUnits];
@@ -66,7 +131,7 @@ __global__ __launch_bounds__(256) void mx_rows_dequant_kernel(const uint8_t *__r
             else if (j == 2) q[i] = u32x2_t{py, q[i].x};
             else if (j == 3) q[i] = u32x2_t{(px >> 16) | (py << 16), py >> 16};
         }
-        byte[i] = scales[row[i] * sstride + (piece[i] >> 2)];
+        byte[i] = scales[mx_scale_at(row[i], nmac) + mac * 256u + (in >> 2)];
     }
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
@@ -106,20 +171,24 @@ __global__ __launch_bounds__(256) void mx_rows_dequant_kernel(const uint8_t *__r
     }
 }
 
-// rows of scales at another stride, zeros behind the blocks
-__global__ __launch_bounds__(256) void mx_pad_scales_kernel(const uint8_t *__restrict__ scales, int64_t rows, int blocks, int sstride, uint8_t *__restrict__ out) {
-    const int64_t n = rows * sstride;
+// scales of an MXFP4 payload, rows of K / 32 bytes one after the other, to where the products read them
+__global__ __launch_bounds__(256) void mx_lay_scales_kernel(const uint8_t *__restrict__ scales, int64_t rows, int blocks, int nmac, uint8_t *__restrict__ out) {
+    const int64_t n = (rows + 31) / 32 * nmac * 32;  // of eight bytes
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / sstride;
-        const int b = static_cast<int>(i - r * sstride);
-        out[i] = b < blocks ? scales[r * blocks + b] : 0;
+        const int64_t rb = i / (nmac * 32);
+        const int in = static_cast<int>(i - rb * (nmac * 32)), mac = in >> 5;
+        const int64_t row = rb * 32 + (in & 31);
+        uint64_t v = 0;
+        if (row < rows)
+            for (int b = 0; b < 8; ++b)
+                if (mac * 8 + b < blocks) v |= static_cast<uint64_t>(scales[row * blocks + mac * 8 + b]) << (8 * b);
+        reinterpret_cast<uint64_t *>(out)[i] = v;
     }
 }
 
 template <int AK, int XD>
 void launch_quantize(const void *x, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st) {
-    const int64_t units = static_cast<int64_t>(M) * (mx_scale_stride(K) * 4);
-    const dim3 grid(static_cast<unsigned>(ceil_div(units, 256 * kUnits)));
+    const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(M) * (mx_macros(K) * 8), 256)));
     const int64_t per16 = XD == MFQ_X_F32 ? 4 : 8;
     if (reinterpret_cast<uintptr_t>(x) % 16 == 0 && (M == 1 || ldx % per16 == 0))
         hipLaunchKernelGGL((mx_quantize_kernel<AK, XD, true>), grid, dim3(256), 0, st, x, ldx, M, K, values, scales);
@@ -150,7 +219,7 @@ extern "C" int mfq_hip_mx_quantized_row_bytes(int kind, int cols) {
     return (kind == 4 || kind == 6) && cols > 0 && cols % 32 == 0 ? static_cast<int>(mx_row_bytes(kind, cols)) : 0;
 }
 
-extern "C" int mfq_hip_mx_scale_stride(int cols) { return cols > 0 && cols % 32 == 0 ? mx_scale_stride(cols) : 0; }
+extern "C" int64_t mfq_hip_mx_scale_bytes(int64_t rows, int cols) { return rows > 0 && cols > 0 && cols % 32 == 0 ? mx_scale_bytes(rows, cols) : 0; }
 
 extern "C" int mfq_hip_mx_quantize_rows(int kind, const void *x, int x_dtype, int64_t ldx, int M, int cols, void *values, void *scales,
                                         mfq_stream_t stream) {
@@ -161,7 +230,7 @@ extern "C" int mfq_hip_mx_quantize_rows(int kind, const void *x, int x_dtype, in
     MFQ_REQUIRE(M == 1 || ldx >= cols, MFQ_ERR_INVALID, "mx_quantize_rows: ldx=%lld < %d", static_cast<long long>(ldx), cols);
     MFQ_REQUIRE(reinterpret_cast<uintptr_t>(x) % (x_dtype == MFQ_X_F32 ? 4 : 2) == 0 && reinterpret_cast<uintptr_t>(values) % 16 == 0 &&
                 reinterpret_cast<uintptr_t>(scales) % 8 == 0, MFQ_ERR_INVALID, "mx_quantize_rows: values must be 16-byte aligned, scales 8-byte aligned");
-    MFQ_REQUIRE(static_cast<int64_t>(M) * cols < (1ll << 40), MFQ_ERR_UNSUPPORTED, "mx_quantize_rows: %d x %d values", M, cols);
+    MFQ_REQUIRE(mx_scale_bytes(M, cols) < (1ll << 32), MFQ_ERR_UNSUPPORTED, "mx_quantize_rows: %d x %d values", M, cols);
     return mx_quantize_launch(kind, x, x_dtype, ldx, M, cols, static_cast<uint8_t *>(values), static_cast<uint8_t *>(scales), as_stream(stream));
 }
 
@@ -174,7 +243,7 @@ extern "C" int mfq_hip_mx_dequant_quantized(int kind, const void *values, const 
     MFQ_REQUIRE(M == 1 || ldo >= cols, MFQ_ERR_INVALID, "mx_dequant_quantized: ldo=%lld < %d", static_cast<long long>(ldo), cols);
     MFQ_REQUIRE(reinterpret_cast<uintptr_t>(values) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % (out_dtype == MFQ_X_F32 ? 4 : 2) == 0, MFQ_ERR_INVALID,
                 "mx_dequant_quantized: values must be 16-byte aligned");
-    MFQ_REQUIRE(static_cast<int64_t>(M) * cols < (1ll << 40), MFQ_ERR_UNSUPPORTED, "mx_dequant_quantized: %d x %d values", M, cols);
+    MFQ_REQUIRE(mx_scale_bytes(M, cols) < (1ll << 32), MFQ_ERR_UNSUPPORTED, "mx_dequant_quantized: %d x %d values", M, cols);
     const int64_t units = static_cast<int64_t>(M) * (cols / 8);
     const dim3 grid(static_cast<unsigned>(ceil_div(units, 256 * kUnits)));
     const bool wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (M == 1 || ldo % (out_dtype == MFQ_X_F32 ? 4 : 8) == 0);
@@ -184,13 +253,12 @@ extern "C" int mfq_hip_mx_dequant_quantized(int kind, const void *values, const 
     return check_launch("mx_dequant_quantized");
 }
 
-extern "C" int mfq_hip_mx_pad_scales(const void *scales, int64_t rows, int cols, void *out, mfq_stream_t stream) {
-    MFQ_REQUIRE(scales && out, MFQ_ERR_INVALID, "mx_pad_scales: null argument");
-    MFQ_REQUIRE(rows > 0 && cols > 0 && cols % 32 == 0, MFQ_ERR_INVALID, "mx_pad_scales: [%lld, %d], columns must be divisible by 32",
+extern "C" int mfq_hip_mx_lay_scales(const void *scales, int64_t rows, int cols, void *out, mfq_stream_t stream) {
+    MFQ_REQUIRE(scales && out && reinterpret_cast<uintptr_t>(out) % 8 == 0, MFQ_ERR_INVALID, "mx_lay_scales: null argument, or out not 8-byte aligned");
+    MFQ_REQUIRE(rows > 0 && cols > 0 && cols % 32 == 0, MFQ_ERR_INVALID, "mx_lay_scales: [%lld, %d], columns must be divisible by 32",
                 static_cast<long long>(rows), cols);
-    const int64_t n = rows * mx_scale_stride(cols);
-    const dim3 grid(static_cast<unsigned>(ceil_div(n, 256) < 65536 ? ceil_div(n, 256) : 65536));
-    hipLaunchKernelGGL(mx_pad_scales_kernel, grid, dim3(256), 0, as_stream(stream), static_cast<const uint8_t *>(scales), rows, cols / 32, mx_scale_stride(cols),
-                       static_cast<uint8_t *>(out));
-    return check_launch("mx_pad_scales");
+    const int64_t n = ceil_div(mx_scale_bytes(rows, cols) / 8, 256);
+    hipLaunchKernelGGL(mx_lay_scales_kernel, dim3(static_cast<unsigned>(n < 65536 ? n : 65536)), dim3(256), 0, as_stream(stream),
+                       static_cast<const uint8_t *>(scales), rows, cols / 32, mx_macros(cols), static_cast<uint8_t *>(out));
+    return check_launch("mx_lay_scales");
 }

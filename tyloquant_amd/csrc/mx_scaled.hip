@@ -117,9 +117,8 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
     };
 
     const uint8_t *wbase = a.wv + static_cast<int64_t>(expert) * a.nrows * wrow;
-    const uint8_t *sbase = a.ws + static_cast<int64_t>(expert) * a.nrows * a.sstride;
     const __amdgpu_buffer_rsrc_t win = wave_window(wbase, static_cast<uint32_t>(a.nrows * wrow));
-    const __amdgpu_buffer_rsrc_t swin = wave_window(sbase, static_cast<uint32_t>(a.nrows) * a.sstride);
+    const __amdgpu_buffer_rsrc_t swin = wave_window(a.ws, 0xffffff00u);  // offsets of 32 bits from the first row: the host sees to it
     uint32_t wv[2 * NB];
     const int piece = lane & 7;
 #pragma unroll
@@ -127,12 +126,12 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
         const int row = 8 * (i & 1) + (lane >> 3);
         wv[i] = static_cast<uint32_t>(neuron(i >> 1, row) * wrow) + 16u * (piece ^ mx_key(row));
     }
-    const uint32_t wsv = static_cast<uint32_t>(neuron(NB == 2 ? lane >> 5 : 0, (lane >> 1) & 15)) * a.sstride + 4u * (lane & 1);
+    const uint32_t wsv = mx_scale_at(a.row0 + expert * a.nrows + neuron(NB == 2 ? lane >> 5 : 0, (lane >> 1) & 15), nmac) + 4u * (lane & 1);
     // rows of a mapped tile lie anywhere: the window is all of them (under 4 GB, the host sees to it); else the block's own
     const int64_t base = MODE == kLinear ? m0 : 0;
     const int span = RES ? 0 : MODE == kLinear ? rows : a.M;
     const __amdgpu_buffer_rsrc_t xwin = wave_window(a.xv + base * xrow, static_cast<uint32_t>(span * xrow));
-    const __amdgpu_buffer_rsrc_t xswin = wave_window(a.xs + base * a.sstride, static_cast<uint32_t>(span) * a.sstride);
+    const __amdgpu_buffer_rsrc_t xswin = wave_window(a.xs, 0xffffff00u);
     uint32_t xv[MT * 2], xv2[MT], xsv = 0;
     if constexpr (!RES) {
 #pragma unroll
@@ -145,7 +144,7 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
             for (int t = 0; t < MT; ++t)
                 xv2[t] = static_cast<uint32_t>((src_of(min(16 * t + (lane >> 2), rows - 1)) - base) * xrow) + 128u + 16u * row_order_quarter(lane >> 2, lane & 3);
         }
-        xsv = static_cast<uint32_t>(src_of(min(MT == 2 ? lane >> 1 : (lane >> 1) & 15, rows - 1)) - base) * a.sstride + 4u * (lane & 1);
+        xsv = mx_scale_at(src_of(min(MT == 2 ? lane >> 1 : (lane >> 1) & 15, rows - 1)), nmac) + 4u * (lane & 1);
     }
 
     uint8_t *ring = lds + wave * (D * S::STAGE);
@@ -164,7 +163,7 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
             if (last < 7) off -= 16u * max(0, (piece ^ mx_key(8 * (i & 1) + (lane >> 3))) - last);
             copy16<2>(win, to + i * 1024, off, mac * 128);
         }
-        if (NB == 2 || lane < 32) copy4(swin, to + S::W, wsv, mac * 8);
+        if (NB == 2 || lane < 32) copy4(swin, to + S::W, wsv, mac * 256);
         if constexpr (!RES) {
             uint8_t *xto = to + S::W + S::WS;
 #pragma unroll
@@ -173,7 +172,7 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t) copy16<0>(xwin, xto + (2 * MT + t) * 1024, xv2[t], xat);
             }
-            if (MT == 2 || lane < 32) copy4(xswin, xto + S::X, xsv, mac * 8);
+            if (MT == 2 || lane < 32) copy4(xswin, xto + S::X, xsv, mac * 256);
         }
     };
 
@@ -211,7 +210,7 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
             }
             for (int u = tid; u < rows * nmac; u += blockDim.x) {
                 const int m = u / nmac, p = u - m * nmac;
-                reinterpret_cast<u32x2_t *>(xres_s)[u] = reinterpret_cast<const u32x2_t *>(a.xs + static_cast<int64_t>(src_of(m)) * a.sstride)[p];
+                reinterpret_cast<u32x2_t *>(xres_s)[u] = *reinterpret_cast<const u32x2_t *>(a.xs + mx_scale_at(src_of(m), nmac) + p * 256);
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -235,7 +234,7 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
         else wait_vmcnt<0>();
         const uint8_t *at = ring + stage * S::STAGE;
         u32x4_t w[2][NB];
-        MxFrag x[2][MT];
+        u32x4_t x[2][MT], tail[MT] = {};
         uint32_t sw[NB], sx[MT];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -250,12 +249,9 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
             const uint8_t *row = RES ? xres + m * xres_row + mac * XMAC : at + S::W + S::WS + t * 2048 + r * 128;
             sx[t] = *reinterpret_cast<const uint16_t *>((RES ? xres_s + m * (nmac * 8) + mac * 8 : at + S::W + S::WS + S::X + t * 128 + r * 8) + 2 * g);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) x[s][t].x = *reinterpret_cast<const u32x4_t *>(row + ((RES ? 2 * g + s : (2 * g + s) ^ key) << 4));
-            if constexpr (AK == 6) {
-                const u32x4_t tail = *reinterpret_cast<const u32x4_t *>(RES ? row + 128 + g * 16 : at + S::W + S::WS + (2 * MT + t) * 1024 + row_order_lane(lane));
-                x[0][t].y = u32x2_t{tail.x, tail.y};
-                x[1][t].y = u32x2_t{tail.z, tail.w};
-            }
+            for (int s = 0; s < 2; ++s) x[s][t] = *reinterpret_cast<const u32x4_t *>(row + ((RES ? 2 * g + s : (2 * g + s) ^ key) << 4));
+            if constexpr (AK == 6)
+                tail[t] = *reinterpret_cast<const u32x4_t *>(RES ? row + 128 + g * 16 : at + S::W + S::WS + (2 * MT + t) * 1024 + row_order_lane(lane));
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is free for the next copies
         if (i + D < mine) issue(stage, wave + (i + D) * nwaves);
@@ -263,8 +259,8 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                acc[b][t] = mx_scale_mfma<AK, 0>(w[0][b], x[0][t], acc[b][t], sw[b], sx[t]);
-                acc[b][t] = mx_scale_mfma<AK, 1>(w[1][b], x[1][t], acc[b][t], sw[b], sx[t]);
+                acc[b][t] = mx_scale_mfma<AK, 0>(w[0][b], x[0][t], tail[t].x, tail[t].y, acc[b][t], sw[b], sx[t]);
+                acc[b][t] = mx_scale_mfma<AK, 1>(w[1][b], x[1][t], tail[t].z, tail[t].w, acc[b][t], sw[b], sx[t]);
             }
         stage = stage + 1 == D ? 0 : stage + 1;
     }
@@ -305,27 +301,35 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
 }
 
 // ---- many rows: tiles -----------------------------------------------------------------------------------------------------------
-// A block of WN * WM waves owns BN neurons x BM rows, a wave BN / WN x BM / WM of them.  The block copies a macro of both operands
-// into one of two stages while it multiplies the other.
-template <int AK, int BN, int BM>
+// A block of WN * WM waves owns BN neurons x BM rows, a wave BN / WN x BM / WM of them in squares of 32.  K goes macro by macro through a
+// ring of R stages in LDS.  Lane (r, h) multiplies block 4 h + s of the macro in step s of four, so its four scales are one word.  While
+// the squares of a step are multiplied the fragments of the next are read; before the last step the macro has been read, its stage
+// takes the macro R further on: one barrier a macro.  The 16-byte pieces of a line are turned by (row / 2) & 7 (FP6's second part: by
+// (row / 4) & 3), with which the four passes of a read meet every bank once.
+// Lines of 64 bytes, half a macro a stage and twice as many stages, were slower (17408 x 5120 at 8192 rows: 635 us where whole lines in two
+// stages of 16 x 16 squares had taken 475): a request fetches lines of 128 bytes.
+template <int AK, int BN, int BM, int R>
 struct TileShape {
-    static constexpr int W = BN * 128, X = BM * mx_macro_bytes(AK), WS = BN * 8, XS = BM * 8;
-    static constexpr int STAGE = W + X + WS + XS;
+    static constexpr int W = BN * 128, X = BM * 128, X2 = AK == 6 ? BM * 64 : 0, WS = BN * 8, XS = BM * 8;
+    static constexpr int STAGE = W + X + X2 + WS + XS;
+    static constexpr int LDS = R * STAGE + BM * 4;  // and the rows of y
 };
+constexpr int kTilePitch = 64 * 4 + 16, kTileOut = 32 * kTilePitch;  // 64 results of 32 rows on their way out
 
-template <int AK, int BN, int BM, int WN, int WM, int MODE>
-__global__ __launch_bounds__(WN *WM * 64) void mxs_tile_kernel(MxsArgs a) {
-    using S = TileShape<AK, BN, BM>;
-    constexpr int NW = WN * WM, TN = BN / 16 / WN, TM = BM / 16 / WM;
-    constexpr int PW = (BN / 8 + NW - 1) / NW, PX = (BM / 8 + NW - 1) / NW;  // requests of a wave: rows of weights, of activations
-    constexpr int QW = (BN / 32 + NW - 1) / NW, QX = (BM / 32 + NW - 1) / NW, PT = (BM / 16 + NW - 1) / NW;  // of scales, of FP6's second parts
-    static_assert(TN % 2 == 0 && BN % 32 == 0 && BM % 32 == 0, "gate and up in one wave; whole requests");
+template <int AK, int BN, int BM, int WN, int WM, int R, int MODE>
+__global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN * BM / (WN * WM) > 8192 ? 1 : 2))) void mxs_tile_kernel(MxsArgs a) {
+    using S = TileShape<AK, BN, BM, R>;
+    constexpr int NW = WN * WM, TN = BN / 32 / WN, TM = BM / 32 / WM;
+    // requests of a wave for a stage; every wave issues as many, some twice
+    constexpr int CW = BN / 8, CX = BM / 8, CT = AK == 6 ? BM / 16 : 0, DW = BN / 32, DX = BM / 32;
+    constexpr int PW = (CW + NW - 1) / NW, PX = (CX + NW - 1) / NW, PT = (CT + NW - 1) / NW, QW = (DW + NW - 1) / NW, QX = (DX + NW - 1) / NW;
+    constexpr int PER = PW + PX + PT + QW + QX, XMAC = mx_macro_bytes(AK);
+    static_assert(TN % 2 == 0 && R >= 2, "gate and up in one wave");
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
-    const int r = lane & 15, g = lane >> 4, key = mx_key(r);
+    const int r = lane & 31, h = lane >> 5;
     const int nblk = a.K / 32, nmac = (nblk + 7) / 8;
-    constexpr int XMAC = mx_macro_bytes(AK);
     const int64_t wrow = a.K / 2, xrow = static_cast<int64_t>(nmac) * XMAC;
     const int width = a.glu ? a.nrows / 2 : a.nrows, step = a.glu ? BN / 2 : BN;  // results of a row; of a tile
     const int tiles_n = (width + step - 1) / step;
@@ -355,190 +359,244 @@ __global__ __launch_bounds__(WN *WM * 64) void mxs_tile_kernel(MxsArgs a) {
         const int p = pair_of(m);
         return MODE == kLinear || a.routed ? p : p / a.R;
     };
-    // neuron of row l of the tile: with GLU the second half of a wave's row-blocks holds the up rows of the first half's gate rows
+    // neuron of row l of the tile: with GLU the second half of a wave's squares holds the up rows of the first half's gate rows
     auto neuron = [&](int l) {
         if (!a.glu) return min(n0 + l, a.nrows - 1);
-        const int j = l >> 4, w_ = j / TN, t = j % TN;
-        const int n = min(n0 + (w_ * (TN / 2) + t % (TN / 2)) * 16 + (l & 15), width - 1);
+        const int j = l >> 5, w_ = j / TN, t = j % TN;
+        const int n = min(n0 + (w_ * (TN / 2) + t % (TN / 2)) * 32 + (l & 31), width - 1);
         return t < TN / 2 ? n : width + n;
     };
+    int *row_of = reinterpret_cast<int *>(lds + R * S::STAGE);
+    for (int m = tid; m < BM; m += NW * 64) row_of[m] = m < rows ? pair_of(m) : -1;
 
     const __amdgpu_buffer_rsrc_t win = wave_window(a.wv + static_cast<int64_t>(expert) * a.nrows * wrow, static_cast<uint32_t>(a.nrows * wrow));
-    const __amdgpu_buffer_rsrc_t swin = wave_window(a.ws + static_cast<int64_t>(expert) * a.nrows * a.sstride, static_cast<uint32_t>(a.nrows) * a.sstride);
+    const __amdgpu_buffer_rsrc_t swin = wave_window(a.ws, 0xffffff00u);  // offsets of 32 bits from the first row: the host sees to it
     const int64_t base = MODE == kLinear ? m0 : 0;
     const int span = MODE == kLinear ? rows : a.M;
     const __amdgpu_buffer_rsrc_t xwin = wave_window(a.xv + base * xrow, static_cast<uint32_t>(span * xrow));
-    const __amdgpu_buffer_rsrc_t xswin = wave_window(a.xs + base * a.sstride, static_cast<uint32_t>(span) * a.sstride);
-    const int piece = lane & 7;
-    uint32_t wv[PW], xv[PX], xv2[PT], wsv[QW], xsv[QX];
+    const __amdgpu_buffer_rsrc_t xswin = wave_window(a.xs, 0xffffff00u);
+    uint32_t wv[PW], xv[PX], xv2[PT > 0 ? PT : 1], wsv[QW], xsv[QX];
+    const int wp = (lane & 7) ^ ((lane >> 4) & 3), wq = wp ^ 4;  // piece of the line that lane's copy takes, in the lower and upper half of 16 rows
 #pragma unroll
     for (int p = 0; p < PW; ++p) {
-        const int l = min(8 * (wave + NW * p), BN - 8) + (lane >> 3);
-        wv[p] = static_cast<uint32_t>(neuron(l) * wrow) + 16u * (piece ^ mx_key(l & 15));
+        const int q = min(wave + NW * p, CW - 1);
+        wv[p] = static_cast<uint32_t>(neuron(q * 8 + (lane >> 3)) * wrow) + 16u * (q & 1 ? wq : wp);
     }
 #pragma unroll
     for (int p = 0; p < PX; ++p) {
-        const int l = min(8 * (wave + NW * p), BM - 8) + (lane >> 3);
-        xv[p] = static_cast<uint32_t>((src_of(min(l, rows - 1)) - base) * xrow) + 16u * (piece ^ mx_key(l & 15));
-    }
-    if constexpr (AK == 6) {
-#pragma unroll
-        for (int p = 0; p < PT; ++p) {
-            const int l = min(16 * (wave + NW * p), BM - 16) + (lane >> 2);
-            xv2[p] = static_cast<uint32_t>((src_of(min(l, rows - 1)) - base) * xrow) + 128u + 16u * row_order_quarter(l & 15, lane & 3);
-        }
+        const int q = min(wave + NW * p, CX - 1);
+        xv[p] = static_cast<uint32_t>((src_of(min(q * 8 + (lane >> 3), rows - 1)) - base) * xrow) + 16u * (q & 1 ? wq : wp);
     }
 #pragma unroll
-    for (int p = 0; p < QW; ++p) wsv[p] = static_cast<uint32_t>(neuron(min(32 * (wave + NW * p), BN - 32) + (lane >> 1))) * a.sstride + 4u * (lane & 1);
+    for (int p = 0; p < PT; ++p)
+        xv2[p] = static_cast<uint32_t>((src_of(min(min(wave + NW * p, CT - 1) * 16 + (lane >> 2), rows - 1)) - base) * xrow) + 128u +
+                 16u * ((lane & 3) ^ ((lane >> 4) & 3));
 #pragma unroll
-    for (int p = 0; p < QX; ++p)
-        xsv[p] = static_cast<uint32_t>(src_of(min(min(32 * (wave + NW * p), BM - 32) + (lane >> 1), rows - 1)) - base) * a.sstride + 4u * (lane & 1);
+    for (int p = 0; p < QW; ++p) wsv[p] = mx_scale_at(a.row0 + neuron(min(wave + NW * p, DW - 1) * 32 + (lane >> 1)) + expert * a.nrows, nmac) + 4u * (lane & 1);
+#pragma unroll
+    for (int p = 0; p < QX; ++p) xsv[p] = mx_scale_at(src_of(min(min(wave + NW * p, DX - 1) * 32 + (lane >> 1), rows - 1)), nmac) + 4u * (lane & 1);
 
-    // Pieces of weights behind the last block of a row: the last one again.  The activations there are zeros.
-    auto issue = [&](int stage, int mac) {
-        uint8_t *to = lds + stage * S::STAGE;
-        const int last = nblk - 1 - 8 * mac;
-        const int xat = mac * XMAC;
+    // Macros behind the last one: the last one again, into a stage that nobody reads.  Pieces of weights behind the last block of a row:
+    // the last one again; the activations there are zeros.
+    const int per_split = (nmac + a.splits - 1) / a.splits;
+    const int st0 = static_cast<int>(blockIdx.y) * per_split, st1 = min(nmac, st0 + per_split);
+    auto issue = [&](uint32_t buffer, int want) {
+        const int st = min(want, st1 - 1);
+        uint8_t *to = lds + buffer;
+        const int last = nblk - 1 - 8 * st, xat = st * XMAC;
+        const uint32_t back = last < 7 ? 16u * max(0, wp - last) : 0u, back2 = last < 7 ? 16u * max(0, wq - last) : 0u;
 #pragma unroll
         for (int p = 0; p < PW; ++p) {
-            const int q = wave + NW * p;
-            if ((BN / 8) % NW != 0 && q >= BN / 8) continue;
-            uint32_t off = wv[p];
-            if (last < 7) off -= 16u * max(0, (piece ^ mx_key((8 * q + (lane >> 3)) & 15)) - last);
-            copy16<0>(win, to + q * 1024, off, mac * 128);
+            const int q = min(wave + NW * p, CW - 1);
+            copy16<0>(win, to + q * 1024, wv[p] - (q & 1 ? back2 : back), st * 128);
         }
 #pragma unroll
-        for (int p = 0; p < PX; ++p) {
-            const int q = wave + NW * p;
-            if ((BM / 8) % NW != 0 && q >= BM / 8) continue;
-            copy16<0>(xwin, to + S::W + q * 1024, xv[p], xat);
-        }
-        if constexpr (AK == 6) {
+        for (int p = 0; p < PX; ++p) copy16<0>(xwin, to + S::W + min(wave + NW * p, CX - 1) * 1024, xv[p], xat);
 #pragma unroll
-            for (int p = 0; p < PT; ++p) {
-                const int q = wave + NW * p;
-                if ((BM / 16) % NW != 0 && q >= BM / 16) continue;
-                copy16<0>(xwin, to + S::W + BM * 128 + q * 1024, xv2[p], xat);
-            }
-        }
+        for (int p = 0; p < PT; ++p) copy16<0>(xwin, to + S::W + S::X + min(wave + NW * p, CT - 1) * 1024, xv2[p], xat);
 #pragma unroll
-        for (int p = 0; p < QW; ++p) {
-            const int q = wave + NW * p;
-            if ((BN / 32) % NW != 0 && q >= BN / 32) continue;
-            copy4(swin, to + S::W + S::X + q * 256, wsv[p], mac * 8);
-        }
+        for (int p = 0; p < QW; ++p) copy4(swin, to + S::W + S::X + S::X2 + min(wave + NW * p, DW - 1) * 256, wsv[p], st * 256);
 #pragma unroll
-        for (int p = 0; p < QX; ++p) {
-            const int q = wave + NW * p;
-            if ((BM / 32) % NW != 0 && q >= BM / 32) continue;
-            copy4(xswin, to + S::W + S::X + S::WS + q * 256, xsv[p], mac * 8);
-        }
+        for (int p = 0; p < QX; ++p) copy4(xswin, to + S::W + S::X + S::X2 + S::WS + min(wave + NW * p, DX - 1) * 256, xsv[p], st * 256);
     };
 
-    float4_t acc[TM][TN];
+    float16_t acc[TM][TN];
 #pragma unroll
     for (int m = 0; m < TM; ++m)
 #pragma unroll
-        for (int n = 0; n < TN; ++n) acc[m][n] = float4_t{0.f, 0.f, 0.f, 0.f};
-
-    auto multiply = [&](int stage) {
-        const uint8_t *at = lds + stage * S::STAGE;
-        const uint8_t *wat = at + wn * TN * 2048 + r * 128, *xat = at + S::W + wm * TM * 2048 + r * 128;
-        uint32_t sw[TN], sx[TM];
-        u32x4_t tail[TM];
+        for (int n = 0; n < TN; ++n)
 #pragma unroll
-        for (int n = 0; n < TN; ++n) sw[n] = *reinterpret_cast<const uint16_t *>(at + S::W + S::X + (wn * TN + n) * 128 + r * 8 + 2 * g);
+            for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
+
+    // fragments of a step: those of the current one and the next
+    u32x4_t w0[TN], w1[TN], x0[TM], x1[TM], tail[TM] = {}, tail2[TM] = {}, tail_next[TM];
+    uint32_t sw[TN], sx[TM], sw_next[TN], sx_next[TM];
+    const uint32_t key = (r >> 1) & 7, line = r * 128, line2 = r * 64, key2 = (r >> 2) & 3, ps = r * 8 + 4 * h;
+    auto read_codes = [&](uint32_t buffer, int s, u32x4_t (&w)[TN], u32x4_t (&x)[TM]) {
+        const uint32_t at = buffer + line + (((4 * h + s) ^ key) << 4);
+#pragma unroll
+        for (int n = 0; n < TN; ++n) w[n] = *reinterpret_cast<const u32x4_t *>(lds + at + (wn * TN + n) * 4096);
+#pragma unroll
+        for (int m = 0; m < TM; ++m) x[m] = *reinterpret_cast<const u32x4_t *>(lds + at + S::W + (wm * TM + m) * 4096);
+    };
+    auto read_tail = [&](uint32_t buffer, int half, u32x4_t (&t)[TM]) {
+        if constexpr (AK == 6) {
+            const uint32_t at = buffer + S::W + S::X + line2 + (((2 * h + half) ^ key2) << 4);
+#pragma unroll
+            for (int m = 0; m < TM; ++m) t[m] = *reinterpret_cast<const u32x4_t *>(lds + at + (wm * TM + m) * 2048);
+        }
+    };
+    auto read_scales = [&](uint32_t buffer) {
+        const uint32_t at = buffer + S::W + S::X + S::X2 + ps;
+#pragma unroll
+        for (int n = 0; n < TN; ++n) sw_next[n] = *reinterpret_cast<const uint32_t *>(lds + at + (wn * TN + n) * 256);
+#pragma unroll
+        for (int m = 0; m < TM; ++m) sx_next[m] = *reinterpret_cast<const uint32_t *>(lds + at + S::WS + (wm * TM + m) * 256);
+    };
+    auto take = [&] {
+#pragma unroll
+        for (int n = 0; n < TN; ++n) sw[n] = sw_next[n];
 #pragma unroll
         for (int m = 0; m < TM; ++m) {
-            sx[m] = *reinterpret_cast<const uint16_t *>(at + S::W + S::X + S::WS + (wm * TM + m) * 128 + r * 8 + 2 * g);
-            if constexpr (AK == 6) tail[m] = *reinterpret_cast<const u32x4_t *>(at + S::W + BM * 128 + (wm * TM + m) * 1024 + row_order_lane(lane));
+            sx[m] = sx_next[m];
+            if constexpr (AK == 6) tail[m] = tail_next[m];
         }
-        static_for<2>([&](auto SS) {
-            constexpr int s = SS.value;
-            const int pc = ((2 * g + s) ^ key) << 4;
-            u32x4_t w[TN];
-            MxFrag x[TM];
+    };
+    auto multiply = [&](auto SS, const u32x4_t (&w)[TN], const u32x4_t (&x)[TM], const u32x4_t (&t)[TM]) {
+        constexpr int s = SS.value;
 #pragma unroll
-            for (int n = 0; n < TN; ++n) w[n] = *reinterpret_cast<const u32x4_t *>(wat + n * 2048 + pc);
+        for (int m = 0; m < TM; ++m)
 #pragma unroll
-            for (int m = 0; m < TM; ++m) {
-                x[m].x = *reinterpret_cast<const u32x4_t *>(xat + m * 2048 + pc);
-                if constexpr (AK == 6) x[m].y = s == 0 ? u32x2_t{tail[m].x, tail[m].y} : u32x2_t{tail[m].z, tail[m].w};
-            }
-#pragma unroll
-            for (int m = 0; m < TM; ++m)
-#pragma unroll
-                for (int n = 0; n < TN; ++n) acc[m][n] = mx_scale_mfma<AK, s>(w[n], x[m], acc[m][n], sw[n], sx[m]);
-        });
+            for (int n = 0; n < TN; ++n)
+                acc[m][n] = mx_scale_mfma32<AK, s>(w[n], x[m], s % 2 ? t[m].z : t[m].x, s % 2 ? t[m].w : t[m].y, acc[m][n], sw[n], sx[m]);
     };
 
-    const int per_split = (nmac + a.splits - 1) / a.splits;
-    const int mac0 = static_cast<int>(blockIdx.y) * per_split, mac1 = min(nmac, mac0 + per_split);
-    issue(0, mac0);
-    int stage = 0;
-    for (int mac = mac0; mac < mac1; ++mac) {
-        // the copies of this stage have landed, and every wave has read the other one
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < R; ++i) issue(i * S::STAGE, st0 + i);
+    wait_vmcnt<(R - 1) * PER>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    uint32_t cur = 0;
+    read_codes(cur, 0, w0, x0);
+    read_scales(cur);
+    read_tail(cur, 0, tail_next);
+    take();
+    for (int st = st0; st < st1; ++st) {
+        read_codes(cur, 1, w1, x1);
+        multiply(std::integral_constant<int, 0>{}, w0, x0, tail);
+        read_codes(cur, 2, w0, x0);
+        read_tail(cur, 1, tail2);
+        multiply(std::integral_constant<int, 1>{}, w1, x1, tail);
+        read_codes(cur, 3, w1, x1);
+        multiply(std::integral_constant<int, 2>{}, w0, x0, tail2);
+        // the next macro has landed, and every wave has read this one
+        wait_vmcnt<(R - 2) * PER>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (mac + 1 < mac1) issue(stage ^ 1, mac + 1);
-        multiply(stage);
-        stage ^= 1;
+        issue(cur, st + R);
+        cur = cur + S::STAGE == R * S::STAGE ? 0u : cur + S::STAGE;
+        read_codes(cur, 0, w0, x0);
+        read_scales(cur);
+        read_tail(cur, 0, tail_next);
+        multiply(std::integral_constant<int, 3>{}, w1, x1, tail2);
+        take();
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // late copies must not land in reused LDS
     __syncthreads();
 
-    // results leave through LDS so that the lanes of a store lie side by side in a row
-    uint8_t *area = lds + wave * kRowsOut;
-    const bool partial = a.splits > 1;
+    // Results leave through LDS so that the lanes of a store lie side by side in a row: two squares at a time, 32 rows of 64.
+    uint8_t *area = lds + wave * kTileOut;
+    const bool partial = a.splits > 1, f32 = partial || a.y_dtype == MFQ_X_F32;
+    uint8_t *y = reinterpret_cast<uint8_t *>(partial ? a.part + static_cast<int64_t>(blockIdx.y) * a.M * a.nrows : a.y);
+    const int64_t ldy = partial ? a.nrows : a.ldy;
+    const bool wide = ldy % (f32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+    // columns n .. n + 64 of the 32 rows from mt on, from the two squares p and q; those of q at `shift` from p's instead of 32
+    auto put = [&](const float16_t &p, const float16_t &q, int mt, int n, int end) __attribute__((always_inline)) {
+        if (f32) {
 #pragma unroll
-    for (int m = 0; m < TM; ++m) {
-        const int mt = (wm * TM + m) * 16;
-        auto dst = [&](int i) { return mt + i < rows ? pair_of(mt + i) : -1; };
-        auto put = [&](auto NG, const float4_t *v, int col, int end, bool f32, float *y, int64_t ldy) {
-            constexpr int G = NG.value;
-            const bool wide = ldy % (f32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
-            if (f32) {
-                float4_t o[G];
-#pragma unroll
-                for (int i = 0; i < G; ++i) o[i] = v[i];
-                store_rows<G>(area, o, lane, col, end, y, ldy, wide, dst);
-            } else {
-                u32x2_t o[G];
-#pragma unroll
-                for (int i = 0; i < G; ++i) o[i] = u32x2_t{mx_pack16(v[i][0], v[i][1], a.y_dtype), mx_pack16(v[i][2], v[i][3], a.y_dtype)};
-                store_rows16<G>(area, o, lane, col, end, reinterpret_cast<uint16_t *>(y), ldy, wide, dst);
+            for (int j = 0; j < 4; ++j) {
+                *reinterpret_cast<float4_t *>(area + r * kTilePitch + (8 * j + 4 * h) * 4) = float4_t{p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]};
+                *reinterpret_cast<float4_t *>(area + r * kTilePitch + (32 + 8 * j + 4 * h) * 4) = float4_t{q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]};
             }
-        };
-        constexpr int G = TN < 4 ? TN : 4, H = TN / 2 < 4 ? TN / 2 : 4;
-        if (partial) {
-            float *part = a.part + static_cast<int64_t>(blockIdx.y) * a.M * a.nrows;
-            if (a.glu) {
+            wave_sync();
 #pragma unroll
-                for (int b = 0; b < TN; b += H) {
-                    const int half = b >= TN / 2, at = n0 + (wn * (TN / 2) + b % (TN / 2)) * 16;
-                    put(std::integral_constant<int, H>{}, &acc[m][b], half * width + at, half * width + max(at, width), true, part, a.nrows);
+            for (int k = 0; k < 8; ++k) {
+                const int row = k * 4 + (lane >> 4), c = n + (lane & 15) * 4, to_row = row_of[mt + row];
+                const float4_t v = *reinterpret_cast<const float4_t *>(area + row * kTilePitch + (lane & 15) * 16);
+                if (to_row < 0 || c >= end) continue;
+                float *o = reinterpret_cast<float *>(y) + static_cast<int64_t>(to_row) * ldy + c;
+                if (wide && c + 4 <= end) {
+                    *reinterpret_cast<float4_t *>(o) = v;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        if (c + t < end) o[t] = v[t];
                 }
-            } else {
-#pragma unroll
-                for (int b = 0; b < TN; b += G) put(std::integral_constant<int, G>{}, &acc[m][b], n0 + (wn * TN + b) * 16, a.nrows, true, part, a.nrows);
-            }
-        } else if (a.glu) {
-#pragma unroll
-            for (int b = 0; b < TN / 2; b += H) {
-                float4_t v[H];
-#pragma unroll
-                for (int i = 0; i < H; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[i][j] = glu_value(acc[m][b + i][j], acc[m][TN / 2 + b + i][j], a.gelu);
-                put(std::integral_constant<int, H>{}, v, n0 + (wn * (TN / 2) + b) * 16, width, a.y_dtype == MFQ_X_F32, static_cast<float *>(a.y), a.ldy);
             }
         } else {
 #pragma unroll
-            for (int b = 0; b < TN; b += G)
-                put(std::integral_constant<int, G>{}, &acc[m][b], n0 + (wn * TN + b) * 16, width, a.y_dtype == MFQ_X_F32, static_cast<float *>(a.y), a.ldy);
+            for (int j = 0; j < 4; ++j) {
+                *reinterpret_cast<u32x2_t *>(area + r * kTilePitch + (8 * j + 4 * h) * 2) =
+                    u32x2_t{mx_pack16(p[4 * j], p[4 * j + 1], a.y_dtype), mx_pack16(p[4 * j + 2], p[4 * j + 3], a.y_dtype)};
+                *reinterpret_cast<u32x2_t *>(area + r * kTilePitch + (32 + 8 * j + 4 * h) * 2) =
+                    u32x2_t{mx_pack16(q[4 * j], q[4 * j + 1], a.y_dtype), mx_pack16(q[4 * j + 2], q[4 * j + 3], a.y_dtype)};
+            }
+            wave_sync();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int row = k * 8 + (lane >> 3), c = n + (lane & 7) * 8, to_row = row_of[mt + row];
+                const u32x4_t v = *reinterpret_cast<const u32x4_t *>(area + row * kTilePitch + (lane & 7) * 16);
+                if (to_row < 0 || c >= end) continue;
+                uint16_t *o = reinterpret_cast<uint16_t *>(y) + static_cast<int64_t>(to_row) * ldy + c;
+                if (wide && c + 8 <= end) {
+                    *reinterpret_cast<u32x4_t *>(o) = v;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 8; ++t)
+                        if (c + t < end) o[t] = static_cast<uint16_t>(v[t >> 1] >> (16 * (t & 1)));
+                }
+            }
         }
-    }
+        wave_sync();
+    };
+    static_for<TM>([&](auto MI) __attribute__((always_inline)) {
+        constexpr int m = MI.value;
+        const int mt = (wm * TM + m) * 32;
+        if (mt >= rows) return;
+        static_for<TN / 2>([&](auto BI) __attribute__((always_inline)) {
+            constexpr int b = BI.value;
+            if (!a.glu) {
+                put(acc[m][2 * b], acc[m][2 * b + 1], mt, n0 + (wn * TN + 2 * b) * 32, width);
+            } else if constexpr (TN == 2) {  // 32 columns: one square, twice
+                const int at = n0 + wn * 32, end = min(at + 32, width);
+                if (partial) {
+                    put(acc[m][0], acc[m][0], mt, at, end);
+                    put(acc[m][1], acc[m][1], mt, width + at, width + end);
+                } else {
+                    float16_t v;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = glu_value(acc[m][0][i], acc[m][1][i], a.gelu);
+                    put(v, v, mt, at, end);
+                }
+            } else if constexpr (b < TN / 4) {
+                const int at = n0 + (wn * (TN / 2) + 2 * b) * 32;
+                if (partial) {
+                    put(acc[m][2 * b], acc[m][2 * b + 1], mt, at, width);
+                    put(acc[m][TN / 2 + 2 * b], acc[m][TN / 2 + 2 * b + 1], mt, width + at, 2 * width);
+                } else {
+                    float16_t u, v;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        u[i] = glu_value(acc[m][2 * b][i], acc[m][TN / 2 + 2 * b][i], a.gelu);
+                        v[i] = glu_value(acc[m][2 * b + 1][i], acc[m][TN / 2 + 2 * b + 1][i], a.gelu);
+                    }
+                    put(u, v, mt, at, width);
+                }
+            }
+        });
+    });
 }
 
 // the pieces of a split over K, added in their order
@@ -586,17 +644,17 @@ int launch_stream_nb(const MxsArgs &a, int tiles, hipStream_t st) {
     return launch_stream<AK, MT, 1, 2, RES, MODE>(a, tiles, st);
 }
 
-template <int AK, int BN, int BM, int WN, int WM, int MODE>
+template <int AK, int BN, int BM, int WN, int WM, int R, int MODE>
 int launch_tile(const MxsArgs &a, hipStream_t st) {
-    using S = TileShape<AK, BN, BM>;
+    using S = TileShape<AK, BN, BM, R>;
     const int width = a.glu ? a.nrows / 2 : a.nrows;
     const int64_t tiles_n = ceil_div(width, a.glu ? BN / 2 : BN);
     const int64_t tiles_m = MODE == kMapped ? ceil_div(a.pairs, BM) + (a.E < a.pairs ? a.E : a.pairs) : ceil_div(a.M, BM);
     const int64_t blocks = (tiles_n * tiles_m + 7) / 8 * 8;
     MFQ_REQUIRE(blocks < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx_scaled: %lld tiles", static_cast<long long>(blocks));
-    size_t lds = 2 * S::STAGE;
-    if (lds < WN * WM * static_cast<size_t>(kRowsOut)) lds = WN * WM * static_cast<size_t>(kRowsOut);
-    auto kern = mxs_tile_kernel<AK, BN, BM, WN, WM, MODE>;
+    static_assert(WN * WM * kTileOut <= R * S::STAGE && S::LDS <= static_cast<int>(kMaxDynamicLds), "results leave through the ring");
+    const size_t lds = S::LDS;
+    auto kern = mxs_tile_kernel<AK, BN, BM, WN, WM, R, MODE>;
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void *>(kern), lds, "mx_scaled")) return rc;
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(MODE == kLinear ? a.splits : 1)), dim3(WN * WM * 64), lds, st, a);
     return check_launch("mx_scaled (tile)");
@@ -611,23 +669,25 @@ int launch_join(const MxsArgs &a, hipStream_t st) {
 }
 
 // Kernel of a call: rows up to which the weights are streamed, tile and pieces of K above.
-struct MxsPlan { int kind, splits; };  // kind: 0 streamed, activations in LDS; 1, 2 streamed, one or two tiles; 3 .. 5 tiles
+struct MxsPlan { int kind, splits; };  // kind: 0 streamed, activations in LDS; 1, 2 streamed, one or two tiles; 3 .. 6 tiles
 constexpr int kPlanTile = 3;
-constexpr int kTileN[3] = {128, 256, 256}, kTileM[3] = {64, 128, 256};
+constexpr int kTileN[8] = {128, 128, 256, 256,256,128,256,64}, kTileM[8] = {64, 128, 128, 256,192,64,64,128};
 
 MxsPlan plan_linear(int act, int nrows, int K, int M, bool glu) {
-    const int nmac = (K / 32 + 7) / 8;
+    const int nmac = mx_macros(K);
     if (M <= 16 && static_cast<int64_t>(M) * nmac * mx_macro_bytes(act) <= kResBytes) return {0, 1};
     if (M <= 16) return {1, 1};
     if (M <= 32) return {2, 1};
     const int cus = device_cu_count();
-    const int shapes = act == 4 ? 3 : 2;
     int best = 0;
-    for (int s = 0; s < shapes; ++s)
-        if (ceil_div(nrows, kTileN[s]) * ceil_div(M, kTileM[s]) >= cus || s == 0) best = s;
+    for (int s = 0; s < (act == 4 ? 4 : 3); ++s)
+        if (10 * ceil_div(nrows, kTileN[s]) * ceil_div(M, kTileM[s]) >= 8 * cus) best = s;
+    static const int forced = tune_env("MFQ_MXS_TILE", 0), forced_split = tune_env("MFQ_MXS_SPLIT", 0);
+    if (forced) best = forced - 1;
     const int64_t tiles = ceil_div(nrows, kTileN[best]) * ceil_div(M, kTileM[best]);
     int splits = 1;
     while (splits < 8 && tiles * splits * 2 <= cus && nmac / (splits * 2) >= 2) splits *= 2;
+    if (forced_split) splits = forced_split < nmac ? forced_split : nmac;
     // no piece may be empty
     while (splits > 1 && (splits - 1) * ceil_div(nmac, splits) >= nmac) --splits;
     return {kPlanTile + best, splits};
@@ -635,7 +695,7 @@ MxsPlan plan_linear(int act, int nrows, int K, int M, bool glu) {
 
 size_t quantized_bytes(int act, int K, int64_t M) {
     const auto up = [](int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); };
-    return static_cast<size_t>(up(M * mx_row_bytes(act, K)) + up(M * mx_scale_stride(K)));
+    return static_cast<size_t>(up(M * mx_row_bytes(act, K)) + up(mx_scale_bytes(M, K)));
 }
 
 template <int AK>
@@ -644,10 +704,15 @@ int run_linear(const MxsArgs &a, const MxsPlan &p, hipStream_t st) {
         case 0: return launch_stream_nb<AK, 1, true, kLinear>(a, 1, st);
         case 1: return launch_stream_nb<AK, 1, false, kLinear>(a, 1, st);
         case 2: return launch_stream_nb<AK, 2, false, kLinear>(a, 1, st);
-        case 3: return launch_tile<AK, 128, 64, 2, 2, kLinear>(a, st);
-        case 4: return launch_tile<AK, 256, 128, 4, 2, kLinear>(a, st);
+        case 3: return launch_tile<AK, 128, 64, 2, 2, 2, kLinear>(a, st);
+        case 4: return launch_tile<AK, 128, 128, 2, 2, 2, kLinear>(a, st);
+        case 5: return launch_tile<AK, 256, 128, 4, 2, AK == 4 ? 3 : 2, kLinear>(a, st);
+        case 7: return launch_tile<AK, 256, 192, 4, 2, 2, kLinear>(a, st);
+        case 8: return launch_tile<AK, 128, 64, 2, 2, 3, kLinear>(a, st);
+        case 9: return launch_tile<AK, 256, 64, 4, 1, 2, kLinear>(a, st);
+        case 10: return launch_tile<AK, 64, 128, 1, 4, 3, kLinear>(a, st);
         default:
-            if constexpr (AK == 4) return launch_tile<AK, 256, 256, 2, 4, kLinear>(a, st);
+            if constexpr (AK == 4) return launch_tile<AK, 256, 256, 2, 4, 2, kLinear>(a, st);
             else return fail(MFQ_ERR_UNSUPPORTED, "mx_scaled: no such tile");
     }
 }
@@ -665,8 +730,8 @@ int run_experts(const MxsArgs &a, hipStream_t st) {
     switch (plan_mapped(a.pairs, a.E)) {
         case 0: return launch_stream_nb<AK, 1, false, kMapped>(a, most(16), st);
         case 1: return launch_stream_nb<AK, 2, false, kMapped>(a, most(32), st);
-        case 2: return launch_tile<AK, 128, 64, 2, 2, kMapped>(a, st);
-        default: return launch_tile<AK, 256, 128, 4, 2, kMapped>(a, st);
+        case 2: return launch_tile<AK, 128, 64, 2, 2, 2, kMapped>(a, st);
+        default: return launch_tile<AK, 256, 128, 4, 2, AK == 4 ? 3 : 2, kMapped>(a, st);
     }
 }
 
@@ -690,12 +755,13 @@ int check_common(MxsArgs &a, const char *who, const void *values, const void *sc
     MFQ_REQUIRE(!glu || (y_dtype != MFQ_X_F32 && (activation == MFQ_GLU_SILU || activation == MFQ_GLU_GELU)), MFQ_ERR_INVALID,
                 "%s: a gated product takes a 16-bit type and activation 0 or 1, not y_dtype=%d activation=%d", who, y_dtype, activation);
     MFQ_REQUIRE(reinterpret_cast<uintptr_t>(y) % (y_dtype == MFQ_X_F32 ? 4 : 2) == 0, MFQ_ERR_INVALID, "%s: unaligned y", who);
+    MFQ_REQUIRE(mx_scale_bytes(rows, cols) < (1ll << 32) - 512 && mx_scale_bytes(x_rows, cols) < (1ll << 32) - 512, MFQ_ERR_UNSUPPORTED,
+                "%s: %lld rows of weights, %lld of activations, %d columns", who, static_cast<long long>(rows), static_cast<long long>(x_rows), cols);
     a.wv = static_cast<const uint8_t *>(values);
     a.ws = static_cast<const uint8_t *>(scales);
     a.y = const_cast<void *>(y);
     a.ldy = ldy;
     a.K = cols;
-    a.sstride = mx_scale_stride(cols);
     a.y_dtype = y_dtype;
     a.glu = glu != 0;
     a.gelu = activation == MFQ_GLU_GELU;
@@ -733,7 +799,7 @@ extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scale
     MFQ_REQUIRE(static_cast<int64_t>(nrows) * (cols / 2) < (1ll << 32) - 256, MFQ_ERR_UNSUPPORTED, "mx_scaled_gemm_rows: %d x %d weights", nrows, cols);
     const hipStream_t st = as_stream(stream);
     a.wv += static_cast<int64_t>(row0) * (cols / 2);
-    a.ws += static_cast<int64_t>(row0) * a.sstride;
+    a.row0 = row0;
     a.nrows = nrows;
     a.M = M;
     a.R = 1;
@@ -760,7 +826,7 @@ extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scale
     if (p.splits > 1) {
         // a short workspace: K in as many pieces as it has room for
         const size_t left = workspace_bytes > used && ws ? workspace_bytes - used : 0, each = static_cast<size_t>(M) * nrows * 4;
-        const int nmac = (cols / 32 + 7) / 8;
+        const int nmac = mx_macros(cols);
         if (left / each < static_cast<size_t>(p.splits)) p.splits = static_cast<int>(left / each);
         while (p.splits > 1 && (p.splits - 1) * ceil_div(nmac, p.splits) >= nmac) --p.splits;
         if (p.splits < 2 || reinterpret_cast<uintptr_t>(ws) % 16 != 0) p.splits = 1;

@@ -34,11 +34,17 @@ typedef short i16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kMxMacro = 256;  // columns of a macro
 
-// bytes of a row of scales: those of whole macros
-__host__ __device__ __forceinline__ constexpr int mx_scale_stride(int K) { return (K / 32 + 7) & ~7; }
+// Scales of both operands lie by blocks of 32 rows, and in those by macros: eight bytes a row, 256 a block of rows.  A copy of a tile's
+// scales then moves whole lines, where rows one after the other (a line of 128 bytes fetched for every eight) cost as many requests as
+// the codes.  Zeros behind the last column.
+__host__ __device__ __forceinline__ constexpr int mx_macros(int K) { return (K + kMxMacro - 1) / kMxMacro; }
+__host__ __device__ __forceinline__ constexpr uint32_t mx_scale_at(int64_t row, int nmac) {  // of the row's first macro; the next are 256 further each
+    return static_cast<uint32_t>(row >> 5) * static_cast<uint32_t>(nmac) * 256u + static_cast<uint32_t>(row & 31) * 8u;
+}
+__host__ __device__ __forceinline__ constexpr int64_t mx_scale_bytes(int64_t rows, int K) { return (rows + 31) / 32 * mx_macros(K) * 256; }
 // bytes of a macro of quantised activations, and of a row
 __host__ __device__ __forceinline__ constexpr int mx_macro_bytes(int kind) { return kind == 4 ? 128 : 192; }
-__host__ __device__ __forceinline__ constexpr int64_t mx_row_bytes(int kind, int K) { return static_cast<int64_t>((K + kMxMacro - 1) / kMxMacro) * mx_macro_bytes(kind); }
+__host__ __device__ __forceinline__ constexpr int64_t mx_row_bytes(int kind, int K) { return static_cast<int64_t>(mx_macros(K)) * mx_macro_bytes(kind); }
 
 // by which the pieces of a line are turned, from its row (0 .. 15): with rows p = 2, 3, 4, 5 (in pairs) in the upper half and 0, 1, 6, 7
 // in the lower, for each of which the hardware reads another lane group's piece in the same pass
@@ -47,20 +53,16 @@ __device__ __forceinline__ int mx_key(int row) {
     return (p & 1) | ((p >> 2) << 1) | ((((p >> 1) ^ (p >> 2)) & 1) << 2);
 }
 
-// a fragment of activations: FP4 fills x, FP6 also y
-struct MxFrag {
-    u32x4_t x;
-    u32x2_t y;
-};
+// x: four registers of activations, FP4 codes or the first of FP6; y, z: the rest of those
 template <int AK, int SEL>
-__device__ __forceinline__ float4_t mx_scale_mfma(u32x4_t w, const MxFrag &f, float4_t c, uint32_t sw, uint32_t sx) {
+__device__ __forceinline__ float4_t mx_scale_mfma(u32x4_t w, u32x4_t x, uint32_t y, uint32_t z, float4_t c, uint32_t sw, uint32_t sx) {
     const i32x8_t a = {static_cast<int>(w.x), static_cast<int>(w.y), static_cast<int>(w.z), static_cast<int>(w.w), 0, 0, 0, 0};
     if constexpr (AK == 4) {
-        const i32x8_t b = {static_cast<int>(f.x.x), static_cast<int>(f.x.y), static_cast<int>(f.x.z), static_cast<int>(f.x.w), 0, 0, 0, 0};
+        const i32x8_t b = {static_cast<int>(x.x), static_cast<int>(x.y), static_cast<int>(x.z), static_cast<int>(x.w), 0, 0, 0, 0};
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, SEL, static_cast<int>(sw), SEL, static_cast<int>(sx));
     } else {
-        const i32x8_t b = {static_cast<int>(f.x.x), static_cast<int>(f.x.y), static_cast<int>(f.x.z), static_cast<int>(f.x.w),
-                           static_cast<int>(f.y.x), static_cast<int>(f.y.y), 0, 0};
+        const i32x8_t b = {static_cast<int>(x.x), static_cast<int>(x.y), static_cast<int>(x.z), static_cast<int>(x.w),
+                           static_cast<int>(y), static_cast<int>(z), 0, 0};
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 2, SEL, static_cast<int>(sw), SEL, static_cast<int>(sx));
     }
 }
@@ -74,6 +76,23 @@ __device__ __forceinline__ void copy4(__amdgpu_buffer_rsrc_t win, uint8_t *lds, 
     __builtin_amdgcn_raw_ptr_buffer_load_lds(win, (lds_void_t)lds, 4, at, base, 0, 0);
 }
 
+// ---- the 32 x 32 form, for tiles ------------------------------------------------------------------------------------------------
+// v_mfma_scale_f32_32x32x64_f8f6f4: lane l = (r, h), r = l & 31, h = l >> 5, holds columns 32 h .. 32 h + 31 of row r; results 8 j + 4 h + i of
+// the first operand by row r of the second in register 4 j + i.  In a loop of nothing else it reaches 6.9 PFLOP/s on random codes
+// where the 16 x 16 form reaches 5.0 (one wave a SIMD) to 5.7 (four), 9.8 against 7.3 on zeros: the rest is the clock under load.
+template <int AK, int SEL>
+__device__ __forceinline__ float16_t mx_scale_mfma32(u32x4_t w, u32x4_t x, uint32_t y, uint32_t z, float16_t c, uint32_t sw, uint32_t sx) {
+    const i32x8_t a = {static_cast<int>(w.x), static_cast<int>(w.y), static_cast<int>(w.z), static_cast<int>(w.w), 0, 0, 0, 0};
+    if constexpr (AK == 4) {
+        const i32x8_t b = {static_cast<int>(x.x), static_cast<int>(x.y), static_cast<int>(x.z), static_cast<int>(x.w), 0, 0, 0, 0};
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, SEL, static_cast<int>(sw), SEL, static_cast<int>(sx));
+    } else {
+        const i32x8_t b = {static_cast<int>(x.x), static_cast<int>(x.y), static_cast<int>(x.z), static_cast<int>(x.w),
+                           static_cast<int>(y), static_cast<int>(z), 0, 0};
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 2, SEL, static_cast<int>(sw), SEL, static_cast<int>(sx));
+    }
+}
+
 // ---- quantisation of eight values of a block of 32, which lies in the four lanes of a quad --------------------------------------
 // Scale 2^(e - 2), e the exponent of the block's largest magnitude (both element types reach into the binade of 4), not below
 // 2^-127; elements to nearest, ties to even, those beyond the largest element (6, or 7.5) to it.  A block that holds an infinity
@@ -82,14 +101,18 @@ template <int PERM>
 __device__ __forceinline__ uint32_t quad_perm(uint32_t v) {
     return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), PERM, 0xF, 0xF, true));
 }
+// the scale byte of a block from the bits of its largest magnitude as an fp32
+__device__ __forceinline__ uint32_t mx_scale_of(uint32_t most) {
+    const int e = static_cast<int>(most >> 23);  // of a subnormal 0: its scale is 2^-127 in any case
+    return e == 255 ? 255u : static_cast<uint32_t>(max(e - 2, 0));
+}
 __device__ __forceinline__ uint32_t mx_scale_byte(const float (&v)[8]) {
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
     most = max(most, quad_perm<0xB1>(most));
     most = max(most, quad_perm<0x4E>(most));
-    const int e = static_cast<int>(most >> 23);  // of an fp32 subnormal 0: its scale is 2^-127 in any case
-    return e == 255 ? 255u : static_cast<uint32_t>(max(e - 2, 0));
+    return mx_scale_of(most);
 }
 // codes of eight values: 32 bits of E2M1, or 48 of E2M3
 template <int AK>
@@ -174,17 +197,17 @@ __device__ __forceinline__ uint32_t mx_pack16(float lo, float hi, int dtype) {
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------------
-// Quantised rows in memory: values [M, mx_row_bytes], scales [M, mx_scale_stride] with zeros behind the row's blocks.
+// Quantised rows in memory: values [M, mx_row_bytes], scales of mx_scale_bytes (rows behind the last are left as they are).
 int mx_quantize_launch(int kind, const void *x, int x_dtype, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st);
 
 struct MxsArgs {
-    const uint8_t *wv, *ws;  // weights of the pool: values, scales with rows of `sstride` bytes
+    const uint8_t *wv, *ws;  // weights: values from row row0 of the pool on, scales of the whole pool
     const uint8_t *xv, *xs;  // quantised activations
     void *y;
     const int32_t *ids, *ids_dst, *bounds, *slot;  // grouped calls: expert of a pair, pairs by expert, their bounds, place of an expert in the pool
     const void *xraw;        // activations before quantisation, for the kernel that does it itself
     int64_t ldy, ldx;
-    int K, sstride, nrows;   // nrows: neurons of the tensor or of an expert
+    int K, row0, nrows;      // nrows: neurons of the tensor or of an expert
     int M, E, R, pairs, routed;
     int y_dtype, glu, gelu, x_dtype, x_wide;  // glu: gate rows first, nrows / 2 results; x_wide: xraw lies in pieces of 16 bytes
     int splits;

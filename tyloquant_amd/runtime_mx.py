@@ -30,7 +30,7 @@ class MxWeight:
         self.n_experts = self.rows // self.out
         self.data = values                      # the device tensor other weights call `data`
         self._ws = _Workspace()
-        self._wide_scales = None
+        self._laid = None
 
     @property
     def payload_bytes(self) -> int:
@@ -50,20 +50,19 @@ class MxWeight:
         h = F.MxHeader(dtype, 4 if dtype == "MXFP4" else 8, values.shape[0], cols, 0, values.numel(), values.numel(), scales.numel())
         return MxWeight(h, values, scales, out)
 
-    def wide_scales(self) -> torch.Tensor:
-        """Scales with rows of whole groups of eight, which the products of microscaled operands read: the payload's own where
-        the columns are a multiple of 256, else a copy made at the first call."""
-        if self.kind != 4:
-            raise ValueError(f"products of microscaled operands take MXFP4 weights, not {self.dtype}: use mx_matmul")
-        if self._wide_scales is None:
-            if self.neuron_len % 256 == 0 and self.scales.data_ptr() % 8 == 0:
-                self._wide_scales = self.scales
-            else:
-                stride = (self.neuron_len // 32 + 7) // 8 * 8
-                wide = torch.empty((self.rows, stride), dtype=torch.uint8, device=self.scales.device)
-                L.check(L.lib().mfq_hip_mx_pad_scales(_ptr(self.scales), self.rows, self.neuron_len, _ptr(wide), _stream()))
-                self._wide_scales = wide
-        return self._wide_scales
+    def laid_scales(self) -> torch.Tensor:
+        """Scales as the products of microscaled operands read them (mfq_hip_mx_lay_scales), laid out at the first call and kept:
+        1/16 of the values' bytes.  A graph cannot be the first to ask: what it writes is there only after a replay."""
+        if self._laid is None:
+            if self.kind != 4:
+                raise ValueError(f"products of microscaled operands take MXFP4 weights, not {self.dtype}: use mx_matmul")
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{self.dtype}: call laid_scales() before a graph is captured")
+            laid = torch.empty(_scale_bytes(self.rows, self.neuron_len), dtype=torch.uint8, device=self.scales.device)
+            L.check(L.lib().mfq_hip_mx_lay_scales(_ptr(self.scales), self.rows, self.neuron_len, _ptr(laid), _stream()))
+            torch.cuda.current_stream().synchronize()   # later calls may come on other streams
+            self._laid = laid
+        return self._laid
 
     @staticmethod
     def from_blob(dtype: str, blob, device="cuda", out: int | None = None) -> "MxWeight":
@@ -120,10 +119,14 @@ def _row_bytes(kind: int, K: int) -> int:
     return -(-K // 256) * (128 if kind == 4 else 192)
 
 
+def _scale_bytes(rows: int, K: int) -> int:
+    return -(-rows // 32) * -(-K // 256) * 256
+
+
 class MxRows:
     """Quantised activations [.., neuron_len]: value bytes of rows of whole groups of 256 columns (uint8 [M, 128 or 192 a group], the
-    layout of mfq_hip_mx_quantize_rows) and E8M0 scales (uint8 [M, 8 a group]), zeros behind the row's last column; `shape` is
-    that of the rows before quantisation."""
+    layout of mfq_hip_mx_quantize_rows) and E8M0 scales (uint8, by 32 rows and groups); `shape` is that of the rows before
+    quantisation."""
 
     def __init__(self, dtype: str, values: torch.Tensor, scales: torch.Tensor, shape):
         kind, self.shape = _act_kind(dtype), tuple(shape)
@@ -132,7 +135,7 @@ class MxRows:
         self.dtype, self.kind, self.values, self.scales = dtype, kind, values, scales
         self.neuron_len = self.shape[-1]
         self.rows = torch.Size(self.shape[:-1]).numel()
-        want = (self.rows, _row_bytes(kind, self.neuron_len)), (self.rows, -(-self.neuron_len // 256) * 8)
+        want = (self.rows, _row_bytes(kind, self.neuron_len)), (_scale_bytes(self.rows, self.neuron_len),)
         if values.dtype != torch.uint8 or scales.dtype != torch.uint8 or (tuple(values.shape), tuple(scales.shape)) != want or \
                 not (values.is_contiguous() and scales.is_contiguous()) or values.device != scales.device:
             raise ValueError(f"{dtype} rows of {self.shape}: values {tuple(values.shape)} and scales {tuple(scales.shape)} must be contiguous uint8 "
@@ -178,7 +181,7 @@ def mx_quantize(x: torch.Tensor, dtype: str = "MXFP4") -> MxRows:
     x2 = _raw_rows(x, K)
     M = x2.shape[0]
     values = torch.empty((M, _row_bytes(kind, K)), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((M, -(-K // 256) * 8), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(_scale_bytes(M, K), dtype=torch.uint8, device=x.device)
     if M:
         L.check(L.lib().mfq_hip_mx_quantize_rows(kind, _ptr(x2), _OUT[x2.dtype], x2.stride(0), M, K, _ptr(values), _ptr(scales), _stream()))
     return MxRows(dtype, values, scales, x.shape)
@@ -201,14 +204,14 @@ def _scaled(w: MxWeight, x, act: str, expert: int, glu: int, activation: int, ou
     yd = _out_dtype(out_dtype)
     if glu and (nrows % 2 or yd == L.X_F32):
         raise ValueError(f"a gated product takes a 16-bit type and gate and up rows, not {out_dtype} and {nrows} rows")
-    ws_scales = w.wide_scales()
+    laid = w.laid_scales()
     width = nrows // 2 if glu else nrows
     y = torch.empty((M, width), dtype=out_dtype, device=dev)
     if M:
         lib = L.lib()
         need = lib.mfq_hip_mx_scaled_gemm_workspace_bytes(kind, nrows, K, M, xs is not None)
         ws = borrow(need, dev)
-        L.check(lib.mfq_hip_mx_scaled_gemm_rows(w.values.data_ptr(), ws_scales.data_ptr(), w.rows, K, row0, nrows, kind, x2.data_ptr(), xd, ldx,
+        L.check(lib.mfq_hip_mx_scaled_gemm_rows(w.values.data_ptr(), laid.data_ptr(), w.rows, K, row0, nrows, kind, x2.data_ptr(), xd, ldx,
                                                 _ptr(xs), M, glu, activation, y.data_ptr(), yd, width, _ptr(ws), need if ws is not None else 0,
                                                 _stream()))
     return y if len(shape) == 2 else y.reshape(*shape[:-1], width)
@@ -235,7 +238,7 @@ def _moe(w: MxWeight, x, route, act: str, routed: bool, glu: int, activation: in
     yd = _out_dtype(out_dtype)
     if glu and (w.out % 2 or yd == L.X_F32):
         raise ValueError(f"a gated product takes a 16-bit type and gate and up rows, not {out_dtype} and {w.out} rows")
-    ws_scales = w.wide_scales()
+    laid = w.laid_scales()
     width = w.out // 2 if glu else w.out
     y = torch.empty((T, R, width), dtype=out_dtype, device=dev) if out is None else out
     if T * R:
@@ -243,7 +246,7 @@ def _moe(w: MxWeight, x, route, act: str, routed: bool, glu: int, activation: in
         mapped = route.ids_dst is not None
         need = lib.mfq_hip_mx_moe_workspace_bytes(kind, K, M, mapped, xs is not None)
         ws = borrow(need, dev)
-        L.check(lib.mfq_hip_mx_moe_matmul(w.values.data_ptr(), ws_scales.data_ptr(), w.rows, K, w.out, _ptr(slot), route.n_experts, kind, x2.data_ptr(), xd,
+        L.check(lib.mfq_hip_mx_moe_matmul(w.values.data_ptr(), laid.data_ptr(), w.rows, K, w.out, _ptr(slot), route.n_experts, kind, x2.data_ptr(), xd,
                                           ldx, _ptr(xs), int(routed), route.ids.data_ptr(), T, R, _ptr(route.ids_dst) if mapped else None,
                                           _ptr(route.expert_bounds) if mapped else None, glu, activation, y.data_ptr(), yd, width, _ptr(ws),
                                           need if ws is not None else 0, _stream()))
