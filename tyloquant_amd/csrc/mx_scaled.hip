@@ -300,6 +300,196 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
     }
 }
 
+// ---- few rows, many neurons ---------------------------------------------------------------------------------------------------
+// The activations of a tile of up to 16 * MT rows lie in LDS for the whole of K; every wave takes row-blocks of 16 neurons by itself (with
+// GLU those of the gate and of the up rows) and goes through their macros as one stream, a ring of D stages ahead across the ends of the
+// row-blocks: no sum meets another wave's, and a launch has a few long blocks where the kernel above has a short one for every 16
+// neurons.  Bound by the weights' way from memory.  61 tokens of 8 routes over 64 experts of 4096 x 2048: the kernel above took 167 us.
+template <int AK, int MT, int NB>
+struct FlowShape {
+    static constexpr int W = NB * 2048, STAGE = W + 256, REQ = 2 * NB + 1;
+    static constexpr int XM = MT * 16 * mx_macro_bytes(AK) + 256;  // a macro of activations and its scales
+};
+
+template <int AK, int MT, int NB, int D, int MODE>
+__global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
+    using S = FlowShape<AK, MT, NB>;
+    static_assert(NB <= 2 && MT <= 2 && D >= 3, "a stage's scales are one request of four bytes a lane");
+    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, nwaves = blockDim.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int nblk = a.K / 32, nmac = (nblk + 7) / 8;
+    constexpr int XMAC = mx_macro_bytes(AK);
+    const int64_t wrow = a.K / 2, xrow = static_cast<int64_t>(nmac) * XMAC;
+    const int width = NB == 2 ? a.nrows / 2 : a.nrows;  // results of a row
+
+    const int tile = static_cast<int>(blockIdx.x) / chunks, chunk = static_cast<int>(blockIdx.x) - tile * chunks;
+    int expert = 0, m0 = 0, first = 0, rows;
+    if constexpr (MODE == kMapped) {
+        mxs_zero_rows(a, blockIdx.x, gridDim.x, tid, blockDim.x);
+        if (tile >= mxs_total_tiles(a, 16 * MT, lane)) return;
+        int t0, count;
+        mxs_find_tile(a, 16 * MT, lane, tile, expert, t0, count);
+        first = a.bounds[expert] + (tile - t0) * 16 * MT;
+        rows = min(16 * MT, a.bounds[expert + 1] - first);
+        if (a.slot) expert = a.slot[expert];
+        expert = __builtin_amdgcn_readfirstlane(expert);
+    } else {
+        m0 = tile * 16 * MT;
+        rows = min(16 * MT, a.M - m0);
+    }
+    auto pair_of = [&](int m) { return MODE == kMapped ? a.ids_dst[first + m] : m0 + m; };
+    auto src_of = [&](int m) {
+        const int p = pair_of(m);
+        return MODE == kLinear || a.routed ? p : p / a.R;
+    };
+    // the block's row-blocks, and how many of them are this wave's: rb0 + wave, rb0 + wave + nwaves, ...
+    const int rbs = (width + 15) / 16;
+    const int rb0 = static_cast<int>(static_cast<int64_t>(rbs) * chunk / chunks), rb1 = static_cast<int>(static_cast<int64_t>(rbs) * (chunk + 1) / chunks);
+    const int mine = max(0, rb1 - rb0 - wave + nwaves - 1) / nwaves, items = mine * nmac;
+
+    // activations, macro after macro as the copies of the kernel above leave them
+    uint8_t *xres = lds + nwaves * (D * S::STAGE);
+    {
+        const int64_t base = MODE == kLinear ? m0 : 0;
+        const int span = MODE == kLinear ? rows : a.M;
+        const __amdgpu_buffer_rsrc_t xwin = wave_window(a.xv + base * xrow, static_cast<uint32_t>(span * xrow));
+        const __amdgpu_buffer_rsrc_t xswin = wave_window(a.xs, 0xffffff00u);
+        uint32_t xv[2 * MT], xv2[MT];
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) {
+            const int row = 8 * i + (lane >> 3);
+            xv[i] = static_cast<uint32_t>((src_of(min(row, rows - 1)) - base) * xrow) + 16u * ((lane & 7) ^ mx_key(row & 15));
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            xv2[t] = static_cast<uint32_t>((src_of(min(16 * t + (lane >> 2), rows - 1)) - base) * xrow) + 128u + 16u * row_order_quarter(lane >> 2, lane & 3);
+        const uint32_t xsv = mx_scale_at(src_of(min(MT == 2 ? lane >> 1 : (lane >> 1) & 15, rows - 1)), nmac) + 4u * (lane & 1);
+        for (int mac = wave; mac < nmac; mac += nwaves) {
+            uint8_t *to = xres + mac * S::XM;
+            const int xat = mac * XMAC;
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) copy16<0>(xwin, to + i * 1024, xv[i], xat);
+            if constexpr (AK == 6) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) copy16<0>(xwin, to + (2 * MT + t) * 1024, xv2[t], xat);
+            }
+            if (MT == 2 || lane < 32) copy4(xswin, to + MT * 16 * XMAC, xsv, mac * 256);
+        }
+    }
+
+    const __amdgpu_buffer_rsrc_t win = wave_window(a.wv + static_cast<int64_t>(expert) * a.nrows * wrow, static_cast<uint32_t>(a.nrows * wrow));
+    const __amdgpu_buffer_rsrc_t swin = wave_window(a.ws, 0xffffff00u);  // offsets of 32 bits from the first row: the host sees to it
+    uint8_t *ring = lds + wave * (D * S::STAGE);
+    const int piece = lane & 7;
+    const uint32_t off0 = static_cast<uint32_t>((lane >> 3) * wrow) + 16u * (piece ^ mx_key(lane >> 3));
+    const uint32_t off1 = static_cast<uint32_t>((8 + (lane >> 3)) * wrow) + 16u * (piece ^ mx_key(8 + (lane >> 3)));
+    // the next copies: stage, row-block, macro
+    int to_stage = 0, to_rb = rb0 + wave, to_mac = 0;
+    uint32_t wsv = 0;
+    auto issue = [&] {
+        if (to_mac == 0) {
+            const int b = NB == 2 ? lane >> 5 : 0;
+            wsv = mx_scale_at(a.row0 + expert * a.nrows + b * width + min(to_rb * 16 + ((lane >> 1) & 15), width - 1), nmac) + 4u * (lane & 1);
+        }
+        uint8_t *to = ring + to_stage * S::STAGE;
+        const int last = nblk - 1 - 8 * to_mac, valid = width - to_rb * 16;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) {
+            const int row = 8 * (i & 1) + (lane >> 3);
+            uint32_t off = i & 1 ? off1 : off0;
+            // neurons behind the last one, and pieces of weights behind the last block of a row: the last ones again
+            if (valid < 16) off -= static_cast<uint32_t>(max(0, row - (valid - 1)) * wrow);
+            if (last < 7) off -= 16u * max(0, (piece ^ mx_key(row)) - last);
+            copy16<2>(win, to + i * 1024, off, static_cast<int>(static_cast<uint32_t>((to_rb * 16 + (i >> 1) * width) * wrow) + to_mac * 128u));
+        }
+        if (NB == 2 || lane < 32) copy4(swin, to + S::W, wsv, to_mac * 256);
+        to_stage = to_stage + 1 == D ? 0 : to_stage + 1;
+        if (++to_mac == nmac) {
+            to_mac = 0;
+            to_rb += nwaves;
+        }
+    };
+    for (int i = 0; i < D; ++i)
+        if (i < items) issue();
+    if (items >= D) wait_vmcnt<D * S::REQ>();
+    else wait_vmcnt<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+
+    int64_t out_row[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) out_row[t] = t * 16 + r < rows ? static_cast<int64_t>(pair_of(t * 16 + r)) * a.ldy : -1;
+    const bool f32 = a.y_dtype == MFQ_X_F32;
+    const bool wide = a.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
+    float4_t acc[NB][MT];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[b][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const int key = mx_key(r);
+    int stage = 0, rb = rb0 + wave, mac = 0;
+    for (int i = 0; i < items; ++i) {
+        // younger than this stage: those of the next D - 1 items, and the stores of results, which only make the wait longer
+        const int left = items - 1 - i;
+        if (left >= D - 1) wait_vmcnt<(D - 1) * S::REQ>();
+        else if (D > 3 && left == 2) wait_vmcnt<2 * S::REQ>();
+        else if (left == 1) wait_vmcnt<S::REQ>();
+        else wait_vmcnt<0>();
+        const uint8_t *at = ring + stage * S::STAGE, *xat = xres + mac * S::XM;
+        u32x4_t w[2][NB], x[2][MT], tail[MT] = {};
+        uint32_t sw[NB], sx[MT];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            sw[b] = *reinterpret_cast<const uint16_t *>(at + S::W + b * 128 + r * 8 + 2 * g);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) w[s][b] = *reinterpret_cast<const u32x4_t *>(at + b * 2048 + r * 128 + (((2 * g + s) ^ key) << 4));
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            sx[t] = *reinterpret_cast<const uint16_t *>(xat + MT * 16 * XMAC + t * 128 + r * 8 + 2 * g);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) x[s][t] = *reinterpret_cast<const u32x4_t *>(xat + t * 2048 + r * 128 + (((2 * g + s) ^ key) << 4));
+            if constexpr (AK == 6) tail[t] = *reinterpret_cast<const u32x4_t *>(xat + (2 * MT + t) * 1024 + row_order_lane(lane));
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is free for the next copies
+        if (i + D < items) issue();
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                acc[b][t] = mx_scale_mfma<AK, 0>(w[0][b], x[0][t], tail[t].x, tail[t].y, acc[b][t], sw[b], sx[t]);
+                acc[b][t] = mx_scale_mfma<AK, 1>(w[1][b], x[1][t], tail[t].z, tail[t].w, acc[b][t], sw[b], sx[t]);
+            }
+        stage = stage + 1 == D ? 0 : stage + 1;
+        if (++mac < nmac) continue;
+        const int n = rb * 16 + 4 * g;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            float4_t v = acc[0][t];
+            acc[0][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+            if constexpr (NB == 2) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = glu_value(v[j], acc[1][t][j], a.gelu);
+                acc[1][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+            }
+            if (out_row[t] < 0 || n >= width) continue;
+            if (wide && n + 4 <= width) {
+                if (f32) *reinterpret_cast<float4_t *>(static_cast<float *>(a.y) + out_row[t] + n) = v;
+                else *reinterpret_cast<u32x2_t *>(static_cast<uint16_t *>(a.y) + out_row[t] + n) =
+                    u32x2_t{mx_pack16(v[0], v[1], a.y_dtype), mx_pack16(v[2], v[3], a.y_dtype)};
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n + j < width) store_rounded(a.y, out_row[t] + n + j, v[j], a.y_dtype);
+            }
+        }
+        mac = 0;
+        rb += nwaves;
+    }
+}
+
 // ---- many rows: tiles -----------------------------------------------------------------------------------------------------------
 // A block of WN * WM waves owns BN neurons x BM rows, a wave BN / WN x BM / WM of them in squares of 32.  K goes macro by macro through a
 // ring of R stages in LDS.  Lane (r, h) multiplies block 4 h + s of the macro in step s of four, so its four scales are one word.  While
@@ -644,6 +834,40 @@ int launch_stream_nb(const MxsArgs &a, int tiles, hipStream_t st) {
     return launch_stream<AK, MT, 1, 2, RES, MODE>(a, tiles, st);
 }
 
+// Waves of a block of the flow kernel: as many as fit the LDS beside the activations, eight at most; 0: K is too long for it.
+template <int AK, int MT, int NB, int D>
+int flow_waves(int K, size_t *lds) {
+    using S = FlowShape<AK, MT, NB>;
+    const size_t x = static_cast<size_t>(mx_macros(K)) * S::XM;
+    for (int n = 8; n >= 2; --n) {
+        *lds = n * static_cast<size_t>(D) * S::STAGE + x;
+        if (*lds <= kMaxDynamicLds) return n;
+    }
+    return 0;
+}
+template <int AK, int MT, int NB, int MODE>
+int launch_flow_nb(const MxsArgs &a, int tiles, int busy, hipStream_t st) {
+    constexpr int D = 3;
+    size_t lds;
+    const int nwaves = flow_waves<AK, MT, NB, D>(a.K, &lds);
+    if (!nwaves) return MFQ_ERR_UNSUPPORTED;
+    const int width = a.glu ? a.nrows / 2 : a.nrows, rbs = static_cast<int>(ceil_div(width, 16));
+    // blocks of a tile: two for each compute unit where the LDS has room for two, while every wave has a row-block
+    const int want = device_cu_count() * (2 * lds <= kMaxDynamicLds ? 2 : 1);
+    int chunks = static_cast<int>(ceil_div(want, busy > 0 ? busy : 1));
+    if (chunks > ceil_div(rbs, nwaves)) chunks = static_cast<int>(ceil_div(rbs, nwaves));
+    auto kern = mxs_flow_kernel<AK, MT, NB, D, MODE>;
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void *>(kern), lds, "mx_scaled")) return rc;
+    MFQ_REQUIRE(static_cast<int64_t>(tiles) * chunks < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx_scaled: %d tiles", tiles);
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles * chunks)), dim3(64 * nwaves), lds, st, a, chunks);
+    return check_launch("mx_scaled (flow)");
+}
+// tiles: at most; busy: about as many have rows
+template <int AK, int MT, int MODE>
+int launch_flow(const MxsArgs &a, int tiles, int busy, hipStream_t st) {
+    return a.glu ? launch_flow_nb<AK, MT, 2, MODE>(a, tiles, busy, st) : launch_flow_nb<AK, MT, 1, MODE>(a, tiles, busy, st);
+}
+
 template <int AK, int BN, int BM, int WN, int WM, int R, int MODE>
 int launch_tile(const MxsArgs &a, hipStream_t st) {
     using S = TileShape<AK, BN, BM, R>;
@@ -728,8 +952,12 @@ int run_experts(const MxsArgs &a, hipStream_t st) {
     if (!a.ids_dst) return launch_stream_nb<AK, 1, true, kPairs>(a, a.pairs, st);
     const auto most = [&](int rows) { return static_cast<int>(ceil_div(a.pairs, rows) + (a.E < a.pairs ? a.E : a.pairs)); };
     switch (plan_mapped(a.pairs, a.E)) {
-        case 0: return launch_stream_nb<AK, 1, false, kMapped>(a, most(16), st);
-        case 1: return launch_stream_nb<AK, 2, false, kMapped>(a, most(32), st);
+        case 0:
+            if (int rc = launch_flow<AK, 1, kMapped>(a, most(16), a.E < a.pairs ? a.E : a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
+            return launch_stream_nb<AK, 1, false, kMapped>(a, most(16), st);
+        case 1:
+            if (int rc = launch_flow<AK, 2, kMapped>(a, most(32), a.E < a.pairs ? a.E : a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
+            return launch_stream_nb<AK, 2, false, kMapped>(a, most(32), st);
         case 2: return launch_tile<AK, 128, 64, 2, 2, 2, kMapped>(a, st);
         default: return launch_tile<AK, 256, 128, 4, 2, AK == 4 ? 3 : 2, kMapped>(a, st);
     }
