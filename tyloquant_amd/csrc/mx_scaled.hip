@@ -892,29 +892,56 @@ int launch_join(const MxsArgs &a, hipStream_t st) {
     return check_launch("mx_scaled (join)");
 }
 
-// Kernel of a call: rows up to which the weights are streamed, tile and pieces of K above.
-struct MxsPlan { int kind, splits; };  // kind: 0 streamed, activations in LDS; 1, 2 streamed, one or two tiles; 3 .. 6 tiles
+// Kernel of a call: streamed with the activations in LDS (0), streamed in one or two tiles of 16 rows (1, 2), or a tile of the list (3 + its
+// index) with K in `splits` pieces.
+struct MxsPlan { int kind, splits; };
 constexpr int kPlanTile = 3;
-constexpr int kTileN[8] = {128, 128, 256, 256,256,128,256,64}, kTileM[8] = {64, 128, 128, 256,192,64,64,128};
+// Tiles and what a launch of them takes, us: f + max(macros * l, rounds * (macros * c + e)), rounds = blocks a compute unit: l is a macro's
+// way from memory with the compute unit to itself, c its share with `per_cu` blocks on it, e the end of a block.  Fitted to 12288 x 4096 and
+// 4096 x 12288 at 40 to 4096 rows, MXFP4 / MXFP6: 12288 x 4096 at 40 rows 13.2, 11.6, 15.2, 19.3, 28.2 us in the order of the list (MXFP4),
+// at 601 rows 31.0, 31.2, 26.6, 25.9, 34.0, at 2048 rows 82.9, 88.6, 71.4, 73.2, 72.8; MXFP6 at 128 rows 13.9 (128 x 64), 24.8, 30.1, at 2048
+// 102.8, 82.0, 103.4, at 4096 279, 206, 182.
+struct MxsTile { int act, n, m, per_cu; double f, l, c, e; };
+constexpr MxsTile kMxsTile[] = {
+    {4, 128, 64, 3, 5.5, 0.48, 0.36, 0.5}, {4, 64, 128, 2, 6.0, 0.36, 0.40, 0.5}, {4, 128, 128, 2, 6.2, 0.56, 0.62, 1.0},
+    {4, 256, 128, 1, 7.3, 0.75, 1.12, 2.6}, {4, 256, 256, 1, 9.6, 1.16, 1.9, 5.0},
+    {6, 128, 64, 1, 5.3, 0.47, 0.65, 0.5}, {6, 256, 128, 1, 7.2, 0.95, 1.35, 3.0}, {6, 256, 192, 1, 8.0, 1.23, 1.95, 4.0}};
+constexpr int kMxsTiles = sizeof(kMxsTile) / sizeof(kMxsTile[0]), kMaxSplits = 16;
 
-MxsPlan plan_linear(int act, int nrows, int K, int M, bool glu) {
+double tile_us(const MxsTile &t, int nrows, int nmac, int M, int splits, int cus) {
+    const double blocks = static_cast<double>(ceil_div(nrows, t.n)) * ceil_div(M, t.m) * splits, q = blocks / cus;
+    const double whole = static_cast<double>(static_cast<int64_t>(q) + (q > static_cast<int64_t>(q) ? 1 : 0));
+    const double rounds = t.per_cu == 1 ? whole : (q + whole) / 2;
+    const double macs = static_cast<double>(ceil_div(nmac, splits));
+    double us = macs * t.l > rounds * (macs * t.c + t.e) ? macs * t.l : rounds * (macs * t.c + t.e);
+    // the pieces are written, read by a second launch and written as the result
+    if (splits > 1) us += 3.0 + static_cast<double>(M) * nrows * 4 * (2 * splits + 1) / 4.5e6;
+    return t.f + us;
+}
+
+MxsPlan plan_linear(int act, int nrows, int K, int M) {
     const int nmac = mx_macros(K);
     if (M <= 16 && static_cast<int64_t>(M) * nmac * mx_macro_bytes(act) <= kResBytes) return {0, 1};
     if (M <= 16) return {1, 1};
     if (M <= 32) return {2, 1};
-    const int cus = device_cu_count();
-    int best = 0;
-    for (int s = 0; s < (act == 4 ? 4 : 3); ++s)
-        if (10 * ceil_div(nrows, kTileN[s]) * ceil_div(M, kTileM[s]) >= 8 * cus) best = s;
     static const int forced = tune_env("MFQ_MXS_TILE", 0), forced_split = tune_env("MFQ_MXS_SPLIT", 0);
-    if (forced) best = forced - 1;
-    const int64_t tiles = ceil_div(nrows, kTileN[best]) * ceil_div(M, kTileM[best]);
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= cus && nmac / (splits * 2) >= 2) splits *= 2;
-    if (forced_split) splits = forced_split < nmac ? forced_split : nmac;
-    // no piece may be empty
-    while (splits > 1 && (splits - 1) * ceil_div(nmac, splits) >= nmac) --splits;
-    return {kPlanTile + best, splits};
+    const int cus = device_cu_count();
+    MxsPlan best = {-1, 1};
+    double least = 0.0;
+    for (int t = 0; t < kMxsTiles; ++t) {
+        if (kMxsTile[t].act != act || (forced && forced != t + 1)) continue;
+        for (int s = 1; s <= kMaxSplits && s <= nmac; ++s) {
+            // no piece may be empty
+            if ((s - 1) * ceil_div(nmac, s) >= nmac || (forced_split && s != forced_split)) continue;
+            const double us = tile_us(kMxsTile[t], nrows, nmac, M, s, cus);
+            if (best.kind < 0 || us < least) {
+                best = {kPlanTile + t, s};
+                least = us;
+            }
+        }
+    }
+    if (best.kind < 0) best = {kPlanTile + (act == 4 ? 2 : 6), 1};
+    return best;
 }
 
 size_t quantized_bytes(int act, int K, int64_t M) {
@@ -928,23 +955,34 @@ int run_linear(const MxsArgs &a, const MxsPlan &p, hipStream_t st) {
         case 0: return launch_stream_nb<AK, 1, true, kLinear>(a, 1, st);
         case 1: return launch_stream_nb<AK, 1, false, kLinear>(a, 1, st);
         case 2: return launch_stream_nb<AK, 2, false, kLinear>(a, 1, st);
-        case 3: return launch_tile<AK, 128, 64, 2, 2, 2, kLinear>(a, st);
-        case 4: return launch_tile<AK, 128, 128, 2, 2, 2, kLinear>(a, st);
-        case 5: return launch_tile<AK, 256, 128, 4, 2, AK == 4 ? 3 : 2, kLinear>(a, st);
-        case 7: return launch_tile<AK, 256, 192, 4, 2, 2, kLinear>(a, st);
-        case 8: return launch_tile<AK, 128, 64, 2, 2, 3, kLinear>(a, st);
-        case 9: return launch_tile<AK, 256, 64, 4, 1, 2, kLinear>(a, st);
-        case 10: return launch_tile<AK, 64, 128, 1, 4, 3, kLinear>(a, st);
-        default:
-            if constexpr (AK == 4) return launch_tile<AK, 256, 256, 2, 4, 2, kLinear>(a, st);
-            else return fail(MFQ_ERR_UNSUPPORTED, "mx_scaled: no such tile");
+        default: break;
+    }
+    if constexpr (AK == 4) {
+        switch (p.kind - kPlanTile) {
+            case 0: return launch_tile<4, 128, 64, 2, 2, 2, kLinear>(a, st);
+            case 1: return launch_tile<4, 64, 128, 1, 4, 3, kLinear>(a, st);
+            case 2: return launch_tile<4, 128, 128, 2, 2, 2, kLinear>(a, st);
+            case 3: return launch_tile<4, 256, 128, 4, 2, 3, kLinear>(a, st);
+            default: return launch_tile<4, 256, 256, 2, 4, 2, kLinear>(a, st);
+        }
+    } else {
+        switch (p.kind - kPlanTile) {
+            case 5: return launch_tile<6, 128, 64, 2, 2, 3, kLinear>(a, st);
+            case 6: return launch_tile<6, 256, 128, 4, 2, 2, kLinear>(a, st);
+            default: return launch_tile<6, 256, 192, 4, 2, 2, kLinear>(a, st);
+        }
     }
 }
 
-// smallest tile of rows that holds the pairs an expert has on average, half as many again
+// Kernel of a call with a route map, from the pairs an expert has on average: 0 and 1 waves that stream row-blocks against 16 or 32 rows
+// (flow kernel), 2 and 3 tiles of 128 x 64 and 256 x 128.  128 experts of 2048 x 2048, gated, MXFP4, 8 routes: at 256 tokens (16 pairs an
+// expert) 81, 74, 64 and 75 us, at 2048 tokens 314, 217, 126 and 140; 32 experts of 2880 x 1440, MXFP6, 4 routes: at 1501 tokens (188
+// pairs) 146, 111, 80 and 65 us.
 int plan_mapped(int64_t pairs, int E) {
+    static const int forced = tune_env("MFQ_MXS_TILE", 0);
+    if (forced) return forced - 1;
     const int64_t mean = ceil_div(pairs, E);
-    return mean <= 10 ? 0 : mean <= 24 ? 1 : mean <= 64 ? 2 : 3;
+    return mean <= 10 ? 0 : mean < 160 ? 2 : 3;
 }
 
 template <int AK>
@@ -1009,7 +1047,7 @@ using namespace mfq;
 
 extern "C" size_t mfq_hip_mx_scaled_gemm_workspace_bytes(int act, int nrows, int cols, int M, int x_quantized) {
     if ((act != 4 && act != 6) || nrows <= 0 || cols <= 0 || cols % 32 != 0 || M <= 0) return 0;
-    const MxsPlan p = plan_linear(act, nrows, cols, M, false);
+    const MxsPlan p = plan_linear(act, nrows, cols, M);
     size_t n = x_quantized || (p.kind == 0 && static_cast<int64_t>(M) * cols <= kFuseValues) ? 0 : quantized_bytes(act, cols, M);
     if (p.splits > 1) n += static_cast<size_t>(p.splits) * M * nrows * 4;
     return n;
@@ -1031,7 +1069,7 @@ extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scale
     a.nrows = nrows;
     a.M = M;
     a.R = 1;
-    MxsPlan p = plan_linear(act, nrows, cols, M, glu != 0);
+    MxsPlan p = plan_linear(act, nrows, cols, M);
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     size_t used = 0;
     if (x_scales) {
