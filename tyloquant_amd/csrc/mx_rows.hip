@@ -7,12 +7,6 @@ namespace {
 
 constexpr int kUnits = 4;  // pieces of eight values a thread of the dequantizer takes, 256 pieces apart: their loads are in flight together
 
-typedef __bf16 bf16x32_t __attribute__((ext_vector_type(32)));
-typedef _Float16 half32_t __attribute__((ext_vector_type(32)));
-typedef uint32_t u32x16_t __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x6_t __attribute__((ext_vector_type(6)));
-typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
-
 // A thread takes a block of 32 values, whose conversion to E2M3 the hardware does in one instruction and to E2M1 in sixteen, from the
 // activations' own type; its codes are 16 bytes (and 8 more of E2M3) next to its neighbour's.  Its loads are 64 or 128 bytes from its
 // neighbour's, which takes the address path four or eight times as long as side by side and still is the lesser evil: with a quad of
@@ -28,75 +22,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const void *__restrict
     const int64_t from = row * ldx + block * 32;
     uint32_t byte = 0;
     u32x6_t q = {};
-    if (block < K / 32) {
-        if constexpr (XD == MFQ_X_F32) {
-            const float *p = static_cast<const float *>(x) + from;
-            float16_t v[2];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float4_t f;
-                if constexpr (VEC) f = reinterpret_cast<const float4_t *>(p)[i];
-                else f = float4_t{p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]};
-#pragma unroll
-                for (int t = 0; t < 4; ++t) v[t & 1][2 * i + (t >> 1)] = f[t];  // even and odd columns: the order of the conversion to E2M3
-            }
-            uint32_t most = 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) most = max(most, __float_as_uint(v[i & 1][i >> 1]) & 0x7fffffffu);
-            byte = mx_scale_of(most);
-            const float scale = __uint_as_float(byte << 23);
-            if constexpr (AK == 6) {
-                q = __builtin_bit_cast(u32x6_t, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(v[0], v[1], scale));
-            } else {
-                static_for<4>([&](auto D) {
-                    constexpr int d = D.value;
-                    static_for<4>([&](auto T) {
-                        constexpr int t = T.value;
-                        q[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q[d], v[0][4 * d + t], v[1][4 * d + t], scale, t);
-                    });
-                });
-            }
-        } else {
-            const uint16_t *p = static_cast<const uint16_t *>(x) + from;
-            u32x16_t v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (VEC) {
-                    const u32x4_t f = reinterpret_cast<const u32x4_t *>(p)[i];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) v[4 * i + t] = f[t];
-                } else {
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) v[4 * i + t] = p[8 * i + 2 * t] | (static_cast<uint32_t>(p[8 * i + 2 * t + 1]) << 16);
-                }
-            }
-            u16x2_t most = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t pair = v[i] & 0x7fff7fffu;
-                most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, pair));
-            }
-            const uint32_t m = max(most.x, most.y);
-            // of fp16 the exponent as an fp32 has it, infinities and NaN with theirs
-            byte = mx_scale_of(XD == MFQ_X_BF16 ? m << 16 : m >= 0x7c00u ? 0x7f800000u : __float_as_uint(f16_to_f32(static_cast<uint16_t>(m))));
-            const float scale = __uint_as_float(byte << 23);
-            if constexpr (AK == 6) {
-                if constexpr (XD == MFQ_X_F16) q = __builtin_bit_cast(u32x6_t, __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(__builtin_bit_cast(half32_t, v), scale));
-                else q = __builtin_bit_cast(u32x6_t, __builtin_amdgcn_cvt_scalef32_pk32_fp6_bf16(__builtin_bit_cast(bf16x32_t, v), scale));
-            } else {
-                static_for<4>([&](auto D) {
-                    constexpr int d = D.value;
-                    static_for<4>([&](auto T) {
-                        constexpr int t = T.value;
-                        const uint32_t pair = v[4 * d + t];  // by itself: a bit cast of the element reads the vector's first
-                        if constexpr (XD == MFQ_X_F16) q[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q[d], __builtin_bit_cast(half2_t, pair), scale, t);
-                        else q[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q[d], __builtin_bit_cast(bf16x2_t, pair), scale, t);
-                    });
-                });
-            }
-        }
-        if (byte == 255u) q = u32x6_t{};
-    }
+    if (block < K / 32) mx_quantize_block<AK, XD, VEC>(x, from, q, byte);
     uint8_t *to = values + row * mx_row_bytes(AK, K) + (block >> 3) * mx_macro_bytes(AK);
     *reinterpret_cast<u32x4_t *>(to + (block & 7) * 16) = u32x4_t{q[0], q[1], q[2], q[3]};
     if constexpr (AK == 6) *reinterpret_cast<u32x2_t *>(to + 128 + (block & 7) * 8) = u32x2_t{q[4], q[5]};

@@ -55,21 +55,22 @@ __device__ __forceinline__ void mxs_zero_rows(const MxsArgs &a, int block, int b
     }
 }
 
-// ---- few rows: the weights are streamed ----------------------------------------------------------------------------------------
-// A block owns NB row-blocks of 16 neurons and up to 16 * MT rows of activations; its waves take the macros of K in turn, each
-// through a ring of D stages of its own in LDS (no barrier in the loop), and their sums meet in LDS.  RES: the activations of the
-// block lie in LDS, quantised by the block itself where they come as bf16 or fp16; else they go through the ring with the weights.
-template <int AK, int MT, int NB, int D, bool RES>
+// ---- few rows, long K -------------------------------------------------------------------------------------------------------------
+// A block owns NB row-blocks of 16 neurons (with GLU one of gate rows and that of their up rows) and up to 16 * MT rows of activations; its
+// waves take the macros of K in turn, each through a ring of two stages of its own in LDS (no barrier in the loop), activations and weights
+// alike, and their sums meet in LDS.  For rows of activations that do not fit the LDS beside the weights' ring (flow kernel, below).
+template <int AK, int MT, int NB>
 struct StreamShape {
-    static constexpr int W = NB * 2048, WS = 256, X = RES ? 0 : MT * 16 * mx_macro_bytes(AK), XS = RES ? 0 : 256;
+    static constexpr int W = NB * 2048, WS = 256, X = MT * 16 * mx_macro_bytes(AK), XS = 256;
     static constexpr int STAGE = W + WS + X + XS;
-    static constexpr int REQ = 2 * NB + 1 + (RES ? 0 : MT * (AK == 4 ? 2 : 3) + 1);  // requests of a stage
+    static constexpr int REQ = 2 * NB + 1 + MT * (AK == 4 ? 2 : 3) + 1;  // requests of a stage
 };
 
-template <int AK, int MT, int NB, int D, bool RES, int MODE>
+template <int AK, int MT, int NB, int MODE>
 __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
-    using S = StreamShape<AK, MT, NB, D, RES>;
-    static_assert(NB <= 2 && MT <= 2 && (D == 2 || D == 3), "a stage's scales are one request of four bytes a lane");
+    using S = StreamShape<AK, MT, NB>;
+    constexpr int D = 2;
+    static_assert(NB <= 2 && MT <= 2, "a stage's scales are one request of four bytes a lane");
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, nwaves = blockDim.x >> 6;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -80,14 +81,7 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
     const int width = a.glu ? a.nrows / 2 : a.nrows;  // results of a row
 
     int expert = 0, m0 = 0, rows = a.M, first = 0;
-    if constexpr (MODE == kPairs) {
-        expert = a.ids[blockIdx.y];
-        if (expert < 0 || expert >= a.E) {
-            if (blockIdx.x == 0) mxs_zero_rows(a, blockIdx.y, a.pairs, tid, blockDim.x);
-            return;
-        }
-        rows = 1;
-    } else if constexpr (MODE == kMapped) {
+    if constexpr (MODE == kMapped) {
         if (blockIdx.x == 0) mxs_zero_rows(a, blockIdx.y, gridDim.y, tid, blockDim.x);
         if (static_cast<int>(blockIdx.y) >= mxs_total_tiles(a, 16 * MT, lane)) return;
         int t0, count;
@@ -104,7 +98,7 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
         expert = __builtin_amdgcn_readfirstlane(expert);
     }
     // row of the activations, and of y, that row m of the block is
-    auto pair_of = [&](int m) { return MODE == kPairs ? static_cast<int>(blockIdx.y) : MODE == kMapped ? a.ids_dst[first + m] : m0 + m; };
+    auto pair_of = [&](int m) { return MODE == kMapped ? a.ids_dst[first + m] : m0 + m; };
     auto src_of = [&](int m) {
         const int p = pair_of(m);
         return MODE == kLinear || a.routed ? p : p / a.R;
@@ -129,11 +123,11 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
     const uint32_t wsv = mx_scale_at(a.row0 + expert * a.nrows + neuron(NB == 2 ? lane >> 5 : 0, (lane >> 1) & 15), nmac) + 4u * (lane & 1);
     // rows of a mapped tile lie anywhere: the window is all of them (under 4 GB, the host sees to it); else the block's own
     const int64_t base = MODE == kLinear ? m0 : 0;
-    const int span = RES ? 0 : MODE == kLinear ? rows : a.M;
+    const int span = MODE == kLinear ? rows : a.M;
     const __amdgpu_buffer_rsrc_t xwin = wave_window(a.xv + base * xrow, static_cast<uint32_t>(span * xrow));
     const __amdgpu_buffer_rsrc_t xswin = wave_window(a.xs, 0xffffff00u);
     uint32_t xv[MT * 2], xv2[MT], xsv = 0;
-    if constexpr (!RES) {
+    {
 #pragma unroll
         for (int i = 0; i < MT * 2; ++i) {
             const int row = 8 * i + (lane >> 3);
@@ -148,9 +142,6 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
     }
 
     uint8_t *ring = lds + wave * (D * S::STAGE);
-    uint8_t *xres = lds + nwaves * (D * S::STAGE);  // RES: rows of whole macros, then their scales
-    const int xres_row = nmac * XMAC;
-    uint8_t *xres_s = xres + rows * xres_row;
 
     // Pieces of weights behind the last block of a row: the last one again.  The activations there are zeros.
     auto issue = [&](int stage, int mac) {
@@ -164,7 +155,7 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
             copy16<2>(win, to + i * 1024, off, mac * 128);
         }
         if (NB == 2 || lane < 32) copy4(swin, to + S::W, wsv, mac * 256);
-        if constexpr (!RES) {
+        {
             uint8_t *xto = to + S::W + S::WS;
 #pragma unroll
             for (int i = 0; i < 2 * MT; ++i) copy16<0>(xwin, xto + i * 1024, xv[i], xat);
@@ -181,43 +172,6 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
     for (int i = 0; i < D; ++i)
         if (i < mine) issue(i, wave + i * nwaves);
 
-    if constexpr (RES) {
-        // the block's rows: quantised here, zeros up to whole macros, or copied
-        if (a.xraw) {
-            const int per_row = nmac * 32;
-            for (int u = tid; u < rows * per_row; u += blockDim.x) {
-                const int m = u / per_row, p = u - m * per_row;
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = 0.f;
-                if (p < a.K / 8) {
-                    const int64_t from = src_of(m) * a.ldx + 8 * p;
-                    if (a.x_dtype == MFQ_X_F32) a.x_wide ? mx_load8<MFQ_X_F32, true>(a.xraw, from, v) : mx_load8<MFQ_X_F32, false>(a.xraw, from, v);
-                    else if (a.x_dtype == MFQ_X_F16) a.x_wide ? mx_load8<MFQ_X_F16, true>(a.xraw, from, v) : mx_load8<MFQ_X_F16, false>(a.xraw, from, v);
-                    else a.x_wide ? mx_load8<MFQ_X_BF16, true>(a.xraw, from, v) : mx_load8<MFQ_X_BF16, false>(a.xraw, from, v);
-                }
-                const uint32_t byte = mx_scale_byte(v);
-                const MxStore o = mx_place<AK>(mx_codes<AK>(v, byte), p);
-                if constexpr (AK == 4) *reinterpret_cast<uint32_t *>(xres + m * xres_row + o.at) = o.q.x;
-                else if (o.any) *reinterpret_cast<u32x2_t *>(xres + m * xres_row + o.at) = o.q;
-                if ((p & 3) == 0) xres_s[m * (nmac * 8) + (p >> 2)] = static_cast<uint8_t>(byte);
-            }
-        } else {
-            const int per_row = xres_row / 16;
-            for (int u = tid; u < rows * per_row; u += blockDim.x) {
-                const int m = u / per_row, p = u - m * per_row;
-                reinterpret_cast<u32x4_t *>(xres + m * xres_row)[p] = reinterpret_cast<const u32x4_t *>(a.xv + src_of(m) * xrow)[p];
-            }
-            for (int u = tid; u < rows * nmac; u += blockDim.x) {
-                const int m = u / nmac, p = u - m * nmac;
-                reinterpret_cast<u32x2_t *>(xres_s)[u] = *reinterpret_cast<const u32x2_t *>(a.xs + mx_scale_at(src_of(m), nmac) + p * 256);
-            }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    }
-
     float4_t acc[NB][MT];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -226,11 +180,9 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
     const int key = mx_key(r);
     int stage = 0;
     for (int i = 0; i < mine; ++i) {
-        const int mac = wave + i * nwaves;
         // younger stages in flight: those of the next D - 1 macros
         const int left = mine - 1 - i;
-        if (D == 3 && left >= 2) wait_vmcnt<(D - 1) * S::REQ>();
-        else if (left >= 1) wait_vmcnt<S::REQ>();
+        if (left >= 1) wait_vmcnt<S::REQ>();
         else wait_vmcnt<0>();
         const uint8_t *at = ring + stage * S::STAGE;
         u32x4_t w[2][NB];
@@ -244,14 +196,11 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
         }
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            // RES: rows one after the other, read as they lie; else as the copies have left them
-            const int m = min(t * 16 + r, rows - 1);
-            const uint8_t *row = RES ? xres + m * xres_row + mac * XMAC : at + S::W + S::WS + t * 2048 + r * 128;
-            sx[t] = *reinterpret_cast<const uint16_t *>((RES ? xres_s + m * (nmac * 8) + mac * 8 : at + S::W + S::WS + S::X + t * 128 + r * 8) + 2 * g);
+            const uint8_t *x0 = at + S::W + S::WS;
+            sx[t] = *reinterpret_cast<const uint16_t *>(x0 + S::X + t * 128 + r * 8 + 2 * g);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) x[s][t] = *reinterpret_cast<const u32x4_t *>(row + ((RES ? 2 * g + s : (2 * g + s) ^ key) << 4));
-            if constexpr (AK == 6)
-                tail[t] = *reinterpret_cast<const u32x4_t *>(RES ? row + 128 + g * 16 : at + S::W + S::WS + (2 * MT + t) * 1024 + row_order_lane(lane));
+            for (int s = 0; s < 2; ++s) x[s][t] = *reinterpret_cast<const u32x4_t *>(x0 + t * 2048 + r * 128 + (((2 * g + s) ^ key) << 4));
+            if constexpr (AK == 6) tail[t] = *reinterpret_cast<const u32x4_t *>(x0 + (2 * MT + t) * 1024 + row_order_lane(lane));
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is free for the next copies
         if (i + D < mine) issue(stage, wave + (i + D) * nwaves);
@@ -300,21 +249,24 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
     }
 }
 
-// ---- few rows, many neurons ---------------------------------------------------------------------------------------------------
-// The activations of a tile of up to 16 * MT rows lie in LDS for the whole of K; every wave takes row-blocks of 16 neurons by itself (with
-// GLU those of the gate and of the up rows) and goes through their macros as one stream, a ring of D stages ahead across the ends of the
-// row-blocks: no sum meets another wave's, and a launch has a few long blocks where the kernel above has a short one for every 16
-// neurons.  Bound by the weights' way from memory.  61 tokens of 8 routes over 64 experts of 4096 x 2048: the kernel above took 167 us.
+// ---- few rows ---------------------------------------------------------------------------------------------------------------------
+// The activations of a tile of up to 16 * MT rows lie in LDS for the whole of K.  A block takes a range of row-blocks of 16 neurons (with GLU
+// those of the gate rows, each with that of its up rows), macro after macro, as one stream that its waves share evenly; a wave keeps a ring of
+// D stages of weights ahead, across the ends of row-blocks.  Sums of a row-block that lies in several waves' shares meet in LDS, in the order
+// of the waves.  Bound by the weights' way from memory.  61 tokens of 8 routes over 64 experts of 4096 x 2048, MXFP4 (295 MB): 57 us, where
+// a block for every 16 neurons, its waves on different macros (stream kernel), took 167; 12288 x 4096 at 16 rows 12.2 us there.
+// SMALL: up to four rows, quantised by the block itself where they come as bf16, fp16 or fp32; only that many are kept.
 template <int AK, int MT, int NB>
 struct FlowShape {
     static constexpr int W = NB * 2048, STAGE = W + 256, REQ = 2 * NB + 1;
     static constexpr int XM = MT * 16 * mx_macro_bytes(AK) + 256;  // a macro of activations and its scales
+    static constexpr int small_macro(int rows) { return (rows * (mx_macro_bytes(AK) + 8) + 15) & ~15; }
 };
 
-template <int AK, int MT, int NB, int D, int MODE>
+template <int AK, int MT, int NB, int D, int MODE, bool SMALL>
 __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
     using S = FlowShape<AK, MT, NB>;
-    static_assert(NB <= 2 && MT <= 2 && D >= 3, "a stage's scales are one request of four bytes a lane");
+    static_assert(NB <= 2 && MT <= 2 && D >= 3 && (!SMALL || MT == 1), "a stage's scales are one request of four bytes a lane");
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, nwaves = blockDim.x >> 6;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -326,7 +278,17 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
 
     const int tile = static_cast<int>(blockIdx.x) / chunks, chunk = static_cast<int>(blockIdx.x) - tile * chunks;
     int expert = 0, m0 = 0, first = 0, rows;
-    if constexpr (MODE == kMapped) {
+    if constexpr (MODE == kPairs) {
+        expert = a.ids[tile];
+        if (expert < 0 || expert >= a.E) {
+            if (chunk == 0) mxs_zero_rows(a, tile, a.pairs, tid, blockDim.x);
+            return;
+        }
+        if (a.slot) expert = a.slot[expert];
+        if (expert < 0) return;
+        expert = __builtin_amdgcn_readfirstlane(expert);
+        rows = 1;
+    } else if constexpr (MODE == kMapped) {
         mxs_zero_rows(a, blockIdx.x, gridDim.x, tid, blockDim.x);
         if (tile >= mxs_total_tiles(a, 16 * MT, lane)) return;
         int t0, count;
@@ -339,19 +301,22 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
         m0 = tile * 16 * MT;
         rows = min(16 * MT, a.M - m0);
     }
-    auto pair_of = [&](int m) { return MODE == kMapped ? a.ids_dst[first + m] : m0 + m; };
+    auto pair_of = [&](int m) { return MODE == kPairs ? tile : MODE == kMapped ? a.ids_dst[first + m] : m0 + m; };
     auto src_of = [&](int m) {
         const int p = pair_of(m);
         return MODE == kLinear || a.routed ? p : p / a.R;
     };
-    // the block's row-blocks, and how many of them are this wave's: rb0 + wave, rb0 + wave + nwaves, ...
+    // the block's row-blocks, and this wave's share of their macros
     const int rbs = (width + 15) / 16;
     const int rb0 = static_cast<int>(static_cast<int64_t>(rbs) * chunk / chunks), rb1 = static_cast<int>(static_cast<int64_t>(rbs) * (chunk + 1) / chunks);
-    const int mine = max(0, rb1 - rb0 - wave + nwaves - 1) / nwaves, items = mine * nmac;
+    const int total = (rb1 - rb0) * nmac, item0 = static_cast<int>(static_cast<int64_t>(total) * wave / nwaves);
+    const int items = static_cast<int>(static_cast<int64_t>(total) * (wave + 1) / nwaves) - item0;
 
-    // activations, macro after macro as the copies of the kernel above leave them
     uint8_t *xres = lds + nwaves * (D * S::STAGE);
-    {
+    const int kept = SMALL ? rows > 2 ? 4 : rows : 16 * MT;  // rows of activations in LDS, a power of two
+    const int xm = SMALL ? S::small_macro(kept) : S::XM, xtail = kept * 128, xsat = kept * XMAC;  // of a macro; where FP6's second part and the scales begin
+    if constexpr (!SMALL) {
+        // macro after macro as the copies of the kernel above leave them
         const int64_t base = MODE == kLinear ? m0 : 0;
         const int span = MODE == kLinear ? rows : a.M;
         const __amdgpu_buffer_rsrc_t xwin = wave_window(a.xv + base * xrow, static_cast<uint32_t>(span * xrow));
@@ -367,7 +332,7 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
             xv2[t] = static_cast<uint32_t>((src_of(min(16 * t + (lane >> 2), rows - 1)) - base) * xrow) + 128u + 16u * row_order_quarter(lane >> 2, lane & 3);
         const uint32_t xsv = mx_scale_at(src_of(min(MT == 2 ? lane >> 1 : (lane >> 1) & 15, rows - 1)), nmac) + 4u * (lane & 1);
         for (int mac = wave; mac < nmac; mac += nwaves) {
-            uint8_t *to = xres + mac * S::XM;
+            uint8_t *to = xres + mac * xm;
             const int xat = mac * XMAC;
 #pragma unroll
             for (int i = 0; i < 2 * MT; ++i) copy16<0>(xwin, to + i * 1024, xv[i], xat);
@@ -375,7 +340,7 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t) copy16<0>(xwin, to + (2 * MT + t) * 1024, xv2[t], xat);
             }
-            if (MT == 2 || lane < 32) copy4(xswin, to + MT * 16 * XMAC, xsv, mac * 256);
+            if (MT == 2 || lane < 32) copy4(xswin, to + xsat, xsv, mac * 256);
         }
     }
 
@@ -386,13 +351,14 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
     const uint32_t off0 = static_cast<uint32_t>((lane >> 3) * wrow) + 16u * (piece ^ mx_key(lane >> 3));
     const uint32_t off1 = static_cast<uint32_t>((8 + (lane >> 3)) * wrow) + 16u * (piece ^ mx_key(8 + (lane >> 3)));
     // the next copies: stage, row-block, macro
-    int to_stage = 0, to_rb = rb0 + wave, to_mac = 0;
+    int to_stage = 0, to_rb = rb0 + item0 / nmac, to_mac = item0 - item0 / nmac * nmac;
     uint32_t wsv = 0;
+    auto scales_of = [&](int rb) {
+        const int b = NB == 2 ? lane >> 5 : 0;
+        return mx_scale_at(a.row0 + expert * a.nrows + b * width + min(rb * 16 + ((lane >> 1) & 15), width - 1), nmac) + 4u * (lane & 1);
+    };
+    wsv = scales_of(to_rb);
     auto issue = [&] {
-        if (to_mac == 0) {
-            const int b = NB == 2 ? lane >> 5 : 0;
-            wsv = mx_scale_at(a.row0 + expert * a.nrows + b * width + min(to_rb * 16 + ((lane >> 1) & 15), width - 1), nmac) + 4u * (lane & 1);
-        }
         uint8_t *to = ring + to_stage * S::STAGE;
         const int last = nblk - 1 - 8 * to_mac, valid = width - to_rb * 16;
 #pragma unroll
@@ -408,13 +374,47 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
         to_stage = to_stage + 1 == D ? 0 : to_stage + 1;
         if (++to_mac == nmac) {
             to_mac = 0;
-            to_rb += nwaves;
+            wsv = scales_of(++to_rb);
         }
     };
     for (int i = 0; i < D; ++i)
         if (i < items) issue();
-    if (items >= D) wait_vmcnt<D * S::REQ>();
-    else wait_vmcnt<0>();
+    if constexpr (SMALL) {
+        // a thread a block of 32 columns: quantised here, or copied
+        const int per_row = nmac * 8;
+        for (int u = tid; u < rows * per_row; u += blockDim.x) {
+            const int m = u / per_row, block = u - m * per_row, p = block & 7;
+            const int64_t src = src_of(m);
+            u32x6_t q = {};
+            uint32_t byte = 0;
+            if (a.xraw) {
+                if (block < nblk) {
+                    const int64_t from = src * a.ldx + 32 * block;
+                    if (a.x_dtype == MFQ_X_F32) a.x_wide ? mx_quantize_block<AK, MFQ_X_F32, true>(a.xraw, from, q, byte) : mx_quantize_block<AK, MFQ_X_F32, false>(a.xraw, from, q, byte);
+                    else if (a.x_dtype == MFQ_X_F16) a.x_wide ? mx_quantize_block<AK, MFQ_X_F16, true>(a.xraw, from, q, byte) : mx_quantize_block<AK, MFQ_X_F16, false>(a.xraw, from, q, byte);
+                    else a.x_wide ? mx_quantize_block<AK, MFQ_X_BF16, true>(a.xraw, from, q, byte) : mx_quantize_block<AK, MFQ_X_BF16, false>(a.xraw, from, q, byte);
+                }
+            } else {
+                const uint8_t *row = a.xv + src * xrow + (block >> 3) * XMAC;
+                const u32x4_t v = *reinterpret_cast<const u32x4_t *>(row + p * 16);
+                q[0] = v.x; q[1] = v.y; q[2] = v.z; q[3] = v.w;
+                if constexpr (AK == 6) {
+                    const u32x2_t t = *reinterpret_cast<const u32x2_t *>(row + 128 + p * 8);
+                    q[4] = t.x; q[5] = t.y;
+                }
+                byte = a.xs[mx_scale_at(src, nmac) + (block >> 3) * 256 + p];
+            }
+            uint8_t *to = xres + (block >> 3) * xm;
+            *reinterpret_cast<u32x4_t *>(to + m * 128 + ((p ^ mx_key(m)) << 4)) = u32x4_t{q[0], q[1], q[2], q[3]};
+            if constexpr (AK == 6) *reinterpret_cast<u32x2_t *>(to + xtail + m * 64 + row_order_quarter(m, p >> 1) * 16 + (p & 1) * 8) = u32x2_t{q[4], q[5]};
+            to[xsat + m * 8 + p] = static_cast<uint8_t>(byte);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    } else {
+        // what is older than the weights' first stages
+        if (items >= D) wait_vmcnt<D * S::REQ>();
+        else wait_vmcnt<0>();
+    }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 
@@ -428,51 +428,15 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[b][t] = float4_t{0.f, 0.f, 0.f, 0.f};
-    const int key = mx_key(r);
-    int stage = 0, rb = rb0 + wave, mac = 0;
-    for (int i = 0; i < items; ++i) {
-        // younger than this stage: those of the next D - 1 items, and the stores of results, which only make the wait longer
-        const int left = items - 1 - i;
-        if (left >= D - 1) wait_vmcnt<(D - 1) * S::REQ>();
-        else if (D > 3 && left == 2) wait_vmcnt<2 * S::REQ>();
-        else if (left == 1) wait_vmcnt<S::REQ>();
-        else wait_vmcnt<0>();
-        const uint8_t *at = ring + stage * S::STAGE, *xat = xres + mac * S::XM;
-        u32x4_t w[2][NB], x[2][MT], tail[MT] = {};
-        uint32_t sw[NB], sx[MT];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            sw[b] = *reinterpret_cast<const uint16_t *>(at + S::W + b * 128 + r * 8 + 2 * g);
-#pragma unroll
-            for (int s = 0; s < 2; ++s) w[s][b] = *reinterpret_cast<const u32x4_t *>(at + b * 2048 + r * 128 + (((2 * g + s) ^ key) << 4));
-        }
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            sx[t] = *reinterpret_cast<const uint16_t *>(xat + MT * 16 * XMAC + t * 128 + r * 8 + 2 * g);
-#pragma unroll
-            for (int s = 0; s < 2; ++s) x[s][t] = *reinterpret_cast<const u32x4_t *>(xat + t * 2048 + r * 128 + (((2 * g + s) ^ key) << 4));
-            if constexpr (AK == 6) tail[t] = *reinterpret_cast<const u32x4_t *>(xat + (2 * MT + t) * 1024 + row_order_lane(lane));
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is free for the next copies
-        if (i + D < items) issue();
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                acc[b][t] = mx_scale_mfma<AK, 0>(w[0][b], x[0][t], tail[t].x, tail[t].y, acc[b][t], sw[b], sx[t]);
-                acc[b][t] = mx_scale_mfma<AK, 1>(w[1][b], x[1][t], tail[t].z, tail[t].w, acc[b][t], sw[b], sx[t]);
-            }
-        stage = stage + 1 == D ? 0 : stage + 1;
-        if (++mac < nmac) continue;
+    // results of row-block rb, from v (and u: gate and up)
+    auto put = [&](int rb, const float4_t (&sum)[NB][MT]) {
         const int n = rb * 16 + 4 * g;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            float4_t v = acc[0][t];
-            acc[0][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+            float4_t v = sum[0][t];
             if constexpr (NB == 2) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = glu_value(v[j], acc[1][t][j], a.gelu);
-                acc[1][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < 4; ++j) v[j] = glu_value(v[j], sum[1][t][j], a.gelu);
             }
             if (out_row[t] < 0 || n >= width) continue;
             if (wide && n + 4 <= width) {
@@ -485,8 +449,99 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
                     if (n + j < width) store_rounded(a.y, out_row[t] + n + j, v[j], a.y_dtype);
             }
         }
+    };
+    const int m_ = r & (kept - 1), key = mx_key(m_), xrow16 = SMALL ? m_ : r;
+    const int wkey = mx_key(r);
+    int stage = 0, rb = rb0 + item0 / nmac, mac = item0 - item0 / nmac * nmac;
+    bool whole = mac == 0;  // of the current row-block from its first macro on
+    float4_t head[NB][MT];  // the sums of a row-block that another wave has begun
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) head[b][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < items; ++i) {
+        // younger than this stage: those of the next D - 1 items, and the stores of results, which only make the wait longer
+        const int left = items - 1 - i;
+        if (left >= D - 1) wait_vmcnt<(D - 1) * S::REQ>();
+        else if (D > 3 && left == 2) wait_vmcnt<2 * S::REQ>();
+        else if (left == 1) wait_vmcnt<S::REQ>();
+        else wait_vmcnt<0>();
+        const uint8_t *at = ring + stage * S::STAGE, *xat = xres + mac * xm;
+        u32x4_t w[2][NB], x[2][MT], tail[MT] = {};
+        uint32_t sw[NB], sx[MT];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            sw[b] = *reinterpret_cast<const uint16_t *>(at + S::W + b * 128 + r * 8 + 2 * g);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) w[s][b] = *reinterpret_cast<const u32x4_t *>(at + b * 2048 + r * 128 + (((2 * g + s) ^ wkey) << 4));
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            sx[t] = *reinterpret_cast<const uint16_t *>(xat + xsat + t * 128 + xrow16 * 8 + 2 * g);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) x[s][t] = *reinterpret_cast<const u32x4_t *>(xat + t * 2048 + xrow16 * 128 + (((2 * g + s) ^ key) << 4));
+            if constexpr (AK == 6)
+                tail[t] = *reinterpret_cast<const u32x4_t *>(xat + xtail + t * 1024 + (SMALL ? m_ * 64 + row_order_quarter(m_, g) * 16 : row_order_lane(lane)));
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is free for the next copies
+        if (i + D < items) issue();
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                acc[b][t] = mx_scale_mfma<AK, 0>(w[0][b], x[0][t], tail[t].x, tail[t].y, acc[b][t], sw[b], sx[t]);
+                acc[b][t] = mx_scale_mfma<AK, 1>(w[1][b], x[1][t], tail[t].z, tail[t].w, acc[b][t], sw[b], sx[t]);
+            }
+        stage = stage + 1 == D ? 0 : stage + 1;
+        if (++mac < nmac) continue;
+        if (whole) put(rb, acc);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                if (!whole) head[b][t] = acc[b][t];
+                acc[b][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+            }
         mac = 0;
-        rb += nwaves;
+        ++rb;
+        whole = true;
+    }
+    if (total % nwaves == 0 && total / nwaves % nmac == 0) return;  // every row-block lies in one wave's share
+    // Row-blocks of several shares: each wave leaves what it has of the one it came into (head) and of the one it stopped in.  A share within one
+    // row-block, begun and not ended by it, is a head as well.
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            if (!whole) head[b][t] = acc[b][t];
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    float4_t *left = reinterpret_cast<float4_t *>(ring);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            left[(b * MT + t) * 64 + lane] = head[b][t];
+            left[(NB * MT + b * MT + t) * 64 + lane] = acc[b][t];
+        }
+    static_assert(2 * NB * MT * 1024 <= D * S::STAGE, "sums in the wave's ring");
+    __syncthreads();
+    auto wave_of = [&](int item) { return static_cast<int>((static_cast<int64_t>(item + 1) * nwaves - 1) / total); };
+    for (int k = wave; k < rb1 - rb0; k += nwaves) {
+        const int w0 = wave_of(k * nmac), w1 = wave_of(k * nmac + nmac - 1);
+        if (w0 == w1) continue;
+        float4_t sum[NB][MT];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                sum[b][t] = reinterpret_cast<const float4_t *>(lds + w0 * (D * S::STAGE))[(NB * MT + b * MT + t) * 64 + lane];
+                for (int o = w0 + 1; o <= w1; ++o) {
+                    const float4_t v = reinterpret_cast<const float4_t *>(lds + o * (D * S::STAGE))[(b * MT + t) * 64 + lane];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum[b][t][j] += v[j];
+                }
+            }
+        put(rb0 + k, sum);
     }
 }
 
@@ -808,64 +863,64 @@ __global__ __launch_bounds__(256) void mxs_join_kernel(MxsArgs a) {
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------
-constexpr int kResBytes = 32 * 1024;   // activations a block keeps in LDS
-constexpr int kFuseValues = 20480;     // values up to which a block quantises its activations itself
+constexpr int kSmallRows = 4;  // rows that a block of the flow kernel may quantise itself
 
-template <int AK, int MT, int NB, int D, bool RES, int MODE>
-int launch_stream(const MxsArgs &a, int tiles, hipStream_t st) {
-    using S = StreamShape<AK, MT, NB, D, RES>;
-    const int nmac = (a.K / 32 + 7) / 8, rows = MODE == kLinear ? (a.M < 16 * MT ? a.M : 16 * MT) : MODE == kPairs ? 1 : 16 * MT;
-    const size_t res = RES ? static_cast<size_t>(rows) * nmac * (mx_macro_bytes(AK) + 8) : 0;
+template <int AK, int MT, int NB, int MODE>
+int launch_stream_nb(const MxsArgs &a, int tiles, hipStream_t st) {
+    using S = StreamShape<AK, MT, NB>;
+    const int nmac = mx_macros(a.K);
     int nwaves = nmac < 8 ? nmac : 8;
-    while (nwaves > 1 && nwaves * static_cast<size_t>(D) * S::STAGE + res > kMaxDynamicLds) --nwaves;
-    size_t lds = nwaves * static_cast<size_t>(D) * S::STAGE + res;
-    const size_t red = static_cast<size_t>(nwaves) * NB * MT * 1024;
-    if (lds < red) lds = red;
+    while (nwaves > 1 && nwaves * static_cast<size_t>(2) * S::STAGE > kMaxDynamicLds) --nwaves;
+    const size_t lds = nwaves * static_cast<size_t>(2) * S::STAGE;
+    static_assert(NB * MT * 1024 <= 2 * S::STAGE, "sums in the ring");
     const int width = a.glu ? a.nrows / 2 : a.nrows, per = 16 * (a.glu ? NB / 2 : NB);
-    auto kern = mxs_stream_kernel<AK, MT, NB, D, RES, MODE>;
+    auto kern = mxs_stream_kernel<AK, MT, NB, MODE>;
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void *>(kern), lds, "mx_scaled")) return rc;
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(ceil_div(width, per)), static_cast<unsigned>(tiles)), dim3(64 * nwaves), lds, st, a);
     return check_launch("mx_scaled (stream)");
 }
-
-template <int AK, int MT, bool RES, int MODE>
-int launch_stream_nb(const MxsArgs &a, int tiles, hipStream_t st) {
-    if (a.glu) return launch_stream<AK, MT, 2, 2, RES, MODE>(a, tiles, st);
-    return launch_stream<AK, MT, 1, 2, RES, MODE>(a, tiles, st);
+template <int AK, int MT, int MODE>
+int launch_stream(const MxsArgs &a, int tiles, hipStream_t st) {
+    return a.glu ? launch_stream_nb<AK, MT, 2, MODE>(a, tiles, st) : launch_stream_nb<AK, MT, 1, MODE>(a, tiles, st);
 }
 
-// Waves of a block of the flow kernel: as many as fit the LDS beside the activations, eight at most; 0: K is too long for it.
-template <int AK, int MT, int NB, int D>
-int flow_waves(int K, size_t *lds) {
-    using S = FlowShape<AK, MT, NB>;
-    const size_t x = static_cast<size_t>(mx_macros(K)) * S::XM;
+// Waves of a block of the flow kernel: as many as fit the LDS beside `x` bytes of activations, eight at most; 0: K is too long for it.
+int flow_waves(size_t ring, size_t x, size_t *lds) {
     for (int n = 8; n >= 2; --n) {
-        *lds = n * static_cast<size_t>(D) * S::STAGE + x;
+        *lds = n * ring + x;
         if (*lds <= kMaxDynamicLds) return n;
     }
     return 0;
 }
-template <int AK, int MT, int NB, int MODE>
+constexpr int kFlowStages = 3;
+template <int AK, int MT, int NB>
+size_t flow_x_bytes(int K, int small_rows) {
+    using S = FlowShape<AK, MT, NB>;
+    return static_cast<size_t>(mx_macros(K)) * (small_rows ? S::small_macro(small_rows > 2 ? 4 : small_rows) : S::XM);
+}
+template <int AK, int MT, int NB, int MODE, bool SMALL>
 int launch_flow_nb(const MxsArgs &a, int tiles, int busy, hipStream_t st) {
-    constexpr int D = 3;
+    constexpr int D = kFlowStages;
+    using S = FlowShape<AK, MT, NB>;
     size_t lds;
-    const int nwaves = flow_waves<AK, MT, NB, D>(a.K, &lds);
+    const int nwaves = flow_waves(static_cast<size_t>(D) * S::STAGE, flow_x_bytes<AK, MT, NB>(a.K, SMALL ? MODE == kPairs ? 1 : a.M : 0), &lds);
     if (!nwaves) return MFQ_ERR_UNSUPPORTED;
     const int width = a.glu ? a.nrows / 2 : a.nrows, rbs = static_cast<int>(ceil_div(width, 16));
-    // blocks of a tile: two for each compute unit where the LDS has room for two, while every wave has a row-block
+    // blocks of a tile: two for each compute unit where the LDS has room for two
     const int want = device_cu_count() * (2 * lds <= kMaxDynamicLds ? 2 : 1);
     int chunks = static_cast<int>(ceil_div(want, busy > 0 ? busy : 1));
-    if (chunks > ceil_div(rbs, nwaves)) chunks = static_cast<int>(ceil_div(rbs, nwaves));
-    auto kern = mxs_flow_kernel<AK, MT, NB, D, MODE>;
+    if (chunks > rbs) chunks = rbs;
+    chunks = static_cast<int>(ceil_div(rbs, ceil_div(rbs, chunks)));  // as many row-blocks in each
+    auto kern = mxs_flow_kernel<AK, MT, NB, D, MODE, SMALL>;
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void *>(kern), lds, "mx_scaled")) return rc;
     MFQ_REQUIRE(static_cast<int64_t>(tiles) * chunks < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx_scaled: %d tiles", tiles);
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles * chunks)), dim3(64 * nwaves), lds, st, a, chunks);
     return check_launch("mx_scaled (flow)");
 }
 // tiles: at most; busy: about as many have rows
-template <int AK, int MT, int MODE>
+template <int AK, int MT, int MODE, bool SMALL = false>
 int launch_flow(const MxsArgs &a, int tiles, int busy, hipStream_t st) {
-    return a.glu ? launch_flow_nb<AK, MT, 2, MODE>(a, tiles, busy, st) : launch_flow_nb<AK, MT, 1, MODE>(a, tiles, busy, st);
+    return a.glu ? launch_flow_nb<AK, MT, 2, MODE, SMALL>(a, tiles, busy, st) : launch_flow_nb<AK, MT, 1, MODE, SMALL>(a, tiles, busy, st);
 }
 
 template <int AK, int BN, int BM, int WN, int WM, int R, int MODE>
@@ -892,8 +947,8 @@ int launch_join(const MxsArgs &a, hipStream_t st) {
     return check_launch("mx_scaled (join)");
 }
 
-// Kernel of a call: streamed with the activations in LDS (0), streamed in one or two tiles of 16 rows (1, 2), or a tile of the list (3 + its
-// index) with K in `splits` pieces.
+// Kernel of a call: the flow kernel on up to four rows (0), on one or two tiles of 16 rows (1, 2; the stream kernel where K is too long), or a
+// tile of the list (3 + its index) with K in `splits` pieces.
 struct MxsPlan { int kind, splits; };
 constexpr int kPlanTile = 3;
 // Tiles and what a launch of them takes, us: f + max(macros * l, rounds * (macros * c + e)), rounds = blocks a compute unit: l is a macro's
@@ -919,9 +974,16 @@ double tile_us(const MxsTile &t, int nrows, int nmac, int M, int splits, int cus
     return t.f + us;
 }
 
+// whether the flow kernel holds up to four rows of K columns, gate and up side by side
+bool small_fits(int act, int K, int M) {
+    size_t lds;
+    return act == 4 ? flow_waves(kFlowStages * FlowShape<4, 1, 2>::STAGE, flow_x_bytes<4, 1, 2>(K, M), &lds) > 0
+                    : flow_waves(kFlowStages * FlowShape<6, 1, 2>::STAGE, flow_x_bytes<6, 1, 2>(K, M), &lds) > 0;
+}
+
 MxsPlan plan_linear(int act, int nrows, int K, int M) {
     const int nmac = mx_macros(K);
-    if (M <= 16 && static_cast<int64_t>(M) * nmac * mx_macro_bytes(act) <= kResBytes) return {0, 1};
+    if (M <= kSmallRows && small_fits(act, K, M)) return {0, 1};
     if (M <= 16) return {1, 1};
     if (M <= 32) return {2, 1};
     static const int forced = tune_env("MFQ_MXS_TILE", 0), forced_split = tune_env("MFQ_MXS_SPLIT", 0);
@@ -952,9 +1014,14 @@ size_t quantized_bytes(int act, int K, int64_t M) {
 template <int AK>
 int run_linear(const MxsArgs &a, const MxsPlan &p, hipStream_t st) {
     switch (p.kind) {
-        case 0: return launch_stream_nb<AK, 1, true, kLinear>(a, 1, st);
-        case 1: return launch_stream_nb<AK, 1, false, kLinear>(a, 1, st);
-        case 2: return launch_stream_nb<AK, 2, false, kLinear>(a, 1, st);
+        case 0:
+            return launch_flow<AK, 1, kLinear, true>(a, 1, 1, st);
+        case 1:
+            if (int rc = launch_flow<AK, 1, kLinear>(a, 1, 1, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
+            return launch_stream<AK, 1, kLinear>(a, 1, st);
+        case 2:
+            if (int rc = launch_flow<AK, 2, kLinear>(a, 1, 1, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
+            return launch_stream<AK, 2, kLinear>(a, 1, st);
         default: break;
     }
     if constexpr (AK == 4) {
@@ -987,15 +1054,18 @@ int plan_mapped(int64_t pairs, int E) {
 
 template <int AK>
 int run_experts(const MxsArgs &a, hipStream_t st) {
-    if (!a.ids_dst) return launch_stream_nb<AK, 1, true, kPairs>(a, a.pairs, st);
+    if (!a.ids_dst) {
+        if (int rc = launch_flow<AK, 1, kPairs, true>(a, a.pairs, a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
+        return fail(MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: %d columns without a route map", a.K);
+    }
     const auto most = [&](int rows) { return static_cast<int>(ceil_div(a.pairs, rows) + (a.E < a.pairs ? a.E : a.pairs)); };
     switch (plan_mapped(a.pairs, a.E)) {
         case 0:
             if (int rc = launch_flow<AK, 1, kMapped>(a, most(16), a.E < a.pairs ? a.E : a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
-            return launch_stream_nb<AK, 1, false, kMapped>(a, most(16), st);
+            return launch_stream<AK, 1, kMapped>(a, most(16), st);
         case 1:
             if (int rc = launch_flow<AK, 2, kMapped>(a, most(32), a.E < a.pairs ? a.E : a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
-            return launch_stream_nb<AK, 2, false, kMapped>(a, most(32), st);
+            return launch_stream<AK, 2, kMapped>(a, most(32), st);
         case 2: return launch_tile<AK, 128, 64, 2, 2, 2, kMapped>(a, st);
         default: return launch_tile<AK, 256, 128, 4, 2, AK == 4 ? 3 : 2, kMapped>(a, st);
     }
@@ -1048,7 +1118,7 @@ using namespace mfq;
 extern "C" size_t mfq_hip_mx_scaled_gemm_workspace_bytes(int act, int nrows, int cols, int M, int x_quantized) {
     if ((act != 4 && act != 6) || nrows <= 0 || cols <= 0 || cols % 32 != 0 || M <= 0) return 0;
     const MxsPlan p = plan_linear(act, nrows, cols, M);
-    size_t n = x_quantized || (p.kind == 0 && static_cast<int64_t>(M) * cols <= kFuseValues) ? 0 : quantized_bytes(act, cols, M);
+    size_t n = x_quantized || p.kind == 0 ? 0 : quantized_bytes(act, cols, M);
     if (p.splits > 1) n += static_cast<size_t>(p.splits) * M * nrows * 4;
     return n;
 }
@@ -1075,7 +1145,7 @@ extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scale
     if (x_scales) {
         a.xv = static_cast<const uint8_t *>(x);
         a.xs = static_cast<const uint8_t *>(x_scales);
-    } else if (p.kind == 0 && static_cast<int64_t>(M) * cols <= kFuseValues) {
+    } else if (p.kind == 0) {
         a.xraw = x;
         a.x_wide = pieces(x, x_dtype, ldx, M);
         a.x_dtype = x_dtype;
@@ -1123,10 +1193,8 @@ extern "C" int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int
     MFQ_REQUIRE(T * R == 1 || ldy >= (glu ? out_per_expert / 2 : out_per_expert), MFQ_ERR_INVALID, "mx_moe_matmul: ldy=%lld", static_cast<long long>(ldy));
     MFQ_REQUIRE(static_cast<int64_t>(out_per_expert) * (cols / 2) < (1ll << 32) - 256 && x_rows * mx_row_bytes(act, cols) < (1ll << 32) - 256,
                 MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: an expert of %d x %d, %d rows of activations", out_per_expert, cols, x_rows);
-    const int nmac = (cols / 32 + 7) / 8;
     if (!ids_dst) {
         MFQ_REQUIRE(T * R <= 65535, MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: %d pairs without a route map", T * R);
-        MFQ_REQUIRE(nmac * mx_macro_bytes(act) <= 64 * 1024, MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: %d columns without a route map", cols);
     } else {
         MFQ_REQUIRE(ceil_div(T * R, 16) + E <= 65535 || plan_mapped(static_cast<int64_t>(T) * R, E) > 1, MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: %d experts, %d pairs", E, T * R);
     }

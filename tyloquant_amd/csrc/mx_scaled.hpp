@@ -93,7 +93,7 @@ __device__ __forceinline__ float16_t mx_scale_mfma32(u32x4_t w, u32x4_t x, uint3
     }
 }
 
-// ---- quantisation of eight values of a block of 32, which lies in the four lanes of a quad --------------------------------------
+// ---- quantisation of a block of 32 values ---------------------------------------------------------------------------------------
 // Scale 2^(e - 2), e the exponent of the block's largest magnitude (both element types reach into the binade of 4), not below
 // 2^-127; elements to nearest, ties to even, those beyond the largest element (6, or 7.5) to it.  A block that holds an infinity
 // or a NaN takes the NaN scale 255 and codes of zero.
@@ -101,92 +101,89 @@ template <int PERM>
 __device__ __forceinline__ uint32_t quad_perm(uint32_t v) {
     return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), PERM, 0xF, 0xF, true));
 }
+typedef __bf16 bf16x32_t __attribute__((ext_vector_type(32)));
+typedef _Float16 half32_t __attribute__((ext_vector_type(32)));
+typedef uint32_t u32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x6_t __attribute__((ext_vector_type(6)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+
 // the scale byte of a block from the bits of its largest magnitude as an fp32
 __device__ __forceinline__ uint32_t mx_scale_of(uint32_t most) {
     const int e = static_cast<int>(most >> 23);  // of a subnormal 0: its scale is 2^-127 in any case
     return e == 255 ? 255u : static_cast<uint32_t>(max(e - 2, 0));
 }
-__device__ __forceinline__ uint32_t mx_scale_byte(const float (&v)[8]) {
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
-    most = max(most, quad_perm<0xB1>(most));
-    most = max(most, quad_perm<0x4E>(most));
-    return mx_scale_of(most);
-}
-// codes of eight values: 32 bits of E2M1, or 48 of E2M3
-template <int AK>
-__device__ __forceinline__ u32x2_t mx_codes(const float (&v)[8], uint32_t byte) {
-    u32x2_t q = {0u, 0u};
-    if constexpr (AK == 4) {
-        // the conversions divide by the power of two in the exponent field, of which 0 is 2^-127, and saturate
-        const float scale = __uint_as_float(byte << 23);
-        q.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q.x, v[0], v[1], scale, 0);
-        q.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q.x, v[2], v[3], scale, 1);
-        q.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q.x, v[4], v[5], scale, 2);
-        q.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q.x, v[6], v[7], scale, 3);
-    } else {
-        // From 1 on the three bits behind an fp32's leading one, rounded, are the code's fraction and what they carry its exponent;
-        // below 1 codes are eighths.  (The hardware converts whole blocks of one lane only.)
-        const float up = byte > 253u ? 0.f : __uint_as_float((254u - byte) << 23);  // 2^(127 - byte); 255 needs none
+// The 32 values from x[from] on; VEC: they lie on a 16-byte boundary.  q: 16 bytes of E2M1 or 24 of E2M3.  The conversions divide by the
+// power of two in the exponent field of their scale, of which 0 is 2^-127, round to nearest even and saturate.
+template <int AK, int XD, bool VEC>
+__device__ __forceinline__ void mx_quantize_block(const void *x, int64_t from, u32x6_t &q, uint32_t &byte) {
+    q = u32x6_t{};
+    if constexpr (XD == MFQ_X_F32) {
+        const float *p = static_cast<const float *>(x) + from;
+        float16_t v[2];  // even and odd columns: the order of the conversion to E2M3
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float a = fabsf(v[i]) * up;
-            const uint32_t bits = __float_as_uint(a);
-            const uint32_t high = ((bits + 0x7ffffu + ((bits >> 20) & 1u)) >> 20) - (127u * 8u - 8u);
-            const uint32_t low = static_cast<uint32_t>(__builtin_rintf(a * 8.f));
-            const uint32_t c = min(a < 1.f ? low : high, 31u) | ((__float_as_uint(v[i]) >> 26) & 32u);
-            if (i < 5) q.x |= c << (6 * i);
-            else if (i == 5) { q.x |= c << 30; q.y |= c >> 2; }
-            else q.y |= c << (6 * i - 32);
+            float4_t f;
+            if constexpr (VEC) f = reinterpret_cast<const float4_t *>(p)[i];
+            else f = float4_t{p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]};
+#pragma unroll
+            for (int t = 0; t < 4; ++t) v[t & 1][2 * i + (t >> 1)] = f[t];
         }
-    }
-    return byte == 255u ? u32x2_t{0u, 0u} : q;
-}
-// Where the codes of piece p (eight columns, lane p & 3 of its quad) go in a row of quantised activations, and what: FP4 a dword a
-// lane; FP6 8 bytes of the block's 24 for lanes 0 to 2, each with what its neighbour holds of them.
-struct MxStore {
-    u32x2_t q;
-    uint32_t at;
-    bool any;
-};
-template <int AK>
-__device__ __forceinline__ MxStore mx_place(u32x2_t q, int p) {
-    const uint32_t mac = static_cast<uint32_t>(p) >> 5, in = p & 31, j = p & 3;
-    if constexpr (AK == 4) return {q, mac * 128u + in * 4u, true};
-    const uint32_t nx = quad_perm<0xF9>(q.x), ny = quad_perm<0xF9>(q.y);  // of the next lane
-    u32x2_t o;
-    if (j == 0) o = u32x2_t{q.x, q.y | (nx << 16)};
-    else if (j == 1) o = u32x2_t{(q.x >> 16) | (q.y << 16), nx};
-    else o = u32x2_t{q.y | (nx << 16), (nx >> 16) | (ny << 16)};
-    const uint32_t block = in >> 2;
-    return {o, mac * 192u + (j < 2 ? block * 16u + j * 8u : 128u + block * 8u), j < 3};
-}
-
-// Eight consecutive values of a row as fp32; VEC: the row's pieces of eight lie on 16-byte boundaries.
-template <int XD, bool VEC>
-__device__ __forceinline__ void mx_load8(const void *x, int64_t at, float (&v)[8]) {
-    if constexpr (XD == MFQ_X_F32) {
-        const float *p = static_cast<const float *>(x) + at;
-        if constexpr (VEC) {
-            const float4_t a = *reinterpret_cast<const float4_t *>(p), b = *reinterpret_cast<const float4_t *>(p + 4);
+        uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+        for (int i = 0; i < 32; ++i) most = max(most, __float_as_uint(v[i & 1][i >> 1]) & 0x7fffffffu);
+        byte = mx_scale_of(most);
+        const float scale = __uint_as_float(byte << 23);
+        if constexpr (AK == 6) {
+            q = __builtin_bit_cast(u32x6_t, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(v[0], v[1], scale));
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = p[i];
+            static_for<4>([&](auto D) {
+                constexpr int d = D.value;
+                static_for<4>([&](auto T) {
+                    constexpr int t = T.value;
+                    q[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q[d], v[0][4 * d + t], v[1][4 * d + t], scale, t);
+                });
+            });
         }
     } else {
-        const uint16_t *p = static_cast<const uint16_t *>(x) + at;
-        if constexpr (VEC) {
-            const u32x4_t q = *reinterpret_cast<const u32x4_t *>(p);
+        const uint16_t *p = static_cast<const uint16_t *>(x) + from;
+        u32x16_t v;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = x_to_f32<XD == MFQ_X_F16>(static_cast<uint16_t>(q[i >> 1] >> (16 * (i & 1))));
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (VEC) {
+                const u32x4_t f = reinterpret_cast<const u32x4_t *>(p)[i];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) v[4 * i + t] = f[t];
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) v[4 * i + t] = p[8 * i + 2 * t] | (static_cast<uint32_t>(p[8 * i + 2 * t + 1]) << 16);
+            }
+        }
+        u16x2_t most = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t pair = v[i] & 0x7fff7fffu;
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, pair));
+        }
+        const uint32_t m = max(most.x, most.y);
+        // of fp16 the exponent as an fp32 has it, infinities and NaN with theirs
+        byte = mx_scale_of(XD == MFQ_X_BF16 ? m << 16 : m >= 0x7c00u ? 0x7f800000u : __float_as_uint(f16_to_f32(static_cast<uint16_t>(m))));
+        const float scale = __uint_as_float(byte << 23);
+        if constexpr (AK == 6) {
+            if constexpr (XD == MFQ_X_F16) q = __builtin_bit_cast(u32x6_t, __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(__builtin_bit_cast(half32_t, v), scale));
+            else q = __builtin_bit_cast(u32x6_t, __builtin_amdgcn_cvt_scalef32_pk32_fp6_bf16(__builtin_bit_cast(bf16x32_t, v), scale));
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = x_to_f32<XD == MFQ_X_F16>(p[i]);
+            static_for<4>([&](auto D) {
+                constexpr int d = D.value;
+                static_for<4>([&](auto T) {
+                    constexpr int t = T.value;
+                    const uint32_t pair = v[4 * d + t];  // by itself: a bit cast of the element reads the vector's first
+                    if constexpr (XD == MFQ_X_F16) q[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q[d], __builtin_bit_cast(half2_t, pair), scale, t);
+                    else q[d] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q[d], __builtin_bit_cast(bf16x2_t, pair), scale, t);
+                });
+            });
         }
     }
+    if (byte == 255u) q = u32x6_t{};
 }
 
 // two values rounded to a 16-bit type
