@@ -220,3 +220,262 @@ def test_moe_matmul(act, T, R, E, out, K, how):
         for gelu in (False, True):
             h = RX.mx_moe_glu(w, x.cuda(), route, act=act, routed=routed, activation=int(gelu), out_dtype=torch.float16)
             P.check(h, P.glu(want, gelu).reshape(T, R, -1), P.glu_bound(want, err, gelu).reshape(T, R, -1), "float16")
+
+
+def test_moe_slots_leave_other_cohorts_alone():
+    """A pool that holds some of the experts, in an order of its own: rows of the others' pairs stay, rows of no expert become zeros."""
+    from tyloquant_amd import runtime_moe as RM
+    from tyloquant_amd import runtime_mx as RX
+    rng = np.random.default_rng(21)
+    E, out, K, held = 9, 80, 352, [7, 2, 4]
+    w, wv = make_weight(rng, len(held) * out, K, out=out)
+    slot = np.full(E, -1, np.int32)
+    slot[held] = np.arange(len(held))
+    for T, R in ((3, 4), (50, 2), (300, 3)):
+        ids = rng.integers(-1, E, (T, R)).astype(np.int32)
+        route = RM.build_moe_route_plan(torch.from_numpy(ids).cuda(), E)
+        x = hidden(rng, T, K).to(torch.bfloat16)
+        xq = quantized(x, "MXFP6")
+        y = torch.full((T, R, out), 7.5, device="cuda")
+        RX.mx_moe_into(w, x.cuda(), route, y, act="MXFP6", slot=torch.from_numpy(slot).cuda())
+        want, err = np.full((T * R, out), 7.5), np.zeros((T * R, out))
+        flat = ids.reshape(-1)
+        want[flat < 0] = 0
+        for e in held:
+            p = np.flatnonzero(flat == e)
+            we = wv[slot[e] * out: slot[e] * out + out]
+            want[p], err[p] = xq[p // R] @ we.T, P.sum_bound(xq[p // R], we)
+        P.check(y, want.reshape(T, R, out), err.reshape(T, R, out), "float32")
+
+
+def mixed_moe(rng, E, out, K):
+    """a NINTM tensor of two MXFP4 cohorts and a NINT4 one between them"""
+    import synth
+    from oracle import mfq_oracle as O
+    from tyloquant_amd import formats as F
+    from tyloquant_amd import runtime_moe as RM
+    order = rng.permutation(E)
+    parts = [np.sort(order[: E // 2]), np.sort(order[E // 2: E - 2]), np.sort(order[E - 2:])]
+    pools, dense = [], np.zeros((E, out, K))
+    for ids, fmt in zip(parts, ("MXFP4", "NINT4", "MXFP4")):
+        if fmt == "MXFP4":
+            v, s, d = P.weight(rng, len(ids) * out, K)
+            blob = F.write_mx("MXFP4", len(ids) * out, K, v, s)
+        else:
+            t = synth.nint_random(rng, len(ids) * out, K, 4, 24, 6)
+            blob, d = O.pack_nint(t), O.dequantize_nint(t).astype(np.float64)
+        pools.append((ids.astype(np.int32), fmt, blob))
+        dense[ids] = d.reshape(len(ids), out, K)
+    return RM.NintMoeWeight.from_blob(F.nintm_blob(E, out, K, pools)), dense, parts
+
+
+@pytest.mark.parametrize("T", [4, 40, 200])
+@pytest.mark.parametrize("act", ACTS)
+def test_mixed_tensor_takes_the_quantised_path_where_it_can(act, T):
+    """NintMoeWeight.forward(act=...): MXFP4 cohorts as mx_moe_matmul, the NINT cohort as before; without act as before."""
+    from tyloquant_amd import runtime_moe as RM
+    rng = np.random.default_rng(T)
+    E, out, K, R = 12, 96, 384, 3
+    w, dense, parts = mixed_moe(rng, E, out, K)
+    ids = rng.integers(0, E, (T, R)).astype(np.int32)
+    route = RM.build_moe_route_plan(torch.from_numpy(ids).cuda(), E)
+    x = hidden(rng, T, K).to(torch.bfloat16)
+    got = w.forward(x.cuda(), route, act=act).double().cpu().numpy().reshape(T * R, out)
+    plain = w.forward(x.cuda(), route).double().cpu().numpy().reshape(T * R, out)
+    xq, x64, flat = quantized(x, act), x.double().numpy(), ids.reshape(-1)
+    for e in range(E):
+        p = np.flatnonzero(flat == e)
+        if not len(p):
+            continue
+        exact = x64[p // R] @ dense[e].T
+        if e in parts[1]:
+            assert np.array_equal(got[p], plain[p])
+        else:
+            want = xq[p // R] @ dense[e].T
+            assert (np.abs(got[p] - want) <= P.sum_bound(xq[p // R], dense[e])).all()
+        assert np.linalg.norm(plain[p] - exact) <= 1e-3 * np.linalg.norm(exact)
+
+
+@pytest.mark.parametrize("T", [1, 20, 150])
+@pytest.mark.parametrize("act", ACTS)
+def test_feed_forward_block_of_quantised_experts(act, T):
+    """nint_moe_ffn_forward(act=...): router, gate/up with its GLU, down and the weighted sum as they run together; against 64 bits
+    with the hidden rows rounded and quantised where the block does."""
+    from tyloquant_amd import formats as F
+    from tyloquant_amd import runtime_moe as RM
+    rng = np.random.default_rng(T + 1)
+    E, H, W, R = 10, 352, 160, 4
+    ids = rng.permutation(E)
+    tensors, dense = [], []
+    for out, K in ((2 * W, H), (H, W)):
+        pools, d = [], np.zeros((E, out, K))
+        for part in (np.sort(ids[:6]), np.sort(ids[6:])):
+            v, s, dv = P.weight(rng, len(part) * out, K)
+            pools.append((part.astype(np.int32), "MXFP4", F.write_mx("MXFP4", len(part) * out, K, v, s)))
+            d[part] = dv.reshape(len(part), out, K)
+        tensors.append(RM.NintMoeWeight.from_blob(F.nintm_blob(E, out, K, pools)))
+        dense.append(d)
+    x = hidden(rng, T, H).to(torch.bfloat16)
+    logits = torch.from_numpy(rng.standard_normal((T, E)).astype(np.float32))
+    out, chosen, weights = RM.nint_moe_ffn_forward(*tensors, x.cuda(), logits.cuda(), R, normalize=True, act=act)
+    chosen, weights = chosen.cpu().numpy(), weights.double().cpu().numpy()
+    route = RM.build_moe_route_plan(torch.from_numpy(chosen).cuda(), E)
+    hid = tensors[0].forward_glu(x.cuda(), route, act=act).cpu()          # fp16, as the block makes it
+    xq = quantized(x, act)
+    want_h, err_h, want, err = np.zeros((T, R, W)), np.zeros((T, R, W)), np.zeros((T, H)), np.zeros((T, H))
+    for t in range(T):
+        for r in range(R):
+            e = chosen[t, r]
+            y, b = xq[t: t + 1] @ dense[0][e].T, P.sum_bound(xq[t: t + 1], dense[0][e])
+            want_h[t, r], err_h[t, r] = P.glu(y)[0], P.glu_bound(y, b)[0]
+            hq = quantized(hid[t, r: r + 1], act)
+            want[t] += weights[t, r] * (hq @ dense[1][e].T)[0]
+            err[t] += abs(weights[t, r]) * P.sum_bound(hq, dense[1][e])[0]
+    P.check(hid, want_h, err_h, "float16")
+    # the weighted sum: R products and sums in fp32, each off by half a step of a partial sum
+    err += (R + 1) * 2.0 ** -23 * (np.abs(want) + err)
+    P.check(out, want, err + 1e-6 * np.abs(want).max(), "float32")
+
+
+# ---- graphs, streams, borders ------------------------------------------------------------------------------------------
+def test_captured_calls_replay():
+    """Linear (fused, few rows, tiles with K split, gated), pairs and routed experts in one graph, replayed between eager work, against
+    eager calls; a first use of a weight under capture is refused."""
+    from tyloquant_amd import runtime_moe as RM
+    from tyloquant_amd import runtime_mx as RX
+    rng = np.random.default_rng(31)
+    w, _ = make_weight(rng, 512, 2048)
+    pool, _ = make_weight(rng, 8 * 128, 288, out=128)
+    x = [torch.randn(m, 2048, device="cuda", dtype=torch.bfloat16) for m in (1, 9, 40)]
+    xe = [torch.randn(t, 288, device="cuda", dtype=torch.bfloat16) for t in (2, 100)]
+    routes_ = [RM.build_moe_route_plan(torch.from_numpy(routes(rng, t, 2, 8, "dropped")).cuda(), 8) for t in (2, 100)]
+
+    def step():
+        y = [RX.mx_scaled_matmul(w, v, act="MXFP6") for v in x] + [RX.mx_scaled_glu(w, x[2], act="MXFP4")]
+        y += [RX.mx_moe_matmul(pool, v, r, act="MXFP4") for v, r in zip(xe, routes_)]
+        return y + [RX.mx_quantize(x[1], "MXFP6").dequantize(torch.bfloat16)]
+
+    eager = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(4):
+        for v in x + xe:
+            v.copy_(torch.randn(v.shape, device="cuda"))
+        eager = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, held)), k
+    fresh, _ = make_weight(rng, 64, 256)
+    with pytest.raises(RuntimeError, match="laid_scales"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            RX.mx_scaled_matmul(fresh, torch.zeros(1, 256, device="cuda", dtype=torch.bfloat16))
+    assert RX.mx_scaled_matmul(fresh, torch.zeros(1, 256, device="cuda", dtype=torch.bfloat16)).shape == (1, 64)
+
+
+def test_two_streams_and_repeated_calls_agree():
+    """The same weight from two streams at once (each call has scratch of its own) gives the bits of one call alone."""
+    from tyloquant_amd import runtime_mx as RX
+    rng = np.random.default_rng(33)
+    w, _ = make_weight(rng, 1024, 1440)
+    xs = [torch.randn(m, 1440, device="cuda", dtype=torch.float16) for m in (1, 12, 70, 500)]
+    alone = [RX.mx_scaled_matmul(w, x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for k in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([RX.mx_scaled_matmul(w, x) for x in xs])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for ys in got for a, b in zip(ys, alone))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 16, 32, 50, 130])
+def test_nothing_behind_the_results_is_written(rows):
+    """The C call with a row stride above the results and rows behind the last; a workspace with no room for pieces of K."""
+    from tyloquant_amd import _lib as L
+    from tyloquant_amd.runtime import _stream
+    rng = np.random.default_rng(rows)
+    out, K, ldy = 102, 1440, 109
+    w, wv = make_weight(rng, out, K)
+    x = hidden(rng, rows, K).to(torch.bfloat16)
+    xd, xq = x.cuda(), quantized(x, "MXFP4")
+    want, err = xq @ wv.T, P.sum_bound(xq, wv)
+    lib = L.lib()
+    need = lib.mfq_hip_mx_scaled_gemm_workspace_bytes(4, out, K, rows, 0)
+    least = 0 if need == 0 else -(-rows * 6 * 128 // 256) * 256 + -(-rows // 32) * 6 * 256
+    for room in {need, least}:
+        for dtype, code in ((torch.float32, L.X_F32), (torch.bfloat16, L.X_BF16)):
+            y = torch.full((rows + 2, ldy), -3.0, dtype=dtype, device="cuda")
+            ws = torch.empty(max(room, 16), dtype=torch.uint8, device="cuda")
+            L.check(lib.mfq_hip_mx_scaled_gemm_rows(w.values.data_ptr(), w.laid_scales().data_ptr(), out, K, 0, out, 4, xd.data_ptr(), L.X_BF16, K, None,
+                                                    rows, 0, 0, y.data_ptr(), code, ldy, ws.data_ptr(), room, _stream()))
+            P.check(y[:rows, :out], want, err, str(dtype)[6:])
+            assert (y[rows:] == -3).all() and (y[:, out:] == -3).all()
+    if need:
+        rc = lib.mfq_hip_mx_scaled_gemm_rows(w.values.data_ptr(), w.laid_scales().data_ptr(), out, K, 0, out, 4, xd.data_ptr(), L.X_BF16, K, None,
+                                             rows, 0, 0, y.data_ptr(), code, ldy, ws.data_ptr(), least - 1, _stream())
+        assert rc == L.ERR_WORKSPACE
+
+
+def test_long_rows():
+    """K past what the LDS holds of activations, for one row, a few and two tiles; offsets of a tensor of many rows."""
+    from tyloquant_amd import runtime_mx as RX
+    rng = np.random.default_rng(41)
+    for out, K, ms in ((20, 70016, (1, 3, 20)), (70000, 64, (1, 5, 40))):
+        w, wv = make_weight(rng, out, K)
+        for m in ms:
+            x = hidden(rng, m, K).to(torch.bfloat16)
+            for act in ACTS:
+                xq = quantized(x, act)
+                P.check(RX.mx_scaled_matmul(w, x.cuda(), act=act), xq @ wv.T, P.sum_bound(xq, wv), "float32", L2)
+
+
+def test_refusals_of_the_host_layer():
+    from tyloquant_amd import runtime_moe as RM
+    from tyloquant_amd import runtime_mx as RX
+    from tyloquant_amd.runtime_mx import MxRows, MxWeight
+    rng = np.random.default_rng(43)
+    w, _ = make_weight(rng, 64, 256, out=32)
+    x = torch.zeros(3, 256, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="MXFP4 or MXFP6"):
+        RX.mx_quantize(x, "MXFP8")
+    with pytest.raises(ValueError, match="divisible by 32"):
+        RX.mx_quantize(x[:, :40])
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        RX.mx_quantize(x.double())
+    with pytest.raises(ValueError, match="current GPU"):
+        RX.mx_quantize(x.cpu())
+    with pytest.raises(ValueError, match="width 128 != neuron length 256"):
+        RX.mx_scaled_matmul(w, x[:, :128])
+    with pytest.raises(ValueError, match="width 128 != neuron length 256"):
+        RX.mx_scaled_matmul(w, RX.mx_quantize(x[:, :128]))
+    with pytest.raises(ValueError, match="MXFP4 or MXFP6"):
+        RX.mx_scaled_matmul(w, x, act="MXFP8")
+    with pytest.raises(TypeError, match="results are"):
+        RX.mx_scaled_matmul(w, x, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="16-bit type"):
+        RX.mx_scaled_glu(w, x, out_dtype=torch.float32)
+    with pytest.raises(IndexError):
+        RX.mx_scaled_matmul(w, x, expert=2)
+    route = RM.build_moe_route_plan(torch.zeros(3, 2, dtype=torch.int32, device="cuda"), 2)
+    with pytest.raises(ValueError, match="3 rows for 3 tokens of 2 routes"):
+        RX.mx_moe_matmul(w, x, route, routed=True)
+    with pytest.raises(ValueError, match="2 experts, a route plan for 3"):
+        RX.mx_moe_matmul(w, x, RM.build_moe_route_plan(route.ids, 3))
+    with pytest.raises(ValueError, match="uint8"):
+        MxRows("MXFP4", torch.zeros(3, 128, device="cuda"), torch.zeros(256, device="cuda"), (3, 256))
+    with pytest.raises(ValueError, match="must be contiguous uint8"):
+        MxRows("MXFP6", torch.zeros(3, 128, device="cuda", dtype=torch.uint8), torch.zeros(256, device="cuda", dtype=torch.uint8), (3, 256))
+    v8, s8 = torch.zeros(128, 128, device="cuda", dtype=torch.uint8), torch.zeros(1, 1, device="cuda", dtype=torch.uint8)
+    with pytest.raises(ValueError, match="use mx_matmul"):
+        RX.mx_scaled_matmul(MxWeight.from_tensors("MXFP8", v8, s8), x[:, :128])
+    with pytest.raises(ValueError, match="values .* and scales"):
+        MxWeight.from_tensors("MXFP4", v8, s8)

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
         wv[i] = static_cast<uint32_t>(neuron(i >> 1, row) * wrow) + 16u * (piece ^ mx_key(row));
     }
     const uint32_t wsv = mx_scale_at(a.row0 + expert * a.nrows + neuron(NB == 2 ? lane >> 5 : 0, (lane >> 1) & 15), nmac) + 4u * (lane & 1);
-    // rows of a mapped tile lie anywhere: the window is all of them (under 4 GB, the host sees to it); else the block's own
+    // rows of a mapped tile lie anywhere: the window is all of them (under 2 GB, the host sees to it); else the block's own
     const int64_t base = MODE == kLinear ? m0 : 0;
     const int span = MODE == kLinear ? rows : a.M;
     const __amdgpu_buffer_rsrc_t xwin = wave_window(a.xv + base * xrow, static_cast<uint32_t>(span * xrow));
@@ -551,6 +551,10 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
 // the squares of a step are multiplied the fragments of the next are read; before the last step the macro has been read, its stage
 // takes the macro R further on: one barrier a macro.  The 16-byte pieces of a line are turned by (row / 2) & 7 (FP6's second part: by
 // (row / 4) & 3), with which the four passes of a read meet every bank once.
+// What bounds it is the way of the operands from L2 to LDS and into L2: 16384 x 10240 at 4096 rows takes 372 us on the 256 x 256 tile, 286 us
+// without its copies, 297 without its products, 180 with copies of the same two macros again and again (all in L2); the clock falls to
+// 1.8 GHz meanwhile.  Tried and no faster: activations through registers half a macro out of step, copies and LDS reads between the
+// squares one by one, lines asked for two to five macros ahead (a compute unit's requests are answered in their order).
 // Lines of 64 bytes, half a macro a stage and twice as many stages, were slower (17408 x 5120 at 8192 rows: 635 us where whole lines in two
 // stages of 16 x 16 squares had taken 475): a request fetches lines of 128 bytes.
 template <int AK, int BN, int BM, int R>
@@ -1132,7 +1136,7 @@ extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scale
     MFQ_REQUIRE(row0 >= 0 && nrows > 0 && static_cast<int64_t>(row0) + nrows <= rows, MFQ_ERR_INVALID, "mx_scaled_gemm_rows: rows %d + %d of %d", row0, nrows, rows);
     MFQ_REQUIRE(!glu || nrows % 2 == 0, MFQ_ERR_INVALID, "mx_scaled_gemm_rows: gate and up in %d rows", nrows);
     MFQ_REQUIRE(M == 1 || ldy >= (glu ? nrows / 2 : nrows), MFQ_ERR_INVALID, "mx_scaled_gemm_rows: ldy=%lld < %d", static_cast<long long>(ldy), glu ? nrows / 2 : nrows);
-    MFQ_REQUIRE(static_cast<int64_t>(nrows) * (cols / 2) < (1ll << 32) - 256, MFQ_ERR_UNSUPPORTED, "mx_scaled_gemm_rows: %d x %d weights", nrows, cols);
+    MFQ_REQUIRE(static_cast<int64_t>(nrows) * (cols / 2) < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx_scaled_gemm_rows: %d x %d weights", nrows, cols);
     const hipStream_t st = as_stream(stream);
     a.wv += static_cast<int64_t>(row0) * (cols / 2);
     a.row0 = row0;
@@ -1191,7 +1195,7 @@ extern "C" int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int
                 "mx_moe_matmul: %d rows are not %d experts of %d", rows, E, out_per_expert);
     MFQ_REQUIRE(!glu || out_per_expert % 2 == 0, MFQ_ERR_INVALID, "mx_moe_matmul: gate and up in %d rows", out_per_expert);
     MFQ_REQUIRE(T * R == 1 || ldy >= (glu ? out_per_expert / 2 : out_per_expert), MFQ_ERR_INVALID, "mx_moe_matmul: ldy=%lld", static_cast<long long>(ldy));
-    MFQ_REQUIRE(static_cast<int64_t>(out_per_expert) * (cols / 2) < (1ll << 32) - 256 && x_rows * mx_row_bytes(act, cols) < (1ll << 32) - 256,
+    MFQ_REQUIRE(static_cast<int64_t>(out_per_expert) * (cols / 2) < (1ll << 31) && x_rows * mx_row_bytes(act, cols) < (1ll << 31),
                 MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: an expert of %d x %d, %d rows of activations", out_per_expert, cols, x_rows);
     if (!ids_dst) {
         MFQ_REQUIRE(T * R <= 65535, MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: %d pairs without a route map", T * R);

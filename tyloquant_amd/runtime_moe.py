@@ -132,9 +132,7 @@ class ForeignCohort:
         from .runtime_vq import NvqsWeight, nepq_hadamard
         lib, dev = L.lib(), x2.device
         if self._slot is None:
-            slot = np.full(n_experts, -1, dtype=np.int32)
-            slot[self.expert_ids[self.live]] = np.arange(len(self.expert_ids), dtype=np.int32)[self.live]
-            self._slot = torch.from_numpy(slot).to(dev)
+            self.slots(n_experts, dev)
             if self.linears:
                 self._wtab = torch.tensor([q.weight.data.data_ptr() for q in self.linears], dtype=torch.int64, device=dev)
         common = (_ptr(self._slot), n_experts)
@@ -158,6 +156,24 @@ class ForeignCohort:
                 L.check(lib.mfq_hip_nvqs_gemv_pairs(C.byref(w0.desc), _ptr(self._wtab), None, self.out, *common, *tail))
             else:
                 L.check(lib.mfq_hip_nvq_gemv_pairs(C.byref(w0.desc), _ptr(self._wtab), *common, *tail))
+
+    def scaled_capable(self) -> bool:
+        """Whether matmul_scaled takes this cohort: a native MXFP4 pool."""
+        return self.mx is not None and self.mx.kind == 4
+
+    def slots(self, n_experts: int, device) -> torch.Tensor:
+        """place of every expert of the tensor in this cohort, -1 for those of others (device int32 [n_experts])"""
+        if self._slot is None:
+            slot = np.full(n_experts, -1, dtype=np.int32)
+            slot[self.expert_ids[self.live]] = np.arange(len(self.expert_ids), dtype=np.int32)[self.live]
+            self._slot = torch.from_numpy(slot).to(device)
+        return self._slot
+
+    def matmul_scaled(self, x, route: MoeRoutePlan, out: torch.Tensor, act: str, routed: bool, glu=False, activation: int = L.GLU_SILU) -> None:
+        """out[t, r] = W[ids[t, r]] . q(x) for the pairs routed to this cohort, activations quantised to `act`: one launch for any batch,
+        nothing read back (mfq_hip_mx_moe_matmul)."""
+        from .runtime_mx import mx_moe_into
+        mx_moe_into(self.mx, x, route, out, act, routed, glu, activation, self.slots(route.n_experts, out.device))
 
     def pairs_capable(self) -> bool:
         """Whether matmul_pairs takes this cohort: every family has the launch; NEPQ1 experts must be whole row-blocks."""
@@ -278,7 +294,7 @@ class NintMoeWeight:
             out[torch.from_numpy(c.expert_ids[c.live].astype(np.int64)).to(out.device)] = c.dequantize()[mask]
         return out
 
-    def _add_foreign(self, x2: torch.Tensor, routed: bool, route: MoeRoutePlan, out: torch.Tensor) -> None:
+    def _add_foreign(self, x2: torch.Tensor, routed: bool, route: MoeRoutePlan, out: torch.Tensor, act: str | None = None) -> None:
         """The rows of the pairs routed to experts of other families: per expert, gather its activation rows, multiply
         on that family's kernels, scatter into `out` [T, R, out_per_expert]; reads the routing table on the host.  A
         decode step (up to ForeignCohort.PAIRS_MAX pairs) instead takes one launch per cohort over all pairs, with the
@@ -286,6 +302,14 @@ class NintMoeWeight:
         T, R = route.tokens, route.routes
         flat = out.view(T * R, self.out_per_expert)
         walk = list(self.foreign)
+        if act is not None:                      # native MXFP4 pools against quantised rows: one launch each, whatever the batch
+            scaled = [c for c in walk if c.scaled_capable()]
+            if len(scaled) > 1:
+                from .runtime_mx import mx_quantize
+                xq = mx_quantize(x2, act)
+            for c in scaled:
+                c.matmul_scaled(x2 if len(scaled) == 1 else xq, route, out, act, routed)
+                walk.remove(c)
         if T * R <= ForeignCohort.PAIRS_MAX:     # a decode step: one launch per cohort, nothing read back
             for c in [c for c in walk if c.pairs_capable()]:
                 c.matmul_pairs(self.n_experts, x2, routed, route.ids, T, R, flat)
@@ -304,9 +328,10 @@ class NintMoeWeight:
                 src = pairs if routed else torch.from_numpy(t_idx.astype(np.int64)).to(out.device)
                 flat[pairs] = c.matmul(local, x2.index_select(0, src))
 
-    def forward(self, x: torch.Tensor, route: MoeRoutePlan) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, route: MoeRoutePlan, act: str | None = None) -> torch.Tensor:
         """NintMoeWeight::forward (cpp_runtime/mfq_decode.cpp:2908-3071): x is [T, K] (shared by the
-        routes of a token) or [T, R, K] (routed input); returns fp32 [T, R, out_per_expert]."""
+        routes of a token) or [T, R, K] (routed input); returns fp32 [T, R, out_per_expert].  act: "MXFP4" or "MXFP6" quantises
+        the activations of native MXFP4 cohorts and multiplies the codes (mx_moe_matmul); other cohorts take them as they are."""
         T, R = route.tokens, route.routes
         routed = x.dim() == 3
         if x.shape[-1] != self.neuron_len or x.shape[0] != T or (routed and x.shape[1] != R):
@@ -315,8 +340,11 @@ class NintMoeWeight:
         if x2.stride(-1) != 1:
             x2 = x2.contiguous()
         if not self.pools:                              # no NINT cohort at all: every row comes from the host loop
-            out = torch.zeros((T, R, self.out_per_expert), dtype=torch.float32, device=x.device)
-            self._add_foreign(x2, routed, route, out)
+            if act is not None and self._all_scaled():      # every row is written: by its cohort, or zeros where the id is none
+                out = torch.empty((T, R, self.out_per_expert), dtype=torch.float32, device=x.device)
+            else:
+                out = torch.zeros((T, R, self.out_per_expert), dtype=torch.float32, device=x.device)
+            self._add_foreign(x2, routed, route, out, act)
             return out
         out = torch.empty((T, R, self.out_per_expert), dtype=torch.float32, device=x.device)
         mapped = route.ids_dst is not None
@@ -334,17 +362,23 @@ class NintMoeWeight:
             _ptr(route.tile_bounds) if mapped else None, _ptr(route.tile_experts) if mapped else None,
             _ptr(out), self.out_per_expert, _ptr(ws), need, _stream()))
         if self.foreign:
-            self._add_foreign(x2, routed, route, out)
+            self._add_foreign(x2, routed, route, out, act)
         return out
 
     __call__ = forward
 
+    def _all_scaled(self) -> bool:
+        """Whether native MXFP4 cohorts alone hold the tensor's experts, every one of them."""
+        return not self.pools and all(c.scaled_capable() for c in self.foreign) and \
+            len({int(e) for c in self.foreign for e in c.expert_ids[c.live]}) == self.n_experts
+
     def forward_glu(self, x: torch.Tensor, route: MoeRoutePlan, activation: int = L.GLU_SILU,
-                    out_dtype=torch.float16) -> torch.Tensor:
+                    out_dtype=torch.float16, act: str | None = None) -> torch.Tensor:
         """act(gate) * up of the routed gate/up projection as 16-bit [T, R, out_per_expert / 2]
         (NintMoeWeight::forward_glu_output, cpp_runtime/mfq_decode.cpp:3073-3127): one pass of the mapped prefill
         kernels with the GLU in their epilogue; the two-call form (forward, then moe_glu) where the library
-        declines -- no route map, a cohort without a prefill body, unaligned activations."""
+        declines -- no route map, a cohort without a prefill body, unaligned activations.  act: as in forward; where
+        MXFP4 cohorts hold every expert the GLU is in the epilogue of their product."""
         T, R = route.tokens, route.routes
         routed = x.dim() == 3
         if x.shape[-1] != self.neuron_len or x.shape[0] != T or (routed and x.shape[1] != R):
@@ -352,6 +386,15 @@ class NintMoeWeight:
         if self.out_per_expert % 2:
             raise RuntimeError("fused gate/up GLU needs an even number of neurons per expert")
         W = self.out_per_expert // 2
+        if act is not None and self._all_scaled():
+            hidden = torch.empty((T, R, W), dtype=out_dtype, device=x.device)
+            x2 = x.reshape(-1, self.neuron_len)
+            if len(self.foreign) > 1:
+                from .runtime_mx import mx_quantize
+                x2 = mx_quantize(x2, act)
+            for c in self.foreign:
+                c.matmul_scaled(x2, route, hidden, act, routed, True, activation)
+            return hidden
         if route.ids_dst is not None and self.out_per_expert % 32 == 0 and not self.foreign:
             x2 = x.reshape(-1, self.neuron_len)
             if x2.stride(-1) != 1:
@@ -370,7 +413,7 @@ class NintMoeWeight:
                     return hidden
                 if rc != L.ERR_UNSUPPORTED:
                     L.check(rc)
-        return moe_glu(self.forward(x, route), out_dtype, activation)
+        return moe_glu(self.forward(x, route, act), out_dtype, activation)
 
     def decode_capable(self, shared: NintWeight | None = None, tokens: int = 1, routes: int = 1, swiglu=False) -> bool:
         """Whether forward_decode takes these cohorts, this shared tensor and this many (token, route) pairs: the
@@ -466,9 +509,10 @@ def moe_weighted_reduce(pair: torch.Tensor, weights: torch.Tensor, shared: torch
 
 def nint_moe_ffn_forward(gate_up: NintMoeWeight, down: NintMoeWeight, x: torch.Tensor, router_logits: torch.Tensor,
                          top_k: int, use_sigmoid=False, use_sqrt_softplus=False, normalize=False,
-                         delayed_softmax=False, router_bias=None, router_scale=1.0, shared=None):
+                         delayed_softmax=False, router_bias=None, router_scale=1.0, shared=None, act=None):
     """cpp_runtime/mfq_decode.cpp:3394-3416.  `shared` = (gate_up NintWeight [2W, H], down NintWeight [H, W]) of the
-    shared expert, added ungated (cpp_runtime/mfq_decode.cpp:11077-11080).  Returns (out, ids, weights)."""
+    shared expert, added ungated (cpp_runtime/mfq_decode.cpp:11077-11080).  act: "MXFP4" or "MXFP6" quantises the activations of
+    native MXFP4 cohorts, those of the block and the hidden ones (NintMoeWeight.forward).  Returns (out, ids, weights)."""
     if gate_up.n_experts != down.n_experts or gate_up.out_per_expert != 2 * down.neuron_len or \
             down.out_per_expert != gate_up.neuron_len:
         raise RuntimeError("incompatible fused gate_up/down NINTM tensors")
@@ -497,8 +541,8 @@ def nint_moe_ffn_forward(gate_up: NintMoeWeight, down: NintMoeWeight, x: torch.T
                 return moe_weighted_reduce(dn[:n].view(T_, R_, -1), w, dn[n:]), ids, w
             hidden, sh_hidden = both[:n].view(T_, R_, -1), both[n:]
     if hidden is None:
-        hidden = gate_up.forward_glu(x, route)
-    dn = down.forward(hidden, route)
+        hidden = gate_up.forward_glu(x, route, act=act)
+    dn = down.forward(hidden, route, act)
     sh = None
     if shared is not None:
         sh = nint_matmul(sdn, moe_swiglu(nint_matmul(sgu, x)) if sh_hidden is None else sh_hidden)

@@ -30,7 +30,7 @@ class MxWeight:
         self.n_experts = self.rows // self.out
         self.data = values                      # the device tensor other weights call `data`
         self._ws = _Workspace()
-        self._laid = None
+        self._laid, self._needs = None, {}
 
     @property
     def payload_bytes(self) -> int:
@@ -123,94 +123,120 @@ def _scale_bytes(rows: int, K: int) -> int:
     return -(-rows // 32) * -(-K // 256) * 256
 
 
+def _out_dtype(dtype) -> int:
+    code = _OUT.get(dtype)
+    if code is None:
+        raise TypeError(f"results are float32, bfloat16 or float16, not {dtype}")
+    return code
+
+
+def _act_kind(act: str) -> int:
+    kind = _ACT.get(act)
+    if kind is None:
+        raise ValueError(f"activations are quantised to MXFP4 or MXFP6, not {act}")
+    return kind
+
+
 class MxRows:
     """Quantised activations [.., neuron_len]: value bytes of rows of whole groups of 256 columns (uint8 [M, 128 or 192 a group], the
     layout of mfq_hip_mx_quantize_rows) and E8M0 scales (uint8, by 32 rows and groups); `shape` is that of the rows before
     quantisation."""
 
     def __init__(self, dtype: str, values: torch.Tensor, scales: torch.Tensor, shape):
-        kind, self.shape = _act_kind(dtype), tuple(shape)
-        if not self.shape or self.shape[-1] <= 0 or self.shape[-1] % 32:
-            raise ValueError(f"{dtype} columns must be divisible by 32: {self.shape}")
-        self.dtype, self.kind, self.values, self.scales = dtype, kind, values, scales
-        self.neuron_len = self.shape[-1]
-        self.rows = torch.Size(self.shape[:-1]).numel()
-        want = (self.rows, _row_bytes(kind, self.neuron_len)), (_scale_bytes(self.rows, self.neuron_len),)
+        shape = tuple(shape)
+        kind = _act_kind(dtype)
+        if not shape or shape[-1] <= 0 or shape[-1] % 32:
+            raise ValueError(f"{dtype} columns must be divisible by 32: {shape}")
+        rows = torch.Size(shape[:-1]).numel()
+        want = (rows, _row_bytes(kind, shape[-1])), (_scale_bytes(rows, shape[-1]),)
         if values.dtype != torch.uint8 or scales.dtype != torch.uint8 or (tuple(values.shape), tuple(scales.shape)) != want or \
                 not (values.is_contiguous() and scales.is_contiguous()) or values.device != scales.device:
-            raise ValueError(f"{dtype} rows of {self.shape}: values {tuple(values.shape)} and scales {tuple(scales.shape)} must be contiguous uint8 "
+            raise ValueError(f"{dtype} rows of {shape}: values {tuple(values.shape)} and scales {tuple(scales.shape)} must be contiguous uint8 "
                              f"{want[0]} and {want[1]} on one device")
+        self._set(dtype, kind, values, scales, shape, rows)
+
+    def _set(self, dtype, kind, values, scales, shape, rows):
+        self.dtype, self.kind, self.values, self.scales, self.shape = dtype, kind, values, scales, shape
+        self.rows, self.neuron_len = rows, shape[-1]
+        return self
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         """element x scale in fp32, rounded once to `dtype`."""
+        code = _out_dtype(dtype)
         out = torch.empty(self.shape, dtype=dtype, device=self.values.device)
         if self.rows:
-            L.check(L.lib().mfq_hip_mx_dequant_quantized(self.kind, _ptr(self.values), _ptr(self.scales), self.rows, self.neuron_len,
-                                                         _out_dtype(dtype), _ptr(out), self.neuron_len, _stream()))
+            _here(out)
+            L.check(L.lib().mfq_hip_mx_dequant_quantized(self.kind, self.values.data_ptr(), self.scales.data_ptr(), self.rows, self.neuron_len, code,
+                                                         out.data_ptr(), self.neuron_len, _stream()))
         return out
 
 
-def _out_dtype(dtype) -> int:
-    try:
-        return _OUT[dtype]
-    except KeyError:
-        raise TypeError(f"results are float32, bfloat16 or float16, not {dtype}") from None
-
-
-def _act_kind(act: str) -> int:
-    try:
-        return _ACT[act]
-    except KeyError:
-        raise ValueError(f"activations are quantised to MXFP4 or MXFP6, not {act}") from None
+def _here(t: torch.Tensor) -> None:
+    """Launches go to the current device's stream: refuse tensors that are elsewhere."""
+    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors must be on the current GPU (cuda:{torch._C._cuda_getDevice()}), got {t.device}")
 
 
 def _raw_rows(x: torch.Tensor, K: int) -> torch.Tensor:
-    """[rows, K] with neighbouring columns side by side"""
+    """[rows, K] with neighbouring columns side by side, and rows that do not lie on one another (a broadcast one is copied)"""
     if x.dtype not in _OUT:
         raise TypeError(f"activations must be float32, bfloat16 or float16, got {x.dtype}")
-    return _as_2d(x, K)
+    x2 = _as_2d(x, K)
+    return x2 if x2.shape[0] == 1 or x2.stride(0) >= K else x2.contiguous()
 
 
 def mx_quantize(x: torch.Tensor, dtype: str = "MXFP4") -> MxRows:
     """Rows of bf16, fp16 or fp32 [..., K] to MXFP4 or MXFP6 with a power of two for every 32 columns: 2^(e - 2), e = the
     exponent of the block's largest magnitude; elements to nearest, ties to even, the largest where they are beyond it.  A block
     that holds an infinity or a NaN becomes NaN."""
-    kind, K = _act_kind(dtype), x.shape[-1]
+    kind, shape = _act_kind(dtype), tuple(x.shape)
+    K = shape[-1] if shape else 0
     if K % 32 or K == 0:
         raise ValueError(f"{dtype} columns must be divisible by 32, got {K}")
     x2 = _raw_rows(x, K)
+    _here(x2)
     M = x2.shape[0]
-    values = torch.empty((M, _row_bytes(kind, K)), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_scale_bytes(M, K), dtype=torch.uint8, device=x.device)
+    values = torch.empty((M, _row_bytes(kind, K)), dtype=torch.uint8, device=x2.device)
+    scales = torch.empty(_scale_bytes(M, K), dtype=torch.uint8, device=x2.device)
     if M:
-        L.check(L.lib().mfq_hip_mx_quantize_rows(kind, _ptr(x2), _OUT[x2.dtype], x2.stride(0), M, K, _ptr(values), _ptr(scales), _stream()))
-    return MxRows(dtype, values, scales, x.shape)
+        L.check(L.lib().mfq_hip_mx_quantize_rows(kind, x2.data_ptr(), _OUT[x2.dtype], x2.stride(0), M, K, values.data_ptr(), scales.data_ptr(), _stream()))
+    return MxRows.__new__(MxRows)._set(dtype, kind, values, scales, shape, M)
 
 
 def _operand(x, K: int, act: str):
-    """(kind, tensor, x_dtype, row stride, scales or None, rows, shape, device) of activations that come quantised or not"""
+    """(kind, tensor, x_dtype, row stride, scales or None, rows, shape) of activations that come quantised or not"""
     if isinstance(x, MxRows):
         if x.neuron_len != K:
             raise ValueError(f"activation width {x.neuron_len} != neuron length {K}")
-        return x.kind, x.values, 0, 0, x.scales, x.rows, x.shape, x.values.device
+        return x.kind, x.values, 0, 0, x.scales, x.rows, x.shape
     x2 = _raw_rows(x, K)
-    return _act_kind(act), x2, _OUT[x2.dtype], x2.stride(0), None, x2.shape[0], x.shape, x.device
+    return _act_kind(act), x2, _OUT[x2.dtype], x2.stride(0), None, x2.shape[0], x.shape
+
+
+def _result_dtype(w: MxWeight, rows: int, glu: int, out_dtype) -> int:
+    code = _out_dtype(out_dtype)
+    if glu and (rows % 2 or code == L.X_F32):
+        raise ValueError(f"{w.dtype}: a gated product takes a 16-bit type and as many gate as up rows, not {out_dtype} and {rows} rows")
+    return code
 
 
 def _scaled(w: MxWeight, x, act: str, expert: int, glu: int, activation: int, out_dtype) -> torch.Tensor:
     row0, nrows = w._rows(expert)
     K = w.neuron_len
-    kind, x2, xd, ldx, xs, M, shape, dev = _operand(x, K, act)
-    yd = _out_dtype(out_dtype)
-    if glu and (nrows % 2 or yd == L.X_F32):
-        raise ValueError(f"a gated product takes a 16-bit type and gate and up rows, not {out_dtype} and {nrows} rows")
+    kind, x2, xd, ldx, xs, M, shape = _operand(x, K, act)
+    yd = _result_dtype(w, nrows, glu, out_dtype)
     laid = w.laid_scales()
+    _here(x2)
+    _here(w.values)
     width = nrows // 2 if glu else nrows
-    y = torch.empty((M, width), dtype=out_dtype, device=dev)
+    y = torch.empty((M, width), dtype=out_dtype, device=x2.device)
     if M:
         lib = L.lib()
-        need = lib.mfq_hip_mx_scaled_gemm_workspace_bytes(kind, nrows, K, M, xs is not None)
-        ws = borrow(need, dev)
+        key = (kind, nrows, M, xs is None)
+        need = w._needs.get(key)
+        if need is None:
+            need = w._needs[key] = lib.mfq_hip_mx_scaled_gemm_workspace_bytes(kind, nrows, K, M, xs is not None)
+        ws = borrow(need, x2.device)
         L.check(lib.mfq_hip_mx_scaled_gemm_rows(w.values.data_ptr(), laid.data_ptr(), w.rows, K, row0, nrows, kind, x2.data_ptr(), xd, ldx,
                                                 _ptr(xs), M, glu, activation, y.data_ptr(), yd, width, _ptr(ws), need if ws is not None else 0,
                                                 _stream()))
@@ -228,37 +254,51 @@ def mx_scaled_glu(w: MxWeight, x, act: str = "MXFP6", activation: int = L.GLU_SI
     return _scaled(w, x, act, expert, 1, int(activation), out_dtype)
 
 
-def _moe(w: MxWeight, x, route, act: str, routed: bool, glu: int, activation: int, out_dtype, slot=None, out=None) -> torch.Tensor:
+def mx_moe_into(w: MxWeight, x, route, out: torch.Tensor, act: str = "MXFP6", routed: bool = False, glu: bool = False, activation: int = L.GLU_SILU,
+                slot: torch.Tensor | None = None) -> torch.Tensor:
+    """The rows out[t, r] of the pairs whose expert `w` holds: expert e is the pool's slot[e] (device int32, -1 for the experts of other
+    pools, whose rows are left as they are), or e itself without `slot`; rows of ids that are none become zeros."""
     K, T, R = w.neuron_len, route.tokens, route.routes
-    kind, x2, xd, ldx, xs, M, shape, dev = _operand(x, K, act)
+    kind, x2, xd, ldx, xs, M, _ = _operand(x, K, act)
     if M != (T * R if routed else T):
         raise ValueError(f"MoE activations must be [{'tokens * routes' if routed else 'tokens'}, K]: {M} rows for {T} tokens of {R} routes")
     if slot is None and w.n_experts != route.n_experts:
         raise ValueError(f"{w.n_experts} experts, a route plan for {route.n_experts}")
-    yd = _out_dtype(out_dtype)
-    if glu and (w.out % 2 or yd == L.X_F32):
-        raise ValueError(f"a gated product takes a 16-bit type and gate and up rows, not {out_dtype} and {w.out} rows")
+    if slot is not None and (slot.dtype != torch.int32 or slot.numel() != route.n_experts or not slot.is_contiguous()):
+        raise ValueError("expert slots must be int32 [experts] side by side")
+    yd = _result_dtype(w, w.out, glu, out.dtype)
     laid = w.laid_scales()
     width = w.out // 2 if glu else w.out
-    y = torch.empty((T, R, width), dtype=out_dtype, device=dev) if out is None else out
+    if tuple(out.shape) != (T, R, width) or not out.is_contiguous():
+        raise ValueError(f"MoE results must be contiguous {(T, R, width)}, got {tuple(out.shape)}")
+    for t in (x2, w.values, out, route.ids):
+        _here(t)
     if T * R:
         lib = L.lib()
         mapped = route.ids_dst is not None
-        need = lib.mfq_hip_mx_moe_workspace_bytes(kind, K, M, mapped, xs is not None)
-        ws = borrow(need, dev)
+        key = (kind, M, mapped, xs is None)
+        need = w._needs.get(key)
+        if need is None:
+            need = w._needs[key] = lib.mfq_hip_mx_moe_workspace_bytes(kind, K, M, mapped, xs is not None)
+        ws = borrow(need, x2.device)
         L.check(lib.mfq_hip_mx_moe_matmul(w.values.data_ptr(), laid.data_ptr(), w.rows, K, w.out, _ptr(slot), route.n_experts, kind, x2.data_ptr(), xd,
                                           ldx, _ptr(xs), int(routed), route.ids.data_ptr(), T, R, _ptr(route.ids_dst) if mapped else None,
-                                          _ptr(route.expert_bounds) if mapped else None, glu, activation, y.data_ptr(), yd, width, _ptr(ws),
+                                          _ptr(route.expert_bounds) if mapped else None, int(glu), int(activation), out.data_ptr(), yd, width, _ptr(ws),
                                           need if ws is not None else 0, _stream()))
-    return y
+    return out
+
+
+def _moe_out(w: MxWeight, route, width: int, out_dtype) -> torch.Tensor:
+    _out_dtype(out_dtype)
+    return torch.empty((route.tokens, route.routes, width), dtype=out_dtype, device=w.values.device)
 
 
 def mx_moe_matmul(w: MxWeight, x, route, act: str = "MXFP6", routed: bool = False, out_dtype=torch.float32) -> torch.Tensor:
     """[tokens, routes, out] of a pool of MXFP4 experts: every (token, route) pair of `route` (build_moe_route_plan) against its expert;
-    zeros where the id is none.  x has a row per token, with `routed` one per pair."""
-    return _moe(w, x, route, act, routed, 0, 0, out_dtype)
+    zeros where the id is none.  x has a row per token, with `routed` one per pair; quantised to `act` by the call, or MxRows."""
+    return mx_moe_into(w, x, route, _moe_out(w, route, w.out, out_dtype), act, routed)
 
 
 def mx_moe_glu(w: MxWeight, x, route, act: str = "MXFP6", activation: int = L.GLU_SILU, routed: bool = False, out_dtype=torch.bfloat16) -> torch.Tensor:
     """act(gate) * up of a pool of gate/up tensors, 16-bit [tokens, routes, out / 2]."""
-    return _moe(w, x, route, act, routed, 1, int(activation), out_dtype)
+    return mx_moe_into(w, x, route, _moe_out(w, route, w.out // 2, out_dtype), act, routed, True, activation)
