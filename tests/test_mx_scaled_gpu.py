@@ -438,6 +438,39 @@ def test_long_rows():
                 P.check(RX.mx_scaled_matmul(w, x.cuda(), act=act), xq @ wv.T, P.sum_bound(xq, wv), "float32", L2)
 
 
+def test_cpp_runtime_linear():
+    """mfq_rt_linear_forward_scaled on a loaded MXFP4 blob: the bits of the Python layer; its refusals."""
+    import ctypes as C
+    from pathlib import Path
+    from tyloquant_amd import _lib as L
+    from tyloquant_amd import formats as F
+    from tyloquant_amd import runtime as R
+    from tyloquant_amd import runtime_mx as RX
+    rt = C.CDLL(str(Path(R.__file__).resolve().parent / "lib" / "libmfq_runtime.so"))
+    rt.mfq_rt_last_error.restype = C.c_char_p
+    rt.mfq_rt_load_quant_linear.argtypes = [C.c_char_p, C.c_char_p, C.c_size_t, C.POINTER(C.c_void_p)]
+    rt.mfq_rt_free_quant_linear.argtypes = [C.c_void_p]
+    rt.mfq_rt_linear_forward_scaled.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int,
+                                                C.c_void_p]
+    rng = np.random.default_rng(51)
+    v, s, _ = P.weight(rng, 160, 1440)
+    blob = F.write_mx("MXFP4", 160, 1440, v, s)
+    lin = R.load_quant_linear("MXFP4", blob).weight
+    h = C.c_void_p()
+    assert rt.mfq_rt_load_quant_linear(b"MXFP4", blob, len(blob), C.byref(h)) == 0
+    for m in (200, 1, 9):
+        x = hidden(rng, m, 1440).to(torch.float16).cuda()
+        for glu, act in ((0, 4), (1, 6)):
+            y = torch.empty((m, 80 if glu else 160), dtype=torch.bfloat16, device="cuda")
+            assert rt.mfq_rt_linear_forward_scaled(h, act, x.data_ptr(), L.X_F16, 1440, m, glu, 0, y.data_ptr(), L.X_BF16, None) == 0
+            torch.cuda.synchronize()
+            call = RX.mx_scaled_glu if glu else RX.mx_scaled_matmul
+            assert torch.equal(y, call(lin, x, act="MXFP4" if act == 4 else "MXFP6", out_dtype=torch.bfloat16))
+    assert rt.mfq_rt_linear_forward_scaled(h, 8, x.data_ptr(), L.X_F16, 1440, 9, 0, 0, y.data_ptr(), L.X_BF16, None) != 0
+    assert b"kind 8" in rt.mfq_rt_last_error()
+    rt.mfq_rt_free_quant_linear(h)
+
+
 def test_refusals_of_the_host_layer():
     from tyloquant_amd import runtime_moe as RM
     from tyloquant_amd import runtime_mx as RX

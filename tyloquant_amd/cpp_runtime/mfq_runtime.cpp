@@ -772,6 +772,23 @@ void mx_dequantize(const MxWeight &w, int expert, float *out, mfq_stream_t strea
     abi_check(mfq_hip_mx_dequant_rows(w.kind, w.values.get(), w.scales.get(), static_cast<int>(w.rows), static_cast<int>(w.cols),
                                       row0, nrows, MFQ_X_F32, out, w.cols, stream));
 }
+void MxWeight::lay_scales(mfq_stream_t stream) const {
+    if (laid.get()) return;
+    if (kind != 4) fail("products of microscaled operands take MXFP4 weights, not " + dtype);
+    laid.ensure(static_cast<size_t>(mfq_hip_mx_scale_bytes(rows, static_cast<int>(cols))));
+    abi_check(mfq_hip_mx_lay_scales(scales.get(), rows, static_cast<int>(cols), laid.get(), stream));
+    hip_check(hipStreamSynchronize(hs(stream)), "mx scales");
+}
+void mx_scaled_matmul(const MxWeight &w, int expert, int act, const void *x, int x_dtype, int64_t ldx, int M, bool glu, int activation, void *y,
+                      int y_dtype, mfq_stream_t stream) {
+    if (expert < 0 || expert >= w.n_experts()) fail(w.dtype + ": expert index out of range");
+    w.lay_scales(stream);
+    const int nrows = static_cast<int>(w.out_per_expert), cols = static_cast<int>(w.cols);
+    const size_t need = mfq_hip_mx_scaled_gemm_workspace_bytes(act, nrows, cols, M, 0);
+    w.workspace.ensure(need);
+    abi_check(mfq_hip_mx_scaled_gemm_rows(w.values.get(), w.laid.get(), static_cast<int>(w.rows), cols, expert * nrows, nrows, act, x, x_dtype, ldx,
+                                          nullptr, M, glu, activation, y, y_dtype, glu ? nrows / 2 : nrows, w.workspace.get(), need, stream));
+}
 void nvq_dequantize(const NvqWeight &w, float *out, mfq_stream_t stream) {
     if (w.streams) {
         abi_check(mfq_hip_nvqs_dequant_f32(&w.sdesc, w.data.get(), out, w.sdesc.neuron_len, stream));
@@ -1841,6 +1858,14 @@ int mfq_rt_linear_reserve(void *h, int max_M) {
 }
 int mfq_rt_linear_forward(void *h, const void *x, int x_dtype, int64_t ldx, int M, float *y, void *stream) {
     return guard([&] { static_cast<QuantLinear *>(h)->forward(x, x_dtype, ldx, M, y, stream); });
+}
+int mfq_rt_linear_forward_scaled(void *h, int act, const void *x, int x_dtype, int64_t ldx, int M, int glu, int activation, void *y, int y_dtype,
+                                 void *stream) {
+    return guard([&] {
+        const QuantLinear *q = static_cast<QuantLinear *>(h);
+        if (!q->mx) fail("products of microscaled operands need an MXFP4 tensor");
+        mx_scaled_matmul(*q->mx, 0, act, x, x_dtype, ldx, M, glu != 0, activation, y, y_dtype, stream);
+    });
 }
 int mfq_rt_linear_forward_glu(void *h, const void *x, int x_dtype, int64_t ldx, int M, int gelu, void *hidden, float *scratch,
                               void *stream) {

@@ -149,10 +149,13 @@ struct MxWeight {
     int64_t rows = 0, cols = 0, out_per_expert = 0;
     std::string dtype;
     DeviceBuffer values, scales;
-    mutable DeviceBuffer workspace;
+    mutable DeviceBuffer workspace, laid;  // laid: the scales as mx_scaled_matmul reads them (lay_scales)
     int64_t out() const { return out_per_expert; }
     int64_t neuron_len() const { return cols; }
     int64_t n_experts() const { return rows / out_per_expert; }
+    // Lays the scales of an MXFP4 tensor out for mx_scaled_matmul, once (1/16 of the values' bytes); waits for the stream.  The first
+    // mx_scaled_matmul does it where nobody has: call it before capturing one into a HIP graph.
+    void lay_scales(mfq_stream_t stream = nullptr) const;
     int64_t payload_bytes() const;
     static MxWeight from_blob(const std::string &dtype, const uint8_t *blob, size_t n, int64_t out_per_expert = 0,
                               mfq_stream_t stream = nullptr);
@@ -161,6 +164,10 @@ bool is_mx_linear_dtype(const std::string &dtype);
 void mx_matmul(const MxWeight &w, int expert, const void *x, int x_dtype, int64_t ldx, int M, float *y,
                mfq_stream_t stream = nullptr);
 void mx_dequantize(const MxWeight &w, int expert, float *out, mfq_stream_t stream = nullptr);
+// y[M, out] = q(x) . W^T of an MXFP4 tensor, activations (bf16, fp16 or fp32) quantised to kind act = 4 (MXFP4) or 6 (MXFP6); with glu
+// y[M, out / 2] = act(gate) * up in 16 bits (gate rows first).  y_dtype MFQ_X_*.  No counterpart in the reference.
+void mx_scaled_matmul(const MxWeight &w, int expert, int act, const void *x, int x_dtype, int64_t ldx, int M, bool glu, int activation, void *y,
+                      int y_dtype, mfq_stream_t stream = nullptr);
 struct NepqWeight {
     mfq_nepq_desc desc{};    // lane-major layout (NEPQ1-S, NEPQ1-L)
     mfq_nvqs_desc sdesc{};   // streams read in place (NEPQ0-S, NEPQ0-L: the product tables of NPQ0): `streams` set
