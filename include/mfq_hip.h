@@ -526,8 +526,9 @@ int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scales, int rows
  * [experts * out_per_expert, cols].  ids device int32 [T, R]; ids outside [0, E) give rows of zeros.  expert_slot (device, [E]) =
  * place of an expert in the pool, -1 for those of other pools, whose rows are left as they are; null: the experts as they lie.
  * ids_dst and expert_bounds from mfq_hip_moe_route_map (any tile_m), or both null: every pair by itself, for a handful of tokens.
- * x has T rows, with routed_input T * R.  Workspace: the quantised rows of calls with a route map. */
-size_t mfq_hip_mx_moe_workspace_bytes(int act, int cols, int x_rows, int mapped, int x_quantized);
+ * x has T rows, with routed_input T * R (x_rows of the query).  Workspace of calls with a route map (mapped != 0): the quantised rows
+ * and a table of the experts' tiles. */
+size_t mfq_hip_mx_moe_workspace_bytes(int act, int cols, int x_rows, int n_pairs, int E, int mapped, int x_quantized);
 int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int rows, int cols, int out_per_expert, const int32_t *expert_slot,
                           int E, int act, const void *x, int x_dtype, int64_t ldx, const void *x_scales, int routed_input,
                           const int32_t *ids, int T, int R, const int32_t *ids_dst, const int32_t *expert_bounds, int glu,

@@ -31,8 +31,11 @@ def test_sizes(lib):
     assert lib.mfq_hip_mx_scaled_gemm_workspace_bytes(4, 4096, 4096, 16, 1) == 0
     assert lib.mfq_hip_mx_scaled_gemm_workspace_bytes(4, 4096, 4096, 16, 0) == 16 * 2048 + 16 * 256
     assert lib.mfq_hip_mx_scaled_gemm_workspace_bytes(5, 4096, 4096, 16, 0) == 0
-    assert lib.mfq_hip_mx_moe_workspace_bytes(6, 288, 100, 1, 0) == 100 * 384 + 128 * 16
-    assert lib.mfq_hip_mx_moe_workspace_bytes(6, 288, 100, 0, 0) == 0 and lib.mfq_hip_mx_moe_workspace_bytes(6, 288, 100, 1, 1) == 0
+    # routed experts: the rows and, where tiles serve the call, 16 bytes for each of at most so many and one
+    moe = lib.mfq_hip_mx_moe_workspace_bytes
+    assert moe(6, 288, 100, 200, 64, 1, 0) == 100 * 384 + 128 * 16 and moe(6, 288, 100, 200, 64, 1, 1) == 0
+    assert moe(6, 288, 100, 1600, 32, 1, 1) == 16 * (25 + 32 + 1) and moe(6, 288, 100, 1600, 32, 1, 0) == 100 * 384 + 128 * 16 + 16 * 58
+    assert moe(6, 288, 100, 200, 64, 0, 0) == 0
 
 
 def test_quantize_checks(lib):
@@ -86,7 +89,7 @@ def moe(lib, **k):
     (dict(E=5), "INVALID", "not 5 experts"), (dict(out=60), "INVALID", "not 4 experts"), (dict(act=8), "INVALID", "kind 8"),
     (dict(glu=1, yd=L.X_F16, out=64, activation=9), "INVALID", "activation=9"), (dict(ldy=10), "INVALID", "ldy"), (dict(ldx=255), "INVALID", "ldx"),
     (dict(T=1 << 16, R=1 << 15), "INVALID", "tokens"), (dict(T=40000, R=2), "UNSUPPORTED", "without a route map"),
-    (dict(dst=A, bounds=A), "WORKSPACE", "workspace"), (dict(dst=A, bounds=A, ws=ODD, nbytes=1 << 20), "WORKSPACE", "unaligned"),
+    (dict(dst=A, bounds=A), "WORKSPACE", "workspace"), (dict(T=1000, xs=A, dst=A, bounds=A), "WORKSPACE", "workspace"), (dict(dst=A, bounds=A, ws=ODD, nbytes=1 << 20), "WORKSPACE", "unaligned"),
     (dict(T=1 << 20, R=16, routed=1, dst=A, bounds=A, ws=A, nbytes=1 << 40), "UNSUPPORTED", "rows of activations")])
 def test_moe_checks(lib, change, status, word):
     assert moe(lib, **change) == getattr(L, "ERR_" + status), _msg(lib)

@@ -146,7 +146,7 @@ _SIGS = {
     "mfq_hip_mx_scaled_gemm_workspace_bytes": (sz, [C.c_int] * 5),
     "mfq_hip_mx_scaled_gemm_rows": (C.c_int, [vp, vp] + [C.c_int] * 5 + [vp, C.c_int, i64, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, i64, vp,
                                     sz, vp]),
-    "mfq_hip_mx_moe_workspace_bytes": (sz, [C.c_int] * 5),
+    "mfq_hip_mx_moe_workspace_bytes": (sz, [C.c_int] * 7),
     "mfq_hip_mx_moe_matmul": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, C.c_int, vp, C.c_int, i64, vp, C.c_int, vp, C.c_int,
                               C.c_int, vp, vp, C.c_int, C.c_int, vp, C.c_int, i64, vp, sz, vp]),
     "mfq_hip_mx_gemm_rows": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, C.c_int, i64, C.c_int, vp, i64,

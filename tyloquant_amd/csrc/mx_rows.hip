@@ -13,7 +13,11 @@ constexpr int kUnits = 4;  // pieces of eight values a thread of the dequantizer
 // threads a block and E2M3 rounded in integers, 2048 x 12288 bf16 to MXFP6 took 23.0 us.
 template <int AK, int XD, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const void *__restrict__ x, int64_t ldx, int M, int K, uint8_t *__restrict__ values,
-                                                          uint8_t *__restrict__ scales) {
+                                                          uint8_t *__restrict__ scales, MxTileTable table) {
+    if (table.out && blockIdx.x == gridDim.x - 1) {
+        mx_write_table(table, threadIdx.x);
+        return;
+    }
     const int nmac = mx_macros(K), per_row = nmac * 8;  // blocks behind the last column are zeros
     const int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int64_t row = static_cast<int64_t>(M) * per_row < (1ll << 31) ? static_cast<int64_t>(static_cast<uint32_t>(u) / static_cast<uint32_t>(per_row)) : u / per_row;
@@ -113,26 +117,27 @@ __global__ __launch_bounds__(256) void mx_lay_scales_kernel(const uint8_t *__res
 }
 
 template <int AK, int XD>
-void launch_quantize(const void *x, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(M) * (mx_macros(K) * 8), 256)));
+void launch_quantize(const void *x, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st, const MxTileTable &table) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(M) * (mx_macros(K) * 8), 256) + (table.out ? 1 : 0)));
     const int64_t per16 = XD == MFQ_X_F32 ? 4 : 8;
     if (reinterpret_cast<uintptr_t>(x) % 16 == 0 && (M == 1 || ldx % per16 == 0))
-        hipLaunchKernelGGL((mx_quantize_kernel<AK, XD, true>), grid, dim3(256), 0, st, x, ldx, M, K, values, scales);
+        hipLaunchKernelGGL((mx_quantize_kernel<AK, XD, true>), grid, dim3(256), 0, st, x, ldx, M, K, values, scales, table);
     else
-        hipLaunchKernelGGL((mx_quantize_kernel<AK, XD, false>), grid, dim3(256), 0, st, x, ldx, M, K, values, scales);
+        hipLaunchKernelGGL((mx_quantize_kernel<AK, XD, false>), grid, dim3(256), 0, st, x, ldx, M, K, values, scales, table);
 }
 
 }  // namespace
 
-int mx_quantize_launch(int kind, const void *x, int x_dtype, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st) {
+int mx_quantize_launch(int kind, const void *x, int x_dtype, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st, const MxTileTable *table) {
+    const MxTileTable t = table ? *table : MxTileTable{};
     if (kind == 4) {
-        if (x_dtype == MFQ_X_F32) launch_quantize<4, MFQ_X_F32>(x, ldx, M, K, values, scales, st);
-        else if (x_dtype == MFQ_X_F16) launch_quantize<4, MFQ_X_F16>(x, ldx, M, K, values, scales, st);
-        else launch_quantize<4, MFQ_X_BF16>(x, ldx, M, K, values, scales, st);
+        if (x_dtype == MFQ_X_F32) launch_quantize<4, MFQ_X_F32>(x, ldx, M, K, values, scales, st, t);
+        else if (x_dtype == MFQ_X_F16) launch_quantize<4, MFQ_X_F16>(x, ldx, M, K, values, scales, st, t);
+        else launch_quantize<4, MFQ_X_BF16>(x, ldx, M, K, values, scales, st, t);
     } else {
-        if (x_dtype == MFQ_X_F32) launch_quantize<6, MFQ_X_F32>(x, ldx, M, K, values, scales, st);
-        else if (x_dtype == MFQ_X_F16) launch_quantize<6, MFQ_X_F16>(x, ldx, M, K, values, scales, st);
-        else launch_quantize<6, MFQ_X_BF16>(x, ldx, M, K, values, scales, st);
+        if (x_dtype == MFQ_X_F32) launch_quantize<6, MFQ_X_F32>(x, ldx, M, K, values, scales, st, t);
+        else if (x_dtype == MFQ_X_F16) launch_quantize<6, MFQ_X_F16>(x, ldx, M, K, values, scales, st, t);
+        else launch_quantize<6, MFQ_X_BF16>(x, ldx, M, K, values, scales, st, t);
     }
     return check_launch("mx_quantize_rows");
 }

@@ -586,17 +586,17 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
     int tn = 0, tm = 0, expert = 0, first = 0, rows, m0 = 0;
     if constexpr (MODE == kMapped) {
         mxs_zero_rows(a, blockIdx.x, gridDim.x, tid, NW * 64);
-        const int total = mxs_total_tiles(a, BM, lane) * tiles_n, per = (total + 7) / 8;
+        const int total = __builtin_amdgcn_readfirstlane(a.table[0].x) * tiles_n, per = (total + 7) / 8;
         const int t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);  // an XCD takes neighbouring tiles
         if (t >= total || static_cast<int>(blockIdx.x >> 3) >= per) return;
-        int t0, count;
-        mxs_find_tile(a, BM, lane, t / tiles_n, expert, t0, count);
-        const int in = t - t0 * tiles_n;  // of the expert's tiles, those of the same neurons side by side
+        const i32x4v_t at = a.table[1 + t / tiles_n];
+        expert = __builtin_amdgcn_readfirstlane(at.x);
+        const int pairs = __builtin_amdgcn_readfirstlane(at.w), count = (pairs + BM - 1) / BM;
+        const int in = t - __builtin_amdgcn_readfirstlane(at.y) * tiles_n;  // of the expert's tiles, those of the same neurons side by side
         tn = in / count;
-        first = a.bounds[expert] + in % count * BM;
-        rows = min(BM, a.bounds[expert + 1] - first);
-        if (a.slot) expert = a.slot[expert];
-        expert = __builtin_amdgcn_readfirstlane(expert);
+        const int i = in % count * BM;
+        first = __builtin_amdgcn_readfirstlane(at.z) + i;
+        rows = min(BM, pairs - i);
     } else {
         if (!tile_of_block(tiles_n, (a.M + BM - 1) / BM, tn, tm)) return;
         m0 = tm * BM;
@@ -927,12 +927,16 @@ int launch_flow(const MxsArgs &a, int tiles, int busy, hipStream_t st) {
     return a.glu ? launch_flow_nb<AK, MT, 2, MODE, SMALL>(a, tiles, busy, st) : launch_flow_nb<AK, MT, 1, MODE, SMALL>(a, tiles, busy, st);
 }
 
+int tile_rows_mapped(int kind) { return kind == 2 ? 64 : 128; }
+// tiles of a call with a route map: at most
+int64_t tiles_mapped(int64_t pairs, int E, int rows) { return ceil_div(pairs, rows) + (E < pairs ? E : pairs); }
+
 template <int AK, int BN, int BM, int WN, int WM, int R, int MODE>
 int launch_tile(const MxsArgs &a, hipStream_t st) {
     using S = TileShape<AK, BN, BM, R>;
     const int width = a.glu ? a.nrows / 2 : a.nrows;
     const int64_t tiles_n = ceil_div(width, a.glu ? BN / 2 : BN);
-    const int64_t tiles_m = MODE == kMapped ? ceil_div(a.pairs, BM) + (a.E < a.pairs ? a.E : a.pairs) : ceil_div(a.M, BM);
+    const int64_t tiles_m = MODE == kMapped ? tiles_mapped(a.pairs, a.E, BM) : ceil_div(a.M, BM);
     const int64_t blocks = (tiles_n * tiles_m + 7) / 8 * 8;
     MFQ_REQUIRE(blocks < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx_scaled: %lld tiles", static_cast<long long>(blocks));
     static_assert(WN * WM * kTileOut <= R * S::STAGE && S::LDS <= static_cast<int>(kMaxDynamicLds), "results leave through the ring");
@@ -1062,7 +1066,7 @@ int run_experts(const MxsArgs &a, hipStream_t st) {
         if (int rc = launch_flow<AK, 1, kPairs, true>(a, a.pairs, a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
         return fail(MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: %d columns without a route map", a.K);
     }
-    const auto most = [&](int rows) { return static_cast<int>(ceil_div(a.pairs, rows) + (a.E < a.pairs ? a.E : a.pairs)); };
+    const auto most = [&](int rows) { return static_cast<int>(tiles_mapped(a.pairs, a.E, rows)); };
     switch (plan_mapped(a.pairs, a.E)) {
         case 0:
             if (int rc = launch_flow<AK, 1, kMapped>(a, most(16), a.E < a.pairs ? a.E : a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
@@ -1177,9 +1181,16 @@ extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scale
     return launch_join(a, st);
 }
 
-extern "C" size_t mfq_hip_mx_moe_workspace_bytes(int act, int cols, int x_rows, int mapped, int x_quantized) {
-    if ((act != 4 && act != 6) || cols <= 0 || cols % 32 != 0 || x_rows <= 0 || !mapped || x_quantized) return 0;
-    return quantized_bytes(act, cols, x_rows);
+namespace {
+size_t table_bytes(int64_t pairs, int E) {
+    const int kind = plan_mapped(pairs, E);
+    return kind < 2 ? 0 : static_cast<size_t>(tiles_mapped(pairs, E, tile_rows_mapped(kind)) + 1) * 16;
+}
+}  // namespace
+
+extern "C" size_t mfq_hip_mx_moe_workspace_bytes(int act, int cols, int x_rows, int n_pairs, int E, int mapped, int x_quantized) {
+    if ((act != 4 && act != 6) || cols <= 0 || cols % 32 != 0 || x_rows <= 0 || n_pairs <= 0 || E <= 0 || !mapped) return 0;
+    return (x_quantized ? 0 : quantized_bytes(act, cols, x_rows)) + table_bytes(n_pairs, E);
 }
 
 extern "C" int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int rows, int cols, int out_per_expert, const int32_t *expert_slot, int E, int act,
@@ -1221,15 +1232,22 @@ extern "C" int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int
         a.x_wide = pieces(x, x_dtype, ldx, x_rows);
         a.x_dtype = x_dtype;
         a.ldx = ldx;
-    } else {
-        const size_t need = quantized_bytes(act, cols, x_rows);
-        MFQ_REQUIRE(workspace && workspace_bytes >= need, MFQ_ERR_WORKSPACE, "mx_moe_matmul: workspace %zu < %zu", workspace_bytes, need);
-        MFQ_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, MFQ_ERR_WORKSPACE, "mx_moe_matmul: unaligned workspace");
+    }
+    if (ids_dst) {
+        const size_t rows_bytes = x_scales ? 0 : quantized_bytes(act, cols, x_rows), tab = table_bytes(a.pairs, E), need = rows_bytes + tab;
+        MFQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), MFQ_ERR_WORKSPACE, "mx_moe_matmul: workspace %zu < %zu", workspace_bytes, need);
+        MFQ_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, MFQ_ERR_WORKSPACE, "mx_moe_matmul: unaligned workspace");
         uint8_t *ws = static_cast<uint8_t *>(workspace);
-        uint8_t *xs = ws + ((static_cast<int64_t>(x_rows) * mx_row_bytes(act, cols) + 255) & ~static_cast<int64_t>(255));
-        if (int rc = mx_quantize_launch(act, x, x_dtype, ldx, x_rows, cols, ws, xs, st)) return rc;
-        a.xv = ws;
-        a.xs = xs;
+        const MxTileTable table = {expert_bounds, expert_slot, E, tile_rows_mapped(plan_mapped(a.pairs, E)), tab ? reinterpret_cast<i32x4v_t *>(ws + rows_bytes) : nullptr};
+        a.table = table.out;
+        uint8_t *xs = ws;
+        if (!x_scales) {
+            xs = ws + ((static_cast<int64_t>(x_rows) * mx_row_bytes(act, cols) + 255) & ~static_cast<int64_t>(255));
+            a.xv = ws;
+            a.xs = xs;
+        }
+        if (!x_scales || tab)
+            if (int rc = mx_quantize_launch(act, x, x_scales ? MFQ_X_BF16 : x_dtype, ldx, x_scales ? 0 : x_rows, cols, ws, xs, st, &table)) return rc;
     }
     return act == 4 ? run_experts<4>(a, st) : run_experts<6>(a, st);
 }

@@ -193,15 +193,56 @@ __device__ __forceinline__ uint32_t mx_pack16(float lo, float hi, int dtype) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
+// ---- tiles of routed experts ------------------------------------------------------------------------------------------------------
+// The pairs bounds[e] .. bounds[e + 1] of expert e are cut into tiles of bm rows.  The table has an entry for each tile, those of an expert side
+// by side: place of the expert in the pool, its first tile, its first pair, its number of pairs; in front of them one with their total.
+typedef int i32x4v_t __attribute__((ext_vector_type(4)));
+struct MxTileTable {
+    const int32_t *bounds, *slot;
+    int E, bm;
+    i32x4v_t *out;
+};
+// by one block of 256 threads
+__device__ __forceinline__ void mx_write_table(const MxTileTable &t, int tid) {
+    __shared__ int upto[256];
+    int before = 0;
+    for (int c = 0; c < t.E; c += 256) {
+        const int e = c + tid;
+        int place = -1, first = 0, pairs = 0;
+        if (e < t.E) {
+            place = t.slot ? t.slot[e] : e;
+            first = t.bounds[e];
+            pairs = place < 0 ? 0 : t.bounds[e + 1] - first;
+        }
+        const int n = (pairs + t.bm - 1) / t.bm;
+        upto[tid] = n;
+        __syncthreads();
+        for (int o = 1; o < 256; o <<= 1) {
+            const int v = tid >= o ? upto[tid - o] : 0;
+            __syncthreads();
+            upto[tid] += v;
+            __syncthreads();
+        }
+        const int t0 = before + upto[tid] - n;
+        for (int i = 0; i < n; ++i) t.out[1 + t0 + i] = i32x4v_t{place, t0, first, pairs};
+        before += upto[255];
+        __syncthreads();
+    }
+    if (tid == 0) t.out[0] = i32x4v_t{before, 0, 0, 0};
+}
+
 // ---- launches -----------------------------------------------------------------------------------------------------------------
 // Quantised rows in memory: values [M, mx_row_bytes], scales of mx_scale_bytes (rows behind the last are left as they are).
-int mx_quantize_launch(int kind, const void *x, int x_dtype, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st);
+// table (optional): written by one more block of the launch; M may be 0 then.
+int mx_quantize_launch(int kind, const void *x, int x_dtype, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st,
+                       const MxTileTable *table = nullptr);
 
 struct MxsArgs {
     const uint8_t *wv, *ws;  // weights: values from row row0 of the pool on, scales of the whole pool
     const uint8_t *xv, *xs;  // quantised activations
     void *y;
     const int32_t *ids, *ids_dst, *bounds, *slot;  // grouped calls: expert of a pair, pairs by expert, their bounds, place of an expert in the pool
+    const i32x4v_t *table;   // and their tiles (mx_write_table)
     const void *xraw;        // activations before quantisation, for the kernel that does it itself
     int64_t ldy, ldx;
     int K, row0, nrows;      // nrows: neurons of the tensor or of an expert

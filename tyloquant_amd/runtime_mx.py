@@ -276,10 +276,10 @@ def mx_moe_into(w: MxWeight, x, route, out: torch.Tensor, act: str = "MXFP6", ro
     if T * R:
         lib = L.lib()
         mapped = route.ids_dst is not None
-        key = (kind, M, mapped, xs is None)
+        key = (kind, M, T * R, route.n_experts, mapped, xs is None)
         need = w._needs.get(key)
         if need is None:
-            need = w._needs[key] = lib.mfq_hip_mx_moe_workspace_bytes(kind, K, M, mapped, xs is not None)
+            need = w._needs[key] = lib.mfq_hip_mx_moe_workspace_bytes(kind, K, M, T * R, route.n_experts, mapped, xs is not None)
         ws = borrow(need, x2.device)
         L.check(lib.mfq_hip_mx_moe_matmul(w.values.data_ptr(), laid.data_ptr(), w.rows, K, w.out, _ptr(slot), route.n_experts, kind, x2.data_ptr(), xd,
                                           ldx, _ptr(xs), int(routed), route.ids.data_ptr(), T, R, _ptr(route.ids_dst) if mapped else None,
