@@ -23,7 +23,7 @@ def _msg(lib):
 
 def test_sizes(lib):
     assert [lib.mfq_hip_mx_quantized_row_bytes(4, k) for k in (32, 256, 288, 4096)] == [128, 128, 256, 2048]
-    assert [lib.mfq_hip_mx_quantized_row_bytes(6, k) for k in (32, 256, 288, 4096)] == [192, 192, 384, 3072]
+    assert [lib.mfq_hip_mx_quantized_row_bytes(6, k) for k in (32, 256, 288, 2048)] == [192, 192, 384, 1536]
     assert lib.mfq_hip_mx_quantized_row_bytes(8, 256) == 0 and lib.mfq_hip_mx_quantized_row_bytes(4, 40) == 0
     assert [lib.mfq_hip_mx_scale_bytes(r, 288) for r in (1, 32, 33)] == [512, 512, 1024] and lib.mfq_hip_mx_scale_bytes(0, 256) == 0
     # a workspace that grows with the rows; none for rows that the kernel quantises itself or that come quantised
