@@ -27,7 +27,8 @@ int mfq_rt_linear_forward(void *handle, const void *x, int x_dtype, int64_t ldx,
 int mfq_rt_linear_dequantize(void *handle, float *out, void *stream);
 /* y = q(x) . W^T of an MXFP4 linear with its activations quantised to kind act = 4 (MXFP4) or 6 (MXFP6): y[M, out] of y_dtype (MFQ_X_*), or
  * with glu act(gate) * up [M, out / 2] in 16 bits (mfq_hip_mx_scaled_gemm_rows).  The first call of a handle lays its scales out and waits
- * for the stream; the workspace grows with M: make the largest call once before capturing. */
+ * for the stream (refused while it captures).  Calls of a handle share its workspace: one stream at a time; make a call of the same M once
+ * before capturing one. */
 int mfq_rt_linear_forward_scaled(void *handle, int act, const void *x, int x_dtype, int64_t ldx, int M, int glu, int activation, void *y, int y_dtype,
                                  void *stream);
 /* QuantLinear::forward_swiglu / nint_matmul_geglu (cpp_runtime/mfq_decode.cpp:9228-9240, 8462-8485) on a NINT gate/up

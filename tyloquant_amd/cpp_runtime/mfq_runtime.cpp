@@ -775,9 +775,13 @@ void mx_dequantize(const MxWeight &w, int expert, float *out, mfq_stream_t strea
 void MxWeight::lay_scales(mfq_stream_t stream) const {
     if (laid.get()) return;
     if (kind != 4) fail("products of microscaled operands take MXFP4 weights, not " + dtype);
-    laid.ensure(static_cast<size_t>(mfq_hip_mx_scale_bytes(rows, static_cast<int>(cols))));
-    abi_check(mfq_hip_mx_lay_scales(scales.get(), rows, static_cast<int>(cols), laid.get(), stream));
+    hipStreamCaptureStatus capture;
+    hip_check(hipStreamIsCapturing(hs(stream), &capture), "mx scales");
+    if (capture != hipStreamCaptureStatusNone) fail(dtype + ": lay_scales, or a first product, before a graph is captured");
+    DeviceBuffer to(static_cast<size_t>(mfq_hip_mx_scale_bytes(rows, static_cast<int>(cols))));
+    abi_check(mfq_hip_mx_lay_scales(scales.get(), rows, static_cast<int>(cols), to.get(), stream));
     hip_check(hipStreamSynchronize(hs(stream)), "mx scales");
+    laid = std::move(to);  // only what is whole is kept
 }
 void mx_scaled_matmul(const MxWeight &w, int expert, int act, const void *x, int x_dtype, int64_t ldx, int M, bool glu, int activation, void *y,
                       int y_dtype, mfq_stream_t stream) {
@@ -785,9 +789,9 @@ void mx_scaled_matmul(const MxWeight &w, int expert, int act, const void *x, int
     w.lay_scales(stream);
     const int nrows = static_cast<int>(w.out_per_expert), cols = static_cast<int>(w.cols);
     const size_t need = mfq_hip_mx_scaled_gemm_workspace_bytes(act, nrows, cols, M, 0);
-    w.workspace.ensure(need);
+    void *room = need ? w.scaled_room.room(need) : nullptr;
     abi_check(mfq_hip_mx_scaled_gemm_rows(w.values.get(), w.laid.get(), static_cast<int>(w.rows), cols, expert * nrows, nrows, act, x, x_dtype, ldx,
-                                          nullptr, M, glu, activation, y, y_dtype, glu ? nrows / 2 : nrows, w.workspace.get(), need, stream));
+                                          nullptr, M, glu, activation, y, y_dtype, glu ? nrows / 2 : nrows, room, need, stream));
 }
 void nvq_dequantize(const NvqWeight &w, float *out, mfq_stream_t stream) {
     if (w.streams) {

@@ -150,6 +150,7 @@ struct MxWeight {
     std::string dtype;
     DeviceBuffer values, scales;
     mutable DeviceBuffer workspace, laid;  // laid: the scales as mx_scaled_matmul reads them (lay_scales)
+    mutable SharedWorkspace scaled_room;   // of mx_scaled_matmul: what it needs does not only grow with the rows
     int64_t out() const { return out_per_expert; }
     int64_t neuron_len() const { return cols; }
     int64_t n_experts() const { return rows / out_per_expert; }
@@ -165,7 +166,9 @@ void mx_matmul(const MxWeight &w, int expert, const void *x, int x_dtype, int64_
                mfq_stream_t stream = nullptr);
 void mx_dequantize(const MxWeight &w, int expert, float *out, mfq_stream_t stream = nullptr);
 // y[M, out] = q(x) . W^T of an MXFP4 tensor, activations (bf16, fp16 or fp32) quantised to kind act = 4 (MXFP4) or 6 (MXFP6); with glu
-// y[M, out / 2] = act(gate) * up in 16 bits (gate rows first).  y_dtype MFQ_X_*.  No counterpart in the reference.
+// y[M, out / 2] = act(gate) * up in 16 bits (gate rows first).  y_dtype MFQ_X_*.  Calls of one weight share its workspace: one stream
+// at a time; a captured call needs one of its rows before the capture, and stays good when later ones ask for more.  No counterpart in the
+// reference.
 void mx_scaled_matmul(const MxWeight &w, int expert, int act, const void *x, int x_dtype, int64_t ldx, int M, bool glu, int activation, void *y,
                       int y_dtype, mfq_stream_t stream = nullptr);
 struct NepqWeight {
