@@ -4,9 +4,12 @@ import ctypes as C
 
 import numpy as np
 import pytest
+import torch
 
 import mx_scaled_ref as P
 from tyloquant_amd import _lib as L
+from tyloquant_amd import formats as F
+from tyloquant_amd.runtime_mx import MxWeight, mx_scaled_matmul
 
 A = C.c_void_p(0x1000)      # an aligned address that a rejected call never dereferences
 ODD = C.c_void_p(0x1001)
@@ -94,6 +97,26 @@ def moe(lib, **k):
 def test_moe_checks(lib, change, status, word):
     assert moe(lib, **change) == getattr(L, "ERR_" + status), _msg(lib)
     assert word in _msg(lib)
+
+
+def test_columns_beyond_the_tiles_offsets(lib):
+    K = (1 << 24) + 32
+    assert gemm(lib, cols=K, ldx=K, rows=2, nrows=2, M=200, ws=A, nbytes=1 << 50) == L.ERR_UNSUPPORTED and f"{K} columns" in _msg(lib)
+    assert moe(lib, cols=K, ldx=K, rows=4, out=1, ldy=1) == L.ERR_UNSUPPORTED and f"{K} columns" in _msg(lib)
+
+
+def test_scales_are_laid_where_they_are():
+    """laid_scales launches on the current GPU: a weight that is elsewhere is refused before anything runs."""
+    w = MxWeight(F.MxHeader("MXFP4", 4, 64, 256, 0, 64 * 128, 64 * 128, 64 * 8), torch.zeros(64, 128, dtype=torch.uint8), torch.zeros(64, 8, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="on the current GPU, got cpu"):
+        w.laid_scales()
+    with pytest.raises(ValueError, match="on the current GPU, got cpu"):
+        mx_scaled_matmul(w, torch.zeros(2, 256))
+
+
+def test_noted_workspaces_stay_few():
+    w = MxWeight(F.MxHeader("MXFP4", 4, 64, 256, 0, 64 * 128, 64 * 128, 64 * 8), torch.zeros(64, 128, dtype=torch.uint8), torch.zeros(64, 8, dtype=torch.uint8))
+    assert [w.note_need(m, 2 * m) for m in range(5000)] == [2 * m for m in range(5000)] and 0 < len(w._needs) <= 1024
 
 
 def test_oracle_quantiser_closed_forms():

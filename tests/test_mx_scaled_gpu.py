@@ -248,6 +248,34 @@ def test_moe_slots_leave_other_cohorts_alone():
         P.check(y, want.reshape(T, R, out), err.reshape(T, R, out), "float32")
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("T,R", [(1300, 3), (30000, 2)])
+def test_hundreds_of_experts_in_tiles(act, T, R):
+    """More experts than the block that writes the table of tiles has threads, part of them in this pool, some without rows."""
+    from tyloquant_amd import runtime_moe as RM
+    from tyloquant_amd import runtime_mx as RX
+    rng = np.random.default_rng(T + R)
+    E, out, K = 300, 40, 64
+    held = np.sort(rng.permutation(E)[:280])
+    w, wv = make_weight(rng, len(held) * out, K, out=out)
+    slot = np.full(E, -1, np.int32)
+    slot[held] = np.arange(len(held))
+    ids = np.minimum(rng.integers(-1, E, (T, R)), E - 9).astype(np.int32)      # eight experts get nothing, the one before many
+    route = RM.build_moe_route_plan(torch.from_numpy(ids).cuda(), E)
+    x = hidden(rng, T, K).to(torch.bfloat16)
+    xq = quantized(x, act)
+    want, err, flat = np.full((T * R, out), -2.5), np.zeros((T * R, out)), ids.reshape(-1)
+    want[flat < 0] = 0
+    for e in held:
+        p = np.flatnonzero(flat == e)
+        we = wv[slot[e] * out: slot[e] * out + out]
+        want[p], err[p] = xq[p // R] @ we.T, P.sum_bound(xq[p // R], we)
+    for rows in (x.cuda(), RX.mx_quantize(x.cuda(), act)):
+        y = torch.full((T, R, out), -2.5, device="cuda")
+        RX.mx_moe_into(w, rows, route, y, act=act, slot=torch.from_numpy(slot).cuda())
+        P.check(y, want.reshape(T, R, out), err.reshape(T, R, out), "float32")
+
+
 def mixed_moe(rng, E, out, K):
     """a NINTM tensor of two MXFP4 cohorts and a NINT4 one between them"""
     import synth
@@ -471,6 +499,51 @@ def test_cpp_runtime_linear():
     rt.mfq_rt_free_quant_linear(h)
 
 
+def test_cpp_runtime_capture():
+    """A first product under capture is refused and leaves the handle good; a captured one replays after calls that need more room."""
+    import ctypes as C
+    from pathlib import Path
+    from tyloquant_amd import _lib as L
+    from tyloquant_amd import formats as F
+    from tyloquant_amd import runtime as R
+    from tyloquant_amd import runtime_mx as RX
+    rt = C.CDLL(str(Path(R.__file__).resolve().parent / "lib" / "libmfq_runtime.so"))
+    rt.mfq_rt_last_error.restype = C.c_char_p
+    rt.mfq_rt_load_quant_linear.argtypes = [C.c_char_p, C.c_char_p, C.c_size_t, C.POINTER(C.c_void_p)]
+    rt.mfq_rt_free_quant_linear.argtypes = [C.c_void_p]
+    rt.mfq_rt_linear_forward_scaled.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int,
+                                                C.c_void_p]
+    rng = np.random.default_rng(53)
+    v, s, _ = P.weight(rng, 512, 2080)
+    blob = F.write_mx("MXFP4", 512, 2080, v, s)
+    lin = R.load_quant_linear("MXFP4", blob).weight
+    h = C.c_void_p()
+    assert rt.mfq_rt_load_quant_linear(b"MXFP4", blob, len(blob), C.byref(h)) == 0
+    x = [hidden(rng, m, 2080).to(torch.bfloat16).cuda() for m in (9, 40, 700)]
+    y = [torch.empty((len(t), 512), device="cuda") for t in x]
+
+    def call(i):
+        return rt.mfq_rt_linear_forward_scaled(h, 6, x[i].data_ptr(), L.X_BF16, 2080, len(x[i]), 0, 0, y[i].data_ptr(), L.X_F32,
+                                               torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        assert call(0) != 0
+        y[2].zero_()
+    assert b"before a graph is captured" in rt.mfq_rt_last_error()
+    assert call(0) == 0
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert call(0) == 0
+    for k in range(3):
+        assert call(1) == 0 and call(2) == 0
+        x[0].copy_(hidden(rng, 9, 2080))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, RX.mx_scaled_matmul(lin, b)) for a, b in zip(y, x)), k
+    del graph
+    rt.mfq_rt_free_quant_linear(h)
+
+
 def test_refusals_of_the_host_layer():
     from tyloquant_amd import runtime_moe as RM
     from tyloquant_amd import runtime_mx as RX
@@ -507,6 +580,12 @@ def test_refusals_of_the_host_layer():
         MxRows("MXFP4", torch.zeros(3, 128, device="cuda"), torch.zeros(256, device="cuda"), (3, 256))
     with pytest.raises(ValueError, match="must be contiguous uint8"):
         MxRows("MXFP6", torch.zeros(3, 128, device="cuda", dtype=torch.uint8), torch.zeros(256, device="cuda", dtype=torch.uint8), (3, 256))
+    with pytest.raises(ValueError, match="current GPU, got cpu"):
+        RX.mx_moe_into(w, x, route, torch.empty(3, 2, 32, device="cuda"), slot=torch.zeros(2, dtype=torch.int32))
+    moe, _, _ = mixed_moe(rng, 8, 64, 96)
+    for call in (moe.forward, moe.forward_glu):
+        with pytest.raises(ValueError, match="MXFP4 or MXFP6"):
+            call(torch.zeros(3, 96, device="cuda"), RM.build_moe_route_plan(route.ids, 8), act="MXFP8")
     v8, s8 = torch.zeros(128, 128, device="cuda", dtype=torch.uint8), torch.zeros(1, 1, device="cuda", dtype=torch.uint8)
     with pytest.raises(ValueError, match="use mx_matmul"):
         RX.mx_scaled_matmul(MxWeight.from_tensors("MXFP8", v8, s8), x[:, :128])

@@ -1057,7 +1057,7 @@ int run_linear(const MxsArgs &a, const MxsPlan &p, hipStream_t st) {
 // pairs) 146, 111, 80 and 65 us.
 int plan_mapped(int64_t pairs, int E) {
     static const int forced = tune_env("MFQ_MXS_TILE", 0);
-    if (forced) return forced - 1;
+    if (forced > 0) return forced < 4 ? forced - 1 : 3;
     const int64_t mean = ceil_div(pairs, E);
     return mean <= 10 ? 0 : mean < 160 ? 2 : 3;
 }
@@ -1081,6 +1081,8 @@ int run_experts(const MxsArgs &a, hipStream_t st) {
     }
 }
 
+constexpr int kMaxCols = 1 << 24;  // with which the 256 quantised rows of a tile lie within 32 bits
+
 // Checks shared by both entry points; fills what they have in common.
 int check_common(MxsArgs &a, const char *who, const void *values, const void *scales, int64_t rows, int cols, int act, const void *x, int x_dtype, int64_t ldx,
                  const void *x_scales, int64_t x_rows, int glu, int activation, const void *y, int y_dtype, int64_t ldy) {
@@ -1101,6 +1103,7 @@ int check_common(MxsArgs &a, const char *who, const void *values, const void *sc
     MFQ_REQUIRE(!glu || (y_dtype != MFQ_X_F32 && (activation == MFQ_GLU_SILU || activation == MFQ_GLU_GELU)), MFQ_ERR_INVALID,
                 "%s: a gated product takes a 16-bit type and activation 0 or 1, not y_dtype=%d activation=%d", who, y_dtype, activation);
     MFQ_REQUIRE(reinterpret_cast<uintptr_t>(y) % (y_dtype == MFQ_X_F32 ? 4 : 2) == 0, MFQ_ERR_INVALID, "%s: unaligned y", who);
+    MFQ_REQUIRE(cols <= kMaxCols, MFQ_ERR_UNSUPPORTED, "%s: %d columns", who, cols);
     MFQ_REQUIRE(mx_scale_bytes(rows, cols) < (1ll << 32) - 512 && mx_scale_bytes(x_rows, cols) < (1ll << 32) - 512, MFQ_ERR_UNSUPPORTED,
                 "%s: %lld rows of weights, %lld of activations, %d columns", who, static_cast<long long>(rows), static_cast<long long>(x_rows), cols);
     a.wv = static_cast<const uint8_t *>(values);

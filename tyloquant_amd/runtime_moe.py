@@ -173,6 +173,7 @@ class ForeignCohort:
         """out[t, r] = W[ids[t, r]] . q(x) for the pairs routed to this cohort, activations quantised to `act`: one launch for any batch,
         nothing read back (mfq_hip_mx_moe_matmul)."""
         from .runtime_mx import mx_moe_into
+        self.mx.laid_scales()                    # before anything of a first call under capture, which it refuses
         mx_moe_into(self.mx, x, route, out, act, routed, glu, activation, self.slots(route.n_experts, out.device))
 
     def pairs_capable(self) -> bool:
@@ -332,6 +333,9 @@ class NintMoeWeight:
         """NintMoeWeight::forward (cpp_runtime/mfq_decode.cpp:2908-3071): x is [T, K] (shared by the
         routes of a token) or [T, R, K] (routed input); returns fp32 [T, R, out_per_expert].  act: "MXFP4" or "MXFP6" quantises
         the activations of native MXFP4 cohorts and multiplies the codes (mx_moe_matmul); other cohorts take them as they are."""
+        if act is not None:
+            from .runtime_mx import check_act
+            check_act(act)
         T, R = route.tokens, route.routes
         routed = x.dim() == 3
         if x.shape[-1] != self.neuron_len or x.shape[0] != T or (routed and x.shape[1] != R):
@@ -379,6 +383,9 @@ class NintMoeWeight:
         kernels with the GLU in their epilogue; the two-call form (forward, then moe_glu) where the library
         declines -- no route map, a cohort without a prefill body, unaligned activations.  act: as in forward; where
         MXFP4 cohorts hold every expert the GLU is in the epilogue of their product."""
+        if act is not None:
+            from .runtime_mx import check_act
+            check_act(act)
         T, R = route.tokens, route.routes
         routed = x.dim() == 3
         if x.shape[-1] != self.neuron_len or x.shape[0] != T or (routed and x.shape[1] != R):

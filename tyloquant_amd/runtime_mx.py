@@ -56,6 +56,7 @@ class MxWeight:
         if self._laid is None:
             if self.kind != 4:
                 raise ValueError(f"products of microscaled operands take MXFP4 weights, not {self.dtype}: use mx_matmul")
+            _here(self.scales)
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError(f"{self.dtype}: call laid_scales() before a graph is captured")
             laid = torch.empty(_scale_bytes(self.rows, self.neuron_len), dtype=torch.uint8, device=self.scales.device)
@@ -63,6 +64,13 @@ class MxWeight:
             torch.cuda.current_stream().synchronize()   # later calls may come on other streams
             self._laid = laid
         return self._laid
+
+    def note_need(self, key, need: int) -> int:
+        """Remembers the workspace of a call's sizes; a program whose every call has other sizes starts over now and then."""
+        if len(self._needs) >= 1024:
+            self._needs.clear()
+        self._needs[key] = need
+        return need
 
     @staticmethod
     def from_blob(dtype: str, blob, device="cuda", out: int | None = None) -> "MxWeight":
@@ -130,7 +138,8 @@ def _out_dtype(dtype) -> int:
     return code
 
 
-def _act_kind(act: str) -> int:
+def check_act(act: str) -> int:
+    """kind of a type that activations are quantised to; refuses others"""
     kind = _ACT.get(act)
     if kind is None:
         raise ValueError(f"activations are quantised to MXFP4 or MXFP6, not {act}")
@@ -144,7 +153,7 @@ class MxRows:
 
     def __init__(self, dtype: str, values: torch.Tensor, scales: torch.Tensor, shape):
         shape = tuple(shape)
-        kind = _act_kind(dtype)
+        kind = check_act(dtype)
         if not shape or shape[-1] <= 0 or shape[-1] % 32:
             raise ValueError(f"{dtype} columns must be divisible by 32: {shape}")
         rows = torch.Size(shape[:-1]).numel()
@@ -173,7 +182,9 @@ class MxRows:
 
 def _here(t: torch.Tensor) -> None:
     """Launches go to the current device's stream: refuse tensors that are elsewhere."""
-    if not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+    if not t.is_cuda:
+        raise ValueError(f"tensors must be on the current GPU, got {t.device}")
+    if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"tensors must be on the current GPU (cuda:{torch._C._cuda_getDevice()}), got {t.device}")
 
 
@@ -189,7 +200,7 @@ def mx_quantize(x: torch.Tensor, dtype: str = "MXFP4") -> MxRows:
     """Rows of bf16, fp16 or fp32 [..., K] to MXFP4 or MXFP6 with a power of two for every 32 columns: 2^(e - 2), e = the
     exponent of the block's largest magnitude; elements to nearest, ties to even, the largest where they are beyond it.  A block
     that holds an infinity or a NaN becomes NaN."""
-    kind, shape = _act_kind(dtype), tuple(x.shape)
+    kind, shape = check_act(dtype), tuple(x.shape)
     K = shape[-1] if shape else 0
     if K % 32 or K == 0:
         raise ValueError(f"{dtype} columns must be divisible by 32, got {K}")
@@ -210,7 +221,7 @@ def _operand(x, K: int, act: str):
             raise ValueError(f"activation width {x.neuron_len} != neuron length {K}")
         return x.kind, x.values, 0, 0, x.scales, x.rows, x.shape
     x2 = _raw_rows(x, K)
-    return _act_kind(act), x2, _OUT[x2.dtype], x2.stride(0), None, x2.shape[0], x.shape
+    return check_act(act), x2, _OUT[x2.dtype], x2.stride(0), None, x2.shape[0], x.shape
 
 
 def _result_dtype(w: MxWeight, rows: int, glu: int, out_dtype) -> int:
@@ -235,7 +246,7 @@ def _scaled(w: MxWeight, x, act: str, expert: int, glu: int, activation: int, ou
         key = (kind, nrows, M, xs is None)
         need = w._needs.get(key)
         if need is None:
-            need = w._needs[key] = lib.mfq_hip_mx_scaled_gemm_workspace_bytes(kind, nrows, K, M, xs is not None)
+            need = w.note_need(key, lib.mfq_hip_mx_scaled_gemm_workspace_bytes(kind, nrows, K, M, xs is not None))
         ws = borrow(need, x2.device)
         L.check(lib.mfq_hip_mx_scaled_gemm_rows(w.values.data_ptr(), laid.data_ptr(), w.rows, K, row0, nrows, kind, x2.data_ptr(), xd, ldx,
                                                 _ptr(xs), M, glu, activation, y.data_ptr(), yd, width, _ptr(ws), need if ws is not None else 0,
@@ -271,7 +282,7 @@ def mx_moe_into(w: MxWeight, x, route, out: torch.Tensor, act: str = "MXFP6", ro
     width = w.out // 2 if glu else w.out
     if tuple(out.shape) != (T, R, width) or not out.is_contiguous():
         raise ValueError(f"MoE results must be contiguous {(T, R, width)}, got {tuple(out.shape)}")
-    for t in (x2, w.values, out, route.ids):
+    for t in (x2, w.values, out, route.ids) if slot is None else (x2, w.values, out, route.ids, slot):
         _here(t)
     if T * R:
         lib = L.lib()
@@ -279,7 +290,7 @@ def mx_moe_into(w: MxWeight, x, route, out: torch.Tensor, act: str = "MXFP6", ro
         key = (kind, M, T * R, route.n_experts, mapped, xs is None)
         need = w._needs.get(key)
         if need is None:
-            need = w._needs[key] = lib.mfq_hip_mx_moe_workspace_bytes(kind, K, M, T * R, route.n_experts, mapped, xs is not None)
+            need = w.note_need(key, lib.mfq_hip_mx_moe_workspace_bytes(kind, K, M, T * R, route.n_experts, mapped, xs is not None))
         ws = borrow(need, x2.device)
         L.check(lib.mfq_hip_mx_moe_matmul(w.values.data_ptr(), laid.data_ptr(), w.rows, K, w.out, _ptr(slot), route.n_experts, kind, x2.data_ptr(), xd,
                                           ldx, _ptr(xs), int(routed), route.ids.data_ptr(), T, R, _ptr(route.ids_dst) if mapped else None,
