@@ -32,11 +32,12 @@ def test_sizes(lib):
     # a workspace that grows with the rows; none for rows that the kernel quantises itself or that come quantised
     assert lib.mfq_hip_mx_scaled_gemm_workspace_bytes(4, 4096, 4096, 1, 0) == 0
     assert lib.mfq_hip_mx_scaled_gemm_workspace_bytes(4, 4096, 4096, 16, 1) == 0
-    assert lib.mfq_hip_mx_scaled_gemm_workspace_bytes(4, 4096, 4096, 16, 0) == 16 * 2048 + 16 * 256
+    assert lib.mfq_hip_mx_scaled_gemm_workspace_bytes(4, 4096, 8192, 16, 0) == 16 * 4096 + 32 * 256
+    assert lib.mfq_hip_mx_scaled_gemm_workspace_bytes(4, 4096, 4096, 16, 0) == 0 and lib.mfq_hip_mx_scaled_gemm_workspace_bytes(4, 4096, 4096, 17, 0) > 0
     assert lib.mfq_hip_mx_scaled_gemm_workspace_bytes(5, 4096, 4096, 16, 0) == 0
     # routed experts: the rows and, where tiles serve the call, 16 bytes for each of at most so many and one
     moe = lib.mfq_hip_mx_moe_workspace_bytes
-    assert moe(6, 288, 100, 200, 64, 1, 0) == 100 * 384 + 128 * 16 and moe(6, 288, 100, 200, 64, 1, 1) == 0
+    assert moe(6, 8192, 100, 200, 64, 1, 0) == 100 * 6144 + 128 * 256 and moe(6, 8192, 100, 200, 64, 1, 1) == 0 and moe(6, 4096, 100, 200, 64, 1, 0) == 0
     assert moe(6, 288, 100, 1600, 32, 1, 1) == 16 * (25 + 32 + 1) and moe(6, 288, 100, 1600, 32, 1, 0) == 100 * 384 + 128 * 16 + 16 * 58
     assert moe(6, 288, 100, 200, 64, 0, 0) == 0
 
@@ -73,8 +74,8 @@ def gemm(lib, **k):
     (dict(glu=1), "INVALID", "16-bit"), (dict(glu=1, yd=L.X_BF16, activation=4), "INVALID", "activation=4"),
     (dict(glu=1, yd=L.X_BF16, nrows=63), "INVALID", "gate and up"), (dict(y=ODD), "INVALID", "unaligned y"), (dict(x=ODD), "INVALID", "unaligned x"),
     (dict(rows=1 << 20, nrows=1 << 20, cols=1 << 13, ldx=1 << 13, ldy=1 << 20), "UNSUPPORTED", "weights"),
-    (dict(M=16), "WORKSPACE", "workspace"), (dict(M=16, ws=A, nbytes=16 * 128), "WORKSPACE", "workspace"),
-    (dict(M=16, ws=ODD, nbytes=1 << 20), "WORKSPACE", "unaligned")])
+    (dict(M=20), "WORKSPACE", "workspace"), (dict(M=20, ws=A, nbytes=20 * 128), "WORKSPACE", "workspace"),
+    (dict(M=20, ws=ODD, nbytes=1 << 20), "WORKSPACE", "unaligned")])
 def test_gemm_checks(lib, change, status, word):
     assert gemm(lib, **change) == getattr(L, "ERR_" + status), _msg(lib)
     assert word in _msg(lib)
@@ -92,7 +93,7 @@ def moe(lib, **k):
     (dict(E=5), "INVALID", "not 5 experts"), (dict(out=60), "INVALID", "not 4 experts"), (dict(act=8), "INVALID", "kind 8"),
     (dict(glu=1, yd=L.X_F16, out=64, activation=9), "INVALID", "activation=9"), (dict(ldy=10), "INVALID", "ldy"), (dict(ldx=255), "INVALID", "ldx"),
     (dict(T=1 << 16, R=1 << 15), "INVALID", "tokens"), (dict(T=40000, R=2), "UNSUPPORTED", "without a route map"),
-    (dict(dst=A, bounds=A), "WORKSPACE", "workspace"), (dict(T=1000, xs=A, dst=A, bounds=A), "WORKSPACE", "workspace"), (dict(dst=A, bounds=A, ws=ODD, nbytes=1 << 20), "WORKSPACE", "unaligned"),
+    (dict(dst=A, bounds=A, cols=8192, ldx=8192), "WORKSPACE", "workspace"), (dict(T=1000, xs=A, dst=A, bounds=A), "WORKSPACE", "workspace"), (dict(dst=A, bounds=A, cols=8192, ldx=8192, ws=ODD, nbytes=1 << 20), "WORKSPACE", "unaligned"),
     (dict(T=1 << 20, R=16, routed=1, dst=A, bounds=A, ws=A, nbytes=1 << 40), "UNSUPPORTED", "rows of activations")])
 def test_moe_checks(lib, change, status, word):
     assert moe(lib, **change) == getattr(L, "ERR_" + status), _msg(lib)

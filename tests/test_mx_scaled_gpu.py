@@ -103,7 +103,7 @@ def test_quantize_fp32_extremes(act):
 
 # ---- one tensor ---------------------------------------------------------------------------------------------------
 SHAPES = [  # rows, out, K: streamed with the rows in LDS, through the ring, two tiles; tiles of three sizes; pieces of K; ragged everything
-    (1, 16, 32), (1, 48, 96), (1, 4096, 4096), (2, 100, 1440), (5, 257, 512), (7, 64, 17408), (13, 1000, 2880), (16, 33, 12288), (3, 4096, 288),
+    (1, 16, 32), (1, 48, 96), (1, 4096, 4096), (2, 100, 1440), (6, 300, 8192), (8, 40, 8224), (9, 64, 4096), (16, 1030, 4096), (15, 48, 4384), (5, 257, 512), (7, 64, 17408), (13, 1000, 2880), (16, 33, 12288), (3, 4096, 288),
     (16, 512, 256), (17, 96, 544), (31, 130, 4096), (32, 2048, 1440), (33, 128, 288), (64, 300, 4096), (65, 129, 1440), (100, 4096, 2048),
     (129, 1000, 2880), (200, 256, 96), (300, 2048, 4096), (257, 17408, 512), (601, 4096, 544), (1024, 9000, 1024), (2049, 4112, 352)]
 
@@ -187,7 +187,7 @@ def routes(rng, T, R, E, kind):
 
 MOE = [  # tokens, routes, experts, out, K, how routed
     (1, 8, 64, 96, 288, "any"), (1, 1, 3, 16, 32, "any"), (5, 4, 8, 130, 1440, "dropped"), (8, 8, 16, 64, 512, "one"), (9, 2, 4, 48, 96, "dropped"),
-    (9, 1, 200, 64, 352, "any"), (30, 4, 32, 300, 544, "dropped"), (61, 8, 64, 256, 512, "dropped"), (40, 4, 8, 144, 2880, "any"), (100, 1, 4, 128, 256, "one"),
+    (9, 1, 200, 64, 352, "any"), (20, 3, 16, 48, 4096, "dropped"), (20, 3, 16, 48, 4128, "any"), (30, 4, 32, 300, 544, "dropped"), (61, 8, 64, 256, 512, "dropped"), (40, 4, 8, 144, 2880, "any"), (100, 1, 4, 128, 256, "one"),
     (200, 4, 16, 500, 288, "any"), (300, 2, 130, 64, 1440, "dropped"), (700, 8, 32, 272, 512, "dropped"), (513, 4, 8, 512, 352, "any"), (400, 2, 70, 96, 64, "one")]
 
 

@@ -255,13 +255,14 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
 // D stages of weights ahead, across the ends of row-blocks.  Sums of a row-block that lies in several waves' shares meet in LDS, in the order
 // of the waves.  Bound by the weights' way from memory.  61 tokens of 8 routes over 64 experts of 4096 x 2048, MXFP4 (295 MB): 57 us, where
 // a block for every 16 neurons, its waves on different macros (stream kernel), took 167; 12288 x 4096 at 16 rows 12.2 us there.
-// SMALL: up to four rows, quantised by the block itself where they come as bf16, fp16 or fp32; only that many are kept.
+// SMALL: rows that the block itself quantises where they come as bf16, fp16 or fp32; only as many as there are are kept (small_rows).
 template <int AK, int MT, int NB>
 struct FlowShape {
     static constexpr int W = NB * 2048, STAGE = W + 256, REQ = 2 * NB + 1;
     static constexpr int XM = MT * 16 * mx_macro_bytes(AK) + 256;  // a macro of activations and its scales
     static constexpr int small_macro(int rows) { return (rows * (mx_macro_bytes(AK) + 8) + 15) & ~15; }
 };
+__host__ __device__ __forceinline__ constexpr int rows_kept(int rows) { return rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows; }
 
 template <int AK, int MT, int NB, int D, int MODE, bool SMALL>
 __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
@@ -313,7 +314,7 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
     const int items = static_cast<int>(static_cast<int64_t>(total) * (wave + 1) / nwaves) - item0;
 
     uint8_t *xres = lds + nwaves * (D * S::STAGE);
-    const int kept = SMALL ? rows > 2 ? 4 : rows : 16 * MT;  // rows of activations in LDS, a power of two
+    const int kept = SMALL ? rows_kept(rows) : 16 * MT;  // rows of activations in LDS, a power of two
     const int xm = SMALL ? S::small_macro(kept) : S::XM, xtail = kept * 128, xsat = kept * XMAC;  // of a macro; where FP6's second part and the scales begin
     if constexpr (!SMALL) {
         // macro after macro as the copies of the kernel above leave them
@@ -869,7 +870,11 @@ __global__ __launch_bounds__(256) void mxs_join_kernel(MxsArgs a) {
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------
-constexpr int kSmallRows = 4;  // rows that a block of the flow kernel may quantise itself
+// Rows that every block of the flow kernel quantises itself, which saves a launch: up to four, and up to sixteen while they hold no more than
+// so many values.  4096 x 4096 at 5 rows 6.4 us in a graph, 7.9 with the quantiser's launch, at 8 rows 7.0 and 8.1, at 16 rows 8.4 and 8.2
+// (12288 x 4096: 11.7 and 11.1); 4096 x 8192 at 16 rows, beyond it, 12.8 and 10.4.  One call after the other from Python: 9.5 and 13.8.
+constexpr int kSmallRows = 4, kSmallValues = 1 << 16;
+constexpr bool small_rows(int64_t M, int K) { return M <= kSmallRows || (M <= 16 && M * K <= kSmallValues); }
 
 template <int AK, int MT, int NB, int MODE>
 int launch_stream_nb(const MxsArgs &a, int tiles, hipStream_t st) {
@@ -902,14 +907,14 @@ constexpr int kFlowStages = 3;
 template <int AK, int MT, int NB>
 size_t flow_x_bytes(int K, int small_rows) {
     using S = FlowShape<AK, MT, NB>;
-    return static_cast<size_t>(mx_macros(K)) * (small_rows ? S::small_macro(small_rows > 2 ? 4 : small_rows) : S::XM);
+    return static_cast<size_t>(mx_macros(K)) * (small_rows ? S::small_macro(rows_kept(small_rows)) : S::XM);
 }
 template <int AK, int MT, int NB, int MODE, bool SMALL>
 int launch_flow_nb(const MxsArgs &a, int tiles, int busy, hipStream_t st) {
     constexpr int D = kFlowStages;
     using S = FlowShape<AK, MT, NB>;
     size_t lds;
-    const int nwaves = flow_waves(static_cast<size_t>(D) * S::STAGE, flow_x_bytes<AK, MT, NB>(a.K, SMALL ? MODE == kPairs ? 1 : a.M : 0), &lds);
+    const int nwaves = flow_waves(static_cast<size_t>(D) * S::STAGE, flow_x_bytes<AK, MT, NB>(a.K, SMALL ? MODE == kPairs ? 1 : MODE == kMapped ? 16 : a.M : 0), &lds);
     if (!nwaves) return MFQ_ERR_UNSUPPORTED;
     const int width = a.glu ? a.nrows / 2 : a.nrows, rbs = static_cast<int>(ceil_div(width, 16));
     // blocks of a tile: two for each compute unit where the LDS has room for two
@@ -957,7 +962,7 @@ int launch_join(const MxsArgs &a, hipStream_t st) {
     return check_launch("mx_scaled (join)");
 }
 
-// Kernel of a call: the flow kernel on up to four rows (0), on one or two tiles of 16 rows (1, 2; the stream kernel where K is too long), or a
+// Kernel of a call: the flow kernel on rows that its blocks quantise (0), on one or two tiles of 16 rows (1, 2; the stream kernel where K is too long), or a
 // tile of the list (3 + its index) with K in `splits` pieces.
 struct MxsPlan { int kind, splits; };
 constexpr int kPlanTile = 3;
@@ -984,7 +989,7 @@ double tile_us(const MxsTile &t, int nrows, int nmac, int M, int splits, int cus
     return t.f + us;
 }
 
-// whether the flow kernel holds up to four rows of K columns, gate and up side by side
+// whether the flow kernel holds M rows of K columns that it quantises, gate and up side by side
 bool small_fits(int act, int K, int M) {
     size_t lds;
     return act == 4 ? flow_waves(kFlowStages * FlowShape<4, 1, 2>::STAGE, flow_x_bytes<4, 1, 2>(K, M), &lds) > 0
@@ -993,7 +998,7 @@ bool small_fits(int act, int K, int M) {
 
 MxsPlan plan_linear(int act, int nrows, int K, int M) {
     const int nmac = mx_macros(K);
-    if (M <= kSmallRows && small_fits(act, K, M)) return {0, 1};
+    if (small_rows(M, K) && small_fits(act, K, M)) return {0, 1};
     if (M <= 16) return {1, 1};
     if (M <= 32) return {2, 1};
     static const int forced = tune_env("MFQ_MXS_TILE", 0), forced_split = tune_env("MFQ_MXS_SPLIT", 0);
@@ -1062,6 +1067,9 @@ int plan_mapped(int64_t pairs, int E) {
     return mean <= 10 ? 0 : mean < 160 ? 2 : 3;
 }
 
+// whether the blocks of a call with a route map quantise their rows themselves
+bool mapped_small(int act, int K, int64_t pairs, int E) { return plan_mapped(pairs, E) == 0 && small_rows(16, K) && small_fits(act, K, 16); }
+
 template <int AK>
 int run_experts(const MxsArgs &a, hipStream_t st) {
     if (!a.ids_dst) {
@@ -1071,6 +1079,7 @@ int run_experts(const MxsArgs &a, hipStream_t st) {
     const auto most = [&](int rows) { return static_cast<int>(tiles_mapped(a.pairs, a.E, rows)); };
     switch (plan_mapped(a.pairs, a.E)) {
         case 0:
+            if (a.xraw) return launch_flow<AK, 1, kMapped, true>(a, most(16), a.E < a.pairs ? a.E : a.pairs, st);
             if (int rc = launch_flow<AK, 1, kMapped>(a, most(16), a.E < a.pairs ? a.E : a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
             return launch_stream<AK, 1, kMapped>(a, most(16), st);
         case 1:
@@ -1195,7 +1204,7 @@ size_t table_bytes(int64_t pairs, int E) {
 
 extern "C" size_t mfq_hip_mx_moe_workspace_bytes(int act, int cols, int x_rows, int n_pairs, int E, int mapped, int x_quantized) {
     if ((act != 4 && act != 6) || cols <= 0 || cols % 32 != 0 || x_rows <= 0 || n_pairs <= 0 || E <= 0 || !mapped) return 0;
-    return (x_quantized ? 0 : quantized_bytes(act, cols, x_rows)) + table_bytes(n_pairs, E);
+    return (x_quantized || mapped_small(act, cols, n_pairs, E) ? 0 : quantized_bytes(act, cols, x_rows)) + table_bytes(n_pairs, E);
 }
 
 extern "C" int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int rows, int cols, int out_per_expert, const int32_t *expert_slot, int E, int act,
@@ -1232,27 +1241,28 @@ extern "C" int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int
     if (x_scales) {
         a.xv = static_cast<const uint8_t *>(x);
         a.xs = static_cast<const uint8_t *>(x_scales);
-    } else if (!ids_dst) {
+    } else if (!ids_dst || mapped_small(act, cols, a.pairs, E)) {
         a.xraw = x;
         a.x_wide = pieces(x, x_dtype, ldx, x_rows);
         a.x_dtype = x_dtype;
         a.ldx = ldx;
     }
     if (ids_dst) {
-        const size_t rows_bytes = x_scales ? 0 : quantized_bytes(act, cols, x_rows), tab = table_bytes(a.pairs, E), need = rows_bytes + tab;
+        const bool quantise = !x_scales && !a.xraw;
+        const size_t rows_bytes = quantise ? quantized_bytes(act, cols, x_rows) : 0, tab = table_bytes(a.pairs, E), need = rows_bytes + tab;
         MFQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), MFQ_ERR_WORKSPACE, "mx_moe_matmul: workspace %zu < %zu", workspace_bytes, need);
         MFQ_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, MFQ_ERR_WORKSPACE, "mx_moe_matmul: unaligned workspace");
         uint8_t *ws = static_cast<uint8_t *>(workspace);
         const MxTileTable table = {expert_bounds, expert_slot, E, tile_rows_mapped(plan_mapped(a.pairs, E)), tab ? reinterpret_cast<i32x4v_t *>(ws + rows_bytes) : nullptr};
         a.table = table.out;
         uint8_t *xs = ws;
-        if (!x_scales) {
+        if (quantise) {
             xs = ws + ((static_cast<int64_t>(x_rows) * mx_row_bytes(act, cols) + 255) & ~static_cast<int64_t>(255));
             a.xv = ws;
             a.xs = xs;
         }
-        if (!x_scales || tab)
-            if (int rc = mx_quantize_launch(act, x, x_scales ? MFQ_X_BF16 : x_dtype, ldx, x_scales ? 0 : x_rows, cols, ws, xs, st, &table)) return rc;
+        if (quantise || tab)
+            if (int rc = mx_quantize_launch(act, x, x_scales ? MFQ_X_BF16 : x_dtype, ldx, quantise ? x_rows : 0, cols, ws, xs, st, &table)) return rc;
     }
     return act == 4 ? run_experts<4>(a, st) : run_experts<6>(a, st);
 }
