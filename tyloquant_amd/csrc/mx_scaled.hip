@@ -378,10 +378,12 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
             wsv = scales_of(++to_rb);
         }
     };
-    for (int i = 0; i < D; ++i)
-        if (i < items) issue();
+    if constexpr (!SMALL)
+        for (int i = 0; i < D; ++i)
+            if (i < items) issue();
     if constexpr (SMALL) {
-        // a thread a block of 32 columns: quantised here, or copied
+        // A thread a block of 32 columns: quantised here, or copied.  Before the first weights are asked for, behind which these reads would come
+        // (4096 x 4096 in a graph, one row 5.7 -> 5.2 us, four 6.2 -> 5.6, sixteen 8.1 -> 7.8).
         const int per_row = nmac * 8;
         for (int u = tid; u < rows * per_row; u += blockDim.x) {
             const int m = u / per_row, block = u - m * per_row, p = block & 7;
@@ -410,6 +412,8 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
             if constexpr (AK == 6) *reinterpret_cast<u32x2_t *>(to + xtail + m * 64 + row_order_quarter(m, p >> 1) * 16 + (p & 1) * 8) = u32x2_t{q[4], q[5]};
             to[xsat + m * 8 + p] = static_cast<uint8_t>(byte);
         }
+        for (int i = 0; i < D; ++i)
+            if (i < items) issue();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     } else {
         // what is older than the weights' first stages
@@ -871,8 +875,8 @@ __global__ __launch_bounds__(256) void mxs_join_kernel(MxsArgs a) {
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------
 // Rows that every block of the flow kernel quantises itself, which saves a launch: up to four, and up to sixteen while they hold no more than
-// so many values.  4096 x 4096 at 5 rows 6.4 us in a graph, 7.9 with the quantiser's launch, at 8 rows 7.0 and 8.1, at 16 rows 8.4 and 8.2
-// (12288 x 4096: 11.7 and 11.1); 4096 x 8192 at 16 rows, beyond it, 12.8 and 10.4.  One call after the other from Python: 9.5 and 13.8.
+// so many values.  4096 x 4096 at 8 rows 6.5 us in a graph, 8.1 with the quantiser's launch, at 16 rows 7.8 and 8.2, 12288 x 4096 at 16 rows 10.9
+// and 11.1; 4096 x 8192 at 16 rows, beyond it, 12.8 and 10.4.  One call after the other from Python: 9.2 and 13.8.
 constexpr int kSmallRows = 4, kSmallValues = 1 << 16;
 constexpr bool small_rows(int64_t M, int K) { return M <= kSmallRows || (M <= 16 && M * K <= kSmallValues); }
 
