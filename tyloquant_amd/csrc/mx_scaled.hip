@@ -253,8 +253,9 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
 // The activations of a tile of up to 16 * MT rows lie in LDS for the whole of K.  A block takes a range of row-blocks of 16 neurons (with GLU
 // those of the gate rows, each with that of its up rows), macro after macro, as one stream that its waves share evenly; a wave keeps a ring of
 // D stages of weights ahead, across the ends of row-blocks.  Sums of a row-block that lies in several waves' shares meet in LDS, in the order
-// of the waves.  Bound by the weights' way from memory.  61 tokens of 8 routes over 64 experts of 4096 x 2048, MXFP4 (295 MB): 57 us, where
-// a block for every 16 neurons, its waves on different macros (stream kernel), took 167; 12288 x 4096 at 16 rows 12.2 us there.
+// of the waves.  Bound by the weights' way from memory.  61 tokens of 8 routes over 64 experts of 4096 x 2048, MXFP4 (295 MB): 57 us with
+// quantised rows, 61 quantising them, where a block for every 16 neurons, its waves on different macros (stream kernel), took 167; 12288 x 4096
+// at 16 rows 10.9 us in a graph, 12.2 there.
 // SMALL: rows that the block itself quantises where they come as bf16, fp16 or fp32; only as many as there are are kept (small_rows).
 template <int AK, int MT, int NB>
 struct FlowShape {
