@@ -939,7 +939,7 @@ int launch_flow(const MxsArgs &a, int tiles, int busy, hipStream_t st) {
     return a.glu ? launch_flow_nb<AK, MT, 2, MODE, SMALL>(a, tiles, busy, st) : launch_flow_nb<AK, MT, 1, MODE, SMALL>(a, tiles, busy, st);
 }
 
-int tile_rows_mapped(int kind) { return kind == 2 ? 64 : 128; }
+int tile_rows_mapped(int kind) { return kind == 1 ? 64 : 128; }
 // tiles of a call with a route map: at most
 int64_t tiles_mapped(int64_t pairs, int E, int rows) { return ceil_div(pairs, rows) + (E < pairs ? E : pairs); }
 
@@ -1061,15 +1061,14 @@ int run_linear(const MxsArgs &a, const MxsPlan &p, hipStream_t st) {
     }
 }
 
-// Kernel of a call with a route map, from the pairs an expert has on average: 0 and 1 waves that stream row-blocks against 16 or 32 rows
-// (flow kernel), 2 and 3 tiles of 128 x 64 and 256 x 128.  128 experts of 2048 x 2048, gated, MXFP4, 8 routes: at 256 tokens (16 pairs an
-// expert) 81, 74, 64 and 75 us, at 2048 tokens 314, 217, 126 and 140; 32 experts of 2880 x 1440, MXFP6, 4 routes: at 1501 tokens (188
-// pairs) 146, 111, 80 and 65 us.
+// Kernel of a call with a route map, from the pairs an expert has on average: 0 waves that stream row-blocks against 16 rows (flow kernel), 1
+// and 2 tiles of 128 x 64 and 256 x 128.  128 experts of 2048 x 2048, gated, MXFP4, 8 routes: at 256 tokens (16 pairs an expert) 81, 64
+// and 75 us, at 2048 tokens 314, 126 and 140; 32 experts of 2880 x 1440, MXFP6, 4 routes: at 1501 tokens (188 pairs) 146, 80 and 65 us.
 int plan_mapped(int64_t pairs, int E) {
     static const int forced = tune_env("MFQ_MXS_TILE", 0);
-    if (forced > 0) return forced < 4 ? forced - 1 : 3;
+    if (forced > 0) return forced < 3 ? forced - 1 : 2;
     const int64_t mean = ceil_div(pairs, E);
-    return mean <= 10 ? 0 : mean < 160 ? 2 : 3;
+    return mean <= 10 ? 0 : mean < 160 ? 1 : 2;
 }
 
 // whether the blocks of a call with a route map quantise their rows themselves
@@ -1087,10 +1086,7 @@ int run_experts(const MxsArgs &a, hipStream_t st) {
             if (a.xraw) return launch_flow<AK, 1, kMapped, true>(a, most(16), a.E < a.pairs ? a.E : a.pairs, st);
             if (int rc = launch_flow<AK, 1, kMapped>(a, most(16), a.E < a.pairs ? a.E : a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
             return launch_stream<AK, 1, kMapped>(a, most(16), st);
-        case 1:
-            if (int rc = launch_flow<AK, 2, kMapped>(a, most(32), a.E < a.pairs ? a.E : a.pairs, st); rc != MFQ_ERR_UNSUPPORTED) return rc;
-            return launch_stream<AK, 2, kMapped>(a, most(32), st);
-        case 2: return launch_tile<AK, 128, 64, 2, 2, 2, kMapped>(a, st);
+        case 1: return launch_tile<AK, 128, 64, 2, 2, 2, kMapped>(a, st);
         default: return launch_tile<AK, 256, 128, 4, 2, AK == 4 ? 3 : 2, kMapped>(a, st);
     }
 }
@@ -1203,7 +1199,7 @@ extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scale
 namespace {
 size_t table_bytes(int64_t pairs, int E) {
     const int kind = plan_mapped(pairs, E);
-    return kind < 2 ? 0 : static_cast<size_t>(tiles_mapped(pairs, E, tile_rows_mapped(kind)) + 1) * 16;
+    return kind < 1 ? 0 : static_cast<size_t>(tiles_mapped(pairs, E, tile_rows_mapped(kind)) + 1) * 16;
 }
 }  // namespace
 
@@ -1230,7 +1226,7 @@ extern "C" int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int
     if (!ids_dst) {
         MFQ_REQUIRE(T * R <= 65535, MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: %d pairs without a route map", T * R);
     } else {
-        MFQ_REQUIRE(ceil_div(T * R, 16) + E <= 65535 || plan_mapped(static_cast<int64_t>(T) * R, E) > 1, MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: %d experts, %d pairs", E, T * R);
+        MFQ_REQUIRE(ceil_div(T * R, 16) + E <= 65535 || plan_mapped(static_cast<int64_t>(T) * R, E) > 0, MFQ_ERR_UNSUPPORTED, "mx_moe_matmul: %d experts, %d pairs", E, T * R);
     }
     const hipStream_t st = as_stream(stream);
     a.nrows = out_per_expert;
