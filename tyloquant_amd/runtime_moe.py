@@ -131,11 +131,7 @@ class ForeignCohort:
         from .runtime import Nint8ZeroWeight
         from .runtime_vq import NvqsWeight, nepq_hadamard
         lib, dev = L.lib(), x2.device
-        if self._slot is None:
-            self.slots(n_experts, dev)
-            if self.linears:
-                self._wtab = torch.tensor([q.weight.data.data_ptr() for q in self.linears], dtype=torch.int64, device=dev)
-        common = (_ptr(self._slot), n_experts)
+        common = (_ptr(self.slots(n_experts, dev)), n_experts)
         if self.nepq is not None and self.nepq.rotation_block:
             x2 = nepq_hadamard(x2, self.nepq.signs, self.nepq.rotation_block)
         tail = (_ptr(x2), _x_dtype(x2), x2.stride(0), int(routed), _ptr(ids), T, R, _ptr(flat), flat.stride(0), _stream())
@@ -162,8 +158,11 @@ class ForeignCohort:
         return self.mx is not None and self.mx.kind == 4
 
     def slots(self, n_experts: int, device) -> torch.Tensor:
-        """place of every expert of the tensor in this cohort, -1 for those of others (device int32 [n_experts])"""
+        """place of every expert of the tensor in this cohort, -1 for those of others (device int32 [n_experts]); where its experts are
+        tensors of their own, their addresses (_wtab) are made with it"""
         if self._slot is None:
+            if self.linears:
+                self._wtab = torch.tensor([q.weight.data.data_ptr() for q in self.linears], dtype=torch.int64, device=device)
             slot = np.full(n_experts, -1, dtype=np.int32)
             slot[self.expert_ids[self.live]] = np.arange(len(self.expert_ids), dtype=np.int32)[self.live]
             self._slot = torch.from_numpy(slot).to(device)
