@@ -30,3 +30,18 @@ def test_slots_come_with_the_addresses_of_the_experts(monkeypatch):
     x, ids, flat = torch.zeros(1, 64, dtype=torch.bfloat16), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(2, 16)
     c.matmul_pairs(4, x, False, ids, 1, 2, flat)
     assert got["wtab"] is not None and c._wtab.tolist() == [q.weight.data.data_ptr() for q in c.linears]
+
+
+def test_tables_of_cohorts_are_there_from_the_start():
+    """A first call may be a captured one, in which nothing can be copied from the host."""
+    parts = [cohort([3, 0], mx=types.SimpleNamespace(kind=4)), cohort([1], linears=1)]
+    w = RM.NintMoeWeight(4, 16, 64, [], [], torch.device("cpu"), parts)
+    assert [None if c._slot is None else c._slot.tolist() for c in w.foreign] == [[1, -1, -1, 0], [-1, 0, -1, -1]]
+    assert w.foreign[1]._wtab is not None
+
+
+def test_scales_of_every_capable_cohort_are_laid_out():
+    laid = []
+    parts = [cohort([i], mx=types.SimpleNamespace(kind=4, laid_scales=lambda i=i: laid.append(i))) for i in (0, 1)] + [cohort([2], linears=1)]
+    RM.NintMoeWeight(3, 16, 64, [], [], torch.device("cpu"), parts).lay_scales()
+    assert laid == [0, 1]

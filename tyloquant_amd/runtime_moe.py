@@ -119,7 +119,7 @@ class ForeignCohort:
             shape = (n, self.linears[0].out, self.linears[0].neuron_len)
         if shape != (n, out_per_expert, neuron_len):
             raise ValueError(f"NINTM pool tensor shape {shape} must be {(n, out_per_expert, neuron_len)}")
-        self._slot = self._wtab = None           # device tables of the one-launch decode form, built on first use
+        self._slot = self._wtab = None           # device tables of the one-launch forms (slots)
         self.live = np.ones(n, dtype=bool)       # experts an expert overlay has not given to a later cohort
 
     PAIRS_MAX = 64   # (token, route) pairs up to which a decode step takes one launch per cohort over all its pairs
@@ -172,7 +172,7 @@ class ForeignCohort:
         """out[t, r] = W[ids[t, r]] . q(x) for the pairs routed to this cohort, activations quantised to `act`: one launch for any batch,
         nothing read back (mfq_hip_mx_moe_matmul)."""
         from .runtime_mx import mx_moe_into
-        self.mx.laid_scales()                    # before anything of a first call under capture, which it refuses
+        self.mx.laid_scales()                    # before anything of a first call under capture, which it refuses where nobody laid them out
         mx_moe_into(self.mx, x, route, out, act, routed, glu, activation, self.slots(route.n_experts, out.device))
 
     def pairs_capable(self) -> bool:
@@ -214,6 +214,8 @@ class NintMoeWeight:
         self.pool_expert_ids = expert_ids
         self.pool_live = pool_live if pool_live is not None else [np.ones(len(ids), dtype=bool) for ids in expert_ids]
         self.foreign: list[ForeignCohort] = list(foreign)
+        for c in self.foreign:                            # now: copies from the host cannot be part of a captured first call
+            c.slots(n_experts, device)
         ep = np.full(n_experts, -1, dtype=np.int32)       # -1: no NINT cohort -- the kernels leave a zero row
         el = np.full(n_experts, -1, dtype=np.int32)
         for pi, (ids, live) in enumerate(zip(expert_ids, self.pool_live)):
@@ -331,7 +333,8 @@ class NintMoeWeight:
     def forward(self, x: torch.Tensor, route: MoeRoutePlan, act: str | None = None) -> torch.Tensor:
         """NintMoeWeight::forward (cpp_runtime/mfq_decode.cpp:2908-3071): x is [T, K] (shared by the
         routes of a token) or [T, R, K] (routed input); returns fp32 [T, R, out_per_expert].  act: "MXFP4" or "MXFP6" quantises
-        the activations of native MXFP4 cohorts and multiplies the codes (mx_moe_matmul); other cohorts take them as they are."""
+        the activations of native MXFP4 cohorts and multiplies the codes (mx_moe_matmul); other cohorts take them as they are.  The
+        first such call lays those cohorts' scales out, which a graph cannot record: lay_scales(), or a call, before a capture."""
         if act is not None:
             from .runtime_mx import check_act
             check_act(act)
@@ -369,6 +372,12 @@ class NintMoeWeight:
         return out
 
     __call__ = forward
+
+    def lay_scales(self) -> None:
+        """Lays the scales of the native MXFP4 cohorts out for calls with `act` (MxWeight.laid_scales), as the first of them would."""
+        for c in self.foreign:
+            if c.scaled_capable():
+                c.mx.laid_scales()
 
     def _all_scaled(self) -> bool:
         """Whether native MXFP4 cohorts alone hold the tensor's experts, every one of them."""

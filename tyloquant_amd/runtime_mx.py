@@ -58,7 +58,7 @@ class MxWeight:
                 raise ValueError(f"products of microscaled operands take MXFP4 weights, not {self.dtype}: use mx_matmul")
             _here(self.scales)
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"{self.dtype}: call laid_scales() before a graph is captured")
+                raise RuntimeError(f"{self.dtype}: call laid_scales() (lay_scales() of a tensor of experts) before a graph is captured")
             laid = torch.empty(_scale_bytes(self.rows, self.neuron_len), dtype=torch.uint8, device=self.scales.device)
             L.check(L.lib().mfq_hip_mx_lay_scales(_ptr(self.scales), self.rows, self.neuron_len, _ptr(laid), _stream()))
             torch.cuda.current_stream().synchronize()   # later calls may come on other streams
