@@ -45,3 +45,21 @@ def test_scales_of_every_capable_cohort_are_laid_out():
     parts = [cohort([i], mx=types.SimpleNamespace(kind=4, laid_scales=lambda i=i: laid.append(i))) for i in (0, 1)] + [cohort([2], linears=1)]
     RM.NintMoeWeight(3, 16, 64, [], [], torch.device("cpu"), parts).lay_scales()
     assert laid == [0, 1]
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_feed_forward_block_refuses_unknown_activation_types(decode, monkeypatch):
+    """Whichever launches would serve the call, and before any of them."""
+    gate_up = RM.NintMoeWeight(2, 32, 64, [], [], torch.device("cpu"))
+    down = RM.NintMoeWeight(2, 64, 16, [], [], torch.device("cpu"))
+    ran = []
+    monkeypatch.setattr(RM, "moe_topk", lambda *a: ran.append("topk") or (torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, 1)))
+    monkeypatch.setattr(RM, "build_moe_route_plan", lambda ids, n: RM.MoeRoutePlan(ids, n))
+    for w in (gate_up, down):
+        w.decode_capable = lambda *a: decode
+        w.forward_decode = lambda *a, **k: ran.append("decode") or torch.zeros(1, 64)
+        w.forward_shared = lambda *a, **k: torch.zeros(2, 64)
+    monkeypatch.setattr(RM, "moe_weighted_reduce", lambda *a: a[0])
+    with pytest.raises(ValueError, match="MXFP4 or MXFP6, not MXFP8"):
+        RM.nint_moe_ffn_forward(gate_up, down, torch.zeros(1, 64), torch.zeros(1, 2), 1, act="MXFP8", shared=(None, None))
+    assert not ran

@@ -528,6 +528,9 @@ def nint_moe_ffn_forward(gate_up: NintMoeWeight, down: NintMoeWeight, x: torch.T
     """cpp_runtime/mfq_decode.cpp:3394-3416.  `shared` = (gate_up NintWeight [2W, H], down NintWeight [H, W]) of the
     shared expert, added ungated (cpp_runtime/mfq_decode.cpp:11077-11080).  act: "MXFP4" or "MXFP6" quantises the activations of
     native MXFP4 cohorts, those of the block and the hidden ones (NintMoeWeight.forward).  Returns (out, ids, weights)."""
+    if act is not None:                  # here too: launches that fuse the NINT cohorts never come to it
+        from .runtime_mx import check_act
+        check_act(act)
     if gate_up.n_experts != down.n_experts or gate_up.out_per_expert != 2 * down.neuron_len or \
             down.out_per_expert != gate_up.neuron_len:
         raise RuntimeError("incompatible fused gate_up/down NINTM tensors")
