@@ -30,7 +30,8 @@ class MxWeight:
         self.n_experts = self.rows // self.out
         self.data = values                      # the device tensor other weights call `data`
         self._ws = _Workspace()
-        self._laid, self._needs = None, {}
+        self._laid = self._laid_of = self._laid_version = None   # scales of laid_scales, and those that they were made from
+        self._needs = {}
 
     @property
     def payload_bytes(self) -> int:
@@ -50,20 +51,25 @@ class MxWeight:
         h = F.MxHeader(dtype, 4 if dtype == "MXFP4" else 8, values.shape[0], cols, 0, values.numel(), values.numel(), scales.numel())
         return MxWeight(h, values, scales, out)
 
-    def laid_scales(self) -> torch.Tensor:
+    def laid_scales(self, again: bool = False) -> torch.Tensor:
         """Scales as the products of microscaled operands read them (mfq_hip_mx_lay_scales), laid out at the first call and kept:
-        1/16 of the values' bytes.  A graph cannot be the first to ask: what it writes is there only after a replay."""
-        if self._laid is None:
-            if self.kind != 4:
-                raise ValueError(f"products of microscaled operands take MXFP4 weights, not {self.dtype}: use mx_matmul")
-            _here(self.scales)
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"{self.dtype}: call laid_scales() (lay_scales() of a tensor of experts) before a graph is captured")
-            laid = torch.empty(_scale_bytes(self.rows, self.neuron_len), dtype=torch.uint8, device=self.scales.device)
-            L.check(L.lib().mfq_hip_mx_lay_scales(_ptr(self.scales), self.rows, self.neuron_len, _ptr(laid), _stream()))
-            torch.cuda.current_stream().synchronize()   # later calls may come on other streams
-            self._laid = laid
-        return self._laid
+        1/16 of the values' bytes.  Scales that torch operations have rewritten in place since are laid out again, to the same place, so
+        that captured products see them too; writes that torch does not count (of other libraries, or where the scales are an inference
+        tensor) need a call with `again`.  A graph cannot be the first to ask: what it writes is there only after a replay."""
+        scales = self.scales
+        if self._laid is not None and not again and self._laid_of is scales and (self._laid_version is None or self._laid_version == scales._version):
+            return self._laid
+        if self.kind != 4:
+            raise ValueError(f"products of microscaled operands take MXFP4 weights, not {self.dtype}: use mx_matmul")
+        _here(scales)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{self.dtype}: call laid_scales() (lay_scales() of a tensor of experts) before a graph is captured")
+        version = None if scales.is_inference() else scales._version
+        laid = self._laid if self._laid is not None else torch.empty(_scale_bytes(self.rows, self.neuron_len), dtype=torch.uint8, device=scales.device)
+        L.check(L.lib().mfq_hip_mx_lay_scales(_ptr(scales), self.rows, self.neuron_len, _ptr(laid), _stream()))
+        torch.cuda.current_stream().synchronize()   # later calls may come on other streams
+        self._laid, self._laid_of, self._laid_version = laid, scales, version
+        return laid
 
     def note_need(self, key, need: int) -> int:
         """Remembers the workspace of a call's sizes; a program whose every call has other sizes starts over now and then."""
