@@ -37,7 +37,7 @@ constexpr int kMxMacro = 256;  // columns of a macro
 // Scales of both operands lie by blocks of 32 rows, and in those by macros: eight bytes a row, 256 a block of rows.  A copy of a tile's
 // scales then moves whole lines, where rows one after the other (a line of 128 bytes fetched for every eight) cost as many requests as
 // the codes.  Zeros behind the last column.
-__host__ __device__ __forceinline__ constexpr int mx_macros(int K) { return (K + kMxMacro - 1) / kMxMacro; }
+__host__ __device__ __forceinline__ constexpr int mx_macros(int K) { return K / kMxMacro + (K % kMxMacro != 0); }  // of any K: K + 255 may not fit
 __host__ __device__ __forceinline__ constexpr uint32_t mx_scale_at(int64_t row, int nmac) {  // of the row's first macro; the next are 256 further each
     return static_cast<uint32_t>(row >> 5) * static_cast<uint32_t>(nmac) * 256u + static_cast<uint32_t>(row & 31) * 8u;
 }
