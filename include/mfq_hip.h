@@ -534,6 +534,11 @@ int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int rows, int 
                           const int32_t *ids, int T, int R, const int32_t *ids_dst, const int32_t *expert_bounds, int glu,
                           int activation, void *y, int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes,
                           mfq_stream_t stream);
+/* Test and tuning hooks, host only: the kernel that such a call takes given the workspace of its query.  0: the flow kernel on rows that
+ * its blocks quantise (or copy); 1, 2: the flow kernel on one or two tiles of 16 quantised rows; 3, 4: the stream kernel on those; 5 + i:
+ * tile i of kMxsTile in csrc/mx_scaled.hip, one tensor's with K in *splits pieces.  -1 for sizes that no call has. */
+int mfq_hip_mx_scaled_plan(int act, int nrows, int cols, int M, int glu, int *splits);
+int mfq_hip_mx_moe_plan(int act, int cols, int n_pairs, int E, int mapped, int glu, int x_quantized);
 
 /* ------------------------------------------------------------------------------------
  * NEPQ1-S / NEPQ1-L (cross-expert table pool, bank id per 96 weights).  Rows are the

@@ -1,6 +1,9 @@
 """Rules of the products of microscaled operands on the host: sizes at their ends, and which kernel a call takes (nothing is launched)."""
+import ctypes as C
+
 import pytest
 
+from test_mx_scaled_plans_gpu import KIND, TILES
 from tyloquant_amd import _lib as L
 
 
@@ -22,3 +25,37 @@ def test_sizes_of_the_longest_rows(lib, act, x_quantized):
     # 40 rows: the pieces of K, as many for a group fewer, and those rows quantised, which that group's codes and scales make longer
     fewer, *need = [lib.mfq_hip_mx_scaled_gemm_workspace_bytes(act, 64, k, 40, x_quantized) for k in (first - 32, first, last)]
     assert [n - fewer for n in need] == [0 if x_quantized else 40 * (128 if act == 4 else 192) + 2 * 256] * 2
+
+
+@pytest.mark.parametrize("act,cus,rows,out,K,plan,pieces", TILES)
+def test_tile_of_a_call(lib, act, cus, rows, out, K, plan, pieces):
+    lib.mfq_hip_set_cu_count(cus)
+    try:
+        got = C.c_int()
+        assert (lib.mfq_hip_mx_scaled_plan(KIND[act], out, K, rows, 0, C.byref(got)), got.value) == (plan, pieces)
+    finally:
+        lib.mfq_hip_set_cu_count(256)
+
+
+def test_every_tile_is_run():
+    """By the tests on the card, whole and with K in pieces (of 256 x 128 MXFP4 no call was found that splits K)."""
+    assert {(plan, pieces > 1) for *_, plan, pieces in TILES} == {(p, s) for p in range(5, 13) for s in (False, True)} - {(8, True)}
+
+
+@pytest.mark.parametrize("act,out,K,rows,glu,plan", [
+    (4, 12288, 4096, 1, 0, 0), (4, 12288, 4096, 16, 0, 0), (4, 12288, 4096, 17, 0, 2), (4, 12288, 4096, 33, 0, 6), (4, 12288, 4096, 601, 0, 7),
+    (4, 17408, 5120, 8192, 0, 9), (6, 24576, 4096, 2048, 1, 11), (6, 4096, 12288, 13, 0, 3), (6, 4096, 12288, 4, 0, 0),
+    (6, 96, 5632, 20, 0, 2), (6, 96, 5632, 20, 1, 4), (4, 96, 8224, 20, 0, 2), (4, 96, 8224, 20, 1, 4), (4, 96, 17440, 5, 1, 3), (4, 96, 17440, 16, 0, 3),
+    (4, 64, 48, 1, 0, -1), (5, 64, 64, 1, 0, -1), (4, 0, 64, 1, 0, -1), (4, 64, 64, 0, 0, -1), (4, 64, (1 << 24) + 32, 40, 0, -1)])
+def test_kernel_of_a_call(lib, act, out, K, rows, glu, plan):
+    assert lib.mfq_hip_mx_scaled_plan(act, out, K, rows, glu, None) == plan
+
+
+@pytest.mark.parametrize("act,K,pairs,E,mapped,glu,x_quantized,plan", [
+    (6, 4096, 8, 64, 0, 1, 0, 0), (4, 2048, 488, 64, 1, 0, 0, 0), (4, 2048, 488, 64, 1, 0, 1, 1), (4, 4128, 60, 16, 1, 0, 0, 1),
+    (4, 2048, 640, 64, 1, 0, 0, 0), (4, 2048, 641, 64, 1, 0, 0, 5), (6, 2048, 641, 64, 1, 0, 0, 10),       # ten pairs an expert
+    (4, 2048, 64 * 159, 64, 1, 0, 0, 5), (4, 2048, 64 * 159 + 1, 64, 1, 0, 0, 8), (6, 1440, 6004, 32, 1, 0, 0, 11),
+    (4, 17440, 24, 8, 1, 0, 0, 3), (6, 12288, 24, 8, 1, 1, 1, 3), (4, 15136, 24, 8, 1, 0, 0, 1), (4, 15136, 24, 8, 1, 1, 0, 3),
+    (8, 64, 1, 1, 1, 0, 0, -1), (4, 40, 1, 1, 1, 0, 0, -1), (4, 64, 0, 1, 1, 0, 0, -1)])
+def test_kernel_of_routed_experts(lib, act, K, pairs, E, mapped, glu, x_quantized, plan):
+    assert lib.mfq_hip_mx_moe_plan(act, K, pairs, E, mapped, glu, x_quantized) == plan

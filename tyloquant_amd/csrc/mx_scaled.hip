@@ -1001,6 +1001,18 @@ bool small_fits(int act, int K, int M) {
                     : flow_waves(kFlowStages * FlowShape<6, 1, 2>::STAGE, flow_x_bytes<6, 1, 2>(K, M), &lds) > 0;
 }
 
+// whether it holds MT tiles of 16 quantised rows; else the stream kernel serves them
+template <int AK, int MT>
+bool flow_fits(int K, bool glu) {
+    size_t lds;
+    return (glu ? flow_waves(kFlowStages * FlowShape<AK, MT, 2>::STAGE, flow_x_bytes<AK, MT, 2>(K, 0), &lds)
+                : flow_waves(kFlowStages * FlowShape<AK, MT, 1>::STAGE, flow_x_bytes<AK, MT, 1>(K, 0), &lds)) > 0;
+}
+bool flow_fits(int act, int tiles, int K, bool glu) {
+    if (act == 4) return tiles == 1 ? flow_fits<4, 1>(K, glu) : flow_fits<4, 2>(K, glu);
+    return tiles == 1 ? flow_fits<6, 1>(K, glu) : flow_fits<6, 2>(K, glu);
+}
+
 MxsPlan plan_linear(int act, int nrows, int K, int M) {
     const int nmac = mx_macros(K);
     if (small_rows(M, K) && small_fits(act, K, M)) return {0, 1};
@@ -1146,6 +1158,14 @@ extern "C" size_t mfq_hip_mx_scaled_gemm_workspace_bytes(int act, int nrows, int
     return n;
 }
 
+extern "C" int mfq_hip_mx_scaled_plan(int act, int nrows, int cols, int M, int glu, int *splits) {
+    if ((act != 4 && act != 6) || nrows <= 0 || cols <= 0 || cols % 32 != 0 || cols > kMaxCols || M <= 0) return -1;
+    const MxsPlan p = plan_linear(act, nrows, cols, M);
+    if (splits) *splits = p.splits;
+    if (p.kind >= kPlanTile) return 5 + p.kind - kPlanTile;
+    return p.kind > 0 && !flow_fits(act, p.kind, cols, glu != 0) ? 2 + p.kind : p.kind;
+}
+
 extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scales, int rows, int cols, int row0, int nrows, int act, const void *x,
                                            int x_dtype, int64_t ldx, const void *x_scales, int M, int glu, int activation, void *y, int y_dtype,
                                            int64_t ldy, void *workspace, size_t workspace_bytes, mfq_stream_t stream) {
@@ -1206,6 +1226,15 @@ size_t table_bytes(int64_t pairs, int E) {
 extern "C" size_t mfq_hip_mx_moe_workspace_bytes(int act, int cols, int x_rows, int n_pairs, int E, int mapped, int x_quantized) {
     if ((act != 4 && act != 6) || cols <= 0 || cols % 32 != 0 || x_rows <= 0 || n_pairs <= 0 || E <= 0 || !mapped) return 0;
     return (x_quantized || mapped_small(act, cols, n_pairs, E) ? 0 : quantized_bytes(act, cols, x_rows)) + table_bytes(n_pairs, E);
+}
+
+extern "C" int mfq_hip_mx_moe_plan(int act, int cols, int n_pairs, int E, int mapped, int glu, int x_quantized) {
+    if ((act != 4 && act != 6) || cols <= 0 || cols % 32 != 0 || cols > kMaxCols || n_pairs <= 0 || E <= 0) return -1;
+    if (!mapped) return 0;
+    const int kind = plan_mapped(n_pairs, E);
+    if (kind > 0) return 5 + (act == 4 ? kind == 1 ? 0 : 3 : kind == 1 ? 5 : 6);
+    if (!x_quantized && mapped_small(act, cols, n_pairs, E)) return 0;
+    return flow_fits(act, 1, cols, glu != 0) ? 1 : 3;
 }
 
 extern "C" int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int rows, int cols, int out_per_expert, const int32_t *expert_slot, int E, int act,
