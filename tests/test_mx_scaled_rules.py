@@ -59,3 +59,13 @@ def test_kernel_of_a_call(lib, act, out, K, rows, glu, plan):
     (8, 64, 1, 1, 1, 0, 0, -1), (4, 40, 1, 1, 1, 0, 0, -1), (4, 64, 0, 1, 1, 0, 0, -1)])
 def test_kernel_of_routed_experts(lib, act, K, pairs, E, mapped, glu, x_quantized, plan):
     assert lib.mfq_hip_mx_moe_plan(act, K, pairs, E, mapped, glu, x_quantized) == plan
+
+
+@pytest.mark.parametrize("act", [4, 6])
+@pytest.mark.parametrize("out", [300, 301, 302, 303, 304, 134, 32])
+def test_partial_sums_begin_on_16_bytes(lib, act, out):
+    """K in pieces: a row of partial sums has two halves, gate and up of a gated call, that 16-byte stores fill from their first column on."""
+    pieces, rows, K = C.c_int(), 64, 4096
+    assert lib.mfq_hip_mx_scaled_plan(act, out, K, rows, 0, C.byref(pieces)) >= 5 and pieces.value > 1
+    half, left = divmod(lib.mfq_hip_mx_scaled_gemm_workspace_bytes(act, out, K, rows, 1), pieces.value * rows * 2)
+    assert left == 0 and half % 16 == 0 and half >= -(-out // 2) * 4

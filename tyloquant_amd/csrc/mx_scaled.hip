@@ -569,6 +569,10 @@ struct TileShape {
     static constexpr int STAGE = W + X + X2 + WS + XS;
     static constexpr int LDS = R * STAGE + BM * 4;  // and the rows of y
 };
+// Partial results of a split over K: rows of two halves, each a whole number of 16 bytes, so that the up rows' sums of a gated product begin on
+// such a boundary as well as the gate rows'.
+__host__ __device__ __forceinline__ constexpr int part_half(int nrows) { return ((nrows + 1) / 2 + 3) / 4 * 4; }
+constexpr int64_t part_bytes(int M, int nrows) { return static_cast<int64_t>(M) * part_half(nrows) * 8; }
 constexpr int kTilePitch = 64 * 4 + 16, kTileOut = 32 * kTilePitch;  // 64 results of 32 rows on their way out
 
 template <int AK, int BN, int BM, int WN, int WM, int R, int MODE>
@@ -766,8 +770,9 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
     // (8192 rows of FP4 by 17408 x 5120, bf16 out: 470 -> 445 us; 2048 rows of FP6 by 24576 x 4096, gated, fp16 out: 187 -> 177).
     uint8_t *area = lds + wave * kTileOut;
     const bool partial = a.splits > 1, f32 = partial || a.y_dtype == MFQ_X_F32;
-    uint8_t *y = reinterpret_cast<uint8_t *>(partial ? a.part + static_cast<int64_t>(blockIdx.y) * a.M * a.nrows : a.y);
-    const int64_t ldy = partial ? a.nrows : a.ldy;
+    const int half = part_half(a.nrows);  // of partial results: where the up rows' begin
+    uint8_t *y = reinterpret_cast<uint8_t *>(partial ? a.part + static_cast<int64_t>(blockIdx.y) * a.M * (2 * half) : a.y);
+    const int64_t ldy = partial ? 2 * half : a.ldy;
     const bool wide = ldy % (f32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
     // columns n .. n + 64 of the 32 rows from mt on, from the two squares p and q; those of q at `shift` from p's instead of 32
     auto put = [&](const float16_t &p, const float16_t &q, int mt, int n, int end) __attribute__((always_inline)) {
@@ -830,7 +835,7 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
                 const int at = n0 + wn * 32, end = min(at + 32, width);
                 if (partial) {
                     put(acc[m][0], acc[m][0], mt, at, end);
-                    put(acc[m][1], acc[m][1], mt, width + at, width + end);
+                    put(acc[m][1], acc[m][1], mt, half + at, half + end);
                 } else {
                     float16_t v;
 #pragma unroll
@@ -841,7 +846,7 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
                 const int at = n0 + (wn * (TN / 2) + 2 * b) * 32;
                 if (partial) {
                     put(acc[m][2 * b], acc[m][2 * b + 1], mt, at, width);
-                    put(acc[m][TN / 2 + 2 * b], acc[m][TN / 2 + 2 * b + 1], mt, width + at, 2 * width);
+                    put(acc[m][TN / 2 + 2 * b], acc[m][TN / 2 + 2 * b + 1], mt, half + at, half + width);
                 } else {
                     float16_t u, v;
 #pragma unroll
@@ -858,16 +863,16 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
 
 // the pieces of a split over K, added in their order
 __global__ __launch_bounds__(256) void mxs_join_kernel(MxsArgs a) {
-    const int width = a.glu ? a.nrows / 2 : a.nrows;
-    const int64_t all = static_cast<int64_t>(a.M) * a.nrows;
+    const int width = a.glu ? a.nrows / 2 : a.nrows, half = part_half(a.nrows);
+    const int64_t all = static_cast<int64_t>(a.M) * (2 * half);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < static_cast<int64_t>(a.M) * width; i += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t m = i / width;
         const int n = static_cast<int>(i - m * width);
-        const float *p = a.part + m * a.nrows + n;
+        const float *p = a.part + m * (2 * half) + n;
         float v = 0.f, u = 0.f;
         for (int s = 0; s < a.splits; ++s) v += p[s * all];
         if (a.glu) {
-            for (int s = 0; s < a.splits; ++s) u += p[s * all + width];
+            for (int s = 0; s < a.splits; ++s) u += p[s * all + half];
             v = glu_value(v, u, a.gelu);
         }
         store_rounded(a.y, m * a.ldy + n, v, a.y_dtype);
@@ -1154,7 +1159,7 @@ extern "C" size_t mfq_hip_mx_scaled_gemm_workspace_bytes(int act, int nrows, int
     if ((act != 4 && act != 6) || nrows <= 0 || cols <= 0 || cols % 32 != 0 || M <= 0) return 0;
     const MxsPlan p = plan_linear(act, nrows, cols, M);
     size_t n = x_quantized || p.kind == 0 ? 0 : quantized_bytes(act, cols, M);
-    if (p.splits > 1) n += static_cast<size_t>(p.splits) * M * nrows * 4;
+    if (p.splits > 1) n += static_cast<size_t>(p.splits) * part_bytes(M, nrows);
     return n;
 }
 
@@ -1204,7 +1209,7 @@ extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scale
     }
     if (p.splits > 1) {
         // a short workspace: K in as many pieces as it has room for
-        const size_t left = workspace_bytes > used && ws ? workspace_bytes - used : 0, each = static_cast<size_t>(M) * nrows * 4;
+        const size_t left = workspace_bytes > used && ws ? workspace_bytes - used : 0, each = part_bytes(M, nrows);
         const int nmac = mx_macros(cols);
         if (left / each < static_cast<size_t>(p.splits)) p.splits = static_cast<int>(left / each);
         while (p.splits > 1 && (p.splits - 1) * ceil_div(nmac, p.splits) >= nmac) --p.splits;

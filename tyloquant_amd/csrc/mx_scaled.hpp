@@ -249,7 +249,7 @@ struct MxsArgs {
     int M, E, R, pairs, routed;
     int y_dtype, glu, gelu, x_dtype, x_wide;  // glu: gate rows first, nrows / 2 results; x_wide: xraw lies in pieces of 16 bytes
     int splits;
-    float *part;             // partial results of a split over K [splits][M][nrows]
+    float *part;             // partial results of a split over K [splits][M][2 part_half(nrows)]
 };
 
 }  // namespace mfq
