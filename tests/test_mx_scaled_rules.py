@@ -1,5 +1,9 @@
 """Rules of the products of microscaled operands on the host: sizes at their ends, and which kernel a call takes (nothing is launched)."""
 import ctypes as C
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 
@@ -69,3 +73,30 @@ def test_partial_sums_begin_on_16_bytes(lib, act, out):
     assert lib.mfq_hip_mx_scaled_plan(act, out, K, rows, 0, C.byref(pieces)) >= 5 and pieces.value > 1
     half, left = divmod(lib.mfq_hip_mx_scaled_gemm_workspace_bytes(act, out, K, rows, 1), pieces.value * rows * 2)
     assert left == 0 and half % 16 == 0 and half >= -(-out // 2) * 4
+
+
+def _plans_with(env):
+    """plans in a process that starts with these knobs: MXFP4 and MXFP6 of 12288 x 4096 at 601 rows and of 64 x 64 at 40, experts with 3, 30 and 300
+    pairs each"""
+    code = ("import ctypes as C\nfrom tyloquant_amd import _lib as L\nl, n = L.lib(), C.c_int()\nl.mfq_hip_set_cu_count(256)\n"
+            "for a in (4, 6):\n    for out, K, M in ((12288, 4096, 601), (64, 64, 40)):\n"
+            "        print(l.mfq_hip_mx_scaled_plan(a, out, K, M, 0, C.byref(n)), n.value)\n"
+            "    print(*[l.mfq_hip_mx_moe_plan(a, 2048, 8 * p, 8, 1, 0, 1) for p in (3, 30, 300)])\n")
+    root = Path(__file__).resolve().parents[1]
+    out = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": str(root), **env}, check=True, capture_output=True, text=True).stdout
+    return [[int(v) for v in line.split()] for line in out.splitlines()]
+
+
+def test_knobs_mean_one_thing():
+    """A tile is heeded by the calls of its kind and no other, pieces where K has as many groups, the experts' kernel by experts alone."""
+    plain = _plans_with({})
+    assert plain[2] == [1, 5, 8] and plain[5] == [1, 10, 11]
+    tile = _plans_with({"MFQ_MXS_TILE": "2"})       # 64 x 128 of MXFP4
+    assert tile[0][0] == tile[1][0] == 6 and tile[2:] == plain[2:]
+    tile = _plans_with({"MFQ_MXS_TILE": "8"})       # 256 x 192 of MXFP6
+    assert tile[3][0] == tile[4][0] == 12 and tile[:3] == plain[:3] and tile[5] == plain[5]
+    assert _plans_with({"MFQ_MXS_TILE": "9"}) == plain and _plans_with({"MFQ_MXS_SPLIT": "17"}) == plain
+    pieces = _plans_with({"MFQ_MXS_SPLIT": "4"})
+    assert [pieces[i][1] for i in (0, 3)] == [4, 4] and [pieces[i] for i in (1, 2, 4, 5)] == [plain[i] for i in (1, 2, 4, 5)]
+    experts = _plans_with({"MFQ_MXS_EXPERTS": "2"})
+    assert experts[2] == [5, 5, 5] and experts[5] == [10, 10, 10] and [experts[i] for i in (0, 1, 3, 4)] == [plain[i] for i in (0, 1, 3, 4)]

@@ -1024,14 +1024,17 @@ MxsPlan plan_linear(int act, int nrows, int K, int M) {
     if (M <= 16) return {1, 1};
     if (M <= 32) return {2, 1};
     static const int forced = tune_env("MFQ_MXS_TILE", 0), forced_split = tune_env("MFQ_MXS_SPLIT", 0);
+    // what the knobs ask for where the call can have it: a tile of its kind, pieces of which none is empty
+    const bool tile = forced > 0 && forced <= kMxsTiles && kMxsTile[forced - 1].act == act;
+    const auto whole = [&](int s) { return s <= nmac && (s - 1) * ceil_div(nmac, s) < nmac; };
+    const bool pieces = forced_split > 0 && forced_split <= kMaxSplits && whole(forced_split);
     const int cus = device_cu_count();
     MxsPlan best = {-1, 1};
     double least = 0.0;
     for (int t = 0; t < kMxsTiles; ++t) {
-        if (kMxsTile[t].act != act || (forced && forced != t + 1)) continue;
+        if (kMxsTile[t].act != act || (tile && forced != t + 1)) continue;
         for (int s = 1; s <= kMaxSplits && s <= nmac; ++s) {
-            // no piece may be empty
-            if ((s - 1) * ceil_div(nmac, s) >= nmac || (forced_split && s != forced_split)) continue;
+            if (!whole(s) || (pieces && s != forced_split)) continue;
             const double us = tile_us(kMxsTile[t], nrows, nmac, M, s, cus);
             if (best.kind < 0 || us < least) {
                 best = {kPlanTile + t, s};
@@ -1039,7 +1042,6 @@ MxsPlan plan_linear(int act, int nrows, int K, int M) {
             }
         }
     }
-    if (best.kind < 0) best = {kPlanTile + (act == 4 ? 2 : 6), 1};
     return best;
 }
 
@@ -1082,8 +1084,8 @@ int run_linear(const MxsArgs &a, const MxsPlan &p, hipStream_t st) {
 // and 2 tiles of 128 x 64 and 256 x 128.  128 experts of 2048 x 2048, gated, MXFP4, 8 routes: at 256 tokens (16 pairs an expert) 81, 64
 // and 75 us, at 2048 tokens 314, 126 and 140; 32 experts of 2880 x 1440, MXFP6, 4 routes: at 1501 tokens (188 pairs) 146, 80 and 65 us.
 int plan_mapped(int64_t pairs, int E) {
-    static const int forced = tune_env("MFQ_MXS_TILE", 0);
-    if (forced > 0) return forced < 3 ? forced - 1 : 2;
+    static const int forced = tune_env("MFQ_MXS_EXPERTS", 0);
+    if (forced > 0 && forced <= 3) return forced - 1;
     const int64_t mean = ceil_div(pairs, E);
     return mean <= 10 ? 0 : mean < 160 ? 1 : 2;
 }

@@ -56,8 +56,9 @@ Knob g_knobs[] = {
     {"MFQ_MX_STAGE_MAX_M", "rows up to which MX matmuls run as 16-row tiles with the activations staged in LDS (default 48)", 0, false},
     {"MFQ_MX_TILE_MAX_M", "rows up to which MX matmuls run on the tile kernel before the fp16 copy + GEMM (default 256)", 0, false},
     {"MFQ_MX_NB", "row-blocks per block of the MX tile kernel (0 = by shape)", 0, false},
-    {"MFQ_MXS_TILE", "tile of products of microscaled operands, 1 + its index (0 = by the model)", 0, false},
+    {"MFQ_MXS_TILE", "tile of a product of microscaled operands, 1 + its index in kMxsTile; only for its kind of activations (0 = by the model)", 0, false},
     {"MFQ_MXS_SPLIT", "pieces of K of a tiled product of microscaled operands (0 = by the model)", 0, false},
+    {"MFQ_MXS_EXPERTS", "kernel of routed experts of microscaled operands with a route map: 1 flow, 2 and 3 tiles of 128 x 64 and 256 x 128 (0 = by their pairs)", 0, false},
     {"MFQ_MX_WAVES", "waves per block the MX tile kernels split K over (0 = by shape)", 0, false},
     {"MFQ_NVQ_PAIRS_MFMA", "0 = a MoE decode step on an NVQ cohort always takes the generic one-row kernel", 0, false},
     {"MFQ_MOE_NB", "row-blocks per wave of the MoE streaming kernel (0 = by shape)", 0, false},
