@@ -21,10 +21,10 @@ __device__ __forceinline__ int mxs_total_tiles(const MxsArgs &a, int rows, int l
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
     return __builtin_amdgcn_readfirstlane(n);
 }
-// the expert that tile t belongs to, the number of its first tile and how many it has; t is below the total
-__device__ __forceinline__ void mxs_find_tile(const MxsArgs &a, int rows, int lane, int t, int &expert, int &first, int &count) {
+// the expert that tile t belongs to and the number of its first tile; t is below the total
+__device__ __forceinline__ void mxs_find_tile(const MxsArgs &a, int rows, int lane, int t, int &expert, int &first) {
     int before = 0;
-    expert = 0; first = 0; count = 0;
+    expert = 0; first = 0;
     for (int c = 0; c < a.E; c += 64) {
         const int n = mxs_tiles_of(a, c + lane, rows);
         int upto = n;
@@ -37,8 +37,7 @@ __device__ __forceinline__ void mxs_find_tile(const MxsArgs &a, int rows, int la
         if (over) {
             const int l = __ffsll(over) - 1;
             expert = c + l;
-            count = __builtin_amdgcn_readlane(n, l);
-            first = before + __builtin_amdgcn_readlane(upto, l) - count;
+            first = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
             return;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
@@ -84,8 +83,8 @@ __global__ __launch_bounds__(512) void mxs_stream_kernel(MxsArgs a) {
     if constexpr (MODE == kMapped) {
         if (blockIdx.x == 0) mxs_zero_rows(a, blockIdx.y, gridDim.y, tid, blockDim.x);
         if (static_cast<int>(blockIdx.y) >= mxs_total_tiles(a, 16 * MT, lane)) return;
-        int t0, count;
-        mxs_find_tile(a, 16 * MT, lane, blockIdx.y, expert, t0, count);
+        int t0;
+        mxs_find_tile(a, 16 * MT, lane, blockIdx.y, expert, t0);
         first = a.bounds[expert] + (static_cast<int>(blockIdx.y) - t0) * 16 * MT;
         rows = min(16 * MT, a.bounds[expert + 1] - first);
     } else {
@@ -268,7 +267,8 @@ __host__ __device__ __forceinline__ constexpr int rows_kept(int rows) { return r
 template <int AK, int MT, int NB, int D, int MODE, bool SMALL>
 __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
     using S = FlowShape<AK, MT, NB>;
-    static_assert(NB <= 2 && MT <= 2 && D >= 3 && (!SMALL || MT == 1), "a stage's scales are one request of four bytes a lane");
+    static_assert(NB <= 2 && MT <= 2 && (!SMALL || MT == 1), "a stage's scales are one request of four bytes a lane");
+    static_assert(D == 3, "the waits of the loop");
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, nwaves = blockDim.x >> 6;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -293,8 +293,8 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
     } else if constexpr (MODE == kMapped) {
         mxs_zero_rows(a, blockIdx.x, gridDim.x, tid, blockDim.x);
         if (tile >= mxs_total_tiles(a, 16 * MT, lane)) return;
-        int t0, count;
-        mxs_find_tile(a, 16 * MT, lane, tile, expert, t0, count);
+        int t0;
+        mxs_find_tile(a, 16 * MT, lane, tile, expert, t0);
         first = a.bounds[expert] + (tile - t0) * 16 * MT;
         rows = min(16 * MT, a.bounds[expert + 1] - first);
         if (a.slot) expert = a.slot[expert];
@@ -469,7 +469,6 @@ __global__ __launch_bounds__(512) void mxs_flow_kernel(MxsArgs a, int chunks) {
         // younger than this stage: those of the next D - 1 items, and the stores of results, which only make the wait longer
         const int left = items - 1 - i;
         if (left >= D - 1) wait_vmcnt<(D - 1) * S::REQ>();
-        else if (D > 3 && left == 2) wait_vmcnt<2 * S::REQ>();
         else if (left == 1) wait_vmcnt<S::REQ>();
         else wait_vmcnt<0>();
         const uint8_t *at = ring + stage * S::STAGE, *xat = xres + mac * xm;
@@ -774,7 +773,7 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
     uint8_t *y = reinterpret_cast<uint8_t *>(partial ? a.part + static_cast<int64_t>(blockIdx.y) * a.M * (2 * half) : a.y);
     const int64_t ldy = partial ? 2 * half : a.ldy;
     const bool wide = ldy % (f32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
-    // columns n .. n + 64 of the 32 rows from mt on, from the two squares p and q; those of q at `shift` from p's instead of 32
+    // columns n .. n + 64 of the 32 rows from mt on, from the two squares p and q; none from `end` on
     auto put = [&](const float16_t &p, const float16_t &q, int mt, int n, int end) __attribute__((always_inline)) {
         if (f32) {
 #pragma unroll

@@ -28,9 +28,7 @@
 
 namespace mfq {
 
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
-typedef short i16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kMxMacro = 256;  // columns of a macro
 
