@@ -510,7 +510,8 @@ int mfq_hip_mx_quantize_rows(int kind, const void *x, int x_dtype, int64_t ldx, 
 /* out[m][c] = element * scale in fp32, rounded once to out_dtype. */
 int mfq_hip_mx_dequant_quantized(int kind, const void *values, const void *scales, int M, int cols, int out_dtype, void *out,
                                  int64_t ldo, mfq_stream_t stream);
-/* Scales of an MXFP4 payload [rows, cols / 32] in that layout, in which the calls below take them (once, at load time). */
+/* Scales of an MXFP4 payload [rows, cols / 32] in that layout, in which the calls below take them (once, at load
+ * time; again, to the same place, where they are rewritten). */
 int mfq_hip_mx_lay_scales(const void *scales, int64_t rows, int cols, void *out, mfq_stream_t stream);
 /* y[M, nrows] = q(x) . W^T over rows [row0, row0 + nrows) of an MXFP4 tensor [rows, cols], fp32 accumulation, rounded once to
  * y_dtype (MFQ_X_*).  `scales`: those of all rows from mfq_hip_mx_lay_scales.  act: kind of q(x).  x is bf16, fp16 or fp32
