@@ -220,6 +220,18 @@ int mfq_hip_nint_gemv_argmax(const mfq_nint_desc *d, const void *weight, const v
                              int64_t ldx, int M, float *logits, int64_t ldl, int64_t *token,
                              void *workspace, size_t workspace_bytes, mfq_stream_t stream);
 
+/* Scores of an answer, from rows of logits [M, V] in bf16, fp16 or fp32 (dtype MFQ_X_*, ldl values from row to row), fp32 throughout:
+ *   logprob[m] = log softmax(logits[m])[tokens[m]], rank[m] = 1 + how many logits are above the token's;
+ *   entropy[m] = - sum p log p, masked logits (-infinity) adding nothing;
+ *   top_ids[m][i], top_logprobs[m][i], i < top <= 64: the most probable tokens in order, of equal logits the lower first.
+ * A token outside [0, V) (padding) has logprob 0 and rank 0.  A row that is masked throughout, or holds +infinity or a NaN, gives NaN
+ * (NaN logits are the last in order).  top = 0: top_ids and top_logprobs are not looked at.  Workspace: 16-byte aligned, size from the
+ * query (0 where there are many rows).  No counterpart in the reference; what it reads is what any LM head above returns. */
+size_t mfq_hip_token_logprobs_workspace_bytes(int M, int V, int top);
+int mfq_hip_token_logprobs(const void *logits, int dtype, int64_t ldl, int M, int V, const int64_t *tokens, int top,
+                           float *logprob, int64_t *rank, float *entropy, int64_t *top_ids, float *top_logprobs,
+                           void *workspace, size_t workspace_bytes, mfq_stream_t stream);
+
 /* mfq_hip_nint_gemv_argmax for callers that cannot allocate device memory or carry a workspace (code under HIP graph
  * capture, tight serving loops, harnesses that forbid allocation): the scratch is a 4 MiB device array built into the
  * library (one copy per GPU, held until the process ends).  No counterpart in the reference.  Same arguments and

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -356,6 +357,57 @@ def nint_matmul_argmax(w: NintWeight, x: torch.Tensor, return_logits: bool = Fal
     if x.dim() != 2:
         token = token.reshape(x.shape[:-1])
     return (token, _like_rows(logits, x)) if return_logits else token
+
+
+class TokenLogprobs(NamedTuple):
+    """Of every row: the given token's log probability and rank (1: none is above it), the entropy in nats, and the most probable
+    tokens in order with their log probabilities (empty where none were asked for)."""
+    logprobs: torch.Tensor
+    ranks: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+MAX_TOP_LOGPROBS = 64
+_LOGITS = {torch.float32: L.X_F32, torch.bfloat16: L.X_BF16, torch.float16: L.X_F16}
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Scores of an answer: logits [..., V] (what any LM head returns; fp32, bf16 or fp16, masked ones -inf) and one token id (int64)
+    a row.  fp32 results, ids and ranks int64; of equal logits the lower token comes first.  An id outside [0, V) marks padding: its
+    log probability and rank are 0.  Rows that are masked throughout, or hold +inf or a NaN, give NaN."""
+    code, shape = _LOGITS.get(logits.dtype), logits.shape
+    if code is None:
+        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if not shape or tokens.dtype != torch.int64 or tokens.shape != shape[:-1]:
+        raise ValueError(f"tokens must be int64 {tuple(shape[:-1])}, one for each row of logits, got {tokens.dtype} {tuple(tokens.shape)}")
+    V, top = shape[-1], int(top)
+    if not 0 <= top <= min(MAX_TOP_LOGPROBS, V):
+        raise ValueError(f"top must be in [0, min({MAX_TOP_LOGPROBS}, tokens)], got {top} of {V}")
+    here = torch._C._cuda_getDevice() if logits.is_cuda and tokens.is_cuda else -1
+    if here < 0 or logits.get_device() != here or tokens.get_device() != here:
+        raise ValueError(f"logits and tokens must be on the current GPU, got {logits.device} and {tokens.device}")
+    z = logits if len(shape) == 2 else logits.reshape(-1, V)
+    M = z.shape[0]
+    if z.stride(1) != 1 or (M > 1 and z.stride(0) < V):
+        z = z.contiguous()
+    tokens = tokens.contiguous()
+    scores = torch.empty((2, M), dtype=torch.float32, device=z.device)
+    ranks = torch.empty((M,), dtype=torch.int64, device=z.device)
+    ids = torch.empty((M, top), dtype=torch.int64, device=z.device)
+    best = torch.empty((M, top), dtype=torch.float32, device=z.device)
+    lp, entropy = scores[0], scores[1]
+    if M:
+        lib = L.lib()
+        need = lib.mfq_hip_token_logprobs_workspace_bytes(M, V, top)
+        ws = borrow(need, z.device)
+        L.check(lib.mfq_hip_token_logprobs(z.data_ptr(), code, z.stride(0), M, V, tokens.data_ptr(), top, lp.data_ptr(), ranks.data_ptr(),
+                                           entropy.data_ptr(), ids.data_ptr(), best.data_ptr(), _ptr(ws), need if ws is not None else 0, _stream()))
+    if len(shape) != 2:
+        lead = shape[:-1]
+        lp, ranks, entropy, ids, best = lp.reshape(lead), ranks.reshape(lead), entropy.reshape(lead), ids.reshape(*lead, top), best.reshape(*lead, top)
+    return TokenLogprobs(lp, ranks, entropy, ids, best)
 
 
 class NintLinearGroup:
