@@ -553,6 +553,41 @@ int mfq_hip_mx_moe_matmul(const void *values, const void *scales, int rows, int 
 int mfq_hip_mx_scaled_plan(int act, int nrows, int cols, int M, int glu, int *splits);
 int mfq_hip_mx_moe_plan(int act, int cols, int n_pairs, int E, int mapped, int glu, int x_quantized);
 
+/* Products of MXFP8 tensors (as they lie in the file) with activations quantised on the device to E4M3, one E8M0 scale for every 128
+ * columns of a row: the smallest power of two, 2^-127 at least, that brings the block's largest magnitude to 448 or below; elements to
+ * nearest, ties to even.  A block that holds an infinity or a NaN takes scale 255 (NaN) and codes 0.  No counterpart in the
+ * reference, which multiplies MXFP8 weights in fp16.
+ * Quantised rows: values [M, cols], 16-byte aligned; scales mfq_hip_mx8_scale_bytes(M, cols) bytes, 4-byte aligned,
+ * [groups of four blocks][M][4].  x: bf16, fp16 or fp32 [M, ldx]; cols must be divisible by 128. */
+int64_t mfq_hip_mx8_scale_bytes(int64_t rows, int cols);
+int mfq_hip_mx8_quantize_rows(const void *x, int x_dtype, int64_t ldx, int M, int cols, void *values, void *scales, mfq_stream_t stream);
+/* out[m][c] = element * scale in fp32, rounded once to out_dtype. */
+int mfq_hip_mx8_dequant_quantized(const void *values, const void *scales, int M, int cols, int out_dtype, void *out, int64_t ldo,
+                                  mfq_stream_t stream);
+/* y[M, nrows] = q(x) . W^T over rows [row0, row0 + nrows), row0 a multiple of 128, of an MXFP8 tensor [rows, cols] (values, and scales
+ * [ceil(rows / 128), cols / 128]), fp32 sums, rounded once to y_dtype (MFQ_X_*).  The matrix cores keep of FP8 products what leaves
+ * 5e-6 to 2e-5 of a result's size.  x is bf16, fp16 or fp32 [M, ldx] and quantised by the call (x_scales null), or the values of
+ * quantised rows with their x_scales (x_dtype and ldx are not looked at then).  glu != 0: gate rows first, y[M, nrows / 2] =
+ * act(gate) * up with `activation` MFQ_GLU_*, 16-bit y_dtype.  Rows of x that hold a NaN or an infinity give NaN.  cols up to 131072.
+ * Workspace (16-byte aligned, size from the query): the quantised rows, and partial sums of a split over K; without room for the latter
+ * K is split into fewer pieces.  Sums have a fixed order. */
+size_t mfq_hip_mx8_scaled_gemm_workspace_bytes(int nrows, int cols, int M, int x_quantized);
+int mfq_hip_mx8_scaled_gemm_rows(const void *values, const void *scales, int rows, int cols, int row0, int nrows, const void *x,
+                                 int x_dtype, int64_t ldx, const void *x_scales, int M, int glu, int activation, void *y, int y_dtype,
+                                 int64_t ldy, void *workspace, size_t workspace_bytes, mfq_stream_t stream);
+/* The same grouped by expert, as mfq_hip_mx_moe_matmul; experts of a pool of several are whole blocks of 128 rows.  Without a route map
+ * cols up to 20480. */
+size_t mfq_hip_mx8_moe_workspace_bytes(int cols, int x_rows, int n_pairs, int E, int mapped, int x_quantized);
+int mfq_hip_mx8_moe_matmul(const void *values, const void *scales, int rows, int cols, int out_per_expert, const int32_t *expert_slot,
+                           int E, const void *x, int x_dtype, int64_t ldx, const void *x_scales, int routed_input, const int32_t *ids,
+                           int T, int R, const int32_t *ids_dst, const int32_t *expert_bounds, int glu, int activation, void *y,
+                           int y_dtype, int64_t ldy, void *workspace, size_t workspace_bytes, mfq_stream_t stream);
+/* Test and tuning hooks, host only: the kernel of such a call.  0: few rows, quantised by its blocks; 1, 2: one or two tiles of 16
+ * quantised rows; 3 + i: tile i of kMx8Tile in csrc/mx8_scaled.hip, one tensor's with K in *splits pieces.  -1 for sizes that no
+ * call has. */
+int mfq_hip_mx8_scaled_plan(int nrows, int cols, int M, int *splits);
+int mfq_hip_mx8_moe_plan(int cols, int n_pairs, int E, int mapped);
+
 /* ------------------------------------------------------------------------------------
  * NEPQ1-S / NEPQ1-L (cross-expert table pool, bank id per 96 weights).  Rows are the
  * flattened [experts * out_per_expert] neurons.  Replaces NepqWeight

@@ -153,6 +153,16 @@ _SIGS = {
                               C.c_int, vp, vp, C.c_int, C.c_int, vp, C.c_int, i64, vp, sz, vp]),
     "mfq_hip_mx_scaled_plan": (C.c_int, [C.c_int] * 5 + [C.POINTER(C.c_int)]),
     "mfq_hip_mx_moe_plan": (C.c_int, [C.c_int] * 7),
+    "mfq_hip_mx8_scale_bytes": (i64, [i64, C.c_int]),
+    "mfq_hip_mx8_quantize_rows": (C.c_int, [vp, C.c_int, i64, C.c_int, C.c_int, vp, vp, vp]),
+    "mfq_hip_mx8_dequant_quantized": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, i64, vp]),
+    "mfq_hip_mx8_scaled_gemm_workspace_bytes": (sz, [C.c_int] * 4),
+    "mfq_hip_mx8_scaled_gemm_rows": (C.c_int, [vp, vp] + [C.c_int] * 4 + [vp, C.c_int, i64, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, i64, vp, sz, vp]),
+    "mfq_hip_mx8_moe_workspace_bytes": (sz, [C.c_int] * 6),
+    "mfq_hip_mx8_moe_matmul": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, i64, vp, C.c_int, vp, C.c_int, C.c_int, vp, vp,
+                               C.c_int, C.c_int, vp, C.c_int, i64, vp, sz, vp]),
+    "mfq_hip_mx8_scaled_plan": (C.c_int, [C.c_int] * 3 + [C.POINTER(C.c_int)]),
+    "mfq_hip_mx8_moe_plan": (C.c_int, [C.c_int] * 4),
     "mfq_hip_mx_gemm_rows": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, C.c_int, i64, C.c_int, vp, i64,
                                        vp, sz, vp]),
     "mfq_hip_nepq_plan": (C.c_int, [C.c_int] * 4 + [C.POINTER(NepqDesc)]),

@@ -1,0 +1,49 @@
+// Products of MXFP8 weights (E4M3FN bytes, a power of two for each block of 128 x 128) with activations quantised to E4M3, a power of
+// two for every 128 columns of a row:
+//   y[m, n] = sum over blocks b of 128 columns  2^(sw[n / 128, b] - 127) * 2^(sx[m, b] - 127) * sum_k w[n, k] * x[m, k]
+// v_mfma_scale_f32_16x16x128_f8f6f4 (32x32x64 for tiles) multiplies codes as they lie in memory and applies the scales itself; its sums
+// are held in fp32.  Of FP8 products it adds eight at a time, aligned to the largest, of which it keeps 14 bits: 5e-6 to 2e-5,
+// 2-norm, from the same sums in 64 bits, an eightieth of what rounding the result to bf16 costs.
+//
+// The scale of a block of activations is the smallest power of two, 2^-127 at least, that brings its largest magnitude to 448, the largest
+// element, or below: nothing saturates.  Elements are rounded to nearest, ties to even.  A block that holds an infinity or a NaN takes
+// scale 255 (NaN) and codes 0.
+//
+// Lanes of the 16 x 16 form, l = (r, g), r = l & 15, g = l >> 4: an operand holds 32 columns of row r; the result of lane l is row
+// 4 g + i of the first operand by row r of the second.  All columns of a block share their scales, so any 32 of its 128 may sit in lane g as
+// long as both operands agree.
+//
+// Quantised rows: values [M, K], scales by groups of four blocks, [ceil(K / 512)][M][4]: a word of scales serves four steps of 128 columns,
+// and the words of a tile's rows lie side by side.
+#pragma once
+#include "mx_scaled.hpp"
+
+namespace mfq {
+
+constexpr int kMx8Block = 128;
+__host__ __device__ __forceinline__ constexpr int64_t mx8_scale_bytes(int64_t rows, int K) { return (static_cast<int64_t>(K) / kMx8Block + 3) / 4 * rows * 4; }
+__host__ __device__ __forceinline__ constexpr int64_t mx8_scale_at(int64_t rows, int64_t row, int block) { return (static_cast<int64_t>(block >> 2) * rows + row) * 4 + (block & 3); }
+
+// the scale byte of a block from the bits of its largest magnitude as an fp32 (448 = 1.75 * 2^8)
+__device__ __forceinline__ uint32_t mx8_scale_of(uint32_t most) {
+    const int e = static_cast<int>(most >> 23);
+    return e == 255 ? 255u : static_cast<uint32_t>(max(e - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0), 0));
+}
+// four values divided by the power of two in the exponent field of `scale` (of which 0 is 2^-127), as E4M3
+__device__ __forceinline__ uint32_t mx8_codes(float a, float b, float c, float d, float scale) {
+    typedef short short2_t __attribute__((ext_vector_type(2)));
+    short2_t q = {0, 0};
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(q, a, b, scale, false);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(q, c, d, scale, true);
+    return __builtin_bit_cast(uint32_t, q);
+}
+
+__device__ __forceinline__ i32x8_t mx8_operand(u32x4_t lo, u32x4_t hi) {
+    return i32x8_t{static_cast<int>(lo.x), static_cast<int>(lo.y), static_cast<int>(lo.z), static_cast<int>(lo.w),
+                   static_cast<int>(hi.x), static_cast<int>(hi.y), static_cast<int>(hi.z), static_cast<int>(hi.w)};
+}
+
+// Rows to values and scales as above.  table (optional): written by one more block of the launch; M may be 0 then.
+int mx8_quantize_launch(const void *x, int x_dtype, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st, const MxTileTable *table = nullptr);
+
+}  // namespace mfq

@@ -5,55 +5,6 @@
 namespace mfq {
 namespace {
 
-enum MxsMode { kLinear = 0, kPairs = 1, kMapped = 2 };
-
-// ---- tiles of routed experts --------------------------------------------------------------------------------------------------
-// Rows of expert e, pairs bounds[e] .. bounds[e + 1] of the route map, are cut into tiles of `rows`.  Every wave finds its tile from the
-// bounds themselves, 64 experts at a time.
-__device__ __forceinline__ int mxs_tiles_of(const MxsArgs &a, int e, int rows) {
-    if (e >= a.E || (a.slot && a.slot[e] < 0)) return 0;
-    return (a.bounds[e + 1] - a.bounds[e] + rows - 1) / rows;
-}
-__device__ __forceinline__ int mxs_total_tiles(const MxsArgs &a, int rows, int lane) {
-    int n = 0;
-    for (int e = lane; e < a.E; e += 64) n += mxs_tiles_of(a, e, rows);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-    return __builtin_amdgcn_readfirstlane(n);
-}
-// the expert that tile t belongs to and the number of its first tile; t is below the total
-__device__ __forceinline__ void mxs_find_tile(const MxsArgs &a, int rows, int lane, int t, int &expert, int &first) {
-    int before = 0;
-    expert = 0; first = 0;
-    for (int c = 0; c < a.E; c += 64) {
-        const int n = mxs_tiles_of(a, c + lane, rows);
-        int upto = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int other = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += other;
-        }
-        const unsigned long long over = __ballot(before + upto > t);
-        if (over) {
-            const int l = __ffsll(over) - 1;
-            expert = c + l;
-            first = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
-            return;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
-    }
-}
-// Pairs whose expert id is none get rows of zeros: each block looks at its share of the pairs.
-__device__ __forceinline__ void mxs_zero_rows(const MxsArgs &a, int block, int blocks, int tid, int nt) {
-    const int cols = a.glu ? a.nrows / 2 : a.nrows, words = cols * (a.y_dtype == MFQ_X_F32 ? 2 : 1);  // of two bytes
-    for (int p = block; p < a.pairs; p += blocks) {
-        const int e = a.ids[p];
-        if (e >= 0 && e < a.E) continue;
-        uint16_t *row = static_cast<uint16_t *>(a.y) + static_cast<int64_t>(p) * a.ldy * (a.y_dtype == MFQ_X_F32 ? 2 : 1);
-        for (int i = tid; i < words; i += nt) row[i] = 0;
-    }
-}
-
 // ---- few rows, long K -------------------------------------------------------------------------------------------------------------
 // A block owns NB row-blocks of 16 neurons (with GLU one of gate rows and that of their up rows) and up to 16 * MT rows of activations; its
 // waves take the macros of K in turn, each through a ring of two stages of its own in LDS (no barrier in the loop), activations and weights
@@ -568,11 +519,6 @@ struct TileShape {
     static constexpr int STAGE = W + X + X2 + WS + XS;
     static constexpr int LDS = R * STAGE + BM * 4;  // and the rows of y
 };
-// Partial results of a split over K: rows of two halves, each a whole number of 16 bytes, so that the up rows' sums of a gated product begin on
-// such a boundary as well as the gate rows'.
-__host__ __device__ __forceinline__ constexpr int part_half(int nrows) { return ((nrows + 1) / 2 + 3) / 4 * 4; }
-constexpr int64_t part_bytes(int M, int nrows) { return static_cast<int64_t>(M) * part_half(nrows) * 8; }
-constexpr int kTilePitch = 64 * 4 + 16, kTileOut = 32 * kTilePitch;  // 64 results of 32 rows on their way out
 
 template <int AK, int BN, int BM, int WN, int WM, int R, int MODE>
 __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN * BM / (WN * WM) > 8192 ? 1 : 2))) void mxs_tile_kernel(MxsArgs a) {
@@ -764,100 +710,7 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // late copies must not land in reused LDS
     __syncthreads();
 
-    // Results leave through LDS so that the lanes of a store lie side by side in a row: two squares at a time, 32 rows of 64.
-    // The stores are nontemporal: results are not read here again, and kept in L2 they push out the operands that other tiles still read
-    // (8192 rows of FP4 by 17408 x 5120, bf16 out: 470 -> 445 us; 2048 rows of FP6 by 24576 x 4096, gated, fp16 out: 187 -> 177).
-    uint8_t *area = lds + wave * kTileOut;
-    const bool partial = a.splits > 1, f32 = partial || a.y_dtype == MFQ_X_F32;
-    const int half = part_half(a.nrows);  // of partial results: where the up rows' begin
-    uint8_t *y = reinterpret_cast<uint8_t *>(partial ? a.part + static_cast<int64_t>(blockIdx.y) * a.M * (2 * half) : a.y);
-    const int64_t ldy = partial ? 2 * half : a.ldy;
-    const bool wide = ldy % (f32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
-    // columns n .. n + 64 of the 32 rows from mt on, from the two squares p and q; none from `end` on
-    auto put = [&](const float16_t &p, const float16_t &q, int mt, int n, int end) __attribute__((always_inline)) {
-        if (f32) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                *reinterpret_cast<float4_t *>(area + r * kTilePitch + (8 * j + 4 * h) * 4) = float4_t{p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]};
-                *reinterpret_cast<float4_t *>(area + r * kTilePitch + (32 + 8 * j + 4 * h) * 4) = float4_t{q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]};
-            }
-            wave_sync();
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int row = k * 4 + (lane >> 4), c = n + (lane & 15) * 4, to_row = row_of[mt + row];
-                const float4_t v = *reinterpret_cast<const float4_t *>(area + row * kTilePitch + (lane & 15) * 16);
-                if (to_row < 0 || c >= end) continue;
-                float *o = reinterpret_cast<float *>(y) + static_cast<int64_t>(to_row) * ldy + c;
-                if (wide && c + 4 <= end) {
-                    __builtin_nontemporal_store(v, reinterpret_cast<float4_t *>(o));
-                } else {
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        if (c + t < end) o[t] = v[t];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                *reinterpret_cast<u32x2_t *>(area + r * kTilePitch + (8 * j + 4 * h) * 2) =
-                    u32x2_t{mx_pack16(p[4 * j], p[4 * j + 1], a.y_dtype), mx_pack16(p[4 * j + 2], p[4 * j + 3], a.y_dtype)};
-                *reinterpret_cast<u32x2_t *>(area + r * kTilePitch + (32 + 8 * j + 4 * h) * 2) =
-                    u32x2_t{mx_pack16(q[4 * j], q[4 * j + 1], a.y_dtype), mx_pack16(q[4 * j + 2], q[4 * j + 3], a.y_dtype)};
-            }
-            wave_sync();
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int row = k * 8 + (lane >> 3), c = n + (lane & 7) * 8, to_row = row_of[mt + row];
-                const u32x4_t v = *reinterpret_cast<const u32x4_t *>(area + row * kTilePitch + (lane & 7) * 16);
-                if (to_row < 0 || c >= end) continue;
-                uint16_t *o = reinterpret_cast<uint16_t *>(y) + static_cast<int64_t>(to_row) * ldy + c;
-                if (wide && c + 8 <= end) {
-                    __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t *>(o));
-                } else {
-#pragma unroll
-                    for (int t = 0; t < 8; ++t)
-                        if (c + t < end) o[t] = static_cast<uint16_t>(v[t >> 1] >> (16 * (t & 1)));
-                }
-            }
-        }
-        wave_sync();
-    };
-    static_for<TM>([&](auto MI) __attribute__((always_inline)) {
-        constexpr int m = MI.value;
-        const int mt = (wm * TM + m) * 32;
-        if (mt >= rows) return;
-        static_for<TN / 2>([&](auto BI) __attribute__((always_inline)) {
-            constexpr int b = BI.value;
-            if (!a.glu) {
-                put(acc[m][2 * b], acc[m][2 * b + 1], mt, n0 + (wn * TN + 2 * b) * 32, width);
-            } else if constexpr (TN == 2) {  // 32 columns: one square, twice
-                const int at = n0 + wn * 32, end = min(at + 32, width);
-                if (partial) {
-                    put(acc[m][0], acc[m][0], mt, at, end);
-                    put(acc[m][1], acc[m][1], mt, half + at, half + end);
-                } else {
-                    float16_t v;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = glu_value(acc[m][0][i], acc[m][1][i], a.gelu);
-                    put(v, v, mt, at, end);
-                }
-            } else if constexpr (b < TN / 4) {
-                const int at = n0 + (wn * (TN / 2) + 2 * b) * 32;
-                if (partial) {
-                    put(acc[m][2 * b], acc[m][2 * b + 1], mt, at, width);
-                    put(acc[m][TN / 2 + 2 * b], acc[m][TN / 2 + 2 * b + 1], mt, half + at, half + width);
-                } else {
-                    float16_t u, v;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        u[i] = glu_value(acc[m][2 * b][i], acc[m][TN / 2 + 2 * b][i], a.gelu);
-                        v[i] = glu_value(acc[m][2 * b + 1][i], acc[m][TN / 2 + 2 * b + 1][i], a.gelu);
-                    }
-                    put(u, v, mt, at, width);
-                }
-            }
-        });
-    });
+    mxs_tile_results<TM, TN>(a, acc, lds + wave * kTileOut, row_of, n0, wn, wm, rows, width, lane);
 }
 
 // the pieces of a split over K, added in their order
@@ -944,9 +797,6 @@ int launch_flow(const MxsArgs &a, int tiles, int busy, hipStream_t st) {
 }
 
 int tile_rows_mapped(int kind) { return kind == 1 ? 64 : 128; }
-// tiles of a call with a route map: at most
-int64_t tiles_mapped(int64_t pairs, int E, int rows) { return ceil_div(pairs, rows) + (E < pairs ? E : pairs); }
-
 template <int AK, int BN, int BM, int WN, int WM, int R, int MODE>
 int launch_tile(const MxsArgs &a, hipStream_t st) {
     using S = TileShape<AK, BN, BM, R>;
@@ -963,13 +813,17 @@ int launch_tile(const MxsArgs &a, hipStream_t st) {
     return check_launch("mx_scaled (tile)");
 }
 
-int launch_join(const MxsArgs &a, hipStream_t st) {
+}  // namespace
+
+int mxs_join_launch(const MxsArgs &a, hipStream_t st) {
     if (a.splits <= 1) return MFQ_OK;
     const int64_t n = static_cast<int64_t>(a.M) * (a.glu ? a.nrows / 2 : a.nrows);
     const int64_t blocks = ceil_div(n, 256);
     hipLaunchKernelGGL(mxs_join_kernel, dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, a);
     return check_launch("mx_scaled (join)");
 }
+
+namespace {
 
 // Kernel of a call: the flow kernel on rows that its blocks quantise (0), on one or two tiles of 16 rows (1, 2; the stream kernel where K is too long), or a
 // tile of the list (3 + its index) with K in `splits` pieces.
@@ -1219,7 +1073,7 @@ extern "C" int mfq_hip_mx_scaled_gemm_rows(const void *values, const void *scale
         a.part = reinterpret_cast<float *>(ws + used);
     }
     if (int rc = act == 4 ? run_linear<4>(a, p, st) : run_linear<6>(a, p, st)) return rc;
-    return launch_join(a, st);
+    return mxs_join_launch(a, st);
 }
 
 namespace {

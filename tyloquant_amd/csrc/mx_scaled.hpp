@@ -250,4 +250,166 @@ struct MxsArgs {
     float *part;             // partial results of a split over K [splits][M][2 part_half(nrows)]
 };
 
+enum MxsMode { kLinear = 0, kPairs = 1, kMapped = 2 };
+
+// ---- tiles of routed experts --------------------------------------------------------------------------------------------------
+// Rows of expert e, pairs bounds[e] .. bounds[e + 1] of the route map, are cut into tiles of `rows`.  Every wave finds its tile from the
+// bounds themselves, 64 experts at a time.
+__device__ __forceinline__ int mxs_tiles_of(const MxsArgs &a, int e, int rows) {
+    if (e >= a.E || (a.slot && a.slot[e] < 0)) return 0;
+    return (a.bounds[e + 1] - a.bounds[e] + rows - 1) / rows;
+}
+__device__ __forceinline__ int mxs_total_tiles(const MxsArgs &a, int rows, int lane) {
+    int n = 0;
+    for (int e = lane; e < a.E; e += 64) n += mxs_tiles_of(a, e, rows);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    return __builtin_amdgcn_readfirstlane(n);
+}
+// the expert that tile t belongs to and the number of its first tile; t is below the total
+__device__ __forceinline__ void mxs_find_tile(const MxsArgs &a, int rows, int lane, int t, int &expert, int &first) {
+    int before = 0;
+    expert = 0; first = 0;
+    for (int c = 0; c < a.E; c += 64) {
+        const int n = mxs_tiles_of(a, c + lane, rows);
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int other = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += other;
+        }
+        const unsigned long long over = __ballot(before + upto > t);
+        if (over) {
+            const int l = __ffsll(over) - 1;
+            expert = c + l;
+            first = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
+            return;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+}
+// Pairs whose expert id is none get rows of zeros: each block looks at its share of the pairs.
+__device__ __forceinline__ void mxs_zero_rows(const MxsArgs &a, int block, int blocks, int tid, int nt) {
+    const int cols = a.glu ? a.nrows / 2 : a.nrows, words = cols * (a.y_dtype == MFQ_X_F32 ? 2 : 1);  // of two bytes
+    for (int p = block; p < a.pairs; p += blocks) {
+        const int e = a.ids[p];
+        if (e >= 0 && e < a.E) continue;
+        uint16_t *row = static_cast<uint16_t *>(a.y) + static_cast<int64_t>(p) * a.ldy * (a.y_dtype == MFQ_X_F32 ? 2 : 1);
+        for (int i = tid; i < words; i += nt) row[i] = 0;
+    }
+}
+
+// tiles of a call with a route map: at most
+inline int64_t tiles_mapped(int64_t pairs, int E, int rows) { return ceil_div(pairs, rows) + (E < pairs ? E : pairs); }
+
+// Partial results of a split over K: rows of two halves, each a whole number of 16 bytes, so that the up rows' sums of a gated product begin on
+// such a boundary as well as the gate rows'.
+__host__ __device__ __forceinline__ constexpr int part_half(int nrows) { return ((nrows + 1) / 2 + 3) / 4 * 4; }
+constexpr int64_t part_bytes(int M, int nrows) { return static_cast<int64_t>(M) * part_half(nrows) * 8; }
+// the pieces of a split over K (a.splits), added in their order, gated where a.glu
+int mxs_join_launch(const MxsArgs &a, hipStream_t st);
+
+constexpr int kTilePitch = 64 * 4 + 16, kTileOut = 32 * kTilePitch;  // 64 results of 32 rows on their way out
+
+// A wave's TM x TN squares of 32 x 32 to y (or, of a split over K, to a.part): rows row_of[32 (wm TM + m) ..], neurons from n0 + 32 wn TN on, with
+// GLU the second half of the squares holding the up rows of the first half's gate rows.  area: kTileOut bytes of LDS that are the wave's.
+template <int TM, int TN>
+__device__ __forceinline__ void mxs_tile_results(const MxsArgs &a, const float16_t (&acc)[TM][TN], uint8_t *area, const int *row_of, int n0, int wn, int wm, int rows,
+                                                 int width, int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    // Results leave through LDS so that the lanes of a store lie side by side in a row: two squares at a time, 32 rows of 64.
+    // The stores are nontemporal: results are not read here again, and kept in L2 they push out the operands that other tiles still read
+    // (8192 rows of FP4 by 17408 x 5120, bf16 out: 470 -> 445 us; 2048 rows of FP6 by 24576 x 4096, gated, fp16 out: 187 -> 177).
+    const bool partial = a.splits > 1, f32 = partial || a.y_dtype == MFQ_X_F32;
+    const int half = part_half(a.nrows);  // of partial results: where the up rows' begin
+    uint8_t *y = reinterpret_cast<uint8_t *>(partial ? a.part + static_cast<int64_t>(blockIdx.y) * a.M * (2 * half) : a.y);
+    const int64_t ldy = partial ? 2 * half : a.ldy;
+    const bool wide = ldy % (f32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+    // columns n .. n + 64 of the 32 rows from mt on, from the two squares p and q; none from `end` on
+    auto put = [&](const float16_t &p, const float16_t &q, int mt, int n, int end) __attribute__((always_inline)) {
+        if (f32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                *reinterpret_cast<float4_t *>(area + r * kTilePitch + (8 * j + 4 * h) * 4) = float4_t{p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]};
+                *reinterpret_cast<float4_t *>(area + r * kTilePitch + (32 + 8 * j + 4 * h) * 4) = float4_t{q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]};
+            }
+            wave_sync();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int row = k * 4 + (lane >> 4), c = n + (lane & 15) * 4, to_row = row_of[mt + row];
+                const float4_t v = *reinterpret_cast<const float4_t *>(area + row * kTilePitch + (lane & 15) * 16);
+                if (to_row < 0 || c >= end) continue;
+                float *o = reinterpret_cast<float *>(y) + static_cast<int64_t>(to_row) * ldy + c;
+                if (wide && c + 4 <= end) {
+                    __builtin_nontemporal_store(v, reinterpret_cast<float4_t *>(o));
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        if (c + t < end) o[t] = v[t];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                *reinterpret_cast<u32x2_t *>(area + r * kTilePitch + (8 * j + 4 * h) * 2) =
+                    u32x2_t{mx_pack16(p[4 * j], p[4 * j + 1], a.y_dtype), mx_pack16(p[4 * j + 2], p[4 * j + 3], a.y_dtype)};
+                *reinterpret_cast<u32x2_t *>(area + r * kTilePitch + (32 + 8 * j + 4 * h) * 2) =
+                    u32x2_t{mx_pack16(q[4 * j], q[4 * j + 1], a.y_dtype), mx_pack16(q[4 * j + 2], q[4 * j + 3], a.y_dtype)};
+            }
+            wave_sync();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int row = k * 8 + (lane >> 3), c = n + (lane & 7) * 8, to_row = row_of[mt + row];
+                const u32x4_t v = *reinterpret_cast<const u32x4_t *>(area + row * kTilePitch + (lane & 7) * 16);
+                if (to_row < 0 || c >= end) continue;
+                uint16_t *o = reinterpret_cast<uint16_t *>(y) + static_cast<int64_t>(to_row) * ldy + c;
+                if (wide && c + 8 <= end) {
+                    __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t *>(o));
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 8; ++t)
+                        if (c + t < end) o[t] = static_cast<uint16_t>(v[t >> 1] >> (16 * (t & 1)));
+                }
+            }
+        }
+        wave_sync();
+    };
+    static_for<TM>([&](auto MI) __attribute__((always_inline)) {
+        constexpr int m = MI.value;
+        const int mt = (wm * TM + m) * 32;
+        if (mt >= rows) return;
+        static_for<TN / 2>([&](auto BI) __attribute__((always_inline)) {
+            constexpr int b = BI.value;
+            if (!a.glu) {
+                put(acc[m][2 * b], acc[m][2 * b + 1], mt, n0 + (wn * TN + 2 * b) * 32, width);
+            } else if constexpr (TN == 2) {  // 32 columns: one square, twice
+                const int at = n0 + wn * 32, end = min(at + 32, width);
+                if (partial) {
+                    put(acc[m][0], acc[m][0], mt, at, end);
+                    put(acc[m][1], acc[m][1], mt, half + at, half + end);
+                } else {
+                    float16_t v;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = glu_value(acc[m][0][i], acc[m][1][i], a.gelu);
+                    put(v, v, mt, at, end);
+                }
+            } else if constexpr (b < TN / 4) {
+                const int at = n0 + (wn * (TN / 2) + 2 * b) * 32;
+                if (partial) {
+                    put(acc[m][2 * b], acc[m][2 * b + 1], mt, at, width);
+                    put(acc[m][TN / 2 + 2 * b], acc[m][TN / 2 + 2 * b + 1], mt, half + at, half + width);
+                } else {
+                    float16_t u, v;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        u[i] = glu_value(acc[m][2 * b][i], acc[m][TN / 2 + 2 * b][i], a.gelu);
+                        v[i] = glu_value(acc[m][2 * b + 1][i], acc[m][TN / 2 + 2 * b + 1][i], a.gelu);
+                    }
+                    put(u, v, mt, at, width);
+                }
+            }
+        });
+    });
+}
+
 }  // namespace mfq

@@ -1,0 +1,170 @@
+"""Products of MXFP8 tensors with activations quantised to FP8 by blocks of 128 columns (see runtime.py, runtime_mx.py).
+
+The weights are the MXFP8 payloads of full-precision MFQ files as they lie in memory (runtime_mx.MxWeight): E4M3 with a power of two for
+each block of 128 x 128.  mx_matmul multiplies them with 16-bit activations; here activations are rounded to E4M3 with a power of two for
+every 128 columns of a row, and the matrix cores multiply the codes.  No counterpart in the reference.
+
+fp32 results carry what the matrix cores keep of FP8 products, 5e-6 to 2e-5 of a result's size; 16-bit ones do not show it."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib as L
+from .runtime import _ptr, _stream, borrow
+from .runtime_mx import _OUT, MxWeight, _here, _out_dtype, _raw_rows, _result_dtype
+
+BLOCK = 128
+
+
+def _columns(shape) -> int:
+    K = shape[-1] if len(shape) else 0
+    if K == 0 or K % BLOCK:
+        raise ValueError(f"MXFP8 columns must be divisible by 128, got {K}")
+    return K
+
+
+def _scale_shape(rows: int, K: int):
+    return -(-K // (4 * BLOCK)), rows, 4
+
+
+class Mx8Rows:
+    """Quantised activations [.., neuron_len]: E4M3 codes (uint8 [M, neuron_len]) and E8M0 scales (uint8 [groups of four blocks, M, 4]);
+    `shape` is that of the rows before quantisation."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, shape):
+        shape = tuple(shape)
+        K = _columns(shape)
+        rows = torch.Size(shape[:-1]).numel()
+        want = (rows, K), _scale_shape(rows, K)
+        if values.dtype != torch.uint8 or scales.dtype != torch.uint8 or (tuple(values.shape), tuple(scales.shape)) != want or \
+                not (values.is_contiguous() and scales.is_contiguous()) or values.device != scales.device:
+            raise ValueError(f"MXFP8 rows of {shape}: values {tuple(values.shape)} and scales {tuple(scales.shape)} must be contiguous uint8 "
+                             f"{want[0]} and {want[1]} on one device")
+        self._set(values, scales, shape, rows)
+
+    def _set(self, values, scales, shape, rows):
+        self.values, self.scales, self.shape, self.rows, self.neuron_len = values, scales, shape, rows, shape[-1]
+        return self
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """element x scale in fp32, rounded once to `dtype`."""
+        code = _out_dtype(dtype)
+        out = torch.empty(self.shape, dtype=dtype, device=self.values.device)
+        if self.rows:
+            _here(out)
+            L.check(L.lib().mfq_hip_mx8_dequant_quantized(self.values.data_ptr(), self.scales.data_ptr(), self.rows, self.neuron_len, code, out.data_ptr(),
+                                                          self.neuron_len, _stream()))
+        return out
+
+
+def mx8_quantize(x: torch.Tensor) -> Mx8Rows:
+    """Rows of bf16, fp16 or fp32 [..., K] to E4M3 with the smallest power of two for every 128 columns that brings the block's largest
+    magnitude to 448 or below; elements to nearest, ties to even.  A block that holds an infinity or a NaN becomes NaN."""
+    shape = tuple(x.shape)
+    K = _columns(shape)
+    x2 = _raw_rows(x, K)
+    _here(x2)
+    M = x2.shape[0]
+    values = torch.empty((M, K), dtype=torch.uint8, device=x2.device)
+    scales = torch.empty(_scale_shape(M, K), dtype=torch.uint8, device=x2.device)
+    if M:
+        L.check(L.lib().mfq_hip_mx8_quantize_rows(x2.data_ptr(), _OUT[x2.dtype], x2.stride(0), M, K, values.data_ptr(), scales.data_ptr(), _stream()))
+    return Mx8Rows.__new__(Mx8Rows)._set(values, scales, shape, M)
+
+
+def _weight(w: MxWeight) -> None:
+    if w.kind != 8:
+        raise ValueError(f"FP8 products take MXFP8 weights, not {w.dtype}: use mx_scaled_matmul")
+
+
+def _operand(x, K: int):
+    """(tensor, x_dtype, row stride, scales or None, rows, shape) of activations that come quantised or not"""
+    if isinstance(x, Mx8Rows):
+        if x.neuron_len != K:
+            raise ValueError(f"activation width {x.neuron_len} != neuron length {K}")
+        return x.values, 0, 0, x.scales, x.rows, x.shape
+    x2 = _raw_rows(x, K)
+    return x2, _OUT[x2.dtype], x2.stride(0), None, x2.shape[0], x.shape
+
+
+def _scaled(w: MxWeight, x, expert: int, glu: int, activation: int, out_dtype) -> torch.Tensor:
+    _weight(w)
+    row0, nrows = w._rows(expert)
+    K = w.neuron_len
+    x2, xd, ldx, xs, M, shape = _operand(x, K)
+    yd = _result_dtype(w, nrows, glu, out_dtype)
+    _here(x2)
+    _here(w.values)
+    width = nrows // 2 if glu else nrows
+    y = torch.empty((M, width), dtype=out_dtype, device=x2.device)
+    if M:
+        lib = L.lib()
+        key = (8, nrows, M, xs is None)
+        need = w._needs.get(key)
+        if need is None:
+            need = w.note_need(key, lib.mfq_hip_mx8_scaled_gemm_workspace_bytes(nrows, K, M, xs is not None))
+        ws = borrow(need, x2.device)
+        L.check(lib.mfq_hip_mx8_scaled_gemm_rows(w.values.data_ptr(), w.scales.data_ptr(), w.rows, K, row0, nrows, x2.data_ptr(), xd, ldx, _ptr(xs), M, glu,
+                                                 activation, y.data_ptr(), yd, width, _ptr(ws), need if ws is not None else 0, _stream()))
+    return y if len(shape) == 2 else y.reshape(*shape[:-1], width)
+
+
+def mx8_scaled_matmul(w: MxWeight, x, expert: int = 0, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """q(x) @ W^T of an MXFP8 tensor, fp32 sums rounded once to `out_dtype`.  x: bf16, fp16 or fp32 [..., K], quantised by the call, or
+    Mx8Rows.  mx_matmul is the product with unquantised activations."""
+    return _scaled(w, x, expert, 0, 0, out_dtype)
+
+
+def mx8_scaled_glu(w: MxWeight, x, activation: int = L.GLU_SILU, expert: int = 0, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """act(gate) * up of an MXFP8 gate/up tensor (gate rows first), in 16 bits."""
+    return _scaled(w, x, expert, 1, int(activation), out_dtype)
+
+
+def mx8_moe_into(w: MxWeight, x, route, out: torch.Tensor, routed: bool = False, glu: bool = False, activation: int = L.GLU_SILU,
+                 slot: torch.Tensor | None = None) -> torch.Tensor:
+    """The rows out[t, r] of the pairs whose expert `w` holds: expert e is the pool's slot[e] (device int32, -1 for the experts of other
+    pools, whose rows are left as they are), or e itself without `slot`; rows of ids that are none become zeros."""
+    _weight(w)
+    K, T, R = w.neuron_len, route.tokens, route.routes
+    x2, xd, ldx, xs, M, _ = _operand(x, K)
+    if M != (T * R if routed else T):
+        raise ValueError(f"MoE activations must be [{'tokens * routes' if routed else 'tokens'}, K]: {M} rows for {T} tokens of {R} routes")
+    if slot is None and w.n_experts != route.n_experts:
+        raise ValueError(f"{w.n_experts} experts, a route plan for {route.n_experts}")
+    if slot is not None and (slot.dtype != torch.int32 or slot.numel() != route.n_experts or not slot.is_contiguous()):
+        raise ValueError("expert slots must be int32 [experts] side by side")
+    yd = _result_dtype(w, w.out, glu, out.dtype)
+    width = w.out // 2 if glu else w.out
+    if tuple(out.shape) != (T, R, width) or not out.is_contiguous():
+        raise ValueError(f"MoE results must be contiguous {(T, R, width)}, got {tuple(out.shape)}")
+    for t in (x2, w.values, out, route.ids) if slot is None else (x2, w.values, out, route.ids, slot):
+        _here(t)
+    if T * R:
+        lib = L.lib()
+        mapped = route.ids_dst is not None
+        key = (8, M, T * R, route.n_experts, mapped, xs is None)
+        need = w._needs.get(key)
+        if need is None:
+            need = w.note_need(key, lib.mfq_hip_mx8_moe_workspace_bytes(K, M, T * R, route.n_experts, mapped, xs is not None))
+        ws = borrow(need, x2.device)
+        L.check(lib.mfq_hip_mx8_moe_matmul(w.values.data_ptr(), w.scales.data_ptr(), w.rows, K, w.out, _ptr(slot), route.n_experts, x2.data_ptr(), xd, ldx,
+                                           _ptr(xs), int(routed), route.ids.data_ptr(), T, R, _ptr(route.ids_dst) if mapped else None,
+                                           _ptr(route.expert_bounds) if mapped else None, int(glu), int(activation), out.data_ptr(), yd, width, _ptr(ws),
+                                           need if ws is not None else 0, _stream()))
+    return out
+
+
+def _moe_out(w: MxWeight, route, width: int, out_dtype) -> torch.Tensor:
+    _out_dtype(out_dtype)
+    return torch.empty((route.tokens, route.routes, width), dtype=out_dtype, device=w.values.device)
+
+
+def mx8_moe_matmul(w: MxWeight, x, route, routed: bool = False, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """[tokens, routes, out] of a pool of MXFP8 experts: every (token, route) pair of `route` (build_moe_route_plan) against its expert;
+    zeros where the id is none.  x has a row per token, with `routed` one per pair; quantised by the call, or Mx8Rows."""
+    return mx8_moe_into(w, x, route, _moe_out(w, route, w.out, out_dtype), routed)
+
+
+def mx8_moe_glu(w: MxWeight, x, route, activation: int = L.GLU_SILU, routed: bool = False, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """act(gate) * up of a pool of gate/up tensors, 16-bit [tokens, routes, out / 2]."""
+    return mx8_moe_into(w, x, route, _moe_out(w, route, w.out // 2, out_dtype), routed, True, activation)
