@@ -588,6 +588,27 @@ int mfq_hip_mx8_moe_matmul(const void *values, const void *scales, int rows, int
 int mfq_hip_mx8_scaled_plan(int nrows, int cols, int M, int *splits);
 int mfq_hip_mx8_moe_plan(int cols, int n_pairs, int E, int mapped);
 
+/* A whole layer of routed experts for up to 16 tokens in two launches, activations unquantised:
+ *   y[t] = sum_j p_j . D[e_j] (act(G[e_j] x[t]) * (U[e_j] x[t]))  (+ the same of an expert that all tokens take, times
+ *   sigmoid(shared_gate[t]) where shared_gate is not NULL)
+ * with e_j, p_j the top k of logits [T, experts] by the rules of mfq_hip_moe_topk, which are also written to ids[T, k] and weights[T, k].
+ * The place of mfq_hip_moe_topk, two grouped products and mfq_hip_moe_weighted_reduce for MX tensors: gate_up [experts * 2 * inter, hidden]
+ * (an expert's gate rows first), down [experts * hidden, inter]; shared_inter = 0: no shared expert.  kind 8: MXFP8 payloads as they lie;
+ * kind 4: MXFP4 values with scales from mfq_hip_mx_lay_scales.  Widths divisible by 128 (kind 8) or 32; at most 1024 experts, k <= 16.
+ * x: bf16 or fp16 [T, ldx]; y: y_dtype (MFQ_X_*) [T, ldy].  Products and sums are fp32's: the hidden rows are not rounded to 16 bits.
+ * A token is touched by its own experts alone, whatever the others' weights hold.  Workspace (16-byte aligned, size from the query):
+ * the hidden rows. */
+typedef struct mfq_mx_layer {
+    int32_t kind, experts, hidden, inter, shared_inter, reserved;
+    const void *gate_up, *gate_up_scales, *down, *down_scales;
+    const void *shared_gate_up, *shared_gate_up_scales, *shared_down, *shared_down_scales;
+} mfq_mx_layer;
+size_t mfq_hip_mx_moe_layer_workspace_bytes(const mfq_mx_layer *layer, int T, int k);
+int mfq_hip_mx_moe_layer(const mfq_mx_layer *layer, const void *x, int x_dtype, int64_t ldx, int T, const float *logits,
+                         const float *bias, int k, int mode, int normalize, float norm_floor, float scale, int activation,
+                         const float *shared_gate, int32_t *ids, float *weights, void *y, int y_dtype, int64_t ldy,
+                         void *workspace, size_t workspace_bytes, mfq_stream_t stream);
+
 /* ------------------------------------------------------------------------------------
  * NEPQ1-S / NEPQ1-L (cross-expert table pool, bank id per 96 weights).  Rows are the
  * flattened [experts * out_per_expert] neurons.  Replaces NepqWeight

@@ -57,6 +57,12 @@ class MoePool(C.Structure):
     _fields_ = [("desc", NintDesc), ("weight", vp)]
 
 
+class MxLayer(C.Structure):
+    _fields_ = [(n, i32) for n in ("kind", "experts", "hidden", "inter", "shared_inter", "reserved")] + \
+               [(n, vp) for n in ("gate_up", "gate_up_scales", "down", "down_scales", "shared_gate_up", "shared_gate_up_scales", "shared_down",
+                                  "shared_down_scales")]
+
+
 class MfqError(RuntimeError):
     pass
 
@@ -163,6 +169,9 @@ _SIGS = {
                                C.c_int, C.c_int, vp, C.c_int, i64, vp, sz, vp]),
     "mfq_hip_mx8_scaled_plan": (C.c_int, [C.c_int] * 3 + [C.POINTER(C.c_int)]),
     "mfq_hip_mx8_moe_plan": (C.c_int, [C.c_int] * 4),
+    "mfq_hip_mx_moe_layer_workspace_bytes": (sz, [C.POINTER(MxLayer), C.c_int, C.c_int]),
+    "mfq_hip_mx_moe_layer": (C.c_int, [C.POINTER(MxLayer), vp, C.c_int, i64, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, C.c_float, C.c_float, C.c_int,
+                             vp, vp, vp, vp, C.c_int, i64, vp, sz, vp]),
     "mfq_hip_mx_gemm_rows": (C.c_int, [C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, C.c_int, i64, C.c_int, vp, i64,
                                        vp, sz, vp]),
     "mfq_hip_nepq_plan": (C.c_int, [C.c_int] * 4 + [C.POINTER(NepqDesc)]),

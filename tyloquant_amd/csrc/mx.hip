@@ -11,6 +11,7 @@
 
 #include "common.hpp"
 #include "gemv_common.hpp"
+#include "mx_cvt.hpp"
 #include "tune.hpp"
 
 namespace mfq {
@@ -218,50 +219,6 @@ __global__ __launch_bounds__(256) void mx_gemv_kernel(MxK k, const uint16_t *__r
 // four dwords are two MFMAs' worth of k as they are (an MFMA does not care which k sits in which slot as long as both
 // operands agree).  A block of the grid owns NB row-blocks of 16 neurons and MT tiles of 16 rows; its waves split the
 // units of K; two units are in flight per wave.  LDS: waves * NB * MT * 1 KB for the sum over the waves.
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-
-template <int XF16>
-__device__ __forceinline__ float4_t mx_mfma(u32x4_t a, u32x4_t b, float4_t c) {
-    if constexpr (XF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-}
-// eight E2M1 codes of a dword -> eight values of the activations' type, times 2^(exponent field of scale - 127)
-template <int XF16>
-__device__ __forceinline__ u32x4_t mx_cvt_fp4(uint32_t q, float scale) {
-    u32x4_t b;
-    if constexpr (XF16) {
-        b.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, scale, 0));
-        b.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, scale, 1));
-        b.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, scale, 2));
-        b.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, scale, 3));
-    } else {
-        b.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 0));
-        b.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 1));
-        b.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 2));
-        b.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 3));
-    }
-    return b;
-}
-// eight E4M3FN codes of two dwords
-template <int XF16>
-__device__ __forceinline__ u32x4_t mx_cvt_fp8(uint32_t q0, uint32_t q1, float scale) {
-    u32x4_t b;
-    if constexpr (XF16) {
-        b.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q0, scale, false));
-        b.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q0, scale, true));
-        b.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q1, scale, false));
-        b.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q1, scale, true));
-    } else {
-        b.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q0, scale, false));
-        b.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q0, scale, true));
-        b.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q1, scale, false));
-        b.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q1, scale, true));
-    }
-    return b;
-}
-
 // SAL: a row's scale bytes start on a 4-byte boundary (MXFP4: cols % 128 == 0), one dword per unit; else four byte reads
 template <int KIND, int XF16, int NB, int MT, bool SAL>
 __global__ __launch_bounds__(1024) void mx_tile_kernel(MxK k, const uint16_t *__restrict__ x_in, int64_t ldx, int M_in,

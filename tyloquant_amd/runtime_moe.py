@@ -567,6 +567,89 @@ def nint_moe_ffn_forward(gate_up: NintMoeWeight, down: NintMoeWeight, x: torch.T
     return moe_weighted_reduce(dn, w, sh), ids, w
 
 
+MX_LAYER_TOKENS, MX_LAYER_EXPERTS = 16, 1024
+
+
+def _mx_scales(w) -> torch.Tensor:
+    return w.laid_scales() if w.kind == 4 else w.scales
+
+
+def _mx_layer(gate_up, down, shared) -> L.MxLayer:
+    """The layer's tensors for mfq_hip_mx_moe_layer; made at the first call and kept with gate_up while none of them has changed."""
+    tensors = (gate_up, down) + (tuple(shared) if shared is not None else ())
+    scales = tuple(_mx_scales(w) for w in tensors)
+    key = tuple(t.data_ptr() for w, s in zip(tensors, scales) for t in (w.values, s))
+    kept = getattr(gate_up, "_layer", None)
+    if kept is not None and kept[0] == key and kept[1] == tuple((w.rows, w.neuron_len, w.out) for w in tensors):
+        return kept[2]
+    if any(w.kind != gate_up.kind for w in tensors):
+        raise ValueError("a layer's tensors are all MXFP8 or all MXFP4: " + ", ".join(w.dtype for w in tensors))
+    E, H, I = gate_up.n_experts, gate_up.neuron_len, down.neuron_len
+    if down.n_experts != E or gate_up.out != 2 * I or down.out != H:
+        raise ValueError(f"incompatible gate_up [{E}, {gate_up.out}, {H}] and down [{down.n_experts}, {down.out}, {I}]")
+    S = 0
+    if shared is not None:
+        sgu, sdn = shared
+        S = sdn.neuron_len
+        if sgu.n_experts != 1 or sdn.n_experts != 1 or (sgu.out, sgu.neuron_len, sdn.out) != (2 * S, H, H):
+            raise ValueError(f"incompatible shared gate_up [{sgu.out}, {sgu.neuron_len}] and down [{sdn.out}, {S}] of a layer of width {H}")
+    if E > MX_LAYER_EXPERTS:
+        raise ValueError(f"a layer has at most {MX_LAYER_EXPERTS} experts, got {E}")
+    layer = L.MxLayer(gate_up.kind, E, H, I, S, 0, *(t.data_ptr() for w, s in zip(tensors, scales) for t in (w.values, s)))
+    gate_up._layer = (key, tuple((w.rows, w.neuron_len, w.out) for w in tensors), layer)
+    return layer
+
+
+def mx_moe_ffn_forward(gate_up, down, x: torch.Tensor, router_logits: torch.Tensor, top_k: int, use_sigmoid=False, use_sqrt_softplus=False,
+                       normalize=False, delayed_softmax=False, router_bias=None, router_scale=1.0, shared=None, shared_gate=None,
+                       activation: int = L.GLU_SILU, out_dtype=torch.float32):
+    """A layer of routed experts for a decode step of up to 16 tokens in two launches (mfq_hip_mx_moe_layer): top k of the router's logits
+    [tokens, experts] as moe_topk has it, gate and up, the activation, down and the weighted sum.  gate_up [experts * 2 * inter, hidden] and
+    down [experts * hidden, inter] are pools of MXFP8 or of MXFP4 experts (MxWeight); `shared` = (gate_up, down) of an expert that all
+    tokens take, times sigmoid(shared_gate) [tokens] where that is given.  x: bf16 or fp16 [tokens, hidden], unquantised, as are the
+    hidden rows (fp32).  Returns (out, ids, weights).  More tokens: moe_topk, build_moe_route_plan and mx8_moe_glu / mx8_moe_matmul
+    or mx_moe_glu / mx_moe_matmul."""
+    from .runtime_mx import _here, _out_dtype
+    if normalize and delayed_softmax:
+        raise ValueError("selected-weight normalization and delayed softmax are mutually exclusive")
+    if use_sigmoid + use_sqrt_softplus + delayed_softmax > 1:
+        raise ValueError("sigmoid, sqrt-softplus and delayed-softmax routing are mutually exclusive")
+    yd, xd, layer = _out_dtype(out_dtype), _x_dtype(x), _mx_layer(gate_up, down, shared)
+    T, H, E = x.shape[0], layer.hidden, layer.experts
+    if x.dim() != 2 or x.shape[1] != H or router_logits.shape != (T, E):
+        raise ValueError(f"a layer takes [tokens, {H}] activations and [tokens, {E}] router logits, got {tuple(x.shape)} and {tuple(router_logits.shape)}")
+    if T > MX_LAYER_TOKENS:
+        raise ValueError(f"a layer in two launches takes at most {MX_LAYER_TOKENS} tokens, got {T}")
+    if not 1 <= top_k <= min(16, E):
+        raise ValueError("top_k must be in [1, min(16, experts)]")
+    if shared_gate is not None and (shared is None or shared_gate.numel() != T):
+        raise ValueError("shared_gate is one logit a token, for a shared expert")
+    if x.stride(1) != 1 or (T > 1 and x.stride(0) < H):
+        x = x.contiguous()
+    logits = router_logits.float().contiguous()
+    bias = None if router_bias is None else router_bias.float().contiguous()
+    if bias is not None and bias.numel() != E:
+        raise ValueError("bias must be contiguous CUDA float32 [experts]")
+    gate = None if shared_gate is None else shared_gate.float().contiguous()
+    for t in (x, logits, bias, gate, gate_up.values, down.values):
+        if t is not None:
+            _here(t)
+    dev = x.device
+    out = torch.empty((T, H), dtype=out_dtype, device=dev)
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    if T:
+        lib = L.lib()
+        need = lib.mfq_hip_mx_moe_layer_workspace_bytes(C.byref(layer), T, top_k)
+        ws = borrow(need, dev)
+        mode = L.TOPK_DELAYED_SOFTMAX if delayed_softmax else L.TOPK_SIGMOID if use_sigmoid else \
+            L.TOPK_SQRT_SOFTPLUS if use_sqrt_softplus else L.TOPK_SOFTMAX
+        L.check(lib.mfq_hip_mx_moe_layer(C.byref(layer), x.data_ptr(), xd, x.stride(0), T, logits.data_ptr(), _ptr(bias), top_k, mode, int(normalize), 1e-20,
+                                         router_scale, int(activation), _ptr(gate), ids.data_ptr(), weights.data_ptr(), out.data_ptr(), yd, H,
+                                         _ptr(ws), need if ws is not None else 0, _stream()))
+    return out, ids, weights
+
+
 # ---------------------------------------------------------------------------------------
 # Expert residency: experts in pinned host memory, a GPU arena of slots for the ones in use
 # ---------------------------------------------------------------------------------------
