@@ -9,8 +9,11 @@ BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
 
 def oracle(z, tokens, top):
-    """in float64, on the CPU; ids by a stable sort: of equal logits the lower token first"""
-    z = z.detach().cpu().double().reshape(-1, z.shape[-1])
+    """in float64, on the CPU; ids by a stable sort: of equal logits the lower token first.  Ranks go by the differences to the largest logit as
+    fp32 has them."""
+    z = z.detach().cpu().float().reshape(-1, z.shape[-1])
+    below = z - torch.where(z.isnan(), -math.inf, z).amax(1, keepdim=True)
+    z = z.double()
     tokens = tokens.cpu().reshape(-1)
     lp = torch.log_softmax(z, 1)
     p = lp.exp()
@@ -19,7 +22,7 @@ def oracle(z, tokens, top):
     at = tokens.clamp(0, z.shape[1] - 1)[:, None]
     given = z.gather(1, at)
     logprob = torch.where(pad, torch.zeros(1, dtype=torch.float64), lp.gather(1, at)[:, 0])
-    rank = torch.where(pad, 0, 1 + (z > given).sum(1))
+    rank = torch.where(pad, 0, 1 + (below > below.gather(1, at)).sum(1))
     order = torch.sort(torch.where(z.isnan(), -math.inf, z), dim=1, descending=True, stable=True).indices
     last = torch.sort(z.isnan().gather(1, order).int(), dim=1, stable=True).indices      # NaN behind -infinity too
     order = order.gather(1, last)[:, :top]
@@ -129,6 +132,22 @@ def test_wide_rows_of_one_size():
     z[4] = z[4] * 40 - 500
     z[5, 11] = 90.0
     check(z, tokens, 5)
+
+
+@pytest.mark.parametrize("V", [3000, 40000])
+@pytest.mark.parametrize("M", [5, 1200])
+def test_ranks_beside_close_neighbours(M, V):
+    """logits above the token's that the difference to the largest tells from it or not: none, a few, more than a block keeps; far below the largest"""
+    z, tokens = logits(8, M, V, FP32)
+    many = {0: 0, 1: 3, 2: 63, 3: 64, 4: 500}
+    for row, n in many.items():
+        g = torch.Generator(device="cuda").manual_seed(row)
+        z[row, 7] = 0.1
+        at = torch.randperm(V - 8, generator=g, device="cuda")[:n] + 8
+        z[row, at] = 0.1 + torch.rand(n, generator=g, device="cuda") * 3e-6
+        z[row, V - 1] = 14.0 if row % 2 else 80.5
+        tokens[row] = 7
+    check(z, tokens, 3)
 
 
 def test_graph_and_streams():

@@ -360,7 +360,7 @@ def nint_matmul_argmax(w: NintWeight, x: torch.Tensor, return_logits: bool = Fal
 
 
 class TokenLogprobs(NamedTuple):
-    """Of every row: the given token's log probability and rank (1: none is above it), the entropy in nats, and the most probable
+    """Of every row: the given token's log probability and rank (1 + how many are more probable, by logit - max in fp32), the entropy in nats, and the most probable
     tokens in order with their log probabilities (empty where none were asked for)."""
     logprobs: torch.Tensor
     ranks: torch.Tensor
