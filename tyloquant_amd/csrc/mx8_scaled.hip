@@ -28,52 +28,80 @@ struct FewShape {
     static constexpr size_t MOST = kMaxDynamicLds - 16 * MT * 4;
 };
 
+// A lane's 32 columns of a block of 128, whose other three lanes are 16, 32 and 48 further: as they lie, and quantised.  16-bit values are compared
+// and converted in pairs as they are: less than half the instructions, and those of a wave's few rows come from memory with the launch.
 template <int XD>
-__device__ __forceinline__ void mx8_quantize_lane(const void *x, int64_t from, bool wide, u32x4_t &lo, u32x4_t &hi, uint32_t &byte) {
-    float v[32];
-    if constexpr (XD == MFQ_X_F32) {
-        const float *p = static_cast<const float *>(x) + from;
+struct LaneColumns {
+    static constexpr int PIECES = XD == MFQ_X_F32 ? 8 : 4;  // of 16 bytes
+    u32x4_t v[PIECES];
+};
+template <int XD>
+__device__ __forceinline__ void load_lane(const void *x, int64_t from, bool wide, LaneColumns<XD> &c) {
+    if (wide) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float4_t f;
-            if (wide) f = reinterpret_cast<const float4_t *>(p)[i];
-            else f = float4_t{p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]};
-#pragma unroll
-            for (int t = 0; t < 4; ++t) v[4 * i + t] = f[t];
-        }
+        for (int i = 0; i < c.PIECES; ++i) c.v[i] = reinterpret_cast<const u32x4_t *>(static_cast<const uint8_t *>(x) + from * (XD == MFQ_X_F32 ? 4 : 2))[i];
     } else {
-        const uint16_t *p = static_cast<const uint16_t *>(x) + from;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            u32x4_t f;
-            if (wide) {
-                f = reinterpret_cast<const u32x4_t *>(p)[i];
-            } else {
+        for (int i = 0; i < c.PIECES; ++i)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) f[t] = p[8 * i + 2 * t] | (static_cast<uint32_t>(p[8 * i + 2 * t + 1]) << 16);
+            for (int t = 0; t < 4; ++t) {
+                if constexpr (XD == MFQ_X_F32) {
+                    c.v[i][t] = static_cast<const uint32_t *>(x)[from + 4 * i + t];
+                } else {
+                    const uint16_t *p = static_cast<const uint16_t *>(x) + from + 8 * i + 2 * t;
+                    c.v[i][t] = p[0] | (static_cast<uint32_t>(p[1]) << 16);
+                }
             }
-#pragma unroll
-            for (int t = 0; t < 8; ++t) v[8 * i + t] = x_to_f32<XD == MFQ_X_F16>(static_cast<uint16_t>(f[t >> 1] >> (16 * (t & 1))));
-        }
     }
+}
+template <int XD>
+__device__ __forceinline__ void quantize_lane(const LaneColumns<XD> &x, u32x4_t &lo, u32x4_t &hi, uint32_t &byte) {
+    typedef short short2_t __attribute__((ext_vector_type(2)));
+    const auto &v = x.v;
     uint32_t most = 0;
+    if constexpr (XD == MFQ_X_F32) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
-    // the block's four lanes
+        for (int i = 0; i < 32; ++i) most = max(most, v[i >> 2][i & 3] & 0x7fffffffu);
+    } else {
+        u16x2_t pair = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t two = v[i >> 2][i & 3] & 0x7fff7fffu;
+            pair = __builtin_elementwise_max(pair, __builtin_bit_cast(u16x2_t, two));
+        }
+        const uint32_t m = max(pair.x, pair.y);
+        // of fp16 as an fp32 has it, infinities and NaN with theirs
+        most = XD == MFQ_X_BF16 ? m << 16 : m >= 0x7c00u ? 0x7f800000u : __float_as_uint(f16_to_f32(static_cast<uint16_t>(m)));
+    }
     most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16, 64)));
     most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32, 64)));
     byte = mx8_scale_of(most);
     const float scale = __uint_as_float(byte << 23);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        lo[i] = mx8_codes(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], scale);
-        hi[i] = mx8_codes(v[16 + 4 * i], v[17 + 4 * i], v[18 + 4 * i], v[19 + 4 * i], scale);
+    for (int i = 0; i < 8; ++i) {
+        uint32_t q;
+        if constexpr (XD == MFQ_X_F32) {
+            q = mx8_codes(__uint_as_float(v[i][0]), __uint_as_float(v[i][1]), __uint_as_float(v[i][2]), __uint_as_float(v[i][3]), scale);
+        } else {
+            const uint32_t a = v[i >> 1][2 * (i & 1)], b = v[i >> 1][2 * (i & 1) + 1];
+            short2_t c = {0, 0};
+            if constexpr (XD == MFQ_X_F16) {
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, __builtin_bit_cast(half2_t, a), scale, false);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, __builtin_bit_cast(half2_t, b), scale, true);
+            } else {
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2_t, a), scale, false);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2_t, b), scale, true);
+            }
+            q = __builtin_bit_cast(uint32_t, c);
+        }
+        (i < 4 ? lo : hi)[i & 3] = byte == 255u ? 0u : q;
     }
-    if (byte == 255u) lo = hi = u32x4_t{0u, 0u, 0u, 0u};
 }
 
+__device__ __forceinline__ void pin(i32x8_t &v) { asm volatile("" : "+v"(v)); }
+
 template <int MT, int NB, int NM>
-__global__ __launch_bounds__(512) void mx8_few_kernel(MxsArgs a, int mode, int chunks, int scale_rows) {
+__global__ __launch_bounds__(512, MT * NM <= 8 ? 4 : 2) void mx8_few_kernel(MxsArgs a, int mode, int chunks, int scale_rows) {
     using S = FewShape<MT, NB>;
     constexpr int D = S::D;
     static_assert(D == 2 || D == 3, "the waits of the loop");
@@ -110,7 +138,9 @@ __global__ __launch_bounds__(512) void mx8_few_kernel(MxsArgs a, int mode, int c
     auto pair_of = [&](int m) { return mode == kPairs ? tile : mode == kMapped ? a.ids_dst[first + m] : m0 + m; };
 
     const int rbs = (width + 15) / 16;
-    const int rb0 = static_cast<int>(static_cast<int64_t>(rbs) * chunk / chunks), rb1 = static_cast<int>(static_cast<int64_t>(rbs) * (chunk + 1) / chunks);
+    // the first blocks of a tile have a row-block more than the last: those that come second to a compute unit
+    const int each = rbs / chunks, more = rbs - each * chunks;
+    const int rb0 = chunk * each + min(chunk, more), rb1 = rb0 + each + (chunk < more ? 1 : 0);
     const int mine = (nkb - wave + nwaves - 1) / nwaves;  // blocks wave, wave + nwaves, ... of K
     const int total = (rb1 - rb0) * mine;
 
@@ -142,53 +172,88 @@ __global__ __launch_bounds__(512) void mx8_few_kernel(MxsArgs a, int mode, int c
         }
     };
 
-    // scales of the weights: those of the rows' blocks of 128, all of K
+    // The first weights are asked for, then what else a wave needs before it can use them, then the next weights: behind all of a wave's
+    // weights the activations would come late, in front of them the weights.
+    if (total > 0) issue();
+    // scales of the weights: those of the rows' blocks of 128, all of K; a byte a thread does for all but long shares
     uint8_t *scales = lds + nwaves * (D * S::STAGE + 2 * S::RED);
     const int row_base = a.row0 + expert * a.nrows;
+    int scale_count[NB];
+    const uint8_t *scale_from[NB];
+    uint32_t scale_first[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int f = (row_base + b * width + rb0 * 16) >> 7, l = (row_base + b * width + min(rb1 * 16, width) - 1) >> 7;
-        for (int i = tid; i < (l - f + 1) * nkb; i += blockDim.x) scales[b * scale_rows * nkb + i] = a.ws[static_cast<int64_t>(f) * nkb + i];
+        scale_count[b] = (l - f + 1) * nkb;
+        scale_from[b] = a.ws + static_cast<int64_t>(f) * nkb;
+        scale_first[b] = scale_from[b][min(tid, scale_count[b] - 1)];
     }
 
-    // the activations, as operands: before the first weights are asked for, behind which these reads would come
+    // the activations, as operands: the reads of two or four blocks of K are in flight together
     i32x8_t x[NM][MT];
     uint32_t sx[(NM + 3) / 4][MT];
 #pragma unroll
     for (int m = 0; m < (NM + 3) / 4; ++m)
 #pragma unroll
         for (int t = 0; t < MT; ++t) sx[m][t] = 0u;
+    int64_t src[MT];
+    bool live[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        const int row = 16 * t + r;
-        const bool live = row < rows;
-        const int p = live ? pair_of(row) : 0;
-        const int64_t src = mode == kLinear || a.routed ? p : p / a.R;
+        live[t] = 16 * t + r < rows;
+        const int p = pair_of(min(16 * t + r, rows - 1));
+        src[t] = mode == kLinear || a.routed ? p : p / a.R;
+    }
+    const auto keep = [&](int m, int t, u32x4_t lo, u32x4_t hi, uint32_t byte) __attribute__((always_inline)) {
+        const bool use = live[t] && m < mine;
+        const u32x4_t none = {0u, 0u, 0u, 0u};
+        x[m][t] = mx8_operand(use ? lo : none, use ? hi : none);
+        sx[m >> 2][t] |= (use ? byte : 0u) << (8 * (m & 3));
+    };
+    const auto block_of = [&](int m) { return min(wave + m * nwaves, nkb - 1); };
+    const auto quantize = [&](auto XD) __attribute__((always_inline)) {
+        constexpr int TYPE = XD.value, GROUP = TYPE == MFQ_X_F32 || NM > 4 ? 2 : 4;
+        static_for<MT * NM / GROUP>([&](auto Q) __attribute__((always_inline)) {
+            constexpr int t = Q.value / (NM / GROUP), m0 = Q.value % (NM / GROUP) * GROUP;
+            LaneColumns<TYPE> c[GROUP];
 #pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            u32x4_t lo = {0u, 0u, 0u, 0u}, hi = lo;
-            uint32_t byte = 0;
-            const int kb = wave + m * nwaves;
-            if (m < mine && live) {  // the four lanes of a row agree
-                if (a.xraw) {
-                    const int64_t from = src * a.ldx + kb * kMx8Block + 32 * g;
-                    if (a.x_dtype == MFQ_X_F32) mx8_quantize_lane<MFQ_X_F32>(a.xraw, from, a.x_wide, lo, hi, byte);
-                    else if (a.x_dtype == MFQ_X_F16) mx8_quantize_lane<MFQ_X_F16>(a.xraw, from, a.x_wide, lo, hi, byte);
-                    else mx8_quantize_lane<MFQ_X_BF16>(a.xraw, from, a.x_wide, lo, hi, byte);
-                } else {
-                    const u32x4_t *q = reinterpret_cast<const u32x4_t *>(a.xv + src * a.K + kb * kMx8Block + 32 * g);
-                    lo = q[0];
-                    hi = q[1];
-                    byte = a.xs[mx8_scale_at(a.M, src, kb)];
-                }
+            for (int m = 0; m < GROUP; ++m) load_lane<TYPE>(a.xraw, src[t] * a.ldx + block_of(m0 + m) * kMx8Block + 32 * g, a.x_wide, c[m]);
+#pragma unroll
+            for (int m = 0; m < GROUP; ++m) {
+                u32x4_t lo, hi;
+                uint32_t byte;
+                quantize_lane<TYPE>(c[m], lo, hi, byte);
+                keep(m0 + m, t, lo, hi, byte);
             }
-            x[m][t] = mx8_operand(lo, hi);
-            sx[m >> 2][t] |= byte << (8 * (m & 3));
+            // operands now, not where they are used: what they are made of takes twice the registers
+#pragma unroll
+            for (int m = 0; m < GROUP; ++m) pin(x[m0 + m][t]);
+        });
+    };
+    static_assert(NM % 2 == 0 && (MT == 2 || NM % 4 == 0), "whole groups");
+    if (a.xraw) {
+        if constexpr (MT == 1) {  // more rows come quantised
+            if (a.x_dtype == MFQ_X_BF16) quantize(std::integral_constant<int, MFQ_X_BF16>{});
+            else if (a.x_dtype == MFQ_X_F16) quantize(std::integral_constant<int, MFQ_X_F16>{});
+            else quantize(std::integral_constant<int, MFQ_X_F32>{});
         }
+    } else {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+                const u32x4_t *q = reinterpret_cast<const u32x4_t *>(a.xv + src[t] * a.K + block_of(m) * kMx8Block + 32 * g);
+                keep(m, t, q[0], q[1], a.xs[mx8_scale_at(a.M, src[t], block_of(m))]);
+            }
     }
 #pragma unroll
-    for (int i = 0; i < D; ++i)
+    for (int i = 1; i < D; ++i)
         if (i < total) issue();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        if (tid < scale_count[b]) scales[b * scale_rows * nkb + tid] = static_cast<uint8_t>(scale_first[b]);
+        for (int i = tid + blockDim.x; i < scale_count[b]; i += blockDim.x) scales[b * scale_rows * nkb + i] = scale_from[b][i];
+    }
 
     const int results = MT * 256;  // of a row-block; result o: row o / 16, neuron o % 16
     __shared__ int row_of[16 * MT];
@@ -277,7 +342,7 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
     using S = Tile8Shape<BN, BM, R>;
     constexpr int NW = WN * WM, TN = BN / 32 / WN, TM = BM / 32 / WM;
     // requests of a wave for a stage; every wave issues as many, some twice
-    constexpr int CW = BN / 8, CX = BM / 8, PW = (CW + NW - 1) / NW, PX = (CX + NW - 1) / NW, PER = PW + PX;
+    constexpr int CW = BN / 8, CX = BM / 8, PW = (CW + NW - 1) / NW, PX = (CX + NW - 1) / NW, PER = PW + PX + 1;
     static_assert(TN % 2 == 0 && R >= 2 && BM / 64 <= NW, "gate and up in one wave, words of scales by a wave for 64 rows");
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -359,21 +424,21 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
         const int q = min(wave + NW * p, CX - 1);
         xv[p] = static_cast<uint32_t>(src_of(min(q * 8 + (lane >> 3), rows - 1)) - base) * static_cast<uint32_t>(a.K) + 16u * (q & 1 ? wq : wp);
     }
-    const uint32_t xsv = wave < BM / 64 ? static_cast<uint32_t>(src_of(min(wave * 64 + lane, rows - 1))) * 4u : 0u;
+    const uint32_t xsv = static_cast<uint32_t>(src_of(min(wave % (BM / 64) * 64 + lane, rows - 1))) * 4u;
 
     // Stages behind the last one: the last one again, where nobody reads it.
     const int per_split = (nkb + a.splits - 1) / a.splits;
     const int st0 = static_cast<int>(blockIdx.y) * per_split, st1 = min(nkb, st0 + per_split);
-    auto issue = [&](uint32_t buffer, int want) {
-        const int st = min(want, st1 - 1);
-        uint8_t *to = lds + buffer;
-        // before the codes: a wait that counts the codes of younger stages then covers it
-        if (((st & 3) == 0 || want == st0) && wave < BM / 64 && want == st)
-            copy4(xswin, lds + S::XS + ((st >> 2) & 1) * (BM * 4) + wave * 256, xsv + static_cast<uint32_t>(st >> 2) * static_cast<uint32_t>(a.M) * 4u, 0);
-#pragma unroll
-        for (int p = 0; p < PW; ++p) copy16<0>(win, to + min(wave + NW * p, CW - 1) * 1024, wv[p], st * kMx8Block);
-#pragma unroll
-        for (int p = 0; p < PX; ++p) copy16<0>(xwin, to + S::W + min(wave + NW * p, CX - 1) * 1024, xv[p], st * kMx8Block);
+    // the words that stage st's scales are bytes of: with every stage, though they serve four, and in every wave, though a few would do, so that
+    // the loop has no branch, behind which the compiler would sink the products
+    auto copy_scales = [&](int st) __attribute__((always_inline)) {
+        copy4(xswin, lds + S::XS + ((st >> 2) & 1) * (BM * 4) + wave % (BM / 64) * 256, xsv + static_cast<uint32_t>(st >> 2) * static_cast<uint32_t>(a.M) * 4u, 0);
+    };
+    auto copy_codes = [&](uint32_t buffer, int st, auto P) __attribute__((always_inline)) {
+        constexpr int p = P.value;
+        if constexpr (p == PW + PX) copy_scales(st);
+        else if constexpr (p < PW) copy16<0>(win, lds + buffer + min(wave + NW * p, CW - 1) * 1024, wv[p], st * kMx8Block);
+        else copy16<0>(xwin, lds + buffer + S::W + min(wave + NW * (p - PW), CX - 1) * 1024, xv[p - PW], st * kMx8Block);
     };
 
     float16_t acc[TM][TN];
@@ -384,63 +449,78 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
 
-    i32x8_t w0[TN], w1[TN], x0[TM], x1[TM];
+    u32x4_t w0[TN][2], w1[TN][2], x0[TM][2], x1[TM][2];
     uint32_t sw[TN], sx[TM];
     const uint32_t key = (r >> 1) & 7, line = r * 128;
-    auto read_codes = [&](uint32_t buffer, int half, i32x8_t (&w)[TN], i32x8_t (&x)[TM]) __attribute__((always_inline)) {
-        const uint32_t lo = buffer + line + (((4 * h + 2 * half) ^ key) << 4), hi = buffer + line + (((4 * h + 2 * half + 1) ^ key) << 4);
-#pragma unroll
-        for (int n = 0; n < TN; ++n)
-            w[n] = mx8_operand(*reinterpret_cast<const u32x4_t *>(lds + lo + (wn * TN + n) * 4096), *reinterpret_cast<const u32x4_t *>(lds + hi + (wn * TN + n) * 4096));
-#pragma unroll
-        for (int m = 0; m < TM; ++m)
-            x[m] = mx8_operand(*reinterpret_cast<const u32x4_t *>(lds + lo + S::W + (wm * TM + m) * 4096),
-                               *reinterpret_cast<const u32x4_t *>(lds + hi + S::W + (wm * TM + m) * 4096));
+    // read q of half a stage's fragments
+    constexpr int READS = 2 * (TN + TM), SQUARES = TM * TN;
+    auto read_codes = [&](uint32_t buffer, int half, u32x4_t (&w)[TN][2], u32x4_t (&x)[TM][2], auto Q) __attribute__((always_inline)) {
+        constexpr int f = Q.value / 2, s = Q.value % 2;
+        const uint32_t at = buffer + line + (((4 * h + 2 * half + s) ^ key) << 4);
+        if constexpr (f < TN) w[f][s] = *reinterpret_cast<const u32x4_t *>(lds + at + (wn * TN + f) * 4096);
+        else x[f - TN][s] = *reinterpret_cast<const u32x4_t *>(lds + at + S::W + (wm * TM + f - TN) * 4096);
     };
-    // the scales of stage st in the lowest byte: the next byte of the word, or the next word
-    auto next_scales = [&](int st, bool fresh) __attribute__((always_inline)) {
-        if ((st & 3) == 0 || fresh) {
-            const uint32_t at = S::XS + ((st >> 2) & 1) * (BM * 4) + r * 4;
+    // the words of stage st's scales, and its scales in their lowest bytes
+    uint32_t ww[TN], wx[TM];
+    auto read_scales = [&](int st) __attribute__((always_inline)) {
+        const uint32_t at = S::XS + ((st >> 2) & 1) * (BM * 4) + r * 4;
 #pragma unroll
-            for (int n = 0; n < TN; ++n) sw[n] = *reinterpret_cast<const uint32_t *>(lds + wsv[n] + (st >> 2) * 4) >> (8 * (st & 3));
+        for (int n = 0; n < TN; ++n) ww[n] = *reinterpret_cast<const uint32_t *>(lds + wsv[n] + (st >> 2) * 4);
 #pragma unroll
-            for (int m = 0; m < TM; ++m) sx[m] = *reinterpret_cast<const uint32_t *>(lds + at + (wm * TM + m) * 128) >> (8 * (st & 3));
-        } else {
-#pragma unroll
-            for (int n = 0; n < TN; ++n) sw[n] >>= 8;
-#pragma unroll
-            for (int m = 0; m < TM; ++m) sx[m] >>= 8;
-        }
+        for (int m = 0; m < TM; ++m) wx[m] = *reinterpret_cast<const uint32_t *>(lds + at + (wm * TM + m) * 128);
     };
-    auto multiply = [&](const i32x8_t (&w)[TN], const i32x8_t (&x)[TM]) __attribute__((always_inline)) {
+    auto take_scales = [&](int st) __attribute__((always_inline)) {
 #pragma unroll
-        for (int m = 0; m < TM; ++m)
+        for (int n = 0; n < TN; ++n) sw[n] = ww[n] >> (8 * (st & 3));
 #pragma unroll
-            for (int n = 0; n < TN; ++n) acc[m][n] = mx8_mfma32(w[n], x[m], acc[m][n], sw[n], sx[m]);
+        for (int m = 0; m < TM; ++m) sx[m] = wx[m] >> (8 * (st & 3));
     };
-
-#pragma unroll
-    for (int i = 0; i < R; ++i) issue(i * S::STAGE, st0 + i);
+    auto multiply = [&](const u32x4_t (&w)[TN][2], const u32x4_t (&x)[TM][2], auto Q) __attribute__((always_inline)) {
+        constexpr int m = Q.value / TN, n = Q.value % TN;
+        acc[m][n] = mx8_mfma32(mx8_operand(w[n][0], w[n][1]), mx8_operand(x[m][0], x[m][1]), acc[m][n], sw[n], sx[m]);
+    };
+    static_for<R>([&](auto I) __attribute__((always_inline)) {
+        static_for<PER>([&](auto P) __attribute__((always_inline)) { copy_codes(I.value * S::STAGE, min(st0 + static_cast<int>(I.value), st1 - 1), P); });
+    });
     wait_vmcnt<(R - 1) * PER>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     uint32_t cur = 0;
-    read_codes(cur, 0, w0, x0);
-    next_scales(st0, true);
+    static_for<READS>([&](auto Q) __attribute__((always_inline)) { read_codes(cur, 0, w0, x0, Q); });
+    read_scales(st0);
+    take_scales(st0);
+    // The squares of half a stage one by one, and between them what can go on meanwhile: reads of the other half's fragments, and with the second
+    // half, whose stage every wave has read by then, the copies of the stage R further on.  Left to itself the compiler puts all squares behind
+    // the barrier, and nothing is multiplied while fragments are read.
     for (int st = st0; st < st1; ++st) {
-        read_codes(cur, 1, w1, x1);
-        multiply(w0, x0);
+        static_for<SQUARES>([&](auto Q) __attribute__((always_inline)) {
+            multiply(w0, x0, Q);
+            static_for<READS>([&](auto P) __attribute__((always_inline)) {
+                if constexpr (P.value >= READS * Q.value / SQUARES && P.value < READS * (Q.value + 1) / SQUARES) read_codes(cur, 1, w1, x1, P);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
         // the next stage has landed, and every wave has read this one
         wait_vmcnt<(R - 2) * PER>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        issue(cur, st + R);
-        cur = cur + S::STAGE == R * S::STAGE ? 0u : cur + S::STAGE;
-        read_codes(cur, 0, w0, x0);
-        multiply(w1, x1);
-        next_scales(st + 1, false);
+        const uint32_t next = cur + S::STAGE == R * S::STAGE ? 0u : cur + S::STAGE;
+        const int ahead = min(st + R, st1 - 1), after = min(st + 1, st1 - 1);
+        read_scales(after);
+        static_for<SQUARES>([&](auto Q) __attribute__((always_inline)) {
+            multiply(w1, x1, Q);
+            static_for<PER>([&](auto P) __attribute__((always_inline)) {
+                if constexpr (P.value >= PER * Q.value / SQUARES && P.value < PER * (Q.value + 1) / SQUARES) copy_codes(cur, ahead, P);
+            });
+            static_for<READS>([&](auto P) __attribute__((always_inline)) {
+                if constexpr (P.value >= READS * Q.value / SQUARES && P.value < READS * (Q.value + 1) / SQUARES) read_codes(next, 0, w0, x0, P);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        cur = next;
+        take_scales(after);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // late copies must not land in reused LDS
     __syncthreads();
@@ -463,14 +543,9 @@ int launch_few_nm(const MxsArgs &a, int mode, int tiles, int busy, hipStream_t s
     const int want = device_cu_count() * (2 * S::lds(nwaves, nkb, 8) <= S::MOST - 64 * MT ? 2 : 1);
     int chunks = static_cast<int>(ceil_div(want, busy > 0 ? busy : 1));
     if (chunks > rbs) chunks = rbs;
-    int each = static_cast<int>(ceil_div(rbs, chunks));
-    chunks = static_cast<int>(ceil_div(rbs, each));  // as many row-blocks in each
-    const auto scale_rows = [&] { return (each * 16 + 127) / 128 + 1; };
-    MFQ_REQUIRE(static_cast<int64_t>(each) * 16 * a.K < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx8_scaled: %d x %d weights", a.nrows, a.K);
-    while (each > 1 && S::lds(nwaves, nkb, scale_rows()) > S::MOST) {  // the scales of fewer rows
-        each = (each + 1) / 2;
-        chunks = static_cast<int>(ceil_div(rbs, each));
-    }
+    const auto scale_rows = [&] { return static_cast<int>((ceil_div(rbs, chunks) * 16 + 127) / 128 + 1); };
+    while (chunks < rbs && S::lds(nwaves, nkb, scale_rows()) > S::MOST) chunks = chunks * 2 < rbs ? chunks * 2 : rbs;  // the scales of fewer rows
+    MFQ_REQUIRE(ceil_div(rbs, chunks) * 16 * a.K < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx8_scaled: %d x %d weights", a.nrows, a.K);
     const size_t lds = S::lds(nwaves, nkb, scale_rows());
     MFQ_REQUIRE(lds <= S::MOST && static_cast<int64_t>(tiles) * chunks < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx8_scaled: %d tiles of %d columns", tiles, a.K);
     auto kern = mx8_few_kernel<MT, NB, NM>;
@@ -518,7 +593,7 @@ constexpr int kPlanTile = 3;
 // Tiles and what a launch of them takes, us: f + max(blocks of K * l, rounds * (blocks of K * c + e)), rounds = blocks a compute unit: l is the
 // way of a block of K from memory with the compute unit to itself, c its share with `per_cu` blocks on it, e the end of a block.
 struct Mx8Tile { int n, m, per_cu; double f, l, c, e; };
-constexpr Mx8Tile kMx8Tile[] = {{128, 64, 3, 5.5, 0.48, 0.30, 0.5}, {128, 128, 2, 6.2, 0.56, 0.52, 1.0}, {256, 128, 1, 7.3, 0.75, 0.95, 2.6}, {256, 256, 1, 9.6, 1.16, 1.6, 5.0}};
+constexpr Mx8Tile kMx8Tile[] = {{128, 64, 3, 2.0, 0.53, 0.325, 0.2}, {128, 128, 2, 4.0, 0.62, 0.47, 1.5}, {256, 128, 1, 4.0, 0.61, 0.867, 3.9}, {256, 256, 1, 3.0, 1.08, 1.48, 11.0}};
 constexpr int kMx8Tiles = sizeof(kMx8Tile) / sizeof(kMx8Tile[0]), kMaxSplits = 16;
 
 double tile_us(const Mx8Tile &t, int nrows, int nkb, int M, int splits, int cus) {
