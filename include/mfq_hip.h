@@ -597,7 +597,7 @@ int mfq_hip_mx8_moe_plan(int cols, int n_pairs, int E, int mapped);
  * kind 4: MXFP4 values with scales from mfq_hip_mx_lay_scales.  Widths divisible by 128 (kind 8) or 32; at most 1024 experts, k <= 16.
  * x: bf16 or fp16 [T, ldx]; y: y_dtype (MFQ_X_*) [T, ldy].  Products and sums are fp32's: the hidden rows are not rounded to 16 bits.
  * A token is touched by its own experts alone, whatever the others' weights hold.  Workspace (16-byte aligned, size from the query):
- * the hidden rows. */
+ * the hidden rows, the selection, and partial results; nothing in it has to be cleared. */
 typedef struct mfq_mx_layer {
     int32_t kind, experts, hidden, inter, shared_inter, reserved;
     const void *gate_up, *gate_up_scales, *down, *down_scales;

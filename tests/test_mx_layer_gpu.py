@@ -174,15 +174,17 @@ def test_layouts():
 
 @pytest.mark.parametrize("fmt", ["MXFP8", "MXFP4"])
 def test_few_compute_units(fmt, cu_count):
-    """blocks that go through many row-blocks, of several experts and the shared one"""
+    """blocks that go through many row-blocks, of several experts and the shared one; results in one piece, some or as many as there can be"""
     from tyloquant_amd import runtime_moe as RM
     layer = Layer(fmt, 6, 384, 256, 128)
-    x, logits = P.make_x(4, 6, 384, BF16), router(5, 6, 6)
-    want = RM.mx_moe_ffn_forward(layer.gate_up, layer.down, x, logits, 3, shared=layer.shared)
-    for n in (1, 3, 7, 100, 1000):
-        cu_count(n)
-        got = RM.mx_moe_ffn_forward(layer.gate_up, layer.down, x, logits, 3, shared=layer.shared)
-        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for T in (1, 6, 16):
+        x, logits = P.make_x(4, T, 384, BF16), router(5, T, 6)
+        for n in (1, 3, 7, 13, 100, 1000):
+            cu_count(n)
+            y, ids, weights = RM.mx_moe_ffn_forward(layer.gate_up, layer.down, x, logits, 3, shared=layer.shared)
+            layer.check(y, x, ids, weights)
+            again = RM.mx_moe_ffn_forward(layer.gate_up, layer.down, x, logits, 3, shared=layer.shared)
+            assert all(torch.equal(a, b) for a, b in zip((y, ids, weights), again))
 
 
 def test_graph_replays_and_streams():

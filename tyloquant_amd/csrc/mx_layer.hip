@@ -12,8 +12,9 @@
 //
 // First launch: every block finds the selection for itself (a wave a token, some 100 instructions a choice), which costs less than a launch of
 // its own would; blocks then share the row-blocks of all experts hit evenly.  Waves split K, their weights come through a ring in LDS (as in
-// mx8_scaled.hip), their activations stay in registers.  Second launch: a block owns 16 results of every token; its waves share the lines of
-// all experts, and an expert's sums are weighted and added, for the tokens that take it and no others, where a wave leaves it.
+// mx8_scaled.hip), their activations stay in registers.  Second launch: waves share the columns of all
+// experts, and an expert's sums are weighted and added, for the tokens that take it and no others, where a wave leaves it.
+// Columns of an operand that are no token's hold another's values, not zeros: their sums are not looked at.
 #include "moe_topk.hpp"
 #include "mx_cvt.hpp"
 #include "mx_scaled.hpp"
@@ -22,6 +23,16 @@ namespace mfq {
 namespace {
 
 constexpr int kMaxTokens = 16, kMaxRoutes = 16, kMaxExperts = 1024, kMaxPairs = kMaxTokens * kMaxRoutes;
+
+// What the first launch leaves of the selection for the second: the experts hit in ascending order, and of each who takes it, with which
+// weight and by which of a token's routes.
+struct LayerTable {
+    int count, pad[3];
+    int expert[kMaxPairs];
+    uint32_t tokens[kMaxPairs];
+    float weight[kMaxPairs][kMaxTokens];
+    uint8_t rank[kMaxPairs][kMaxTokens];
+};
 
 struct LayerArgs {
     mfq_mx_layer w;
@@ -37,6 +48,10 @@ struct LayerArgs {
     int64_t ldy;
     uint16_t *hidden;         // three parts of [T * k][inter], bf16
     uint16_t *shared_hidden;  // three parts of [T][shared_inter]
+    LayerTable *table;
+    int pieces;               // of the columns of all experts, in the second launch
+    float *partial;           // [groups of 64 results][pieces][T][64]
+    int32_t *arrived;         // [groups]: pieces that are there
 };
 
 // Bytes of a row, lines of 128 bytes of it; columns of a line, and operands of 32 columns that they make.
@@ -179,6 +194,8 @@ __device__ __forceinline__ u32x4_t activations(const LayerArgs &a, int t, int pa
     return v;
 }
 
+__device__ __forceinline__ void pin(u32x4_t &v) { asm volatile("" : "+v"(v)); }
+
 // NL: lines of K a wave has at most, whose activations stay in registers (0: any number, read again for every row-block); SETS of 16 columns.
 template <int KIND, int NL, int SETS>
 __global__ __launch_bounds__(512) void mx_layer_up_kernel(LayerArgs a) {
@@ -198,24 +215,36 @@ __global__ __launch_bounds__(512) void mx_layer_up_kernel(LayerArgs a) {
     // this lane's columns of activations
     const int mine = (nlines - wave + nwaves - 1) / nwaves;  // lines wave, wave + nwaves, ...
     const int parts = a.x_f16 ? 2 : 1;
-    auto column = [&](int s, int &t, int &part) {  // whether column r of set s is one
-        part = SETS == 1 ? r / T : s;
-        t = SETS == 1 ? r - part * T : r;
-        return part < parts && t < T;
-    };
-    auto operand = [&](int s, int line, int f) {
-        int t, part;
+    // token and part of column r of each set; the first of both where it has none
+    int token[SETS], part[SETS];
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+        const int p = SETS == 1 ? r / T : s, c = SETS == 1 ? r - p * T : r;
+        const bool is = p < parts && c < T;
+        token[s] = is ? c : 0;
+        part[s] = is ? p : 0;
+    }
+    auto operand = [&](int s, int line, int f) __attribute__((always_inline)) {
         const int col = line * Line::COLS + g * (Line::COLS / 4) + 8 * f;
-        return column(s, t, part) && col < H ? activations(a, t, part, col) : u32x4_t{0u, 0u, 0u, 0u};
+        const u32x4_t v = activations(a, token[s], part[s], min(col, H - 8));
+        return KIND == 8 || col < H ? v : u32x4_t{0u, 0u, 0u, 0u};
     };
     u32x4_t x[NL > 0 ? NL : 1][SETS][FR];
     if constexpr (NL > 0) {
-#pragma unroll
-        for (int m = 0; m < NL; ++m)
+        // a line's reads together, and its operands before the next line's
+        static_for<NL>([&](auto MI) __attribute__((always_inline)) {
+            constexpr int m = MI.value;
 #pragma unroll
             for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                for (int f = 0; f < FR; ++f) x[m][s][f] = m < mine ? operand(s, wave + m * nwaves, f) : u32x4_t{0u, 0u, 0u, 0u};
+                for (int f = 0; f < FR; ++f) x[m][s][f] = operand(s, min(wave + m * nwaves, nlines - 1), f);
+            if (a.x_f16) {
+#pragma unroll
+                for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                    for (int f = 0; f < FR; ++f) pin(x[m][s][f]);
+            }
+        });
     }
 
     for (int e = tid; e < a.w.experts; e += nt) sel.place[e] = 0u;
@@ -231,6 +260,21 @@ __global__ __launch_bounds__(512) void mx_layer_up_kernel(LayerArgs a) {
         }
     list_experts(sel, a.w.experts, T, a.k, tid, nt);
     const int count = __builtin_amdgcn_readfirstlane(sel.count);
+    if (blockIdx.x == gridDim.x - 1) {
+        for (int i = tid; i < (H + 63) / 64; i += nt) a.arrived[i] = 0;
+        if (tid == 0) a.table->count = count;
+        for (int l = tid; l < count; l += nt) {
+            a.table->expert[l] = sel.expert[l];
+            a.table->tokens[l] = sel.tokens[l];
+        }
+        for (int p = tid; p < count * kMaxTokens; p += nt) {
+            const int l = p / kMaxTokens, t = p % kMaxTokens;
+            const bool takes = t < T && (sel.tokens[l] >> t & 1u);
+            const int rank = takes ? sel.rank[l][t] : 0;
+            a.table->weight[l][t] = takes ? sel.weights[t * a.k + rank] : 0.f;
+            a.table->rank[l][t] = static_cast<uint8_t>(rank);
+        }
+    }
 
     // this block's row-blocks of 16 gate rows with their up rows, of all experts one after the other, the shared one last
     const int rbs = I / 16, all = count * rbs + a.w.shared_inter / 16;
@@ -402,88 +446,119 @@ __global__ __launch_bounds__(512) void mx_layer_up_kernel(LayerArgs a) {
 }
 
 // ---- down and the weighted sum -------------------------------------------------------------------------------------------------------
-constexpr int kDownWaves = 16;
+// A block owns 64 results of every token, and of the columns of all experts one after the other (the shared one last) a piece, which its waves
+// share in units of 128: an operand of hidden rows then serves four of weights, where reading it for each took more of a compute unit's
+// address path than the weights (16 results a block: 67 MB of MXFP8 in 20 us, 116 MB for 16 tokens in 66).  The pieces of a result are added
+// in their order by the block that comes last to them.
+constexpr int kDownWaves = 8, kDownRows = 64, kMaxPieces = 16;
 
-// PACKED: the three parts of all tokens in one set of columns (T <= 5), else a set for each part
+// PACKED: the three parts of all tokens in one set of columns (T <= 5), else a set for each part.  U: units of a wave in flight.
 template <int KIND, bool PACKED>
 __global__ __launch_bounds__(kDownWaves * 64) void mx_layer_down_kernel(LayerArgs a) {
-    using Line = LineOf<KIND>;
-    constexpr int FR = Line::FR, SETS = PACKED ? 1 : 3;
-    __shared__ Selection sel;
+    constexpr int SETS = PACKED ? 1 : 3, U = (PACKED ? 2 : 1) * (KIND == 4 ? 2 : 1), PIECES = KIND == 8 ? 2 : 1;  // pieces of 16 bytes of a lane's 32 columns
     __shared__ float s_weight[kMaxPairs][kMaxTokens];
-    __shared__ float4_t red[kDownWaves][64];
+    __shared__ int s_expert[kMaxPairs];
+    __shared__ uint32_t s_tokens[kMaxPairs];
+    __shared__ uint32_t s_rank[kMaxPairs][kMaxTokens / 4];
+    __shared__ int s_listed, s_last;
+    __shared__ float4_t red[kDownWaves][4][64];
     const int tid = threadIdx.x, lane = tid & 63, nt = kDownWaves * 64;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
     const int H = a.w.hidden, I = a.w.inter, T = a.T, k = a.k;
-    for (int e = tid; e < a.w.experts; e += nt) sel.place[e] = 0u;
-    for (int p = tid; p < T * k; p += nt) {
-        sel.ids[p] = a.ids[p];
-        sel.weights[p] = a.weights[p];
+    const int group = static_cast<int>(blockIdx.x) / a.pieces, piece = static_cast<int>(blockIdx.x) - group * a.pieces;
+    {   // the table, as far as it can reach: entries behind the last are not looked at
+        const int most = min(T * k, a.w.experts);
+        if (tid == 0) s_listed = a.table->count;
+        if (tid < most) {
+            s_expert[tid] = a.table->expert[tid];
+            s_tokens[tid] = a.table->tokens[tid];
+        }
+        for (int p = tid; p < most * (kMaxTokens / 4); p += nt) s_rank[0][p] = reinterpret_cast<const uint32_t *>(a.table->rank)[p];
+        for (int p = tid; p < most * kMaxTokens; p += nt) s_weight[0][p] = a.table->weight[0][p];
     }
     __syncthreads();
-    list_experts(sel, a.w.experts, T, k, tid, nt);
-    const int count = __builtin_amdgcn_readfirstlane(sel.count);
-    for (int p = tid; p < count * kMaxTokens; p += nt) {
-        const int l = p / kMaxTokens, t = p % kMaxTokens;
-        s_weight[l][t] = t < T && (sel.tokens[l] >> t & 1u) ? sel.weights[t * k + sel.rank[l][t]] : 0.f;
-    }
-    __syncthreads();
+    const int count = __builtin_amdgcn_readfirstlane(s_listed);
 
-    const int row = min(static_cast<int>(blockIdx.x) * 16 + r, H - 1);  // behind the last one: the last one again
-    const int lines = Line::lines(I), shared_lines = a.w.shared_inter ? Line::lines(a.w.shared_inter) : 0;
-    const int all = count * lines + shared_lines;
-    const int lo = static_cast<int>(static_cast<int64_t>(all) * wave / kDownWaves), hi = static_cast<int>(static_cast<int64_t>(all) * (wave + 1) / kDownWaves);
+    int row[4];  // behind the last one: the last one again
+#pragma unroll
+    for (int b = 0; b < 4; ++b) row[b] = min(group * kDownRows + 16 * b + r, H - 1);
+    const int units = (I + 127) / 128, shared_units = (a.w.shared_inter + 127) / 128;
+    const int all = count * units + shared_units, shares = a.pieces * kDownWaves, mine = piece * kDownWaves + wave;
+    const int lo = static_cast<int>(static_cast<int64_t>(all) * mine / shares), hi = static_cast<int>(static_cast<int64_t>(all) * (mine + 1) / shares);
 
-    float4_t sum = {0.f, 0.f, 0.f, 0.f};
+    float4_t sum[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) sum[b] = float4_t{0.f, 0.f, 0.f, 0.f};
     for (int at = lo; at < hi;) {
-        const int l = min(at / lines, count);
+        const int l = min(at / units, count);
         const bool shared = l == count;
-        const int first = at - l * lines, n = min(hi - at, (shared ? shared_lines : lines) - first);
+        const int first = at - l * units, n = min(hi - at, (shared ? shared_units : units) - first);
         const int K = shared ? a.w.shared_inter : I;
-        const int64_t e = shared ? 0 : __builtin_amdgcn_readfirstlane(sel.expert[min(l, kMaxPairs - 1)]);
-        const uint32_t takers = shared ? (1u << T) - 1u : __builtin_amdgcn_readfirstlane(static_cast<int>(sel.tokens[min(l, kMaxPairs - 1)]));
-        const uint8_t *values = static_cast<const uint8_t *>(shared ? a.w.shared_down : a.w.down) + (e * H + row) * Line::bytes(K);
+        const int64_t e = shared ? 0 : __builtin_amdgcn_readfirstlane(s_expert[min(l, kMaxPairs - 1)]);
+        const uint32_t takers = shared ? (1u << T) - 1u : __builtin_amdgcn_readfirstlane(static_cast<int>(s_tokens[min(l, kMaxPairs - 1)]));
+        const uint8_t *values = static_cast<const uint8_t *>(shared ? a.w.shared_down : a.w.down) + e * H * LineOf<KIND>::bytes(K);
         const uint8_t *scales = static_cast<const uint8_t *>(shared ? a.w.shared_down_scales : a.w.down_scales);
-        if constexpr (KIND == 8) scales += ((e * H + row) >> 7) * (shared ? shared_lines : lines);
-        else scales += mx_scale_at(e * H + row, shared ? shared_lines : lines) + 2 * g;
-        // the lane's column of hidden rows in each set
+        const uint8_t *wrow[4], *srow[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            wrow[b] = values + row[b] * LineOf<KIND>::bytes(K);
+            // MXFP8: of the 64 rows, which lie within a block of 128; MXFP4: each row's
+            srow[b] = KIND == 8 ? scales + ((e * H + row[0]) >> 7) * (shared ? shared_units : units) : scales + mx_scale_at(e * H + row[b], mx_macros(K)) + g;
+        }
+        // the lane's column of hidden rows in each set; that of the expert's first token where it is none of its own
+        const int someone = __ffs(takers) - 1;
         const uint16_t *h[SETS];
-        bool live[SETS];
 #pragma unroll
         for (int s = 0; s < SETS; ++s) {
-            const int part = PACKED ? r / T : s, t = PACKED ? r - part * T : r;
-            live[s] = part < 3 && t < T && (takers >> t & 1u);
-            const int64_t rows = shared ? T : T * k, at_row = !live[s] ? 0 : shared ? t : t * k + sel.rank[l][t];
-            h[s] = (shared ? a.shared_hidden : a.hidden) + (static_cast<int64_t>(live[s] ? part : 0) * rows + at_row) * K;
+            const int p = PACKED ? r / T : s, c = PACKED ? r - p * T : r;
+            const bool live = p < 3 && c < T && (takers >> c & 1u);
+            const int t = live ? c : someone;
+            const int64_t rows = shared ? T : T * k, at_row = shared ? t : t * k + (s_rank[min(l, kMaxPairs - 1)][t >> 2] >> (8 * (t & 3)) & 255u);
+            h[s] = (shared ? a.shared_hidden : a.hidden) + ((live ? p : 0) * rows + at_row) * K;
         }
-        const int nblk = K / 32;
-        float4_t acc = {0.f, 0.f, 0.f, 0.f};
-        for (int j = 0; j < n; ++j) {
-            const int line = first + j;
-            u32x4_t w[2];
-            uint32_t raw;
-            const int last = KIND == 8 ? 7 : nblk - 1 - 8 * line;  // as above
+        const int last = K / 32 - 1;  // of an MXFP4 row's pieces, blocks of 32 columns
+        float4_t acc[4];
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-                w[b] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(values + static_cast<int64_t>(line) * 128 + 16 * min(2 * g + b, last)));
-            if constexpr (KIND == 8) raw = scales[line];
-            else raw = *reinterpret_cast<const uint16_t *>(scales + static_cast<int64_t>(line) * 256);
-            u32x4_t x[SETS][FR];
+        for (int b = 0; b < 4; ++b) acc[b] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int j0 = 0; j0 < n; j0 += U) {
+            u32x4_t w[U][4][PIECES], x[U][SETS][4];
+            uint32_t raw[U][4];
 #pragma unroll
-            for (int s = 0; s < SETS; ++s)
+            for (int j = 0; j < U; ++j) {
+                const int u = first + min(j0 + j, n - 1);
+                const int block = min(4 * u + g, last);
 #pragma unroll
-                for (int f = 0; f < FR; ++f) {
-                    const int col = line * Line::COLS + g * (Line::COLS / 4) + 8 * f;
-                    x[s][f] = live[s] && col < K ? *reinterpret_cast<const u32x4_t *>(h[s] + col) : u32x4_t{0u, 0u, 0u, 0u};
+                for (int b = 0; b < 4; ++b) {
+#pragma unroll
+                    for (int q = 0; q < PIECES; ++q)
+                        w[j][b][q] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(wrow[b] + (KIND == 8 ? 128 * u + 32 * g : 16 * block) + 16 * q));
+                    if (KIND == 4 || b == 0) raw[j][b] = KIND == 8 ? srow[0][u] : srow[b][static_cast<int64_t>(u >> 1) * 256 + (u & 1) * 4];
                 }
 #pragma unroll
-            for (int f = 0; f < FR; ++f) {
-                u32x4_t v;
-                if constexpr (KIND == 8) v = mx_cvt_fp8<0>(w[f >> 1][2 * (f & 1)], w[f >> 1][2 * (f & 1) + 1], __uint_as_float(raw << 23));
-                else v = mx_cvt_fp4<0>(w[f >> 2][f & 3], __uint_as_float((raw >> (8 * (f >> 2)) & 255u) << 23));
+                for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                for (int s = 0; s < SETS; ++s) acc = mx_mfma<0>(x[s][f], v, acc);
+                    for (int f = 0; f < 4; ++f) x[j][s][f] = *reinterpret_cast<const u32x4_t *>(h[s] + 32 * block + 8 * f);
+            }
+            asm volatile("" ::: "memory");  // all asked for before the first is used
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                if (j0 + j >= n) break;
+                const bool none = KIND == 4 && 4 * (first + j0 + j) + g > last;  // columns behind the last
+#pragma unroll
+                for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) x[j][s][f] = none ? u32x4_t{0u, 0u, 0u, 0u} : x[j][s][f];
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) {
+                        u32x4_t v;
+                        if constexpr (KIND == 8) v = mx_cvt_fp8<0>(w[j][b][f >> 1][2 * (f & 1)], w[j][b][f >> 1][2 * (f & 1) + 1], __uint_as_float(raw[j][0] << 23));
+                        else v = mx_cvt_fp4<0>(w[j][b][0][f], __uint_as_float(raw[j][b] << 23));
+#pragma unroll
+                        for (int s = 0; s < SETS; ++s) acc[b] = mx_mfma<0>(x[j][s][f], v, acc[b]);
+                    }
             }
         }
         // columns 4 g + i of the expert's tokens
@@ -494,22 +569,48 @@ __global__ __launch_bounds__(kDownWaves * 64) void mx_layer_down_kernel(LayerArg
             float p = 1.f;
             if (!shared) p = s_weight[l][t];
             else if (a.shared_gate && takes) p = 1.f / (1.f + expf(-a.shared_gate[t]));
-            sum[i] = takes ? fmaf(p, acc[i], sum[i]) : sum[i];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) sum[b][i] = takes ? fmaf(p, acc[b][i], sum[b][i]) : sum[b][i];
         }
         at += n;
     }
-    red[wave][lane] = sum;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) red[wave][b][lane] = sum[b];
     __syncthreads();
-    for (int o = tid; o < T * 16; o += nt) {
-        const int t = o >> 4, n = o & 15;
-        if (static_cast<int>(blockIdx.x) * 16 + n >= H) continue;
+    // what this block has of result o: token o / 64, row o % 64
+    const auto own = [&](int o) {
+        const int t = o >> 6, n = o & 63;
         float v = 0.f;
         for (int p = 0; p < (PACKED ? 3 : 1); ++p) {
             const int c = p * T + t;
-            const float *at = reinterpret_cast<const float *>(red) + ((c >> 2) * 16 + n) * 4 + (c & 3);
-            for (int w = 0; w < kDownWaves; ++w) v += at[w * 256];
+            const float *at = reinterpret_cast<const float *>(red) + (n >> 4) * 256 + ((c >> 2) * 16 + (n & 15)) * 4 + (c & 3);
+            for (int w = 0; w < kDownWaves; ++w) v += at[w * 1024];
         }
-        store_rounded(a.y, t * a.ldy + blockIdx.x * 16 + n, v, a.y_dtype);
+        return v;
+    };
+    const int live = min(kDownRows, H - group * kDownRows);
+    if (a.pieces == 1) {
+        for (int o = tid; o < T * 64; o += nt)
+            if ((o & 63) < live) store_rounded(a.y, (o >> 6) * a.ldy + group * kDownRows + (o & 63), own(o), a.y_dtype);
+        return;
+    }
+    // Blocks on other dies see these through memory: stores and loads of device scope, which pass by the caches that a die has to itself, and the
+    // counter raised when the stores have arrived.  Fences of that scope would write those caches back and empty them: 50 us here.
+    float *part = a.partial + static_cast<int64_t>(group) * a.pieces * (T * 64);
+    for (int o = tid; o < T * 64; o += nt) __hip_atomic_store(part + piece * (T * 64) + o, own(o), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) s_last = __hip_atomic_fetch_add(a.arrived + group, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.pieces - 1;
+    __syncthreads();
+    if (!s_last) return;
+    asm volatile("" ::: "memory");
+    for (int o = tid; o < T * 64; o += nt) {
+        if ((o & 63) >= live) continue;
+        float v[kMaxPieces], y = 0.f;
+#pragma unroll
+        for (int s = 0; s < kMaxPieces; ++s) v[s] = __hip_atomic_load(part + min(s, a.pieces - 1) * (T * 64) + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int s = 0; s < kMaxPieces; ++s) y += s < a.pieces ? v[s] : 0.f;
+        store_rounded(a.y, (o >> 6) * a.ldy + group * kDownRows + (o & 63), y, a.y_dtype);
     }
 }
 
@@ -539,13 +640,33 @@ int launch_up_sets(const LayerArgs &a, hipStream_t st) {
 template <int KIND>
 int run_layer(const LayerArgs &a, hipStream_t st) {
     if (int rc = a.x_f16 && 2 * a.T > 16 ? launch_up_sets<KIND, 2>(a, st) : launch_up_sets<KIND, 1>(a, st)) return rc;
-    const dim3 grid(static_cast<unsigned>(ceil_div(a.w.hidden, 16)));
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.w.hidden, kDownRows) * a.pieces));
     if (3 * a.T <= 16) hipLaunchKernelGGL((mx_layer_down_kernel<KIND, true>), grid, dim3(kDownWaves * 64), 0, st, a);
     else hipLaunchKernelGGL((mx_layer_down_kernel<KIND, false>), grid, dim3(kDownWaves * 64), 0, st, a);
     return check_launch("mx_moe_layer (down)");
 }
 
-int64_t hidden_bytes(int64_t rows, int width) { return (3 * rows * width * 2 + 255) & ~static_cast<int64_t>(255); }
+int64_t up256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
+int64_t hidden_bytes(int64_t rows, int width) { return up256(3 * rows * width * 2); }
+// pieces of the columns: as many as make a block for each compute unit
+int pieces_of(int hidden) {
+    const int64_t groups = ceil_div(hidden, kDownRows), n = device_cu_count() / groups;
+    return static_cast<int>(n < 1 ? 1 : n > kMaxPieces ? kMaxPieces : n);
+}
+// the workspace: hidden rows, the shared expert's, the table, partial results and their counters
+struct LayerSpace {
+    int64_t shared_hidden, table, partial, arrived, bytes;
+};
+LayerSpace space_of(const mfq_mx_layer &w, int T, int k, int pieces) {
+    LayerSpace s;
+    const int64_t groups = ceil_div(w.hidden, kDownRows);
+    s.shared_hidden = hidden_bytes(static_cast<int64_t>(T) * k, w.inter);
+    s.table = s.shared_hidden + hidden_bytes(T, w.shared_inter);
+    s.partial = s.table + up256(sizeof(LayerTable));
+    s.arrived = s.partial + (pieces > 1 ? groups * pieces * T * 64 * 4 : 0);
+    s.bytes = s.arrived + up256(groups * 4);
+    return s;
+}
 
 }  // namespace
 }  // namespace mfq
@@ -553,8 +674,8 @@ int64_t hidden_bytes(int64_t rows, int width) { return (3 * rows * width * 2 + 2
 using namespace mfq;
 
 extern "C" size_t mfq_hip_mx_moe_layer_workspace_bytes(const mfq_mx_layer *layer, int T, int k) {
-    if (!layer || T < 1 || T > kMaxTokens || k < 1 || k > kMaxRoutes || layer->inter < 1 || layer->shared_inter < 0) return 0;
-    return static_cast<size_t>(hidden_bytes(static_cast<int64_t>(T) * k, layer->inter) + hidden_bytes(T, layer->shared_inter));
+    if (!layer || T < 1 || T > kMaxTokens || k < 1 || k > kMaxRoutes || layer->hidden < 1 || layer->inter < 1 || layer->shared_inter < 0) return 0;
+    return static_cast<size_t>(space_of(*layer, T, k, pieces_of(layer->hidden)).bytes);
 }
 
 extern "C" int mfq_hip_mx_moe_layer(const mfq_mx_layer *layer, const void *x, int x_dtype, int64_t ldx, int T, const float *logits, const float *bias, int k, int mode,
@@ -615,7 +736,13 @@ extern "C" int mfq_hip_mx_moe_layer(const mfq_mx_layer *layer, const void *x, in
     a.y = y;
     a.y_dtype = y_dtype;
     a.ldy = ldy;
-    a.hidden = static_cast<uint16_t *>(workspace);
-    a.shared_hidden = reinterpret_cast<uint16_t *>(static_cast<uint8_t *>(workspace) + hidden_bytes(static_cast<int64_t>(T) * k, w.inter));
+    a.pieces = pieces_of(w.hidden);
+    const LayerSpace space = space_of(w, T, k, a.pieces);
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    a.hidden = reinterpret_cast<uint16_t *>(ws);
+    a.shared_hidden = reinterpret_cast<uint16_t *>(ws + space.shared_hidden);
+    a.table = reinterpret_cast<LayerTable *>(ws + space.table);
+    a.partial = reinterpret_cast<float *>(ws + space.partial);
+    a.arrived = reinterpret_cast<int32_t *>(ws + space.arrived);
     return w.kind == 8 ? run_layer<8>(a, as_stream(stream)) : run_layer<4>(a, as_stream(stream));
 }
