@@ -230,7 +230,7 @@ __global__ __launch_bounds__(512, MT * NM <= 8 ? 4 : 2) void mx8_few_kernel(MxsA
             for (int m = 0; m < GROUP; ++m) pin(x[m0 + m][t]);
         });
     };
-    static_assert(NM % 2 == 0 && (MT == 2 || NM % 4 == 0), "whole groups");
+    static_assert(NM % 4 == 0, "whole groups");
     if (a.xraw) {
         if constexpr (MT == 1) {  // more rows come quantised
             if (a.x_dtype == MFQ_X_BF16) quantize(std::integral_constant<int, MFQ_X_BF16>{});
@@ -328,7 +328,10 @@ __global__ __launch_bounds__(512, MT * NM <= 8 ? 4 : 2) void mx8_few_kernel(MxsA
 // ring of R stages in LDS, a line of 128 bytes a row, whose 16-byte pieces are turned by (row / 2) & 7: the four passes of a read meet every
 // bank once.  Lane (r, h) multiplies pieces 4 h, 4 h + 1 and then 4 h + 2, 4 h + 3 of both operands.  While the squares of one half are
 // multiplied the fragments of the other are read: one barrier a stage.  Scales: a word holds a row's next four blocks; the activations' words
-// come with every fourth stage, the weights' lie in LDS for all of K.
+// come with every stage, the weights' lie in LDS for all of K.
+// A loop of nothing but 32 x 32 x 64 products of random codes reaches 3.4 PFLOP/s with one wave a SIMD and 3.8 with two (4.9 on zeros: the rest
+// is the clock), which is why the largest tile has eight waves and not four of twice the squares (17408 x 5120 at 8192 rows 630 -> 585 us).
+// What is left there: a stage's way from L2, one stage ahead of its use, and 5 us of start and end of each of 9 tiles a compute unit.
 __host__ __device__ __forceinline__ constexpr int tile_scale_rows(int BN) { return 2 * (BN / 256 + 2); }  // blocks of 128 rows that gate and up rows touch
 template <int BN, int BM, int R>
 struct Tile8Shape {
@@ -529,10 +532,11 @@ __global__ __launch_bounds__(WN *WM * 64) __attribute__((amdgpu_waves_per_eu(BN 
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------
 constexpr int kFewWaves = 8;
-constexpr int kMostOperands = 20;  // registers hold so many blocks of 128 columns of 16 rows, half as many of 32
+constexpr int kMostOperands = 20;  // registers hold so many blocks of 128 columns of 16 rows
 
-// whether a wave's share of K fits its registers
-bool few_fits(int K, int tiles) { return ceil_div(K / kMx8Block, kFewWaves) * tiles <= kMostOperands; }
+// Whether a wave's share of K fits its registers.  Of 32 rows those of 4096 columns: longer ones are faster in tiles, with K in pieces
+// (4096 x 12288 at 17 rows 27 us, in a tile 22; 12288 x 4096 17 and 19).
+bool few_fits(int K, int tiles) { return ceil_div(K / kMx8Block, kFewWaves) <= (tiles == 1 ? kMostOperands : 4); }
 
 template <int MT, int NB, int NM>
 int launch_few_nm(const MxsArgs &a, int mode, int tiles, int busy, hipStream_t st) {
@@ -557,10 +561,11 @@ template <int MT, int NB>
 int launch_few_nb(const MxsArgs &a, int mode, int tiles, int busy, hipStream_t st) {
     const int64_t n = ceil_div(a.K / kMx8Block, kFewWaves);
     if (n <= 4) return launch_few_nm<MT, NB, 4>(a, mode, tiles, busy, st);
-    if (n <= 8) return launch_few_nm<MT, NB, 8>(a, mode, tiles, busy, st);
-    if constexpr (MT == 1)
+    if constexpr (MT == 1) {
+        if (n <= 8) return launch_few_nm<1, NB, 8>(a, mode, tiles, busy, st);
         if (n <= 12) return launch_few_nm<1, NB, 12>(a, mode, tiles, busy, st);
-    if (n <= kMostOperands / MT) return launch_few_nm<MT, NB, kMostOperands / MT>(a, mode, tiles, busy, st);
+        if (n <= kMostOperands) return launch_few_nm<1, NB, kMostOperands>(a, mode, tiles, busy, st);
+    }
     return fail(MFQ_ERR_UNSUPPORTED, "mx8_scaled: %d columns", a.K);
 }
 // tiles: at most; busy: about as many have rows
@@ -592,8 +597,10 @@ struct Mx8Plan { int kind, splits; };
 constexpr int kPlanTile = 3;
 // Tiles and what a launch of them takes, us: f + max(blocks of K * l, rounds * (blocks of K * c + e)), rounds = blocks a compute unit: l is the
 // way of a block of K from memory with the compute unit to itself, c its share with `per_cu` blocks on it, e the end of a block.
+// Fitted to 12288 x 4096 and 4096 x 12288 at 40 to 8192 rows: 12288 x 4096 at 256 rows 23.7, 26.4, 27.4, 43.5 us in the order of the list, at 2048
+// rows 130, 101, 97.5, 98.2, at 8192 rows 498, 397, 376, 330; 4096 x 12288 at 8192 rows 499, 372, 346, 314 (2.6 PFLOP/s).
 struct Mx8Tile { int n, m, per_cu; double f, l, c, e; };
-constexpr Mx8Tile kMx8Tile[] = {{128, 64, 3, 2.0, 0.53, 0.325, 0.2}, {128, 128, 2, 4.0, 0.62, 0.47, 1.5}, {256, 128, 1, 4.0, 0.61, 0.867, 3.9}, {256, 256, 1, 3.0, 1.08, 1.48, 11.0}};
+constexpr Mx8Tile kMx8Tile[] = {{128, 64, 3, 2.0, 0.53, 0.325, 0.2}, {128, 128, 2, 4.0, 0.62, 0.47, 1.5}, {256, 128, 1, 4.0, 0.61, 0.867, 3.9}, {256, 256, 1, 2.0, 1.05, 1.5, 5.0}};
 constexpr int kMx8Tiles = sizeof(kMx8Tile) / sizeof(kMx8Tile[0]), kMaxSplits = 16;
 
 double tile_us(const Mx8Tile &t, int nrows, int nkb, int M, int splits, int cus) {
@@ -638,25 +645,26 @@ Mx8Plan plan_linear(int nrows, int K, int M) {
 int64_t up256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 size_t quantized_bytes(int K, int64_t M) { return static_cast<size_t>(up256(M * K) + up256(mx8_scale_bytes(M, K))); }
 
-template <int MODE>
-int run_tile(const MxsArgs &a, int index, hipStream_t st) {
+int run_linear_tile(const MxsArgs &a, int index, hipStream_t st) {
     switch (index) {
-        case 0: return launch_tile<128, 64, 2, 2, 2, MODE>(a, st);
-        case 1: return launch_tile<128, 128, 2, 2, 2, MODE>(a, st);
-        case 2: return launch_tile<256, 128, 4, 2, 3, MODE>(a, st);
-        default: return launch_tile<256, 256, 2, 2, 2, MODE>(a, st);
+        case 0: return launch_tile<128, 64, 2, 2, 2, kLinear>(a, st);
+        case 1: return launch_tile<128, 128, 2, 2, 2, kLinear>(a, st);
+        case 2: return launch_tile<256, 128, 4, 2, 3, kLinear>(a, st);
+        default: return launch_tile<256, 256, 2, 4, 2, kLinear>(a, st);
     }
 }
 
-// Kernel of a call with a route map, from the pairs an expert has on average: 0 the few-rows kernel, tiles of 16 pairs; else 1 + the index of a tile.
+// Kernel of a call with a route map, from the pairs an expert has on average: 0 the few-rows kernel, tiles of 16 pairs; 1 and 2 tiles of
+// 128 x 64 and 256 x 128.  64 experts of 4096 x 4096, gated, 8 routes: at 16 tokens (2 pairs an expert) 124, 150 and 158 us, at 61 (8)
+// 243, 201 and 211, at 800 (100) -, 306 and 278; 128 experts of 2048 x 1024 at 61 tokens (4) 48, 46 and 54, at 1500 (94) -, 90 and 97.
 int plan_mapped(int64_t pairs, int E, int K) {
     static const int forced = tune_env("MFQ_MX8_EXPERTS", 0);
-    if (forced > 0 && forced <= 1 + kMx8Tiles && (forced > 1 || few_fits(K, 1))) return forced - 1;
+    if (forced > 0 && forced <= 3 && (forced > 1 || few_fits(K, 1))) return forced - 1;
     const int64_t mean = ceil_div(pairs, E);
-    if (mean <= 12 && few_fits(K, 1)) return 0;
-    return mean < 96 ? 1 : mean < 384 ? 2 : 3;
+    if (mean <= 4 && few_fits(K, 1)) return 0;
+    return mean < 96 ? 1 : 2;
 }
-int mapped_rows(int plan) { return plan == 0 ? 16 : kMx8Tile[plan - 1].m; }
+int mapped_rows(int plan) { return plan == 0 ? 16 : plan == 1 ? 64 : 128; }
 
 constexpr int kMaxCols = 1 << 17;  // whose scales fit the LDS beside a tile
 
@@ -763,7 +771,7 @@ extern "C" int mfq_hip_mx8_scaled_gemm_rows(const void *values, const void *scal
         a.splits = p.splits;
         a.part = reinterpret_cast<float *>(ws + used);
     }
-    if (int rc = run_tile<kLinear>(a, p.kind - kPlanTile, st)) return rc;
+    if (int rc = run_linear_tile(a, p.kind - kPlanTile, st)) return rc;
     return mxs_join_launch(a, st);
 }
 
@@ -786,7 +794,7 @@ extern "C" int mfq_hip_mx8_moe_plan(int cols, int n_pairs, int E, int mapped) {
     if (cols <= 0 || cols % kMx8Block != 0 || cols > kMaxCols || n_pairs <= 0 || E <= 0) return -1;
     if (!mapped) return 0;
     const int plan = plan_mapped(n_pairs, E, cols);
-    return plan == 0 ? small_rows(16, cols) ? 0 : 1 : kPlanTile + plan - 1;
+    return plan == 0 ? small_rows(16, cols) ? 0 : 1 : plan == 1 ? kPlanTile : kPlanTile + 2;
 }
 
 extern "C" int mfq_hip_mx8_moe_matmul(const void *values, const void *scales, int rows, int cols, int out_per_expert, const int32_t *expert_slot, int E,
@@ -844,5 +852,5 @@ extern "C" int mfq_hip_mx8_moe_matmul(const void *values, const void *scales, in
     if (rows_bytes || table)
         if (int rc = mx8_quantize_launch(x, x_scales ? MFQ_X_BF16 : x_dtype, ldx, rows_bytes ? x_rows : 0, cols, ws, ws + (rows_bytes ? up256(static_cast<int64_t>(x_rows) * cols) : 0), st, &tab)) return rc;
     if (plan == 0) return launch_few<1>(a, kMapped, static_cast<int>(tiles_mapped(a.pairs, E, 16)), E < a.pairs ? E : a.pairs, st);
-    return run_tile<kMapped>(a, plan - 1, st);
+    return plan == 1 ? launch_tile<128, 64, 2, 2, 2, kMapped>(a, st) : launch_tile<256, 128, 4, 2, 3, kMapped>(a, st);
 }
