@@ -129,7 +129,7 @@ void launch_quantize(const void *x, int64_t ldx, int M, int K, uint8_t *values, 
         hipLaunchKernelGGL((mx8_quantize_kernel<XD, false>), grid, dim3(256), 0, st, x, ldx, M, K, values, scales, table);
 }
 
-constexpr int64_t kMaxRowsTimesCols = 1ll << 40;  // blocks of a launch fit its grid
+constexpr int64_t kMaxRowsTimesCols = 1ll << 36;  // a launch has fewer than 2^32 threads, of 32 values each
 int check_shape(const char *who, int M, int cols) {
     MFQ_REQUIRE(M > 0 && cols > 0 && cols % kMx8Block == 0, MFQ_ERR_INVALID, "%s: [%d, %d], columns must be divisible by 128", who, M, cols);
     MFQ_REQUIRE(static_cast<int64_t>(M) * cols < kMaxRowsTimesCols, MFQ_ERR_UNSUPPORTED, "%s: %d x %d values", who, M, cols);

@@ -575,13 +575,8 @@ def _mx_scales(w) -> torch.Tensor:
 
 
 def _mx_layer(gate_up, down, shared) -> L.MxLayer:
-    """The layer's tensors for mfq_hip_mx_moe_layer; made at the first call and kept with gate_up while none of them has changed."""
+    """The layer's tensors for mfq_hip_mx_moe_layer, which fit one another."""
     tensors = (gate_up, down) + (tuple(shared) if shared is not None else ())
-    scales = tuple(_mx_scales(w) for w in tensors)
-    key = tuple(t.data_ptr() for w, s in zip(tensors, scales) for t in (w.values, s))
-    kept = getattr(gate_up, "_layer", None)
-    if kept is not None and kept[0] == key and kept[1] == tuple((w.rows, w.neuron_len, w.out) for w in tensors):
-        return kept[2]
     if any(w.kind != gate_up.kind for w in tensors):
         raise ValueError("a layer's tensors are all MXFP8 or all MXFP4: " + ", ".join(w.dtype for w in tensors))
     E, H, I = gate_up.n_experts, gate_up.neuron_len, down.neuron_len
@@ -595,9 +590,7 @@ def _mx_layer(gate_up, down, shared) -> L.MxLayer:
             raise ValueError(f"incompatible shared gate_up [{sgu.out}, {sgu.neuron_len}] and down [{sdn.out}, {S}] of a layer of width {H}")
     if E > MX_LAYER_EXPERTS:
         raise ValueError(f"a layer has at most {MX_LAYER_EXPERTS} experts, got {E}")
-    layer = L.MxLayer(gate_up.kind, E, H, I, S, 0, *(t.data_ptr() for w, s in zip(tensors, scales) for t in (w.values, s)))
-    gate_up._layer = (key, tuple((w.rows, w.neuron_len, w.out) for w in tensors), layer)
-    return layer
+    return L.MxLayer(gate_up.kind, E, H, I, S, 0, *(t.data_ptr() for w in tensors for t in (w.values, _mx_scales(w))))
 
 
 def mx_moe_ffn_forward(gate_up, down, x: torch.Tensor, router_logits: torch.Tensor, top_k: int, use_sigmoid=False, use_sqrt_softplus=False,
@@ -631,7 +624,7 @@ def mx_moe_ffn_forward(gate_up, down, x: torch.Tensor, router_logits: torch.Tens
     if bias is not None and bias.numel() != E:
         raise ValueError("bias must be contiguous CUDA float32 [experts]")
     gate = None if shared_gate is None else shared_gate.float().contiguous()
-    for t in (x, logits, bias, gate, gate_up.values, down.values):
+    for t in (x, logits, bias, gate, *(w.values for w in (gate_up, down, *(shared or ())))):
         if t is not None:
             _here(t)
     dev = x.device
