@@ -450,12 +450,14 @@ __global__ __launch_bounds__(512) void mx_layer_up_kernel(LayerArgs a) {
 // share in units of 128: an operand of hidden rows then serves four of weights, where reading it for each took more of a compute unit's
 // address path than the weights (16 results a block: 67 MB of MXFP8 in 20 us, 116 MB for 16 tokens in 66).  The pieces of a result are added
 // in their order by the block that comes last to them.
+//
+// The three parts of an expert's hidden rows are columns beside one another where it has five tokens or fewer, which at 16 tokens is most of
+// them: a third of the reads and of the products (16 tokens of 64 experts, 8 each: 129 -> 98 us).  MANY: some may have more (T > 5), and then
+// a set of columns for each part.
 constexpr int kDownWaves = 8, kDownRows = 64, kMaxPieces = 16;
-
-// PACKED: the three parts of all tokens in one set of columns (T <= 5), else a set for each part.  U: units of a wave in flight.
-template <int KIND, bool PACKED>
+template <int KIND, bool MANY>
 __global__ __launch_bounds__(kDownWaves * 64) void mx_layer_down_kernel(LayerArgs a) {
-    constexpr int SETS = PACKED ? 1 : 3, U = (PACKED ? 2 : 1) * (KIND == 4 ? 2 : 1), PIECES = KIND == 8 ? 2 : 1;  // pieces of 16 bytes of a lane's 32 columns
+    constexpr int PIECES = KIND == 8 ? 2 : 1;  // of 16 bytes of a lane's 32 columns of a row
     __shared__ float s_weight[kMaxPairs][kMaxTokens];
     __shared__ int s_expert[kMaxPairs];
     __shared__ uint32_t s_tokens[kMaxPairs];
@@ -484,16 +486,20 @@ __global__ __launch_bounds__(kDownWaves * 64) void mx_layer_down_kernel(LayerArg
 #pragma unroll
     for (int b = 0; b < 4; ++b) row[b] = min(group * kDownRows + 16 * b + r, H - 1);
     const int units = (I + 127) / 128, shared_units = (a.w.shared_inter + 127) / 128;
-    const int all = count * units + shared_units, shares = a.pieces * kDownWaves, mine = piece * kDownWaves + wave;
-    const int lo = static_cast<int>(static_cast<int64_t>(all) * mine / shares), hi = static_cast<int>(static_cast<int64_t>(all) * (mine + 1) / shares);
+    const int all = count * units + shared_units;
+    const int lo = static_cast<int>(static_cast<int64_t>(all) * piece / a.pieces), hi = static_cast<int>(static_cast<int64_t>(all) * (piece + 1) / a.pieces);
+    // The waves take neighbouring runs of units, so that the block reads its rows from memory in whole lengths: 98 -> 95 us there, and 47 -> 45 for five
+    // tokens of MXFP4.  Runs half as long have sums weighted twice as often: 97, and one token of MXFP8 20.6 us for 19.2.
+    const int run = max(1, min(KIND == 4 ? 8 : 4, (hi - lo + kDownWaves - 1) / kDownWaves));
 
     float4_t sum[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) sum[b] = float4_t{0.f, 0.f, 0.f, 0.f};
-    for (int at = lo; at < hi;) {
+    int at = lo + wave * run, end = min(at + run, hi);
+    while (at < hi) {
         const int l = min(at / units, count);
         const bool shared = l == count;
-        const int first = at - l * units, n = min(hi - at, (shared ? shared_units : units) - first);
+        const int first = at - l * units, n = min(end - at, (shared ? shared_units : units) - first);
         const int K = shared ? a.w.shared_inter : I;
         const int64_t e = shared ? 0 : __builtin_amdgcn_readfirstlane(s_expert[min(l, kMaxPairs - 1)]);
         const uint32_t takers = shared ? (1u << T) - 1u : __builtin_amdgcn_readfirstlane(static_cast<int>(s_tokens[min(l, kMaxPairs - 1)]));
@@ -506,73 +512,121 @@ __global__ __launch_bounds__(kDownWaves * 64) void mx_layer_down_kernel(LayerArg
             // MXFP8: of the 64 rows, which lie within a block of 128; MXFP4: each row's
             srow[b] = KIND == 8 ? scales + ((e * H + row[0]) >> 7) * (shared ? shared_units : units) : scales + mx_scale_at(e * H + row[b], mx_macros(K)) + g;
         }
-        // the lane's column of hidden rows in each set; that of the expert's first token where it is none of its own
-        const int someone = __ffs(takers) - 1;
-        const uint16_t *h[SETS];
-#pragma unroll
-        for (int s = 0; s < SETS; ++s) {
-            const int p = PACKED ? r / T : s, c = PACKED ? r - p * T : r;
-            const bool live = p < 3 && c < T && (takers >> c & 1u);
-            const int t = live ? c : someone;
-            const int64_t rows = shared ? T : T * k, at_row = shared ? t : t * k + (s_rank[min(l, kMaxPairs - 1)][t >> 2] >> (8 * (t & 3)) & 255u);
-            h[s] = (shared ? a.shared_hidden : a.hidden) + ((live ? p : 0) * rows + at_row) * K;
-        }
         const int last = K / 32 - 1;  // of an MXFP4 row's pieces, blocks of 32 columns
+        const int someone = __ffs(takers) - 1, ntakers = __popc(takers);
+        const uint16_t *hidden = shared ? a.shared_hidden : a.hidden;
+        const int64_t rows = shared ? T : T * k;
         float4_t acc[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) acc[b] = float4_t{0.f, 0.f, 0.f, 0.f};
-        for (int j0 = 0; j0 < n; j0 += U) {
-            u32x4_t w[U][4][PIECES], x[U][SETS][4];
-            uint32_t raw[U][4];
+        const auto multiply = [&](auto Sets) __attribute__((always_inline)) {
+            constexpr int SETS = Sets.value, U = (SETS == 1 ? 2 : 1) * (KIND == 4 ? 2 : 1);  // units in flight
+            // the lane's column of hidden rows in each set; that of the expert's first token where it is none
+            const uint16_t *h[SETS];
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                const int u = first + min(j0 + j, n - 1);
-                const int block = min(4 * u + g, last);
+            for (int s = 0; s < SETS; ++s) {
+                int t = someone, p = 0;
+                if constexpr (SETS == 1) {
+                    const int q = r / ntakers;
+                    if (q < 3) {
+                        uint32_t left = takers;
+                        for (int i = r - q * ntakers; i > 0; --i) left &= left - 1;
+                        t = __ffs(left) - 1;
+                        p = q;
+                    }
+                } else if (r < T && (takers >> r & 1u)) {
+                    t = r;
+                    p = s;
+                }
+                const int64_t at_row = shared ? t : t * k + (s_rank[min(l, kMaxPairs - 1)][t >> 2] >> (8 * (t & 3)) & 255u);
+                h[s] = hidden + (p * rows + at_row) * K;
+            }
+            for (int j0 = 0; j0 < n; j0 += U) {
+                u32x4_t w[U][4][PIECES], x[U][SETS][4];
+                uint32_t raw[U][4];
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    const int u = first + min(j0 + j, n - 1);
+                    const int block = min(4 * u + g, last);
+                    // MXFP8: a read of the four lanes of a row is 64 bytes side by side, so a lane's 32 columns are 16 of either half of the unit
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+#pragma unroll
+                        for (int q = 0; q < PIECES; ++q)
+                            w[j][b][q] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(wrow[b] + (KIND == 8 ? 128 * u + 64 * q + 16 * g : 16 * block)));
+                        if (KIND == 4 || b == 0) raw[j][b] = KIND == 8 ? srow[0][u] : srow[b][static_cast<int64_t>(u >> 1) * 256 + (u & 1) * 4];
+                    }
+#pragma unroll
+                    for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                        for (int f = 0; f < 4; ++f)
+                            x[j][s][f] = *reinterpret_cast<const u32x4_t *>(h[s] + (KIND == 8 ? 128 * u + 64 * (f >> 1) + 16 * g + 8 * (f & 1) : 32 * block + 8 * f));
+                }
+                asm volatile("" ::: "memory");  // all asked for before the first is used
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    if (j0 + j >= n) break;
+                    const bool none = KIND == 4 && 4 * (first + j0 + j) + g > last;  // columns behind the last
+#pragma unroll
+                    for (int s = 0; s < SETS; ++s)
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) x[j][s][f] = none ? u32x4_t{0u, 0u, 0u, 0u} : x[j][s][f];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) {
+                            u32x4_t v;
+                            if constexpr (KIND == 8) v = mx_cvt_fp8<0>(w[j][b][f >> 1][2 * (f & 1)], w[j][b][f >> 1][2 * (f & 1) + 1], __uint_as_float(raw[j][0] << 23));
+                            else v = mx_cvt_fp4<0>(w[j][b][0][f], __uint_as_float(raw[j][b] << 23));
+#pragma unroll
+                            for (int s = 0; s < SETS; ++s) acc[b] = mx_mfma<0>(x[j][s][f], v, acc[b]);
+                        }
+                }
+            }
+        };
+        // Sums of a token are in its own column 4 g + i, or, side by side, in one a part: those go by way of the wave's place in LDS.
+        float4_t got[4];
+        if (!MANY || 3 * ntakers <= 16) {
+            multiply(std::integral_constant<int, 1>{});
+#pragma unroll
+            for (int b = 0; b < 4; ++b) red[wave][b][lane] = acc[b];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const float *at_col = reinterpret_cast<const float *>(red[wave]) + 4 * r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int nth = __popc(takers & ((1u << (4 * g + i)) - 1u));  // of the tokens in front; no more than five
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
+                    float v = 0.f;
 #pragma unroll
-                    for (int q = 0; q < PIECES; ++q)
-                        w[j][b][q] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(wrow[b] + (KIND == 8 ? 128 * u + 32 * g : 16 * block) + 16 * q));
-                    if (KIND == 4 || b == 0) raw[j][b] = KIND == 8 ? srow[0][u] : srow[b][static_cast<int64_t>(u >> 1) * 256 + (u & 1) * 4];
-                }
-#pragma unroll
-                for (int s = 0; s < SETS; ++s)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) x[j][s][f] = *reinterpret_cast<const u32x4_t *>(h[s] + 32 * block + 8 * f);
-            }
-            asm volatile("" ::: "memory");  // all asked for before the first is used
-#pragma unroll
-            for (int j = 0; j < U; ++j) {
-                if (j0 + j >= n) break;
-                const bool none = KIND == 4 && 4 * (first + j0 + j) + g > last;  // columns behind the last
-#pragma unroll
-                for (int s = 0; s < SETS; ++s)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) x[j][s][f] = none ? u32x4_t{0u, 0u, 0u, 0u} : x[j][s][f];
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) {
-                        u32x4_t v;
-                        if constexpr (KIND == 8) v = mx_cvt_fp8<0>(w[j][b][f >> 1][2 * (f & 1)], w[j][b][f >> 1][2 * (f & 1) + 1], __uint_as_float(raw[j][0] << 23));
-                        else v = mx_cvt_fp4<0>(w[j][b][0][f], __uint_as_float(raw[j][b] << 23));
-#pragma unroll
-                        for (int s = 0; s < SETS; ++s) acc[b] = mx_mfma<0>(x[j][s][f], v, acc[b]);
+                    for (int p = 0; p < 3; ++p) {
+                        const int c = p * ntakers + nth;
+                        v += at_col[b * 256 + (c >> 2) * 64 + (c & 3)];
                     }
+                    got[b][i] = v;
+                }
             }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        } else if constexpr (MANY) {
+            multiply(std::integral_constant<int, 3>{});
+#pragma unroll
+            for (int b = 0; b < 4; ++b) got[b] = acc[b];
         }
-        // columns 4 g + i of the expert's tokens
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int c = 4 * g + i, t = PACKED ? c % T : c;
-            const bool takes = (PACKED ? c < 3 * T : c < T) && (takers >> t & 1u);
+            const int t = 4 * g + i;
+            const bool takes = t < T && (takers >> t & 1u);
             float p = 1.f;
             if (!shared) p = s_weight[l][t];
             else if (a.shared_gate && takes) p = 1.f / (1.f + expf(-a.shared_gate[t]));
 #pragma unroll
-            for (int b = 0; b < 4; ++b) sum[b][i] = takes ? fmaf(p, acc[b][i], sum[b][i]) : sum[b][i];
+            for (int b = 0; b < 4; ++b) sum[b][i] = takes ? fmaf(p, got[b][i], sum[b][i]) : sum[b][i];
         }
         at += n;
+        if (at == end) {
+            at += (kDownWaves - 1) * run;
+            end = min(at + run, hi);
+        }
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) red[wave][b][lane] = sum[b];
@@ -580,12 +634,9 @@ __global__ __launch_bounds__(kDownWaves * 64) void mx_layer_down_kernel(LayerArg
     // what this block has of result o: token o / 64, row o % 64
     const auto own = [&](int o) {
         const int t = o >> 6, n = o & 63;
+        const float *at = reinterpret_cast<const float *>(red) + (n >> 4) * 256 + ((t >> 2) * 16 + (n & 15)) * 4 + (t & 3);
         float v = 0.f;
-        for (int p = 0; p < (PACKED ? 3 : 1); ++p) {
-            const int c = p * T + t;
-            const float *at = reinterpret_cast<const float *>(red) + (n >> 4) * 256 + ((c >> 2) * 16 + (n & 15)) * 4 + (c & 3);
-            for (int w = 0; w < kDownWaves; ++w) v += at[w * 1024];
-        }
+        for (int w = 0; w < kDownWaves; ++w) v += at[w * 1024];
         return v;
     };
     const int live = min(kDownRows, H - group * kDownRows);
@@ -641,7 +692,7 @@ template <int KIND>
 int run_layer(const LayerArgs &a, hipStream_t st) {
     if (int rc = a.x_f16 && 2 * a.T > 16 ? launch_up_sets<KIND, 2>(a, st) : launch_up_sets<KIND, 1>(a, st)) return rc;
     const dim3 grid(static_cast<unsigned>(ceil_div(a.w.hidden, kDownRows) * a.pieces));
-    if (3 * a.T <= 16) hipLaunchKernelGGL((mx_layer_down_kernel<KIND, true>), grid, dim3(kDownWaves * 64), 0, st, a);
+    if (3 * a.T > 16) hipLaunchKernelGGL((mx_layer_down_kernel<KIND, true>), grid, dim3(kDownWaves * 64), 0, st, a);
     else hipLaunchKernelGGL((mx_layer_down_kernel<KIND, false>), grid, dim3(kDownWaves * 64), 0, st, a);
     return check_launch("mx_moe_layer (down)");
 }
