@@ -110,7 +110,7 @@ def test_sizes_reach_every_kernel():
     splits = C.c_int()
     kinds = {L.lib().mfq_hip_mx8_scaled_plan(out, K, M, C.byref(splits)) for out, K, M in SIZES + FORCED}
     assert kinds == {0, 1, 2, 3, 4, 5, 6}
-    assert {L.lib().mfq_hip_mx8_moe_plan(K, T * R, E, T > 8) for T, R, E, _, K in EXPERTS} == {0, 1, 3, 5}
+    assert {L.lib().mfq_hip_mx8_moe_plan(K, T * R, E, T > 8) for T, R, E, _, K in EXPERTS} == {0, 1, 3, 4, 5}
 
 
 
@@ -236,7 +236,7 @@ def check_pairs(got, xd, wd, ids, out, E, routed, glu, holds=None):
 
 
 EXPERTS = [(1, 8, 16, 256, 256), (5, 2, 4, 128, 640), (8, 1, 3, 384, 128), (9, 2, 8, 256, 384), (61, 4, 12, 128, 512), (200, 2, 5, 256, 1024), (700, 8, 16, 384, 256),
-           (2100, 2, 4, 256, 128), (40, 2, 70, 128, 256), (100, 2, 8, 128, 20608), (12, 2, 8, 128, 4608)]
+           (2100, 2, 4, 256, 128), (40, 2, 70, 128, 256), (100, 2, 8, 128, 20608), (12, 2, 8, 128, 4608), (150, 2, 3, 128, 2176)]
 
 
 @pytest.mark.parametrize("T,R,E,out,K", EXPERTS)

@@ -654,15 +654,18 @@ int run_linear_tile(const MxsArgs &a, int index, hipStream_t st) {
     }
 }
 
-// Kernel of a call with a route map, from the pairs an expert has on average: 0 the few-rows kernel, tiles of 16 pairs; 1 and 2 tiles of
-// 128 x 64 and 256 x 128.  64 experts of 4096 x 4096, gated, 8 routes: at 16 tokens (2 pairs an expert) 124, 150 and 158 us, at 61 (8)
-// 243, 201 and 211, at 800 (100) -, 306 and 278; 128 experts of 2048 x 1024 at 61 tokens (4) 48, 46 and 54, at 1500 (94) -, 90 and 97.
+// Kernel of a call with a route map, from the pairs an expert has on average: 0 the few-rows kernel, tiles of 16 pairs; 1 + i tile i
+// of kMx8Tile.  64 experts of 4096 x 4096, gated, 8 routes: at 16 tokens (2 pairs an expert) 124 us, in tiles of 128 x 64 150 and of 256 x 128 158, at 61
+// (8) 243, 201 and 211, at 800 (100) -, 306 and 278; 128 experts of 2048 x 1024 at 61 tokens (4) 48, 46 and 54, at 1500 (94) -, 90 and 97.
+// Two tiles of 128 x 128 fit a compute unit, so that one's start and end go beside the other's squares, which counts where K is short: 128 experts
+// of 2048 x 768 at 4096 tokens 201 us in tiles of 256 x 128, 185 in these, 1024 columns at 2048 144 and 139, 8 experts of 4096 x 2048 gated
+// 128 and 124; 64 of 4096 x 4096 at 2048 432 and 480.
 int plan_mapped(int64_t pairs, int E, int K) {
     static const int forced = tune_env("MFQ_MX8_EXPERTS", 0);
-    if (forced > 0 && forced <= 3 && (forced > 1 || few_fits(K, 1))) return forced - 1;
+    if (forced > 0 && forced <= 4 && (forced > 1 || few_fits(K, 1))) return forced - 1;
     const int64_t mean = ceil_div(pairs, E);
     if (mean <= 4 && few_fits(K, 1)) return 0;
-    return mean < 96 ? 1 : 2;
+    return mean < 96 ? 1 : K <= 2048 ? 2 : 3;
 }
 int mapped_rows(int plan) { return plan == 0 ? 16 : plan == 1 ? 64 : 128; }
 
@@ -794,7 +797,7 @@ extern "C" int mfq_hip_mx8_moe_plan(int cols, int n_pairs, int E, int mapped) {
     if (cols <= 0 || cols % kMx8Block != 0 || cols > kMaxCols || n_pairs <= 0 || E <= 0) return -1;
     if (!mapped) return 0;
     const int plan = plan_mapped(n_pairs, E, cols);
-    return plan == 0 ? small_rows(16, cols) ? 0 : 1 : plan == 1 ? kPlanTile : kPlanTile + 2;
+    return plan == 0 ? small_rows(16, cols) ? 0 : 1 : kPlanTile + plan - 1;
 }
 
 extern "C" int mfq_hip_mx8_moe_matmul(const void *values, const void *scales, int rows, int cols, int out_per_expert, const int32_t *expert_slot, int E,
@@ -852,5 +855,6 @@ extern "C" int mfq_hip_mx8_moe_matmul(const void *values, const void *scales, in
     if (rows_bytes || table)
         if (int rc = mx8_quantize_launch(x, x_scales ? MFQ_X_BF16 : x_dtype, ldx, rows_bytes ? x_rows : 0, cols, ws, ws + (rows_bytes ? up256(static_cast<int64_t>(x_rows) * cols) : 0), st, &tab)) return rc;
     if (plan == 0) return launch_few<1>(a, kMapped, static_cast<int>(tiles_mapped(a.pairs, E, 16)), E < a.pairs ? E : a.pairs, st);
-    return plan == 1 ? launch_tile<128, 64, 2, 2, 2, kMapped>(a, st) : launch_tile<256, 128, 4, 2, 3, kMapped>(a, st);
+    if (plan == 1) return launch_tile<128, 64, 2, 2, 2, kMapped>(a, st);
+    return plan == 2 ? launch_tile<128, 128, 2, 2, 2, kMapped>(a, st) : launch_tile<256, 128, 4, 2, 3, kMapped>(a, st);
 }

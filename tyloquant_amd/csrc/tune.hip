@@ -61,7 +61,7 @@ Knob g_knobs[] = {
     {"MFQ_MXS_EXPERTS", "kernel of routed experts of microscaled operands with a route map: 1 flow, 2 and 3 tiles of 128 x 64 and 256 x 128 (0 = by their pairs)", 0, false},
     {"MFQ_MX8_TILE", "tile of a product of MXFP8 weights and quantised activations, 1 + its index in kMx8Tile (0 = by the model)", 0, false},
     {"MFQ_MX8_SPLIT", "pieces of K of such a tiled product (0 = by the model)", 0, false},
-    {"MFQ_MX8_EXPERTS", "kernel of routed experts of such products with a route map: 1 the few-rows kernel, 2 tiles of 128 x 64, 3 of 256 x 128 (0 = by pairs an expert)", 0, false},
+    {"MFQ_MX8_EXPERTS", "kernel of routed experts of such products with a route map: 1 the few-rows kernel, 2 tiles of 128 x 64, 3 of 128 x 128, 4 of 256 x 128 (0 = by pairs an expert and K)", 0, false},
     {"MFQ_MX_WAVES", "waves per block the MX tile kernels split K over (0 = by shape)", 0, false},
     {"MFQ_NVQ_PAIRS_MFMA", "0 = a MoE decode step on an NVQ cohort always takes the generic one-row kernel", 0, false},
     {"MFQ_MOE_NB", "row-blocks per wave of the MoE streaming kernel (0 = by shape)", 0, false},
