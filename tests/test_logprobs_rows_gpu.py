@@ -141,3 +141,16 @@ def test_rows_far_from_zero(copies):
     z[5, 11] = 90.0
     z, tokens = z.repeat(copies, 1), tokens.repeat(copies)
     check_rows(scores(z, tokens, 5), z, tokens, 5, 15 + 16)
+
+
+def test_rows_of_equal_logits():
+    """log softmax and entropy of V equal logits are log V: sums of ones are exact, what is left is one logarithm, off by one step at most
+    (2^-23 relative)"""
+    wrong = []
+    for V in [*range(2, 200, 7), *range(1000, 160000, 2111)]:
+        z = torch.zeros(1, V, device="cuda")
+        got = scores(z, torch.zeros(1, dtype=torch.int64, device="cuda"), 1)
+        for value, want in ((got.logprobs, -math.log(V)), (got.entropy, math.log(V)), (got.top_logprobs, -math.log(V))):
+            if abs(float(value) - want) > 2 * U * math.log(V):
+                wrong.append((V, float(value) - want))
+    assert not wrong, wrong

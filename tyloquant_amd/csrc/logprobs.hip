@@ -1,6 +1,6 @@
 // Scores of an answer from rows of logits z[0 .. V): of a given token its log probability and rank, the entropy of the row, and the
 // most probable tokens with theirs.
-//   m = max z, p_i = (z_i - m) log2 e, s = sum 2^p_i, t = sum p_i 2^p_i:   log softmax_i = (z_i - m) - ln 2 log2 s,   entropy = ln 2 (log2 s - t / s)
+//   m = max z, p_i = (z_i - m) log2 e, s = sum 2^p_i, t = sum p_i 2^p_i:   log softmax_i = (z_i - m) - log s,   entropy = log s - ln 2 t / s
 // One pass over the logits.  A thread keeps m, s and t of what it has seen, rescaled once for every 8 or 16 values (a tile of its block is 2048
 // or 4096 of them), which are added by a tree and then to the rest by a compensated sum; threads, waves, blocks and the pieces of a row
 // are joined by the same rule.  A piece of -infinity alone has s = 0; a row of nothing else, or with +infinity or a NaN in it, gives NaN
@@ -107,10 +107,21 @@ __device__ __forceinline__ float logit_at(const void *p, int64_t i) {
     else return x_to_f32<DT == MFQ_X_F16>(static_cast<const uint16_t *>(p)[i]);
 }
 
-__device__ __forceinline__ float log_probability(const Sums &s, float z) { return (z - s.m) - log2f(s.s) * kLn2; }
+// log s of s = 2^k f, f from sqrt(1/2) to sqrt(2): logf(s) and ln 2 log2 s are both off by up to a step and a half of log2 s (1.6e-6 of rows that are
+// flat over 100000 tokens), log f by a few 1e-8
+__device__ __forceinline__ float log_of(float s) {
+    int k;
+    float f = frexpf(s, &k);
+    if (f < 0.70710678f) {
+        f *= 2.f;
+        --k;
+    }
+    return fmaf(static_cast<float>(k), kLn2, logf(f));
+}
+__device__ __forceinline__ float log_probability(const Sums &s, float z) { return (z - s.m) - log_of(s.s); }
 // what is written of a whole row but its token's rank; `given`: the token's logit
 __device__ __forceinline__ void put_scores(const LogprobArgs &a, int64_t row, const Sums &s, bool any, float given) {
-    a.entropy[row] = (log2f(s.s) - s.t / s.s) * kLn2;
+    a.entropy[row] = log_of(s.s) - s.t / s.s * kLn2;
     a.logprob[row] = any ? log_probability(s, given) : 0.f;
 }
 // how many of the n logits kept in `near` are as probable as the given one; whether that is all it takes
