@@ -27,6 +27,8 @@ inline int check_launch(const char *what) {
 inline hipStream_t as_stream(mfq_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// a launch has fewer than 2^32 threads along an axis
+constexpr bool grid_fits(int64_t blocks, int threads) { return blocks < (1ll << 32) / threads; }
 
 // ---- device helpers --------------------------------------------------------------------
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2_t;

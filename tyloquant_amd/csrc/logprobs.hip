@@ -463,7 +463,7 @@ extern "C" int mfq_hip_token_logprobs(const void *logits, int dtype, int64_t ldl
     MFQ_REQUIRE(reinterpret_cast<uintptr_t>(logits) % size == 0, MFQ_ERR_INVALID, "token_logprobs: unaligned logits");
     const LogprobPlan p = plan_of(M, V, top);
     LogprobArgs a = {logits, ldl, V, top, p.parts, p.per, tokens, logprob, entropy, top_logprobs, rank, top_ids, nullptr, nullptr, nullptr};
-    MFQ_REQUIRE(static_cast<int64_t>(M) * a.parts < (1ll << 31), MFQ_ERR_UNSUPPORTED, "token_logprobs: %d rows", M);
+    MFQ_REQUIRE(grid_fits(static_cast<int64_t>(M) * a.parts, 256), MFQ_ERR_UNSUPPORTED, "token_logprobs: %d rows", M);
     if (a.parts > 1) {
         const size_t need = workspace_of(M, a.parts, top);
         MFQ_REQUIRE(workspace && workspace_bytes >= need, MFQ_ERR_WORKSPACE, "token_logprobs: workspace %zu < %zu", workspace_bytes, need);

@@ -129,16 +129,20 @@ void launch_quantize(const void *x, int64_t ldx, int M, int K, uint8_t *values, 
         hipLaunchKernelGGL((mx8_quantize_kernel<XD, false>), grid, dim3(256), 0, st, x, ldx, M, K, values, scales, table);
 }
 
-constexpr int64_t kMaxRowsTimesCols = 1ll << 36;  // a launch has fewer than 2^32 threads, of 32 values each
+// blocks of 256 threads, and one more with a table
+int check_values(const char *who, int M, int cols) {
+    MFQ_REQUIRE(grid_fits(ceil_div(static_cast<int64_t>(M) * (cols / 8), 256 * kUnits) + 1, 256), MFQ_ERR_UNSUPPORTED, "%s: %d x %d values", who, M, cols);
+    return MFQ_OK;
+}
 int check_shape(const char *who, int M, int cols) {
     MFQ_REQUIRE(M > 0 && cols > 0 && cols % kMx8Block == 0, MFQ_ERR_INVALID, "%s: [%d, %d], columns must be divisible by 128", who, M, cols);
-    MFQ_REQUIRE(static_cast<int64_t>(M) * cols < kMaxRowsTimesCols, MFQ_ERR_UNSUPPORTED, "%s: %d x %d values", who, M, cols);
-    return MFQ_OK;
+    return check_values(who, M, cols);
 }
 
 }  // namespace
 
 int mx8_quantize_launch(const void *x, int x_dtype, int64_t ldx, int M, int K, uint8_t *values, uint8_t *scales, hipStream_t st, const MxTileTable *table) {
+    if (int rc = check_values("mx8_quantize_rows", M, K)) return rc;
     const MxTileTable t = table ? *table : MxTileTable{};
     if (x_dtype == MFQ_X_F32) launch_quantize<MFQ_X_F32>(x, ldx, M, K, values, scales, st, t);
     else if (x_dtype == MFQ_X_F16) launch_quantize<MFQ_X_F16>(x, ldx, M, K, values, scales, st, t);

@@ -551,7 +551,7 @@ int launch_few_nm(const MxsArgs &a, int mode, int tiles, int busy, hipStream_t s
     while (chunks < rbs && S::lds(nwaves, nkb, scale_rows()) > S::MOST) chunks = chunks * 2 < rbs ? chunks * 2 : rbs;  // the scales of fewer rows
     MFQ_REQUIRE(ceil_div(rbs, chunks) * 16 * a.K < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx8_scaled: %d x %d weights", a.nrows, a.K);
     const size_t lds = S::lds(nwaves, nkb, scale_rows());
-    MFQ_REQUIRE(lds <= S::MOST && static_cast<int64_t>(tiles) * chunks < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx8_scaled: %d tiles of %d columns", tiles, a.K);
+    MFQ_REQUIRE(lds <= S::MOST && grid_fits(static_cast<int64_t>(tiles) * chunks, 64 * nwaves), MFQ_ERR_UNSUPPORTED, "mx8_scaled: %d tiles of %d columns", tiles, a.K);
     auto kern = mx8_few_kernel<MT, NB, NM>;
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void *>(kern), lds, "mx8_scaled")) return rc;
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles * chunks)), dim3(64 * nwaves), lds, st, a, mode, chunks, scale_rows());
@@ -574,14 +574,17 @@ int launch_few(const MxsArgs &a, int mode, int tiles, int busy, hipStream_t st) 
     return a.glu ? launch_few_nb<MT, 2>(a, mode, tiles, busy, st) : launch_few_nb<MT, 1>(a, mode, tiles, busy, st);
 }
 
+// blocks of a launch of tiles of n x m
+int64_t tile_blocks(const MxsArgs &a, int n, int m, bool mapped) {
+    const int width = a.glu ? a.nrows / 2 : a.nrows;
+    const int64_t tiles_m = mapped ? tiles_mapped(a.pairs, a.E, m) : ceil_div(a.M, m);
+    return (ceil_div(width, a.glu ? n / 2 : n) * tiles_m + 7) / 8 * 8;
+}
+// the callers have seen to it that the grid fits (check_tiles)
 template <int BN, int BM, int WN, int WM, int R, int MODE>
 int launch_tile(const MxsArgs &a, hipStream_t st) {
     using S = Tile8Shape<BN, BM, R>;
-    const int width = a.glu ? a.nrows / 2 : a.nrows;
-    const int64_t tiles_n = ceil_div(width, a.glu ? BN / 2 : BN);
-    const int64_t tiles_m = MODE == kMapped ? tiles_mapped(a.pairs, a.E, BM) : ceil_div(a.M, BM);
-    const int64_t blocks = (tiles_n * tiles_m + 7) / 8 * 8;
-    MFQ_REQUIRE(blocks < (1ll << 31), MFQ_ERR_UNSUPPORTED, "mx8_scaled: %lld tiles", static_cast<long long>(blocks));
+    const int64_t blocks = tile_blocks(a, BN, BM, MODE == kMapped);
     static_assert(WN * WM * kTileOut <= R * S::STAGE, "results leave through the ring");
     const size_t lds = S::lds(a.K / kMx8Block);
     MFQ_REQUIRE(lds <= kMaxDynamicLds, MFQ_ERR_UNSUPPORTED, "mx8_scaled: %d columns", a.K);
@@ -599,9 +602,18 @@ constexpr int kPlanTile = 3;
 // way of a block of K from memory with the compute unit to itself, c its share with `per_cu` blocks on it, e the end of a block.
 // Fitted to 12288 x 4096 and 4096 x 12288 at 40 to 8192 rows: 12288 x 4096 at 256 rows 23.7, 26.4, 27.4, 43.5 us in the order of the list, at 2048
 // rows 130, 101, 97.5, 98.2, at 8192 rows 498, 397, 376, 330; 4096 x 12288 at 8192 rows 499, 372, 346, 314 (2.6 PFLOP/s).
-struct Mx8Tile { int n, m, per_cu; double f, l, c, e; };
-constexpr Mx8Tile kMx8Tile[] = {{128, 64, 3, 2.0, 0.53, 0.325, 0.2}, {128, 128, 2, 4.0, 0.62, 0.47, 1.5}, {256, 128, 1, 4.0, 0.61, 0.867, 3.9}, {256, 256, 1, 2.0, 1.05, 1.5, 5.0}};
+struct Mx8Tile { int n, m, threads, per_cu; double f, l, c, e; };
+constexpr Mx8Tile kMx8Tile[] = {{128, 64, 256, 3, 2.0, 0.53, 0.325, 0.2}, {128, 128, 256, 2, 4.0, 0.62, 0.47, 1.5}, {256, 128, 512, 1, 4.0, 0.61, 0.867, 3.9},
+                                {256, 256, 512, 1, 2.0, 1.05, 1.5, 5.0}};
 constexpr int kMx8Tiles = sizeof(kMx8Tile) / sizeof(kMx8Tile[0]), kMaxSplits = 16;
+
+// before anything of a call is launched
+int check_tiles(const MxsArgs &a, int index, bool mapped) {
+    const Mx8Tile &t = kMx8Tile[index];
+    const int64_t blocks = tile_blocks(a, t.n, t.m, mapped);
+    MFQ_REQUIRE(grid_fits(blocks, t.threads), MFQ_ERR_UNSUPPORTED, "mx8_scaled: %lld tiles", static_cast<long long>(blocks));
+    return MFQ_OK;
+}
 
 double tile_us(const Mx8Tile &t, int nrows, int nkb, int M, int splits, int cus) {
     const double blocks = static_cast<double>(ceil_div(nrows, t.n)) * ceil_div(M, t.m) * splits, q = blocks / cus;
@@ -746,6 +758,8 @@ extern "C" int mfq_hip_mx8_scaled_gemm_rows(const void *values, const void *scal
     a.R = 1;
     a.ldy = ldy;
     Mx8Plan p = plan_linear(nrows, cols, M);
+    if (p.kind >= kPlanTile)
+        if (int rc = check_tiles(a, p.kind - kPlanTile, false)) return rc;
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     size_t used = 0;
     if (x_scales) {
@@ -842,6 +856,8 @@ extern "C" int mfq_hip_mx8_moe_matmul(const void *values, const void *scales, in
     MFQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), MFQ_ERR_WORKSPACE, "mx8_moe_matmul: workspace %zu < %zu", workspace_bytes, need);
     MFQ_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, MFQ_ERR_WORKSPACE, "mx8_moe_matmul: unaligned workspace");
     const int plan = plan_mapped(a.pairs, E, cols);
+    if (plan > 0)
+        if (int rc = check_tiles(a, plan - 1, true)) return rc;
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     const size_t rows_bytes = need - table;
     const MxTileTable tab = {expert_bounds, expert_slot, E, mapped_rows(plan), table ? reinterpret_cast<i32x4v_t *>(ws + rows_bytes) : nullptr};
