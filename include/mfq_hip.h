@@ -576,7 +576,7 @@ int mfq_hip_mx8_scaled_gemm_rows(const void *values, const void *scales, int row
                                  int x_dtype, int64_t ldx, const void *x_scales, int M, int glu, int activation, void *y, int y_dtype,
                                  int64_t ldy, void *workspace, size_t workspace_bytes, mfq_stream_t stream);
 /* The same grouped by expert, as mfq_hip_mx_moe_matmul; experts of a pool of several are whole blocks of 128 rows.  Without a route map
- * cols up to 20480. */
+ * cols up to 20480 (the host layer makes a map for longer rows). */
 size_t mfq_hip_mx8_moe_workspace_bytes(int cols, int x_rows, int n_pairs, int E, int mapped, int x_quantized);
 int mfq_hip_mx8_moe_matmul(const void *values, const void *scales, int rows, int cols, int out_per_expert, const int32_t *expert_slot,
                            int E, const void *x, int x_dtype, int64_t ldx, const void *x_scales, int routed_input, const int32_t *ids,

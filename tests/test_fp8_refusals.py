@@ -33,3 +33,12 @@ def test_tiles_of_a_product(lib, kw):
 ])
 def test_tiles_of_experts(lib, kw):
     refused(lib, moe(lib, **kw), L.ERR_UNSUPPORTED, "tiles")
+
+
+def test_no_kernel_for_pairs_of_long_rows(lib):
+    """the host's limit is the one that a call without a route map is held to"""
+    from tyloquant_amd import runtime_mx8 as R8
+    most = R8.MAX_PAIR_COLUMNS
+    assert [lib.mfq_hip_mx8_moe_plan(K, 8, 4, 0) for K in (128, most, most + 128)] == [0, 0, -1]
+    assert lib.mfq_hip_mx8_moe_plan(most + 128, 8, 4, 1) > 0
+    refused(lib, moe(lib, dst=None, bounds=None, cols=most + 128, ldx=most + 128), L.ERR_UNSUPPORTED, "without a route map")

@@ -809,7 +809,7 @@ extern "C" size_t mfq_hip_mx8_moe_workspace_bytes(int cols, int x_rows, int n_pa
 
 extern "C" int mfq_hip_mx8_moe_plan(int cols, int n_pairs, int E, int mapped) {
     if (cols <= 0 || cols % kMx8Block != 0 || cols > kMaxCols || n_pairs <= 0 || E <= 0) return -1;
-    if (!mapped) return 0;
+    if (!mapped) return few_fits(cols, 1) ? 0 : -1;
     const int plan = plan_mapped(n_pairs, E, cols);
     return plan == 0 ? small_rows(16, cols) ? 0 : 1 : kPlanTile + plan - 1;
 }

@@ -14,6 +14,7 @@ from .runtime import _ptr, _stream, borrow
 from .runtime_mx import _OUT, MxWeight, _here, _out_dtype, _raw_rows, _result_dtype
 
 BLOCK = 128
+MAX_PAIR_COLUMNS = 20480    # of experts without a route map
 
 
 def _columns(shape) -> int:
@@ -141,15 +142,19 @@ def mx8_moe_into(w: MxWeight, x, route, out: torch.Tensor, routed: bool = False,
         _here(t)
     if T * R:
         lib = L.lib()
-        mapped = route.ids_dst is not None
+        ids_dst, bounds = route.ids_dst, route.expert_bounds
+        if ids_dst is None and K > MAX_PAIR_COLUMNS:     # a plan of a few tokens has no map: these columns need one
+            from .runtime_moe import build_expert_map
+            ids_dst, bounds = build_expert_map(route.ids, route.n_experts, lib.mfq_hip_moe_tile_m())[:2]
+        mapped = ids_dst is not None
         key = (8, M, T * R, route.n_experts, mapped, xs is None)
         need = w._needs.get(key)
         if need is None:
             need = w.note_need(key, lib.mfq_hip_mx8_moe_workspace_bytes(K, M, T * R, route.n_experts, mapped, xs is not None))
         ws = borrow(need, x2.device)
         L.check(lib.mfq_hip_mx8_moe_matmul(w.values.data_ptr(), w.scales.data_ptr(), w.rows, K, w.out, _ptr(slot), route.n_experts, x2.data_ptr(), xd, ldx,
-                                           _ptr(xs), int(routed), route.ids.data_ptr(), T, R, _ptr(route.ids_dst) if mapped else None,
-                                           _ptr(route.expert_bounds) if mapped else None, int(glu), int(activation), out.data_ptr(), yd, width, _ptr(ws),
+                                           _ptr(xs), int(routed), route.ids.data_ptr(), T, R, _ptr(ids_dst) if mapped else None,
+                                           _ptr(bounds) if mapped else None, int(glu), int(activation), out.data_ptr(), yd, width, _ptr(ws),
                                            need if ws is not None else 0, _stream()))
     return out
 
