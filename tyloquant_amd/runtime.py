@@ -376,12 +376,15 @@ _LOGITS = {torch.float32: L.X_F32, torch.bfloat16: L.X_BF16, torch.float16: L.X_
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
     """Scores of an answer: logits [..., V] (what any LM head returns; fp32, bf16 or fp16, masked ones -inf) and one token id (int64)
     a row.  fp32 results, ids and ranks int64; of equal logits the lower token comes first.  An id outside [0, V) marks padding: its
-    log probability and rank are 0.  Rows that are masked throughout, or hold +inf or a NaN, give NaN."""
+    log probability and rank are 0.  Rows that are masked throughout, or hold +inf or a NaN, give NaN.  No backward pass: logits that
+    a gradient is wanted of are refused."""
     code, shape = _LOGITS.get(logits.dtype), logits.shape
     if code is None:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
     if not shape or tokens.dtype != torch.int64 or tokens.shape != shape[:-1]:
         raise ValueError(f"tokens must be int64 {tuple(shape[:-1])}, one for each row of logits, got {tokens.dtype} {tuple(tokens.shape)}")
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("token_logprobs has no backward pass: call it under torch.no_grad() or on logits.detach()")
     V, top = shape[-1], int(top)
     if not 0 <= top <= min(MAX_TOP_LOGPROBS, V):
         raise ValueError(f"top must be in [0, min({MAX_TOP_LOGPROBS}, tokens)], got {top} of {V}")
