@@ -222,6 +222,7 @@ int mfq_hip_nint_gemv_argmax(const mfq_nint_desc *d, const void *weight, const v
 
 /* Scores of an answer, from rows of logits [M, V] in bf16, fp16 or fp32 (dtype MFQ_X_*, ldl values from row to row), fp32 throughout:
  *   logprob[m] = log softmax(logits[m])[tokens[m]], rank[m] = 1 + how many tokens are more probable: by logit - max, in fp32;
+ *   logits that this difference does not tell apart have one rank, so top_ids[m][i], in the order of the logits, has rank i + 1 or less;
  *   entropy[m] = - sum p log p, masked logits (-infinity) adding nothing;
  *   top_ids[m][i], top_logprobs[m][i], i < top <= 64: the most probable tokens in order, of equal logits the lower first.
  * A token outside [0, V) (padding) has logprob 0 and rank 0.  A row that is masked throughout, or holds +infinity or a NaN, gives NaN

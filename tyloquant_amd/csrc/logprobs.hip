@@ -7,12 +7,15 @@
 // as its softmax does.
 //
 // The most probable: each wave keeps its best so far as whole numbers that order logits, of equal ones the lower token first, and looks at
-// single values of a tile only where the tile's largest reaches the last of them, which is rare after the first tiles.  The first bar is
-// the top-th largest of the 64 lanes' maxima in the first tile.  The numbers decide, not the waves: results do not depend on
-// the order in which waves run.
+// single values of a tile only where the tile's largest reaches the last of them, which is rare after the first tiles of logits that differ.
+// The first bar is the top-th largest of the 64 lanes' maxima in the first tile.  The numbers decide, not the waves: results do not
+// depend on the order in which waves run.  Where a mask leaves fewer than `top` tokens in a wave's first tiles the bar is the mask's own value, which
+// every tile reaches: each of its values is read again then, and so it is in long runs of equal logits at the bar.  2048 rows of 151936,
+// 5 alternatives: 787 us with 50 tokens left, 214 unmasked, 192 either way without alternatives.
 //
 // A token's rank counts the tokens of larger z - m in fp32, the difference that log probabilities are formed of: logits so close together
-// that it does not tell them apart are as probable as one another.  m is known at the end of the row only, so what is counted on the way is
+// that it does not tell them apart are as probable as one another and have one rank, as equal ones have (the alternatives are in the order of
+// the logits, so number i of them has rank i at most, from 1 on).  m is known at the end of the row only, so what is counted on the way is
 // logits above the given one, and the few that lie within 2^-17 above it are kept: of those the equal ones are taken off again.  Rows
 // whose m is more than 64 above the given logit (where fp32 differences are farther apart), or with more of such neighbours than are kept,
 // are read once more.

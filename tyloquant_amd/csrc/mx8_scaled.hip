@@ -627,6 +627,9 @@ double tile_us(const Mx8Tile &t, int nrows, int nkb, int M, int splits, int cus)
 }
 
 // Rows that every block of the few-rows kernel quantises itself, which saves a launch: while the blocks' reads of them are little beside the weights.
+// In a graph, by the blocks and with the quantiser's launch: 12288 x 4096 at 4 rows 13.5 and 14.6 us, at 8 15.5 and 15.9, at 12 17.0 and 16.8, at 16
+// 18.2 and 17.4; 4096 x 4096 at 4 rows 8.4 and 9.8, at 16 10.5 and 11.3; 6144 x 2048 at 4 rows 9.7 and 10.1, at 16 13.4 and 12.8.  So
+// from 12 rows on the two differ by 5 % either way, and one call after the other the launch costs 4 us of the host's.
 constexpr int kSmallValues = 1 << 16;
 bool small_rows(int64_t M, int K) { return M <= 16 && (M <= 4 || M * K <= kSmallValues); }
 
@@ -671,7 +674,9 @@ int run_linear_tile(const MxsArgs &a, int index, hipStream_t st) {
 // (8) 243, 201 and 211, at 800 (100) -, 306 and 278; 128 experts of 2048 x 1024 at 61 tokens (4) 48, 46 and 54, at 1500 (94) -, 90 and 97.
 // Two tiles of 128 x 128 fit a compute unit, so that one's start and end go beside the other's squares, which counts where K is short: 128 experts
 // of 2048 x 768 at 4096 tokens 201 us in tiles of 256 x 128, 185 in these, 1024 columns at 2048 144 and 139, 8 experts of 4096 x 2048 gated
-// 128 and 124; 64 of 4096 x 4096 at 2048 432 and 480.
+// 128 and 124; 64 of 4096 x 4096 at 2048 432 and 480.  Columns between 2048 and 4096 were not measured, nor cards of other numbers of compute units.
+// An expert's last tile is half empty on average, and empty rows are multiplied like others: of tiles of 128 rows a third with 128 pairs an expert, a
+// fifth with 256.
 int plan_mapped(int64_t pairs, int E, int K) {
     static const int forced = tune_env("MFQ_MX8_EXPERTS", 0);
     if (forced > 0 && forced <= 4 && (forced > 1 || few_fits(K, 1))) return forced - 1;

@@ -4,7 +4,8 @@
 // MXFP8 or MXFP4 tensors, activations as they come.  Every expert that some token takes is read once, for all of its tokens: bound by the
 // weights' way from memory.
 //
-// The weights' codes are converted to bf16 with their scales, exactly, and v_mfma_f32_16x16x32_bf16 multiplies them with up to 16 columns of
+// The weights' codes are converted to bf16 with their scales, exactly (but for the smallest codes of scales 2^-127 and 2^-126, which bf16's
+// subnormals cut: 1e-6 of a result), and v_mfma_f32_16x16x32_bf16 multiplies them with up to 16 columns of
 // activations.  Values that bf16 does not hold go as sums of such: fp16 as two parts, the hidden rows, which are fp32, as three, each part the
 // rounding of what the ones before leave.  Parts of few tokens are columns beside one another (one column a part and token); else they
 // are multiplied one after the other into the same sums.  So products are exact to 2^-24 and sums are fp32: nothing is rounded to 16 bits

@@ -360,8 +360,9 @@ def nint_matmul_argmax(w: NintWeight, x: torch.Tensor, return_logits: bool = Fal
 
 
 class TokenLogprobs(NamedTuple):
-    """Of every row: the given token's log probability and rank (1 + how many are more probable, by logit - max in fp32), the entropy in nats, and the most probable
-    tokens in order with their log probabilities (empty where none were asked for)."""
+    """Of every row: the given token's log probability and rank (1 + how many are more probable, by logit - max in fp32: logits that this
+    difference does not tell apart have one rank, so top_ids[i] has rank i + 1 or less), the entropy in nats, and the most probable tokens in
+    the order of their logits with their log probabilities (empty where none were asked for)."""
     logprobs: torch.Tensor
     ranks: torch.Tensor
     entropy: torch.Tensor
